@@ -1,0 +1,85 @@
+/*
+ * r9vx_fp8.h -- block-scaled 8-bit floating point on MI355X: the operators of
+ * r9vx.h for checkpoints whose weights are e4m3 with one f32 scale per
+ * 128 x 128 block, beside the GGUF schemes.  No counterpart in the reference,
+ * whose T0 matmul has an e4m3 branch (crates/r9v-t0/src/matmul.rs:1820) and
+ * no device tier for it.
+ *
+ * Conventions are r9vx.h's: caller-owned buffers and workspaces, nothing
+ * allocated in a launch, stream order, refusals before anything is enqueued,
+ * r9vx_last_error().
+ *
+ * Numbers.  e4m3 is the OCP format without infinities (largest 448, smallest
+ * 2^-9, NaN 0x7F).  KB = ceil(K / 128).  Rounding is to nearest, ties to
+ * even, once, of the exact value.  A row of activations is quantized by
+ *     s[m, b] = max(max |x[m, 128 b .. 128 b + 127]| / 448, 2^-126)   (f32)
+ *     q[m, k] = e4m3(x[m, k] / s[m, k / 128])
+ * and a block that holds a NaN or an infinity gets a NaN scale and NaN codes:
+ * every output of that row is NaN, the other rows are as they would be.
+ * Scales are used as given; they may have any sign and value.
+ */
+#ifndef R9VX_FP8_H_
+#define R9VX_FP8_H_
+
+#include "r9vx.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Element type of codes: this path's own code, outside the reference's DType. */
+#define R9VX_DTYPE_E4M3 0x100u
+
+/* ---------------------------------------------------------------- quantize */
+
+typedef struct r9vx_quantize_fp8_args {
+    const void *x;  /* [m, k] of in_dtype, 16-byte aligned */
+    uint8_t *q;     /* e4m3 [m, k], 16-byte aligned */
+    float *scales;  /* f32 [m, KB] */
+    uint64_t m;
+    uint32_t k;        /* a positive multiple of 16 */
+    uint32_t in_dtype; /* F32 or BF16 */
+} r9vx_quantize_fp8_args;
+
+/* One launch; x, q and scales may not overlap. */
+int r9vx_quantize_fp8_launch(const r9vx_quantize_fp8_args *args, r9vx_stream_t stream);
+
+/* ------------------------------------------------------------------ matmul */
+
+typedef struct r9vx_matmul_fp8_static {
+    uint32_t m_bucket;  /* the launch's m <= m_bucket; it, not m, picks the kernels */
+    uint32_t n;         /* output columns, any positive number */
+    uint32_t k;         /* a positive multiple of 16 */
+    uint32_t in_dtype;  /* F32 or BF16 (quantized within the launch) or E4M3 */
+    uint32_t out_dtype; /* F32 or BF16 */
+    uint32_t epilogue;  /* enum r9vx_epilogue */
+} r9vx_matmul_fp8_static;
+
+typedef struct r9vx_matmul_fp8_args {
+    const uint8_t *w;      /* e4m3 [N, K], 16-byte aligned; SWIGLU: [2N, K], gate rows [0, N) then up rows */
+    const float *w_scales; /* f32 [ceil(N / 128), KB]; SWIGLU: the gate rows' and then the up rows' */
+    const void *x;         /* [m, K] of in_dtype, 16-byte aligned */
+    const float *x_scales; /* f32 [m, KB] with E4M3 activations, otherwise NULL */
+    const float *bias;     /* f32 [N] with the BIAS epilogue */
+    const float *residual; /* f32 [m, N] with the RESIDUAL epilogue; may be y */
+    void *y;               /* [m, N] of out_dtype, 16-byte aligned */
+    uint8_t *workspace;    /* r9vx_matmul_fp8_workspace_bytes, 256-byte aligned; NULL when 0 */
+    uint32_t m;
+    uint32_t _tail_pad;
+} r9vx_matmul_fp8_args;
+
+/* y = x . w^T with both operands in e4m3:
+ *     a[m, n] = sum_b xs[m, b] * ws[n / 128, b] * sum_{k in block b} xq[m, k] * wq[n, k]
+ * accumulated in f32, then the epilogue (bias, residual, or
+ * silu(gate) * up), then one rounding to out_dtype.  A row's output bits
+ * depend on the static and the row alone. */
+int r9vx_matmul_fp8_launch(const r9vx_matmul_fp8_static *st, const r9vx_matmul_fp8_args *args, r9vx_stream_t stream);
+size_t r9vx_matmul_fp8_workspace_bytes(const r9vx_matmul_fp8_static *st);
+/* Algorithmic bytes (weights, scales, x, y) and 2 m N K operations (SWIGLU: twice the weights and 4 m N K). */
+uint64_t r9vx_matmul_fp8_static_bytes(const r9vx_matmul_fp8_static *st, uint32_t m);
+uint64_t r9vx_matmul_fp8_static_flops(const r9vx_matmul_fp8_static *st, uint32_t m);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

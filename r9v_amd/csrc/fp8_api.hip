@@ -1,0 +1,139 @@
+/*
+ * fp8_api.hip -- the C ABI of include/r9vx_fp8.h: every problem of a call is
+ * reported and nothing is enqueued when any is found.
+ */
+#include "r9vx_e4m3.h"
+#include "r9vx_host.h"
+
+namespace {
+
+bool float_dtype(uint32_t d) { return d == R9VX_DTYPE_F32 || d == R9VX_DTYPE_BF16; }
+
+void check_k(uint32_t k, Problems &pr) {
+    if (k == 0 || k % 16) pr.add(R9VX_ERR_INVALID, "k=%u must be a positive multiple of 16", k);
+    else if (k > (1u << 20)) pr.add(R9VX_ERR_UNSUPPORTED, "k=%u exceeds 2^20", k); /* 256 rows are addressed by 32 bits */
+}
+
+uint64_t scale_blocks(uint32_t n, uint32_t k) { return (uint64_t)r9vx_fp8_kb(n) * r9vx_fp8_kb(k); }
+
+bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + nb && y < x + na;
+}
+
+}  // namespace
+
+extern "C" {
+
+int r9vx_quantize_fp8_launch(const r9vx_quantize_fp8_args *a, r9vx_stream_t stream) {
+    Problems pr;
+    if (!a) {
+        pr.add(R9VX_ERR_NULL, "args must be non-NULL");
+        return pr.finish("quantize_fp8");
+    }
+    check_k(a->k, pr);
+    if (!float_dtype(a->in_dtype)) pr.add(R9VX_ERR_UNSUPPORTED, "in_dtype %u: only f32 and bf16 are quantized", a->in_dtype);
+    if (a->m > (1ull << 40)) pr.add(R9VX_ERR_INVALID, "m=%llu exceeds 2^40", (unsigned long long)a->m);
+    if (a->m && (!a->x || !a->q || !a->scales)) pr.add(R9VX_ERR_NULL, "x, q and scales are required");
+    if (!aligned16(a->x) || !aligned16(a->q)) pr.add(R9VX_ERR_ALIGN, "x and q must be 16-byte aligned");
+    if ((uintptr_t)a->scales & 3u) pr.add(R9VX_ERR_ALIGN, "scales must be 4-byte aligned");
+    if (pr.code == R9VX_OK && a->m) {
+        const uint64_t nx = a->m * a->k * (a->in_dtype == R9VX_DTYPE_F32 ? 4 : 2), nq = a->m * a->k,
+                       ns = a->m * r9vx_fp8_kb(a->k) * 4;
+        if (overlap(a->x, nx, a->q, nq) || overlap(a->x, nx, a->scales, ns) || overlap(a->q, nq, a->scales, ns))
+            pr.add(R9VX_ERR_INVALID, "x, q and scales must not overlap");
+    }
+    const int rc = pr.finish("quantize_fp8");
+    if (rc || a->m == 0) return rc;
+    return hip_status("quantize_fp8", r9vx_launch_quantize_fp8(a->x, a->in_dtype, a->m, a->k, a->q, a->scales,
+                                                               reinterpret_cast<hipStream_t>(stream)));
+}
+
+static void check_matmul_fp8_static(const r9vx_matmul_fp8_static *st, Problems &pr) {
+    check_k(st->k, pr);
+    if (st->n == 0) pr.add(R9VX_ERR_INVALID, "n must be positive");
+    if (st->n > (1u << 30)) pr.add(R9VX_ERR_UNSUPPORTED, "n=%u exceeds 2^30", st->n);
+    if (st->m_bucket > (1u << 24)) pr.add(R9VX_ERR_UNSUPPORTED, "m_bucket=%u exceeds 2^24", st->m_bucket);
+    if (!float_dtype(st->in_dtype) && st->in_dtype != R9VX_DTYPE_E4M3)
+        pr.add(R9VX_ERR_UNSUPPORTED, "in_dtype %u: only f32, bf16 and e4m3 activations", st->in_dtype);
+    if (!float_dtype(st->out_dtype)) pr.add(R9VX_ERR_UNSUPPORTED, "out_dtype %u: only f32 and bf16 outputs", st->out_dtype);
+    if (st->epilogue > R9VX_EPILOGUE_SWIGLU)
+        pr.add(R9VX_ERR_UNSUPPORTED, "epilogue %u: only none/bias/residual/swiglu", st->epilogue);
+}
+
+static bool matmul_fp8_static_ok(const r9vx_matmul_fp8_static *st) {
+    if (!st) return false;
+    Problems pr;
+    check_matmul_fp8_static(st, pr);
+    return pr.code == R9VX_OK;
+}
+
+size_t r9vx_matmul_fp8_workspace_bytes(const r9vx_matmul_fp8_static *st) {
+    return matmul_fp8_static_ok(st) ? r9vx_fp8_workspace_bytes(st->m_bucket, st->k, st->n, st->in_dtype, st->epilogue) : 0;
+}
+
+uint64_t r9vx_matmul_fp8_static_bytes(const r9vx_matmul_fp8_static *st, uint32_t m) {
+    if (!matmul_fp8_static_ok(st)) return 0;
+    const uint64_t pair = st->epilogue == R9VX_EPILOGUE_SWIGLU ? 2 : 1;
+    const uint64_t x = st->in_dtype == R9VX_DTYPE_E4M3 ? (uint64_t)m * (st->k + 4ull * r9vx_fp8_kb(st->k))
+                                                       : (uint64_t)m * st->k * (st->in_dtype == R9VX_DTYPE_F32 ? 4 : 2);
+    return pair * ((uint64_t)st->n * st->k + 4 * scale_blocks(st->n, st->k)) + x +
+           (uint64_t)m * st->n * (st->out_dtype == R9VX_DTYPE_F32 ? 4 : 2);
+}
+
+uint64_t r9vx_matmul_fp8_static_flops(const r9vx_matmul_fp8_static *st, uint32_t m) {
+    if (!matmul_fp8_static_ok(st)) return 0;
+    return (st->epilogue == R9VX_EPILOGUE_SWIGLU ? 4ull : 2ull) * m * st->n * st->k;
+}
+
+int r9vx_matmul_fp8_launch(const r9vx_matmul_fp8_static *st, const r9vx_matmul_fp8_args *a, r9vx_stream_t stream) {
+    Problems pr;
+    if (!st || !a) {
+        pr.add(R9VX_ERR_NULL, "static and args must be non-NULL");
+        return pr.finish("matmul_fp8");
+    }
+    check_matmul_fp8_static(st, pr);
+    if (a->m > st->m_bucket) pr.add(R9VX_ERR_INVALID, "m=%u exceeds m_bucket=%u", a->m, st->m_bucket);
+    const bool codes = st->in_dtype == R9VX_DTYPE_E4M3;
+    if (a->m > 0) {
+        if (!a->w || !a->w_scales) pr.add(R9VX_ERR_NULL, "w and w_scales are required");
+        if (!a->x) pr.add(R9VX_ERR_NULL, "x is NULL");
+        if (!a->y) pr.add(R9VX_ERR_NULL, "y is NULL");
+        if (codes && !a->x_scales) pr.add(R9VX_ERR_NULL, "e4m3 activations without x_scales");
+    }
+    if (!codes && a->x_scales) pr.add(R9VX_ERR_INVALID, "x_scales given with activations that are quantized within the launch");
+    if (st->epilogue == R9VX_EPILOGUE_BIAS && a->m > 0 && !a->bias) pr.add(R9VX_ERR_NULL, "bias epilogue without bias");
+    if (st->epilogue != R9VX_EPILOGUE_BIAS && a->bias) pr.add(R9VX_ERR_INVALID, "bias given without bias epilogue");
+    if (st->epilogue == R9VX_EPILOGUE_RESIDUAL && a->m > 0 && !a->residual)
+        pr.add(R9VX_ERR_NULL, "residual epilogue without residual");
+    if (st->epilogue != R9VX_EPILOGUE_RESIDUAL && a->residual)
+        pr.add(R9VX_ERR_INVALID, "residual given without residual epilogue");
+    if (!aligned16(a->w) || !aligned16(a->x) || !aligned16(a->y) || !aligned16(a->bias) || !aligned16(a->residual))
+        pr.add(R9VX_ERR_ALIGN, "w, x, y, bias and residual must be 16-byte aligned");
+    if (((uintptr_t)a->w_scales | (uintptr_t)a->x_scales) & 3u) pr.add(R9VX_ERR_ALIGN, "scales must be 4-byte aligned");
+    const size_t ws = r9vx_matmul_fp8_workspace_bytes(st);
+    if (ws && a->m > 0 && !a->workspace)
+        pr.add(R9VX_ERR_WORKSPACE, "workspace of r9vx_matmul_fp8_workspace_bytes (%zu) required", ws);
+    if ((uintptr_t)a->workspace & 255u) pr.add(R9VX_ERR_ALIGN, "workspace must be 256-byte aligned");
+    const int rc = pr.finish("matmul_fp8");
+    if (rc || a->m == 0) return rc;
+    r9vx_fp8_problem p{};
+    p.w = a->w;
+    p.w_scales = a->w_scales;
+    p.x = a->x;
+    p.x_scales = a->x_scales;
+    p.bias = a->bias;
+    p.residual = a->residual;
+    p.y = a->y;
+    p.workspace = a->workspace;
+    p.m = a->m;
+    p.m_bucket = st->m_bucket;
+    p.n = st->n;
+    p.k = st->k;
+    p.x_dtype = st->in_dtype;
+    p.y_dtype = st->out_dtype;
+    p.epilogue = st->epilogue;
+    return hip_status("matmul_fp8", r9vx_launch_matmul_fp8(p, reinterpret_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,85 @@
+/*
+ * fp8_quant.hip -- activations to e4m3 with one f32 scale per row and 128
+ * columns.
+ *
+ *   s[m, b] = max(max |x[m, 128 b ..]| / 448, 2^-126)      (f32)
+ *   q[m, k] = e4m3, nearest-even, of the exact x[m, k] / s[m, k / 128]
+ *
+ * One pass: eight lanes hold a block in registers, sixteen values each, take
+ * its maximum by three cross-lane steps and write codes and scale.  Bound by
+ * memory: 3 bytes (bf16) or 5 (f32) per value.
+ */
+#include "r9vx_e4m3.h"
+
+using namespace r9vx;
+
+namespace {
+
+template <bool F32>
+__global__ __launch_bounds__(256) void quantize_fp8_kernel(const void *__restrict__ x, uint32_t blocks, uint32_t k, uint32_t kb,
+                                                           uint8_t *__restrict__ q, float *__restrict__ scales) {
+    const uint32_t blk = blockIdx.x * 32 + (threadIdx.x >> 3);
+    if (blk >= blocks) return; /* whole groups of eight lanes */
+    const uint32_t part = threadIdx.x & 7u;
+    const uint32_t row = blk / kb, b = blk - row * kb;
+    const uint32_t left = k - b * kFp8Block; /* columns from the block's first; k is a multiple of 16 */
+    const uint64_t at = (uint64_t)row * k + b * kFp8Block;
+    float v[16];
+    uint32_t amax = 0;
+    /* a lane holds groups of consecutive columns, the lanes' groups side by
+     * side, so that each load instruction reads whole 128-byte lines */
+    constexpr int G = F32 ? 4 : 8, N = 16 / G;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t c = (j * 8 + part) * G;
+        r9vx_u32x4 w = {0u, 0u, 0u, 0u};
+        if (c < left)
+            w = __builtin_nontemporal_load(reinterpret_cast<const r9vx_u32x4 *>(static_cast<const uint8_t *>(x) + (at + c) * (F32 ? 4 : 2)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = w[i]; /* a copy: bit_cast of a vector's element takes its first one */
+            if constexpr (F32) {
+                v[j * 4 + i] = __builtin_bit_cast(float, u);
+            } else {
+                v[j * 8 + 2 * i] = __builtin_bit_cast(float, u << 16);
+                v[j * 8 + 2 * i + 1] = __builtin_bit_cast(float, u & 0xFFFF0000u);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) amax = max(amax, fp8_absbits(v[i]));
+    const Fp8Scale s = fp8_scale(fp8_max8(amax));
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t c = (j * 8 + part) * G;
+        const uint32_t lo = fp8_code4(v[j * G], v[j * G + 1], v[j * G + 2], v[j * G + 3], s);
+        if constexpr (F32) {
+            if (c < left) *reinterpret_cast<uint32_t *>(q + at + c) = lo;
+        } else {
+            const uint32_t hi = fp8_code4(v[j * G + 4], v[j * G + 5], v[j * G + 6], v[j * G + 7], s);
+            if (c < left) *reinterpret_cast<r9vx_u32x2 *>(q + at + c) = r9vx_u32x2{lo, hi};
+        }
+    }
+    if (part == 0) scales[blk] = s.s;
+}
+
+}  // namespace
+
+int r9vx_launch_quantize_fp8(const void *x, uint32_t x_dtype, uint64_t m, uint32_t k, uint8_t *q, float *scales,
+                             hipStream_t stream) {
+    const uint32_t kb = r9vx_fp8_kb(k);
+    const uint64_t rows = (1u << 31) / kb; /* a launch numbers its blocks in 32 bits */
+    for (uint64_t r0 = 0; r0 < m; r0 += rows) {
+        const uint32_t n = (uint32_t)((m - r0 < rows ? m - r0 : rows) * kb);
+        const dim3 grid((n + 31) / 32);
+        if (x_dtype == R9VX_DTYPE_F32)
+            hipLaunchKernelGGL(quantize_fp8_kernel<true>, grid, dim3(256), 0, stream, static_cast<const float *>(x) + r0 * k, n, k, kb,
+                               q + r0 * k, scales + r0 * kb);
+        else
+            hipLaunchKernelGGL(quantize_fp8_kernel<false>, grid, dim3(256), 0, stream, static_cast<const uint16_t *>(x) + r0 * k, n, k, kb,
+                               q + r0 * k, scales + r0 * kb);
+        const int e = (int)hipGetLastError();
+        if (e) return e;
+    }
+    return 0;
+}

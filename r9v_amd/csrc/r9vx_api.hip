@@ -14,42 +14,12 @@
 #include <mutex>
 #include <string>
 
+#include "r9vx_host.h"
 #include "r9vx_internal.h"
 #include "r9vx_moe.h"
 #include "r9vx_probe.h"
 
 namespace {
-
-thread_local std::string g_last_error;
-
-struct Problems {
-    std::string text;
-    int code = R9VX_OK;
-    void add(int c, const char *fmt, ...) {
-        char buf[256];
-        va_list ap;
-        va_start(ap, fmt);
-        vsnprintf(buf, sizeof buf, fmt, ap);
-        va_end(ap);
-        if (!text.empty()) text += "; ";
-        text += buf;
-        if (code == R9VX_OK) code = c;
-    }
-    int finish(const char *op) {
-        if (code != R9VX_OK) g_last_error = std::string(op) + ": " + text;
-        return code;
-    }
-};
-
-int hip_status(const char *op, int rc) {
-    if (rc != 0) {
-        g_last_error = std::string(op) + ": HIP error " + std::to_string(rc) + " (" +
-                       hipGetErrorString((hipError_t)rc) + ")";
-    }
-    return rc;
-}
-
-bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 /* Schemes read as GGUF wire blocks (every op), the ones read in the split
  * layout of r9vx_repack_launch (body + d array), and IQ3_S, read as the
@@ -111,6 +81,8 @@ void check_weight_keys(const char *what, uint32_t scheme, uint32_t dtype, uint32
 uint64_t device_row_bytes(uint32_t s, uint32_t k) { return r9vx_row_bytes(s, k); }
 
 }  // namespace
+
+static thread_local std::string g_last_error;
 
 /* Sets the calling thread's r9vx_last_error() text (used by the other host
  * sources of the library). */

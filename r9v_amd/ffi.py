@@ -19,6 +19,7 @@ LIB_PATH = PKG / "libr9vx.so"
 
 # enums (include/r9vx.h)
 F32, F16, BF16, I8, I4, U32 = 0, 1, 2, 5, 6, 8
+E4M3 = 0x100                      # this path's own code (include/r9vx_fp8.h)
 LAYOUT_L0, LAYOUT_L1, LAYOUT_L1S = 1, 2, 3                      # the reference's layouts: refused
 LAYOUT_GGUF_WIRE, LAYOUT_SPLIT, LAYOUT_IQ3S_112 = 0x100, 0x101, 0x102
 # weight schemes: the reference's SchemeId codes (I4K, I4Xs, I6K, I8B32F, Iq3S;
@@ -52,6 +53,20 @@ class MatmulArgs(ctypes.Structure):
     _fields_ = [("w", _P), ("w_scales", _P), ("w_indices", _P), ("x", _P), ("x_scale", _P),
                 ("bias", _P), ("residual", _P), ("y", _P), ("workspace", _P), ("m", _U32),
                 ("_tail_pad", _U32)]
+
+
+class QuantizeFp8Args(ctypes.Structure):
+    _fields_ = [("x", _P), ("q", _P), ("scales", _P), ("m", _U64), ("k", _U32), ("in_dtype", _U32)]
+
+
+class MatmulFp8Static(ctypes.Structure):
+    _fields_ = [("m_bucket", _U32), ("n", _U32), ("k", _U32), ("in_dtype", _U32), ("out_dtype", _U32),
+                ("epilogue", _U32)]
+
+
+class MatmulFp8Args(ctypes.Structure):
+    _fields_ = [("w", _P), ("w_scales", _P), ("x", _P), ("x_scales", _P), ("bias", _P), ("residual", _P), ("y", _P),
+                ("workspace", _P), ("m", _U32), ("_tail_pad", _U32)]
 
 
 class MoeRouteStatic(ctypes.Structure):
@@ -117,6 +132,12 @@ EXPORTS = [
     ("r9vx_scheme_from_ggml_type", [_U32], _U32),
     ("r9vx_last_error", [], ctypes.c_char_p),
     ("r9vx_abi_version", [], _U32),
+    # include/r9vx_fp8.h
+    ("r9vx_quantize_fp8_launch", [_P, _P], ctypes.c_int),
+    ("r9vx_matmul_fp8_launch", [_P, _P, _P], ctypes.c_int),
+    ("r9vx_matmul_fp8_workspace_bytes", [_P], ctypes.c_size_t),
+    ("r9vx_matmul_fp8_static_bytes", [_P, _U32], ctypes.c_uint64),
+    ("r9vx_matmul_fp8_static_flops", [_P, _U32], ctypes.c_uint64),
     # include/r9vx_probe.h
     ("r9vx_probe_stream_launch", [_P, ctypes.c_uint64, _P, _P], ctypes.c_int),
     ("r9vx_probe_stream_blocks", [ctypes.c_uint64], _U32),
@@ -475,6 +496,126 @@ def moe_sort(ids, e, dm=256, dff=256, workspace=None, stream=None):
     _check(load().r9vx_moe_sort_launch(ctypes.byref(st), _ptr(ids), t, _ptr(workspace), _ptr(counts),
                                        _ptr(offsets), _ptr(order), _stream(torch, stream)))
     return counts, offsets, order
+
+
+# ---------------------------------------------------------------- block-scaled e4m3
+
+FP8_BLOCK = 128                   # columns of an activation scale, rows and columns of a weight scale
+
+
+def _fp8_operands(dtypes, **tensors):
+    """torch, after checking that every given operand is a dense row-major
+    tensor of one of its dtypes (names of torch dtypes, by operand) on the
+    current device."""
+    import torch
+
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _need_gpu(t)  # raises: no device at all, or an operand in host memory
+        if device is None:
+            device = t.device
+            if device.index != torch.cuda.current_device():
+                raise R9vxError(-104, f"{name} is on {device}, the current device is cuda:{torch.cuda.current_device()}")
+        elif t.device != device:
+            raise R9vxError(-104, f"{name} is on {t.device}, other operands on {device}")
+        if not t.is_contiguous():
+            raise R9vxError(-103, f"{name} must be contiguous")
+        want = dtypes.get(name)
+        if want and str(t.dtype)[6:] not in want:
+            raise R9vxError(-103, f"{name} is {t.dtype}: it must be one of {', '.join(want)}")
+    return torch
+
+
+def _shape(name, t, *want):
+    if t is not None and tuple(t.shape) != want:
+        raise R9vxError(-103, f"{name} has shape {tuple(t.shape)}: it must be {want}")
+
+
+def _used_on(stream, *tensors):
+    """Memory that was allocated here and is used on a stream of the caller's
+    is not given to others before that stream is through with it."""
+    if stream is not None:
+        for t in tensors:
+            if t is not None:
+                t.record_stream(stream)
+
+
+_FLOATS, _CODES = ("float32", "bfloat16"), ("float8_e4m3fn", "uint8")
+_ACT = _FLOATS + _CODES
+
+
+def _fp8_kb(k):
+    return -(-k // FP8_BLOCK)
+
+
+def quantize_fp8(x, q=None, scales=None, stream=None):
+    """f32 or bf16 x [m, k] -> (e4m3 codes [m, k], f32 scales [m, ceil(k / 128)]):
+    scale = max(max|x| / 448, 2^-126) over a row's 128 columns, code = the e4m3
+    number nearest to x / scale.  k is a multiple of 16."""
+    torch = _fp8_operands({"x": _FLOATS, "q": _CODES, "scales": ("float32",)}, x=x, q=q, scales=scales)
+    m, k = x.shape
+    mine_q = mine_s = None
+    if q is None:
+        q = mine_q = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
+    if scales is None:
+        scales = mine_s = torch.empty((m, _fp8_kb(k)), dtype=torch.float32, device=x.device)
+    _shape("q", q, m, k)
+    _shape("scales", scales, m, _fp8_kb(k))
+    args = QuantizeFp8Args(x.data_ptr(), q.data_ptr(), scales.data_ptr(), m, k, _dtype_code(x))
+    _check(load().r9vx_quantize_fp8_launch(ctypes.byref(args), _stream(torch, stream)))
+    _used_on(stream, mine_q, mine_s)
+    return q, scales
+
+
+def matmul_fp8_workspace_bytes(st: MatmulFp8Static) -> int:
+    return int(load().r9vx_matmul_fp8_workspace_bytes(ctypes.byref(st)))
+
+
+def matmul_fp8(w, w_scales, x, x_scales=None, out_dtype=F32, bias=None, residual=None, y=None, workspace=None,
+               stream=None, swiglu=False, m_bucket=None):
+    """y[m, n] = x . w^T over e4m3 weights w [n, k] with one f32 scale per 128 x 128
+    block, w_scales [ceil(n / 128), ceil(k / 128)] (+ bias [n] | + residual [m, n]).
+    x: f32 or bf16 [m, k], quantized within the call, or the codes and x_scales of
+    `quantize_fp8`.  swiglu: w holds 2n rows, gate [0, n) then up [n, 2n), w_scales
+    the gate's blocks then the up's; y = silu(gate) * up.  m_bucket (default: m)
+    picks the kernels."""
+    torch = _fp8_operands({"w": _CODES, "w_scales": ("float32",), "x": _ACT, "x_scales": ("float32",), "bias": ("float32",),
+                           "residual": ("float32",), "y": ("float32",) if out_dtype == F32 else ("bfloat16",),
+                           "workspace": ("uint8",)},
+                          w=w, w_scales=w_scales, x=x, x_scales=x_scales, bias=bias, residual=residual, y=y, workspace=workspace)
+    m, k = x.shape
+    pair = 2 if swiglu else 1
+    n = w.shape[0] // pair
+    if x_scales is None and x.element_size() == 1:
+        raise R9vxError(-103, "e4m3 activations need x_scales")
+    _shape("w", w, pair * n, k)
+    _shape("w_scales", w_scales, pair * _fp8_kb(n), _fp8_kb(k))
+    _shape("x_scales", x_scales, m, _fp8_kb(k))
+    _shape("bias", bias, n)
+    _shape("residual", residual, m, n)
+    _shape("y", y, m, n)
+    if (bias is not None) + (residual is not None) + swiglu > 1:
+        raise R9vxError(-103, "one epilogue: bias, residual or swiglu")
+    epi = EPILOGUE_BIAS if bias is not None else EPILOGUE_RESIDUAL if residual is not None else \
+        EPILOGUE_SWIGLU if swiglu else EPILOGUE_NONE
+    st = MatmulFp8Static(m_bucket or max(m, 1), n, k, _dtype_code(x) if x_scales is None else E4M3, out_dtype, epi)
+    mine_y = mine_w = None
+    if y is None:
+        y = mine_y = torch.empty((m, n), dtype=torch.float32 if out_dtype == F32 else torch.bfloat16, device=x.device)
+    nbytes = matmul_fp8_workspace_bytes(st)
+    if workspace is None:
+        if nbytes:
+            workspace = mine_w = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    elif workspace.numel() < nbytes:
+        raise R9vxError(-5, f"workspace of {workspace.numel()} bytes: {nbytes} needed")
+    args = MatmulFp8Args(w.data_ptr(), w_scales.data_ptr(), x.data_ptr(), _ptr(x_scales), _ptr(bias), _ptr(residual),
+                         y.data_ptr(), _ptr(workspace), m, 0)
+    _check(load().r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
+    _used_on(stream, mine_y, mine_w)
+    return y
 
 
 # ---------------------------------------------------------------- ceilings

@@ -1,0 +1,117 @@
+"""The block-scaled e4m3 entry points on the CPU: struct layouts and host-side
+refusals (made before any device call), and the figures they report."""
+from __future__ import annotations
+
+import ctypes
+import pathlib
+import subprocess
+
+import pytest
+
+from r9v_amd import ffi
+
+ROOT = pathlib.Path(__file__).resolve().parent.parent
+FAKE = 1 << 20  # aligned, never dereferenced: every call below is refused or has no rows
+INVALID, UNSUPPORTED, NULL, ALIGN, WORKSPACE = -1, -2, -3, -4, -5
+lib = ffi.load()
+
+STRUCTS = {"r9vx_quantize_fp8_args": ffi.QuantizeFp8Args, "r9vx_matmul_fp8_static": ffi.MatmulFp8Static,
+           "r9vx_matmul_fp8_args": ffi.MatmulFp8Args}
+
+
+def refused(fn, *structs, code, text):
+    rc = fn(*[None if s is None else ctypes.byref(s) for s in structs], None)
+    assert rc == code, (rc, lib.r9vx_last_error())
+    assert text in lib.r9vx_last_error().decode()
+
+
+def test_struct_layouts(tmp_path):
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "r9vx_fp8.h"', "int main(void){"]
+    for name, cls in STRUCTS.items():
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        lines += [f'printf("%zu\\n", offsetof({name}, {f}));' for f, _ in cls._fields_]
+    (tmp_path / "s.c").write_text("\n".join([*lines, "return 0;}"]))
+    subprocess.run(["gcc", "-std=c11", "-I", str(ROOT / "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()]
+    want = []
+    for cls in STRUCTS.values():
+        want += [ctypes.sizeof(cls), *(getattr(cls, f).offset for f, _ in cls._fields_)]
+    assert got == want
+
+
+def quant(**kw):
+    a = dict(x=FAKE, q=FAKE + (1 << 16), scales=FAKE + (2 << 16), m=4, k=256, in_dtype=ffi.BF16)
+    a.update(kw)
+    return ffi.QuantizeFp8Args(**a)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(k=0), INVALID, "multiple of 16"), (dict(k=136), INVALID, "multiple of 16"), (dict(k=(1 << 20) + 16), UNSUPPORTED, "2^20"),
+    (dict(in_dtype=ffi.F16), UNSUPPORTED, "in_dtype 1"), (dict(in_dtype=ffi.E4M3), UNSUPPORTED, "in_dtype"),
+    (dict(x=None), NULL, "required"), (dict(q=None), NULL, "required"), (dict(scales=None), NULL, "required"),
+    (dict(x=FAKE + 8), ALIGN, "16-byte"), (dict(scales=FAKE + (2 << 16) + 2), ALIGN, "4-byte"),
+    (dict(q=FAKE + 1024), INVALID, "overlap"), (dict(scales=FAKE + (1 << 16)), INVALID, "overlap"),
+    (dict(m=1 << 41), INVALID, "2^40")])
+def test_quantize_refusals(kw, code, text):
+    refused(lib.r9vx_quantize_fp8_launch, quant(**kw), code=code, text=text)
+
+
+def test_quantize_without_rows_or_arguments():
+    assert lib.r9vx_quantize_fp8_launch(ctypes.byref(quant(m=0, x=None, q=None, scales=None)), None) == 0
+    assert lib.r9vx_quantize_fp8_launch(None, None) == NULL
+
+
+def mm(**kw):
+    st = dict(m_bucket=8, n=200, k=256, in_dtype=ffi.BF16, out_dtype=ffi.F32, epilogue=ffi.EPILOGUE_NONE)
+    a = dict(w=FAKE, w_scales=FAKE, x=FAKE, y=FAKE, workspace=FAKE, m=4)
+    for k, v in kw.items():
+        (st if k in st else a)[k] = v
+    return ffi.MatmulFp8Static(**st), ffi.MatmulFp8Args(**a)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(k=100), INVALID, "multiple of 16"), (dict(n=0), INVALID, "n must be positive"), (dict(n=1 << 31), UNSUPPORTED, "2^30"),
+    (dict(m_bucket=1 << 25), UNSUPPORTED, "m_bucket"), (dict(m=9), INVALID, "exceeds m_bucket"),
+    (dict(in_dtype=ffi.F16), UNSUPPORTED, "in_dtype"), (dict(in_dtype=ffi.I8), UNSUPPORTED, "in_dtype"),
+    (dict(out_dtype=ffi.E4M3), UNSUPPORTED, "out_dtype"), (dict(epilogue=4), UNSUPPORTED, "epilogue 4"),
+    (dict(w=None), NULL, "w and w_scales"), (dict(w_scales=None), NULL, "w and w_scales"), (dict(x=None), NULL, "x is NULL"),
+    (dict(y=None), NULL, "y is NULL"), (dict(in_dtype=ffi.E4M3), NULL, "x_scales"), (dict(x_scales=FAKE), INVALID, "x_scales"),
+    (dict(epilogue=ffi.EPILOGUE_BIAS), NULL, "bias"), (dict(bias=FAKE), INVALID, "bias given"),
+    (dict(epilogue=ffi.EPILOGUE_RESIDUAL), NULL, "residual"), (dict(residual=FAKE), INVALID, "residual given"),
+    (dict(w=FAKE + 4), ALIGN, "16-byte"), (dict(w_scales=FAKE + 1), ALIGN, "4-byte"), (dict(workspace=None), WORKSPACE, "workspace"),
+    (dict(workspace=FAKE + 16), ALIGN, "256-byte")])
+def test_matmul_refusals(kw, code, text):
+    refused(lib.r9vx_matmul_fp8_launch, *mm(**kw), code=code, text=text)
+
+
+def test_matmul_reports_every_problem():
+    refused(lib.r9vx_matmul_fp8_launch, *mm(k=100, n=0, w=None, epilogue=9), code=INVALID, text="epilogue 9")
+    msg = lib.r9vx_last_error().decode()
+    assert "multiple of 16" in msg and "n must be positive" in msg and "w and w_scales" in msg
+
+
+def test_matmul_without_rows_needs_no_operands():
+    st, _ = mm()
+    assert lib.r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(ffi.MatmulFp8Args()), None) == 0
+    assert lib.r9vx_matmul_fp8_launch(None, None, None) == NULL
+
+
+def test_figures():
+    st, _ = mm(m_bucket=64, n=200, k=272)
+    assert ffi.matmul_fp8_workspace_bytes(st) >= 64 * 272 + 64 * 3 * 4
+    assert lib.r9vx_matmul_fp8_static_bytes(ctypes.byref(st), 5) == 200 * 272 + 4 * 2 * 3 + 5 * 272 * 2 + 5 * 200 * 4
+    assert lib.r9vx_matmul_fp8_static_flops(ctypes.byref(st), 5) == 2 * 5 * 200 * 272
+    st.in_dtype, st.epilogue, st.out_dtype = ffi.E4M3, ffi.EPILOGUE_SWIGLU, ffi.BF16
+    assert lib.r9vx_matmul_fp8_static_bytes(ctypes.byref(st), 5) == 2 * (200 * 272 + 4 * 2 * 3) + 5 * (272 + 12) + 5 * 200 * 2
+    assert lib.r9vx_matmul_fp8_static_flops(ctypes.byref(st), 5) == 4 * 5 * 200 * 272
+    st.k = 100
+    assert ffi.matmul_fp8_workspace_bytes(st) == 0 and lib.r9vx_matmul_fp8_static_bytes(ctypes.byref(st), 5) == 0
+
+
+def test_python_calls_refuse_host_tensors():
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(4, 256)
+    with pytest.raises(ffi.R9vxError):
+        ffi.quantize_fp8(x)
+    with pytest.raises(ffi.R9vxError):
+        ffi.matmul_fp8(torch.zeros(8, 256, dtype=torch.uint8), torch.ones(1, 2), x)
