@@ -249,6 +249,48 @@ int r9vx_status_read(const uint32_t *device_word, uint32_t *status, r9vx_stream_
 uint64_t r9vx_moe_route_static_bytes(const r9vx_moe_route_static *st, uint32_t t);
 uint64_t r9vx_moe_route_static_flops(const r9vx_moe_route_static *st, uint32_t t);
 
+/* Grouped routing: scores, a bias that only selects, groups, top-K.  The
+ * reference names the group key (MoeGroup, crates/r9v-ir/src/op.rs:152-157) and
+ * refuses it (crates/r9v-t0/src/moe_route.rs:198-203), so the definition is this:
+ *     s = softmax(logits) or sigmoid(logits);   c = s + bias
+ *     score of a group (E / n_group consecutive experts) = its largest c, or
+ *         the sum of its two largest
+ *     the topk_group groups of the largest score stay; expert_ids = the top_k
+ *         experts of the largest c among theirs, descending, ties to the lower index
+ *     weights = s (without bias), over their sum if renormalize, times scale
+ * compared as f64 has them; weights are rounded once to f32.  Unlike moe_route,
+ * the bias is not in the weights and the scale is applied after
+ * the renormalisation (there it cancels).
+ *
+ * Rows are refused one by one, where moe_route refuses the whole batch: a row
+ * with a non-finite logit or bias, or whose selected scores sum to zero under
+ * renormalize, gets expert ids 0xFFFFFFFF (moe_ffn and moe_ffn_fp8 refuse them)
+ * and weights 0, and its bit is or-ed into the status word; the other rows are
+ * routed.  So no launch waits for a check of all rows, and one word can gather
+ * a whole step's layers: the caller clears it (zero fill) when it likes and
+ * reads it with r9vx_status_read. */
+enum r9vx_group_score { R9VX_GROUP_MAX = 0, R9VX_GROUP_TOP2 = 1 };
+
+typedef struct r9vx_moe_route_group_static {
+    uint32_t t_bucket;
+    uint32_t e_total;     /* E <= 1024, a multiple of n_group */
+    uint32_t top_k;       /* K <= 32, K <= topk_group * E / n_group */
+    uint32_t scoring;     /* enum r9vx_scoring */
+    uint32_t renormalize; /* 0 / 1 */
+    uint32_t n_group;     /* 1 .. 64; 1: no groups */
+    uint32_t topk_group;  /* 1 .. n_group */
+    uint32_t group_score; /* enum r9vx_group_score; TOP2: groups of at least two experts */
+    uint32_t scale_bits;  /* IEEE-754 bits of the f32 scale, finite and > 0 */
+    uint32_t has_bias;    /* 0 / 1 */
+} r9vx_moe_route_group_static;
+
+/* args as for moe_route (logits and bias 4-byte aligned); status: a device u32
+ * or NULL.  One launch. */
+int r9vx_moe_route_group_launch(const r9vx_moe_route_group_static *st, const r9vx_moe_route_args *args,
+                                uint32_t *status, r9vx_stream_t stream);
+uint64_t r9vx_moe_route_group_static_bytes(const r9vx_moe_route_group_static *st, uint32_t t);
+uint64_t r9vx_moe_route_group_static_flops(const r9vx_moe_route_group_static *st, uint32_t t);
+
 /* Routing from hidden states (the router-logits matmul feeding moe_route,
  * fused; decode form, t_bucket <= 8).  No single op of the reference: it replaces the
  * graph's router matmul (f32 weight [E, dm], the GGUF ffn_gate_inp tensor)

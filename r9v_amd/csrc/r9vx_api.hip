@@ -404,6 +404,63 @@ int r9vx_status_read(const uint32_t *word, uint32_t *status, r9vx_stream_t strea
     return hip_status("status_read", rc);
 }
 
+uint64_t r9vx_moe_route_group_static_bytes(const r9vx_moe_route_group_static *st, uint32_t t) {
+    if (!st) return 0;
+    return (uint64_t)t * st->e_total * 4 + (st->has_bias ? 4ull * st->e_total : 0) + (uint64_t)t * st->top_k * 8;
+}
+
+/* Per expert the score's four operations, the bias add and the comparisons of
+ * group and expert; per selection the weight's. */
+uint64_t r9vx_moe_route_group_static_flops(const r9vx_moe_route_group_static *st, uint32_t t) {
+    if (!st) return 0;
+    return (uint64_t)t * ((6ull + (st->has_bias ? 1u : 0u)) * st->e_total + (st->renormalize ? 3ull : 1ull) * st->top_k);
+}
+
+int r9vx_moe_route_group_launch(const r9vx_moe_route_group_static *st, const r9vx_moe_route_args *a, uint32_t *status,
+                                r9vx_stream_t stream) {
+    Problems pr;
+    if (!st || !a) {
+        pr.add(R9VX_ERR_NULL, "static and args must be non-NULL");
+        return pr.finish("moe_route_group");
+    }
+    float scale;
+    memcpy(&scale, &st->scale_bits, 4);
+    if (!(scale > 0.0f) || !(scale < __builtin_huge_valf()))
+        pr.add(R9VX_ERR_INVALID, "scale must be finite and > 0, got %g", (double)scale);
+    if (st->e_total == 0) pr.add(R9VX_ERR_INVALID, "E must be > 0");
+    if (st->e_total > 1024) pr.add(R9VX_ERR_UNSUPPORTED, "E=%u exceeds 1024", st->e_total);
+    if (st->top_k == 0) pr.add(R9VX_ERR_INVALID, "top_k must be > 0");
+    if (st->top_k > 32) pr.add(R9VX_ERR_UNSUPPORTED, "top_k=%u exceeds 32", st->top_k);
+    if (st->n_group > 64) pr.add(R9VX_ERR_UNSUPPORTED, "n_group=%u exceeds 64", st->n_group);
+    if (st->n_group == 0 || st->e_total % st->n_group)
+        pr.add(R9VX_ERR_INVALID, "E=%u is no multiple of n_group=%u", st->e_total, st->n_group);
+    else {
+        const uint32_t per = st->e_total / st->n_group;
+        if (st->topk_group == 0 || st->topk_group > st->n_group)
+            pr.add(R9VX_ERR_INVALID, "topk_group=%u must be 1 .. n_group=%u", st->topk_group, st->n_group);
+        else if (st->top_k > st->topk_group * per)
+            pr.add(R9VX_ERR_INVALID, "top_k=%u exceeds the %u experts of topk_group=%u groups", st->top_k, st->topk_group * per,
+                   st->topk_group);
+        if (st->group_score == R9VX_GROUP_TOP2 && per < 2)
+            pr.add(R9VX_ERR_INVALID, "group_score TOP2 needs groups of at least two experts");
+    }
+    if (st->group_score > R9VX_GROUP_TOP2) pr.add(R9VX_ERR_UNSUPPORTED, "group_score %u", st->group_score);
+    if (st->scoring > R9VX_SCORING_SIGMOID) pr.add(R9VX_ERR_UNSUPPORTED, "scoring %u", st->scoring);
+    if (a->t > st->t_bucket) pr.add(R9VX_ERR_INVALID, "t=%u exceeds t_bucket=%u", a->t, st->t_bucket);
+    if (a->t > 0 && (!a->logits || !a->expert_ids || !a->weights))
+        pr.add(R9VX_ERR_NULL, "logits, expert_ids and weights are required");
+    if (st->has_bias && a->t > 0 && !a->bias) pr.add(R9VX_ERR_NULL, "has_bias set but bias is NULL");
+    if (!st->has_bias && a->bias) pr.add(R9VX_ERR_INVALID, "bias given but has_bias is 0");
+    if (((uintptr_t)a->logits | (uintptr_t)a->bias | (uintptr_t)a->expert_ids | (uintptr_t)a->weights | (uintptr_t)status) & 3u)
+        pr.add(R9VX_ERR_ALIGN, "logits, bias, expert_ids, weights and the status word must be 4-byte aligned");
+    const int rc = pr.finish("moe_route_group");
+    if (rc || a->t == 0) return rc;
+    const r9vx_route_group_problem p{a->logits,     a->bias,         a->expert_ids,  a->weights,                  status,
+                                     a->t,          st->e_total,     st->top_k,      st->n_group,                 st->topk_group,
+                                     st->group_score, st->scoring, st->renormalize ? 1u : 0u, scale};
+    return hip_status("moe_route_group", r9vx_launch_route_group(p, reinterpret_cast<hipStream_t>(stream)));
+}
+
 static void check_route_static(const r9vx_moe_route_static *st, uint32_t t, Problems &pr, float &scale) {
     memcpy(&scale, &st->scale_bits, 4);
     if (st->top_k == 0) pr.add(R9VX_ERR_INVALID, "top_k must be > 0");

@@ -144,6 +144,17 @@ int r9vx_launch_route(const r9vx_route_problem &p, hipStream_t stream, bool *no_
 /* Streams per device that can make plain moe_route launches. */
 uint32_t r9vx_route_stream_words();
 
+struct r9vx_route_group_problem {
+    const float *logits;
+    const float *bias; /* selection only; NULL: none */
+    uint32_t *ids;
+    float *weights;
+    uint32_t *status; /* bits are or-ed into it; NULL: none kept */
+    uint32_t t, e, k, n_group, topk_group, group_score, scoring, renormalize;
+    float scale;
+};
+int r9vx_launch_route_group(const r9vx_route_group_problem &p, hipStream_t stream);
+
 struct r9vx_route_hidden_problem {
     const uint16_t *x; /* bf16 [t, dm] */
     const float *w;    /* f32 [e, dm] */

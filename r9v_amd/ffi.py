@@ -30,6 +30,7 @@ GGML_Q4_K, GGML_IQ4_XS, GGML_Q6_K, GGML_Q8_0, GGML_IQ3_S = 12, 23, 14, 8, 21
 SCHEME_OF_GGML = {GGML_Q4_K: Q4_K, GGML_IQ4_XS: IQ4_XS, GGML_Q6_K: Q6_K, GGML_Q8_0: Q8_0, GGML_IQ3_S: IQ3_S}
 EPILOGUE_NONE, EPILOGUE_BIAS, EPILOGUE_RESIDUAL, EPILOGUE_SWIGLU = 0, 1, 2, 3
 SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
+GROUP_MAX, GROUP_TOP2 = 0, 1
 ACT_SILU = 0
 STATUS_NONFINITE, STATUS_DEGENERATE, STATUS_BAD_EXPERT = 1, 2, 4
 BLOCK_BYTES = {Q4_K: 144, IQ4_XS: 136, Q6_K: 210, Q8_0: 34, IQ3_S: 110}
@@ -75,6 +76,11 @@ class MoeRouteStatic(ctypes.Structure):
                 ("has_bias", _U32)]
 
 
+class MoeRouteGroupStatic(ctypes.Structure):
+    _fields_ = [("t_bucket", _U32), ("e_total", _U32), ("top_k", _U32), ("scoring", _U32), ("renormalize", _U32),
+                ("n_group", _U32), ("topk_group", _U32), ("group_score", _U32), ("scale_bits", _U32), ("has_bias", _U32)]
+
+
 class MoeRouteArgs(ctypes.Structure):
     _fields_ = [("logits", _P), ("bias", _P), ("expert_ids", _P), ("weights", _P), ("t", _U32),
                 ("_tail_pad", _U32)]
@@ -114,6 +120,9 @@ EXPORTS = [
     ("r9vx_status_read", [_P, _P, _P], ctypes.c_int),
     ("r9vx_moe_route_static_bytes", [_P, _U32], ctypes.c_uint64),
     ("r9vx_moe_route_static_flops", [_P, _U32], ctypes.c_uint64),
+    ("r9vx_moe_route_group_launch", [_P, _P, _P, _P], ctypes.c_int),
+    ("r9vx_moe_route_group_static_bytes", [_P, _U32], ctypes.c_uint64),
+    ("r9vx_moe_route_group_static_flops", [_P, _U32], ctypes.c_uint64),
     ("r9vx_moe_route_hidden_launch", [_P, _P, _P], ctypes.c_int),
     ("r9vx_moe_route_hidden_workspace_bytes", [_P], ctypes.c_size_t),
     ("r9vx_moe_route_hidden_status", [_P, _P, _P, _P], ctypes.c_int),
@@ -500,6 +509,8 @@ def moe_sort(ids, e, dm=256, dff=256, workspace=None, stream=None):
 
 # ---------------------------------------------------------------- block-scaled e4m3
 
+# the operators of a checkpoint with e4m3 weights: activations, products, grouped routing, experts
+
 FP8_BLOCK = 128                   # columns of an activation scale, rows and columns of a weight scale
 
 
@@ -549,6 +560,34 @@ _ACT = _FLOATS + _CODES
 
 def _fp8_kb(k):
     return -(-k // FP8_BLOCK)
+
+
+def moe_route_group(logits, k, n_group, topk_group, bias=None, scoring=SCORING_SIGMOID, group_score=GROUP_TOP2,
+                    renormalize=True, scale=1.0, ids=None, weights=None, status=None, stream=None, t_bucket=None):
+    """Grouped routing of f32 logits [t, e]: the k experts of the largest score + bias
+    within the topk_group (of n_group) groups of the largest group score; ids int32
+    and weights f32 [t, k], the weights from the scores without the bias,
+    renormalised, times scale.  A row that cannot be routed (non-finite, or a zero
+    sum) gets ids -1 and weights 0 and its bits are or-ed into `status`
+    (a device int32 of one element, cleared by the caller)."""
+    torch = _fp8_operands({"logits": ("float32",), "bias": ("float32",), "ids": ("int32", "uint32"), "weights": ("float32",),
+                           "status": ("int32", "uint32")},
+                          logits=logits, bias=bias, ids=ids, weights=weights, status=status)
+    t, e = logits.shape
+    mine_i = mine_w = None
+    if ids is None:
+        ids = mine_i = torch.empty((t, k), dtype=torch.int32, device=logits.device)
+    if weights is None:
+        weights = mine_w = torch.empty((t, k), dtype=torch.float32, device=logits.device)
+    _shape("ids", ids, t, k)
+    _shape("weights", weights, t, k)
+    _shape("bias", bias, e)
+    st = MoeRouteGroupStatic(t_bucket or max(t, 1), e, k, scoring, int(renormalize), n_group, topk_group, group_score,
+                             struct.unpack("<I", struct.pack("<f", scale))[0], int(bias is not None))
+    args = MoeRouteArgs(logits.data_ptr(), _ptr(bias), ids.data_ptr(), weights.data_ptr(), t, 0)
+    _check(load().r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(args), _ptr(status), _stream(torch, stream)))
+    _used_on(stream, mine_i, mine_w)
+    return ids, weights
 
 
 def quantize_fp8(x, q=None, scales=None, stream=None):

@@ -15,7 +15,7 @@ FAKE = 1 << 20  # aligned, never dereferenced: every call below is refused or ha
 INVALID, UNSUPPORTED, NULL, ALIGN, WORKSPACE = -1, -2, -3, -4, -5
 lib = ffi.load()
 
-STRUCTS = {"r9vx_quantize_fp8_args": ffi.QuantizeFp8Args, "r9vx_matmul_fp8_static": ffi.MatmulFp8Static,
+STRUCTS = {"r9vx_moe_route_group_static": ffi.MoeRouteGroupStatic, "r9vx_quantize_fp8_args": ffi.QuantizeFp8Args, "r9vx_matmul_fp8_static": ffi.MatmulFp8Static,
            "r9vx_matmul_fp8_args": ffi.MatmulFp8Args}
 
 
@@ -115,3 +115,38 @@ def test_python_calls_refuse_host_tensors():
         ffi.quantize_fp8(x)
     with pytest.raises(ffi.R9vxError):
         ffi.matmul_fp8(torch.zeros(8, 256, dtype=torch.uint8), torch.ones(1, 2), x)
+
+
+def route(**kw):
+    st = dict(t_bucket=8, e_total=64, top_k=8, scoring=1, renormalize=1, n_group=8, topk_group=4, group_score=1,
+              scale_bits=0x3F800000, has_bias=0)
+    a = dict(logits=FAKE, bias=None, expert_ids=FAKE, weights=FAKE, t=4)
+    for k, v in kw.items():
+        (st if k in st else a)[k] = v
+    return ffi.MoeRouteGroupStatic(**st), ffi.MoeRouteArgs(**a)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(e_total=0), INVALID, "E must be"), (dict(e_total=1032), UNSUPPORTED, "exceeds 1024"), (dict(top_k=0), INVALID, "top_k"),
+    (dict(top_k=33), UNSUPPORTED, "top_k=33"), (dict(n_group=0), INVALID, "multiple of n_group"),
+    (dict(n_group=7), INVALID, "multiple of n_group"), (dict(e_total=1024, n_group=128), UNSUPPORTED, "n_group=128"),
+    (dict(topk_group=0), INVALID, "topk_group"), (dict(topk_group=9), INVALID, "topk_group"),
+    (dict(top_k=9, topk_group=1), INVALID, "exceeds the 8 experts"), (dict(n_group=64, topk_group=16), INVALID, "at least two"),
+    (dict(group_score=2), UNSUPPORTED, "group_score 2"), (dict(scoring=2), UNSUPPORTED, "scoring 2"), (dict(t=9), INVALID, "t_bucket"),
+    (dict(logits=None), NULL, "required"), (dict(expert_ids=None), NULL, "required"), (dict(weights=None), NULL, "required"),
+    (dict(has_bias=1), NULL, "bias is NULL"), (dict(bias=FAKE), INVALID, "bias given"), (dict(scale_bits=0), INVALID, "scale"),
+    (dict(scale_bits=0x7F800000), INVALID, "scale"), (dict(logits=FAKE + 2), ALIGN, "4-byte")])
+def test_route_group_refusals(kw, code, text):
+    st, a = route(**kw)
+    assert lib.r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(a), None, None) == code
+    assert text in lib.r9vx_last_error().decode()
+
+
+def test_route_group_other_calls():
+    st, a = route(t=0, logits=None)
+    assert lib.r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(a), None, None) == 0
+    assert lib.r9vx_moe_route_group_launch(None, None, None, None) == NULL
+    st, a = route()
+    assert lib.r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(a), ctypes.c_void_p(FAKE + 1), None) == ALIGN
+    assert lib.r9vx_moe_route_group_static_bytes(ctypes.byref(st), 5) == 5 * 64 * 4 + 5 * 8 * 8
+    assert lib.r9vx_moe_route_group_static_flops(ctypes.byref(st), 5) == 5 * (6 * 64 + 3 * 8)
