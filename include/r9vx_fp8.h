@@ -79,6 +79,51 @@ size_t r9vx_matmul_fp8_workspace_bytes(const r9vx_matmul_fp8_static *st);
 uint64_t r9vx_matmul_fp8_static_bytes(const r9vx_matmul_fp8_static *st, uint32_t m);
 uint64_t r9vx_matmul_fp8_static_flops(const r9vx_matmul_fp8_static *st, uint32_t m);
 
+/* ----------------------------------------------------------------- moe_ffn */
+
+typedef struct r9vx_moe_ffn_fp8_static {
+    uint32_t t_bucket;       /* the launch's t <= t_bucket; it, not t, picks the kernels */
+    uint32_t e_local;        /* routed experts E <= 1024 */
+    uint32_t k_topk;         /* K <= 32 */
+    uint32_t dm;             /* hidden size, a positive multiple of 128 */
+    uint32_t dff;            /* expert intermediate size, a positive multiple of 128 */
+    uint32_t out_dtype;      /* F32 or BF16 */
+    uint32_t shared_experts; /* S shared experts stored after the E routed ones */
+} r9vx_moe_ffn_fp8_static;
+
+typedef struct r9vx_moe_ffn_fp8_args {
+    const void *x;                 /* bf16 [t, Dm], 16-byte aligned */
+    const uint32_t *expert_ids;    /* [t, K] */
+    const float *weights;          /* [t, K] */
+    const uint8_t *w_gate_up;      /* e4m3 [E + S, 2 Dff, Dm]: gate rows, then up rows; 16-byte aligned */
+    const float *w_gate_up_scales; /* f32 [E + S, 2 Dff / 128, Dm / 128] */
+    const uint8_t *w_down;         /* e4m3 [E + S, Dm, Dff], 16-byte aligned */
+    const float *w_down_scales;    /* f32 [E + S, Dm / 128, Dff / 128] */
+    void *y;                       /* [t, Dm] of out_dtype, 16-byte aligned */
+    uint8_t *workspace;            /* r9vx_moe_ffn_fp8_workspace_bytes, 256-byte aligned */
+    uint32_t t;
+    uint32_t _tail_pad;
+} r9vx_moe_ffn_fp8_args;
+
+/* moe_ffn of r9vx.h over e4m3 experts: x is quantized once; an expert's gate
+ * and up products, h = silu(g) * u in f32, h quantized as activations are, the
+ * down product; y[t] = the token's expert outputs times their weights, added
+ * in ascending (expert, slot) order in f32, plus the shared experts' outputs.
+ * A row's output bits depend on the static, the row and its experts alone.
+ * An expert id >= E refuses the whole call: y is not written and
+ * R9VX_STATUS_BAD_EXPERT is set in the workspace. */
+int r9vx_moe_ffn_fp8_launch(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ffn_fp8_args *args, r9vx_stream_t stream);
+size_t r9vx_moe_ffn_fp8_workspace_bytes(const r9vx_moe_ffn_fp8_static *st);
+/* Synchronises `stream` and returns the status bits the last launch with this
+ * workspace left in it. */
+int r9vx_moe_ffn_fp8_status(const r9vx_moe_ffn_fp8_static *st, const uint8_t *workspace, uint32_t *status,
+                            r9vx_stream_t stream);
+/* One expert's weight and scale bytes; an upper bound on a launch's bytes (as
+ * r9vx_moe_ffn_static_bytes); 6 Dm Dff operations per routed and shared row. */
+uint64_t r9vx_moe_ffn_fp8_expert_bytes(const r9vx_moe_ffn_fp8_static *st);
+uint64_t r9vx_moe_ffn_fp8_static_bytes(const r9vx_moe_ffn_fp8_static *st, uint32_t t);
+uint64_t r9vx_moe_ffn_fp8_static_flops(const r9vx_moe_ffn_fp8_static *st, uint32_t t);
+
 #ifdef __cplusplus
 }
 #endif

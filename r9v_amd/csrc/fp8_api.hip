@@ -136,4 +136,110 @@ int r9vx_matmul_fp8_launch(const r9vx_matmul_fp8_static *st, const r9vx_matmul_f
     return hip_status("matmul_fp8", r9vx_launch_matmul_fp8(p, reinterpret_cast<hipStream_t>(stream)));
 }
 
+static void check_moe_fp8_static(const r9vx_moe_ffn_fp8_static *st, Problems &pr) {
+    if (st->e_local == 0) pr.add(R9VX_ERR_INVALID, "E must be > 0");
+    if (st->e_local > 1024) pr.add(R9VX_ERR_UNSUPPORTED, "E=%u exceeds 1024", st->e_local);
+    if (st->k_topk == 0) pr.add(R9VX_ERR_INVALID, "top-k must be > 0");
+    if (st->k_topk > 32) pr.add(R9VX_ERR_UNSUPPORTED, "top-k %u exceeds 32", st->k_topk);
+    if (st->dm == 0 || st->dm % kFp8Block) pr.add(R9VX_ERR_INVALID, "dm=%u must be a positive multiple of 128", st->dm);
+    if (st->dff == 0 || st->dff % kFp8Block) pr.add(R9VX_ERR_INVALID, "dff=%u must be a positive multiple of 128", st->dff);
+    if (st->dm > (1u << 16) || st->dff > (1u << 16)) pr.add(R9VX_ERR_UNSUPPORTED, "dm=%u or dff=%u exceeds 2^16", st->dm, st->dff);
+    if (st->shared_experts > 64) pr.add(R9VX_ERR_UNSUPPORTED, "%u shared experts exceed 64", st->shared_experts);
+    /* rows are addressed by 32 bits */
+    if ((uint64_t)st->t_bucket * st->dm >= (1ull << 32))
+        pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u times dm=%u reaches 2^32", st->t_bucket, st->dm);
+    if ((uint64_t)st->t_bucket * (st->k_topk + (uint64_t)st->shared_experts) >= (1ull << 26))
+        pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u rows of %u experts reach 2^26", st->t_bucket, st->k_topk + st->shared_experts);
+    if (!float_dtype(st->out_dtype)) pr.add(R9VX_ERR_UNSUPPORTED, "out_dtype %u: only f32 and bf16 outputs", st->out_dtype);
+}
+
+static bool moe_fp8_static_ok(const r9vx_moe_ffn_fp8_static *st) {
+    if (!st) return false;
+    Problems pr;
+    check_moe_fp8_static(st, pr);
+    return pr.code == R9VX_OK;
+}
+
+static r9vx_moe_fp8_problem moe_fp8_problem(const r9vx_moe_ffn_fp8_static *st) {
+    r9vx_moe_fp8_problem p{};
+    p.t_bucket = st->t_bucket;
+    p.e = st->e_local;
+    p.k = st->k_topk;
+    p.dm = st->dm;
+    p.dff = st->dff;
+    p.shared = st->shared_experts;
+    p.y_dtype = st->out_dtype;
+    return p;
+}
+
+size_t r9vx_moe_ffn_fp8_workspace_bytes(const r9vx_moe_ffn_fp8_static *st) {
+    return moe_fp8_static_ok(st) ? r9vx_moe_fp8_workspace_bytes(moe_fp8_problem(st)) : 0;
+}
+
+uint64_t r9vx_moe_ffn_fp8_expert_bytes(const r9vx_moe_ffn_fp8_static *st) {
+    if (!moe_fp8_static_ok(st)) return 0;
+    return 3ull * st->dm * st->dff + 12ull * (st->dm / kFp8Block) * (st->dff / kFp8Block);
+}
+
+uint64_t r9vx_moe_ffn_fp8_static_bytes(const r9vx_moe_ffn_fp8_static *st, uint32_t t) {
+    if (!moe_fp8_static_ok(st)) return 0;
+    const uint64_t pairs = (uint64_t)t * st->k_topk;
+    const uint64_t experts = (pairs < st->e_local ? pairs : st->e_local) + st->shared_experts;
+    return experts * r9vx_moe_ffn_fp8_expert_bytes(st) + (uint64_t)t * st->dm * (2 + (st->out_dtype == R9VX_DTYPE_F32 ? 4 : 2)) + pairs * 8;
+}
+
+uint64_t r9vx_moe_ffn_fp8_static_flops(const r9vx_moe_ffn_fp8_static *st, uint32_t t) {
+    if (!moe_fp8_static_ok(st)) return 0;
+    return 6ull * t * (st->k_topk + st->shared_experts) * st->dm * st->dff;
+}
+
+int r9vx_moe_ffn_fp8_launch(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ffn_fp8_args *a, r9vx_stream_t stream) {
+    Problems pr;
+    if (!st || !a) {
+        pr.add(R9VX_ERR_NULL, "static and args must be non-NULL");
+        return pr.finish("moe_ffn_fp8");
+    }
+    check_moe_fp8_static(st, pr);
+    if (a->t > st->t_bucket) pr.add(R9VX_ERR_INVALID, "t=%u exceeds t_bucket=%u", a->t, st->t_bucket);
+    if (a->t > 0) {
+        if (!a->x || !a->expert_ids || !a->weights || !a->y) pr.add(R9VX_ERR_NULL, "x, expert_ids, weights and y are required");
+        if (!a->w_gate_up || !a->w_gate_up_scales || !a->w_down || !a->w_down_scales)
+            pr.add(R9VX_ERR_NULL, "w_gate_up, w_down and their scales are required");
+        if (!a->workspace) pr.add(R9VX_ERR_WORKSPACE, "workspace of r9vx_moe_ffn_fp8_workspace_bytes required");
+    }
+    if (!aligned16(a->x) || !aligned16(a->w_gate_up) || !aligned16(a->w_down) || !aligned16(a->y))
+        pr.add(R9VX_ERR_ALIGN, "x, w_gate_up, w_down and y must be 16-byte aligned");
+    if (((uintptr_t)a->expert_ids | (uintptr_t)a->weights | (uintptr_t)a->w_gate_up_scales | (uintptr_t)a->w_down_scales) & 3u)
+        pr.add(R9VX_ERR_ALIGN, "expert_ids, weights and scales must be 4-byte aligned");
+    if ((uintptr_t)a->workspace & 255u) pr.add(R9VX_ERR_ALIGN, "workspace must be 256-byte aligned");
+    const int rc = pr.finish("moe_ffn_fp8");
+    if (rc || a->t == 0) return rc;
+    r9vx_moe_fp8_problem p = moe_fp8_problem(st);
+    p.x = reinterpret_cast<const uint16_t *>(a->x);
+    p.ids = a->expert_ids;
+    p.weights = a->weights;
+    p.w_gu = a->w_gate_up;
+    p.w_dn = a->w_down;
+    p.s_gu = a->w_gate_up_scales;
+    p.s_dn = a->w_down_scales;
+    p.y = a->y;
+    p.ws = a->workspace;
+    p.t = a->t;
+    return hip_status("moe_ffn_fp8", r9vx_launch_moe_fp8(p, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int r9vx_moe_ffn_fp8_status(const r9vx_moe_ffn_fp8_static *st, const uint8_t *workspace, uint32_t *status, r9vx_stream_t stream) {
+    Problems pr;
+    if (!st || !workspace || !status) {
+        pr.add(R9VX_ERR_NULL, "static, workspace and status are required");
+        return pr.finish("moe_ffn_fp8_status");
+    }
+    check_moe_fp8_static(st, pr);
+    const int rc = pr.finish("moe_ffn_fp8_status");
+    if (rc) return rc;
+    r9vx_moe_fp8_problem p = moe_fp8_problem(st);
+    p.ws = const_cast<uint8_t *>(workspace);
+    return r9vx_status_read(r9vx_moe_fp8_status_word(p), status, stream);
+}
+
 }  // extern "C"

@@ -25,7 +25,7 @@ template <int MT, int NT, int W, int XT, bool GATED>
 __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a) {
     __shared__ __attribute__((aligned(16))) r9vx_f32x4 part[W * NT * MT * 64];
     const uint32_t strip = blockIdx.x, m0 = blockIdx.y * (MT * 16);
-    Fp8Rows r;
+    Fp8Rows r{};
     r.w = a.w;
     r.ws = a.ws;
     r.m0 = m0;
@@ -46,16 +46,16 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(Fp8Args a) {
     const uint32_t q = tiles >> 3, rem = tiles & 7u;
     const uint32_t at = x * q + (x < rem ? x : rem) + i;
     const uint32_t nt = at / a.m_tiles, mt = at - nt * a.m_tiles;
-    Fp8Rows r;
+    Fp8Rows r{};
     r.w = a.w;
     r.ws = a.ws;
     r.m0 = mt * BM;
     r.rows = a.m - r.m0 < (uint32_t)BM ? a.m - r.m0 : (uint32_t)BM;
     T t;
     if (r.rows > BM - 16)
-        t.template run<true>(a, r, nt, lds, nullptr);
+        t.template run<true>(a, r, nt, lds);
     else
-        t.template run<false>(a, r, nt, lds, nullptr);
+        t.template run<false>(a, r, nt, lds);
     t.drain(lds, [&](uint32_t t0) {
         for (uint32_t o = threadIdx.x; o < T::kPass * (T::kCols / 4); o += 512) {
             const uint32_t row = o / (T::kCols / 4), quad = o % (T::kCols / 4), n = nt * T::kCols + quad * 4;

@@ -1,0 +1,289 @@
+/*
+ * fp8_moe.hip -- moe_ffn over block-scaled e4m3 experts.
+ *
+ *   quantize x -> permute (the stable counting sort of moe.hip) -> per expert
+ *   gate / up product, silu(g) * u, quantize h -> down product -> weighted
+ *   sum per token.
+ *
+ * Rows of h and o stand in sorted order (the pairs of an expert together,
+ * then the shared experts' rows), so an expert's rows are one run.  The sort
+ * leaves a list of tiles of up to 256 rows of one expert; both products walk
+ * it: few rows per expert through the streaming loop, many through the tiles
+ * of r9vx_e4m3_gemm.h.
+ */
+#include "r9vx_e4m3_gemm.h"
+#include "r9vx_moe.h"
+
+using namespace r9vx;
+
+namespace {
+
+struct Fp8MoeLayout {
+    MoeLayout sort; /* the sort's regions */
+    uint64_t xq, xs, h, hq, hs, o, total;
+    bool stream; /* few rows per expert */
+};
+
+/* Few rows: the streaming form. */
+bool moe_streams(const r9vx_moe_fp8_problem &p) { return p.t_bucket <= 64; }
+
+Fp8MoeLayout moe_layout(const r9vx_moe_fp8_problem &p) {
+    Fp8MoeLayout L{};
+    const uint64_t pairs = (uint64_t)p.t_bucket * p.k, rows = pairs + (uint64_t)p.shared * p.t_bucket;
+    const uint64_t nchunk = (pairs + 255) / 256;
+    uint64_t off = 0;
+    auto take = [&](uint64_t bytes) {
+        const uint64_t at = off;
+        off += (bytes + 255) & ~255ull;
+        return at;
+    };
+    MoeLayout &s = L.sort;
+    s.max_tiles3 = (uint32_t)(rows / kMoeTileM3 + (pairs < p.e ? pairs : p.e) + p.shared);
+    s.status = take(64);
+    s.counts = take(4ull * p.e);
+    s.offsets = take(4ull * (p.e + 1));
+    s.sorted = take(4 * pairs);
+    s.inv = take(4 * pairs);
+    s.rank = take(4 * pairs);
+    s.ccount = take(4ull * p.e * nchunk);
+    s.cbase = take(4ull * p.e * nchunk);
+    s.cbad = take(4 * nchunk);
+    s.tiles3 = take(16ull * s.max_tiles3 + 16);
+    L.stream = moe_streams(p);
+    L.xq = take((uint64_t)p.t_bucket * p.dm);
+    L.xs = take(4ull * p.t_bucket * (p.dm / kFp8Block));
+    L.h = take(L.stream ? 4 * rows * p.dff : 0);
+    L.hq = take(rows * p.dff);
+    L.hs = take(4 * rows * (p.dff / kFp8Block));
+    L.o = take(4 * rows * p.dm);
+    L.total = off;
+    return L;
+}
+
+struct Fp8MoeArgs {
+    Fp8Args g;      /* n, k, kb, nb, xq, xs of this product; w, ws of expert 0 */
+    uint8_t *ws;
+    Fp8MoeLayout L;
+    uint32_t p, t, topk;
+    float *out;     /* f32 rows of h (streaming gate / up) or o */
+    uint8_t *hq;
+    float *hs;
+};
+
+/* Tile `at` of the list: the rows of one expert. */
+__device__ __forceinline__ r9vx_u32x4 moe_tile(const Fp8MoeArgs &a, uint32_t at) {
+    return reinterpret_cast<const r9vx_u32x4 *>(a.ws + a.L.sort.tiles3)[at];
+}
+__device__ __forceinline__ uint32_t moe_word(const Fp8MoeArgs &a, uint32_t i) {
+    return reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.status)[i];
+}
+/* The token of row i of a tile that starts at sorted position `first`. */
+__device__ __forceinline__ uint32_t moe_token(const Fp8MoeArgs &a, uint32_t pos) {
+    if (pos >= a.p) return (pos - a.p) % a.t; /* a shared expert's row */
+    return reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.sorted)[pos] / a.topk;
+}
+
+/* UP: gate / up, rows gathered by token, h stored; else down on h's rows. */
+template <int MT, int NT, int W, bool UP>
+__global__ __launch_bounds__(W * 64) void fp8_moe_stream_kernel(Fp8MoeArgs a) {
+    __shared__ __attribute__((aligned(16))) r9vx_f32x4 part[W * NT * MT * 64];
+    __shared__ uint32_t token[256];
+    if (moe_word(a, 0) != 0u || blockIdx.y >= moe_word(a, 4)) return;
+    const r9vx_u32x4 tile = moe_tile(a, blockIdx.y);
+    Fp8Rows r{};
+    r.w = a.g.w + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.n * a.g.k;
+    r.ws = a.g.ws + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.nb * a.g.kb;
+    if (UP) {
+        for (uint32_t i = threadIdx.x; i < tile.z; i += W * 64) token[i] = moe_token(a, tile.y + i);
+        __syncthreads();
+        r.list = token;
+    }
+    for (uint32_t m0 = 0; m0 < tile.z; m0 += MT * 16) {
+        r.m0 = (UP ? 0u : tile.y) + m0;
+        r.rows = tile.z - m0 < MT * 16u ? tile.z - m0 : MT * 16u;
+        fp8_stream<MT, NT, W, 0, UP>(a.g, r, blockIdx.x, part, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
+            *reinterpret_cast<r9vx_f32x4 *>(a.out + (uint64_t)(tile.y + m0 + row) * a.g.n + n) = v;
+        });
+        __syncthreads(); /* the partial sums have been read */
+    }
+}
+
+template <bool UP>
+__global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
+    typedef Fp8Tile<256, 256, 2, UP, false> T;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::kLds];
+    __shared__ uint32_t token[256];
+    if (moe_word(a, 0) != 0u) return;
+    /* each XCD takes one run of the list, a tile's column blocks side by side */
+    const uint32_t cols = (a.g.n + T::kCols - 1) / T::kCols, tiles = moe_word(a, 4) * cols;
+    const uint32_t x = blockIdx.x & 7u, i = blockIdx.x >> 3, q = tiles >> 3, rem = tiles & 7u;
+    if (i >= q + (x < rem ? 1u : 0u)) return;
+    const uint32_t at = x * q + (x < rem ? x : rem) + i, nt = at % cols;
+    const r9vx_u32x4 tile = moe_tile(a, at / cols);
+    Fp8Rows r{};
+    r.w = a.g.w + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.n * a.g.k;
+    r.ws = a.g.ws + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.nb * a.g.kb;
+    r.rows = tile.z;
+    r.m0 = UP ? 0u : tile.y;
+    if (UP) {
+        for (uint32_t j = threadIdx.x; j < tile.z; j += 512) token[j] = moe_token(a, tile.y + j);
+        __syncthreads();
+        r.list = token;
+    }
+    T t;
+    if (r.rows > 240)
+        t.template run<true>(a.g, r, nt, lds);
+    else
+        t.template run<false>(a.g, r, nt, lds);
+    t.drain(lds, [&](uint32_t t0) {
+        if constexpr (UP) {
+            /* a row's 128 columns are one block of h: eight lanes, sixteen values each */
+            const uint32_t part = threadIdx.x & 7u;
+            for (uint32_t row = threadIdx.x >> 3; row < T::kPass && t0 + row < r.rows; row += 64) {
+                r9vx_f32x4 v[4];
+                uint32_t amax = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = *reinterpret_cast<const r9vx_f32x4 *>(lds + T::at(row, part * 4 + j));
+                    amax = max(max(amax, max(fp8_absbits(v[j].x), fp8_absbits(v[j].y))), max(fp8_absbits(v[j].z), fp8_absbits(v[j].w)));
+                }
+                const Fp8Scale s = fp8_scale(fp8_max8(amax));
+                r9vx_u32x4 c;
+                c.x = fp8_code4(v[0].x, v[0].y, v[0].z, v[0].w, s);
+                c.y = fp8_code4(v[1].x, v[1].y, v[1].z, v[1].w, s);
+                c.z = fp8_code4(v[2].x, v[2].y, v[2].z, v[2].w, s);
+                c.w = fp8_code4(v[3].x, v[3].y, v[3].z, v[3].w, s);
+                const uint64_t pos = tile.y + t0 + row;
+                *reinterpret_cast<r9vx_u32x4 *>(a.hq + pos * a.g.n + nt * 128 + part * 16) = c;
+                if (part == 0) a.hs[pos * a.g.nb + nt] = s.s;
+            }
+        } else {
+            for (uint32_t o = threadIdx.x; o < T::kPass * (T::kCols / 4); o += 512) {
+                const uint32_t row = o / (T::kCols / 4), quad = o % (T::kCols / 4), n = nt * T::kCols + quad * 4;
+                if (t0 + row < r.rows && n < a.g.n)
+                    *reinterpret_cast<r9vx_f32x4 *>(a.out + (uint64_t)(tile.y + t0 + row) * a.g.n + n) =
+                        *reinterpret_cast<const r9vx_f32x4 *>(lds + T::at(row, quad));
+            }
+        }
+    });
+}
+
+struct Fp8CombineArgs {
+    const float *weights;
+    const float *o;
+    void *y;
+    const uint8_t *ws;
+    Fp8MoeLayout L;
+    uint32_t t, k, dm, shared, p, y_bf16;
+};
+
+/* y[t] = sum over the token's rows in ascending sorted position (= ascending
+ * (expert, slot)) of w * o, then the shared experts' rows.  A workgroup takes
+ * 1024 columns of one token. */
+__global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) {
+    __shared__ uint32_t spos[kMoeMaxK], opos[kMoeMaxK];
+    __shared__ float sw[kMoeMaxK], ow[kMoeMaxK];
+    if (reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.status)[0] != 0u) return; /* a refused call writes no y */
+    const uint32_t t = blockIdx.x, kk = a.k;
+    if (threadIdx.x < kk) {
+        spos[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.inv)[(uint64_t)t * kk + threadIdx.x];
+        sw[threadIdx.x] = a.weights[(uint64_t)t * kk + threadIdx.x];
+    }
+    __syncthreads();
+    if (threadIdx.x < kk) {
+        const uint32_t p = spos[threadIdx.x];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < kk; ++j) rank += spos[j] < p ? 1u : 0u;
+        opos[rank] = p;
+        ow[rank] = sw[threadIdx.x];
+    }
+    __syncthreads();
+    const uint32_t d = (blockIdx.y * 256 + threadIdx.x) * 4;
+    if (d >= a.dm) return;
+    r9vx_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t j = 0; j < kk; ++j) {
+        const r9vx_f32x4 v = *reinterpret_cast<const r9vx_f32x4 *>(a.o + (uint64_t)opos[j] * a.dm + d);
+        acc = acc + ow[j] * v;
+    }
+    for (uint32_t s = 0; s < a.shared; ++s)
+        acc = acc + *reinterpret_cast<const r9vx_f32x4 *>(a.o + ((uint64_t)a.p + (uint64_t)s * a.t + t) * a.dm + d);
+    const uint64_t at = (uint64_t)t * a.dm + d;
+    if (a.y_bf16)
+        *reinterpret_cast<r9vx_u32x2 *>(static_cast<uint16_t *>(a.y) + at) =
+            r9vx_u32x2{(uint32_t)r9vx_f32_to_bf16(acc.x) | ((uint32_t)r9vx_f32_to_bf16(acc.y) << 16),
+                       (uint32_t)r9vx_f32_to_bf16(acc.z) | ((uint32_t)r9vx_f32_to_bf16(acc.w) << 16)};
+    else
+        *reinterpret_cast<r9vx_f32x4 *>(static_cast<float *>(a.y) + at) = acc;
+}
+
+}  // namespace
+
+size_t r9vx_moe_fp8_workspace_bytes(const r9vx_moe_fp8_problem &p) { return moe_layout(p).total; }
+
+const uint32_t *r9vx_moe_fp8_status_word(const r9vx_moe_fp8_problem &p) {
+    return reinterpret_cast<const uint32_t *>(p.ws + moe_layout(p).sort.status);
+}
+
+int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
+    const Fp8MoeLayout L = moe_layout(p);
+    uint8_t *const xq = p.ws + L.xq, *const hq = p.ws + L.hq;
+    float *const xs = reinterpret_cast<float *>(p.ws + L.xs), *const hs = reinterpret_cast<float *>(p.ws + L.hs);
+    float *const h = reinterpret_cast<float *>(p.ws + L.h), *const o = reinterpret_cast<float *>(p.ws + L.o);
+    int rc = r9vx_launch_quantize_fp8(p.x, R9VX_DTYPE_BF16, p.t, p.dm, xq, xs, stream);
+    if (rc) return rc;
+    r9vx_moe_problem sp{};
+    sp.ids = p.ids;
+    sp.ws = p.ws;
+    sp.t = p.t;
+    sp.e = p.e;
+    sp.k = p.k;
+    sp.shared = p.shared;
+    rc = r9vx_moe_sort_stage(sp, L.sort, stream, false);
+    if (rc) return rc;
+    const uint32_t pairs = p.t * p.k, rows = pairs + p.shared * p.t;
+    Fp8MoeArgs up{}, dn{};
+    up.ws = dn.ws = p.ws;
+    up.L = dn.L = L;
+    up.p = dn.p = pairs;
+    up.t = dn.t = p.t;
+    up.topk = dn.topk = p.k;
+    up.g.w = p.w_gu;
+    up.g.ws = p.s_gu;
+    up.g.xq = xq;
+    up.g.xs = xs;
+    up.g.n = p.dff;
+    up.g.k = p.dm;
+    up.g.nb = p.dff / kFp8Block;
+    up.g.kb = p.dm / kFp8Block;
+    up.out = h;
+    up.hq = hq;
+    up.hs = hs;
+    dn.g.w = p.w_dn;
+    dn.g.ws = p.s_dn;
+    dn.g.xq = hq;
+    dn.g.xs = hs;
+    dn.g.n = p.dm;
+    dn.g.k = p.dff;
+    dn.g.nb = p.dm / kFp8Block;
+    dn.g.kb = p.dff / kFp8Block;
+    dn.out = o;
+    /* the launch's tiles are at most this many (the list's own count is on the device) */
+    const uint32_t tiles = rows / kMoeTileM3 + (pairs < p.e ? pairs : p.e) + p.shared;
+    if (L.stream) {
+        hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 8, true>), dim3(p.dff / 16, tiles), dim3(512), 0, stream, up);
+        rc = (int)hipGetLastError();
+        if (!rc) rc = r9vx_launch_quantize_fp8(h, R9VX_DTYPE_F32, rows, p.dff, hq, hs, stream);
+        if (rc) return rc;
+        hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 8, false>), dim3(p.dm / 32, tiles), dim3(512), 0, stream, dn);
+    } else {
+        hipLaunchKernelGGL((fp8_moe_tile_kernel<true>), dim3(tiles * ((p.dff + 127) / 128) + 7), dim3(512), 0, stream, up);
+        rc = (int)hipGetLastError();
+        if (rc) return rc;
+        hipLaunchKernelGGL((fp8_moe_tile_kernel<false>), dim3(tiles * ((p.dm + 255) / 256) + 7), dim3(512), 0, stream, dn);
+    }
+    rc = (int)hipGetLastError();
+    if (rc) return rc;
+    const Fp8CombineArgs c{p.weights, o, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16};
+    hipLaunchKernelGGL(fp8_moe_combine_kernel, dim3(p.t, (p.dm / 4 + 255) / 256), dim3(256), 0, stream, c);
+    return (int)hipGetLastError();
+}

@@ -148,4 +148,19 @@ struct r9vx_fp8_problem {
 size_t r9vx_fp8_workspace_bytes(uint32_t m_bucket, uint32_t k, uint32_t n, uint32_t x_dtype, uint32_t epilogue);
 int r9vx_launch_matmul_fp8(const r9vx_fp8_problem &p, hipStream_t stream);
 
+struct r9vx_moe_fp8_problem {
+    const uint16_t *x;
+    const uint32_t *ids;
+    const float *weights;
+    const uint8_t *w_gu, *w_dn;
+    const float *s_gu, *s_dn;
+    void *y;
+    uint8_t *ws;
+    uint32_t t, t_bucket, e, k, dm, dff, shared, y_dtype;
+};
+size_t r9vx_moe_fp8_workspace_bytes(const r9vx_moe_fp8_problem &p);
+int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream);
+/* Device address of the status word in a workspace. */
+const uint32_t *r9vx_moe_fp8_status_word(const r9vx_moe_fp8_problem &p);
+
 #endif

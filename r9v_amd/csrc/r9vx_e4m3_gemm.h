@@ -22,11 +22,12 @@ struct Fp8Args {
 };
 
 /* The weights and activation rows of one workgroup: rows m0 .. m0 + rows - 1,
- * or with an index list rows list[i]. */
+ * or, with an index list, rows list[m0] .. list[m0 + rows - 1]. */
 struct Fp8Rows {
     const uint8_t *w;
     const float *ws;
     uint32_t m0, rows;
+    const uint32_t *list; /* NULL: none */
 };
 
 #ifdef __HIPCC__
@@ -110,6 +111,7 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
     for (int i = 0; i < MT; ++i) {
         uint32_t m = i * 16 + c;
         m = r.m0 + (m < r.rows ? m : r.rows - 1);
+        if (r.list) m = r.list[m];
         xrow[i] = a.xq + (uint64_t)m * a.k;
         srow[i] = a.xs + (uint64_t)m * a.kb;
     }
@@ -202,10 +204,9 @@ struct Fp8Tile {
                      : "memory", "m0");
     }
 
-    /* list: the activation row of each tile row (NULL: rows m0 on).  ALL: every
-     * row tile of the workgroup holds rows. */
+    /* ALL: every row tile of the workgroup holds rows. */
     template <bool ALL>
-    __device__ __forceinline__ void run(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds, const uint32_t *list) {
+    __device__ __forceinline__ void run(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds) {
         const uint32_t lane = threadIdx.x & 63u;
         const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
         const uint32_t wm = wave / WN, wn = wave % WN;
@@ -216,13 +217,13 @@ struct Fp8Tile {
 
         /* sources of this lane's copies, from the tile's first row */
         uint32_t xo[IX], wo[IW];
-        const uint8_t *xbase = list ? a.xq : a.xq + (uint64_t)r.m0 * a.k;
+        const uint8_t *xbase = r.list ? a.xq : a.xq + (uint64_t)r.m0 * a.k;
         const uint8_t *wg = r.w + (uint64_t)n0 * a.k, *wu = wg + (uint64_t)a.n * a.k;
 #pragma unroll
         for (int i = 0; i < IX; ++i) {
             const uint32_t row = (wave * IX + i) * 8 + (lane >> 3), c = (lane & 7u) ^ ((row >> 1) & 7u); /* the chunk at this lane's slot */
             const uint32_t in = row < r.rows ? row : r.rows - 1;
-            xo[i] = (list ? list[in] : in) * a.k + c * 16;
+            xo[i] = (r.list ? r.list[r.m0 + in] : in) * a.k + c * 16;
         }
 #pragma unroll
         for (int i = 0; i < IW; ++i) {
@@ -232,10 +233,10 @@ struct Fp8Tile {
             wo[i] = j * a.k + c * 16;
         }
         uint32_t so = 0;
-        const float *sbase = list ? a.xs : a.xs + (uint64_t)r.m0 * a.kb;
+        const float *sbase = r.list ? a.xs : a.xs + (uint64_t)r.m0 * a.kb;
         if (wave < IX) {
             const uint32_t row = wave * 64 + lane, in = row < r.rows ? row : r.rows - 1;
-            so = (list ? list[in] : in) * a.kb * 4;
+            so = (r.list ? r.list[r.m0 + in] : in) * a.kb * 4;
         }
         /* this lane's chunk of an even and of an odd copy's row, in bytes */
         const uint32_t ce = ((lane & 7u) ^ (lane >> 4)) * 16, co = ce ^ 64u;

@@ -70,6 +70,16 @@ class MatmulFp8Args(ctypes.Structure):
                 ("workspace", _P), ("m", _U32), ("_tail_pad", _U32)]
 
 
+class MoeFfnFp8Static(ctypes.Structure):
+    _fields_ = [("t_bucket", _U32), ("e_local", _U32), ("k_topk", _U32), ("dm", _U32), ("dff", _U32), ("out_dtype", _U32),
+                ("shared_experts", _U32)]
+
+
+class MoeFfnFp8Args(ctypes.Structure):
+    _fields_ = [("x", _P), ("expert_ids", _P), ("weights", _P), ("w_gate_up", _P), ("w_gate_up_scales", _P), ("w_down", _P),
+                ("w_down_scales", _P), ("y", _P), ("workspace", _P), ("t", _U32), ("_tail_pad", _U32)]
+
+
 class MoeRouteStatic(ctypes.Structure):
     _fields_ = [("t_bucket", _U32), ("e_total", _U32), ("top_k", _U32), ("scoring", _U32),
                 ("renormalize", _U32), ("n_group", _U32), ("topk_group", _U32), ("scale_bits", _U32),
@@ -147,6 +157,12 @@ EXPORTS = [
     ("r9vx_matmul_fp8_workspace_bytes", [_P], ctypes.c_size_t),
     ("r9vx_matmul_fp8_static_bytes", [_P, _U32], ctypes.c_uint64),
     ("r9vx_matmul_fp8_static_flops", [_P, _U32], ctypes.c_uint64),
+    ("r9vx_moe_ffn_fp8_launch", [_P, _P, _P], ctypes.c_int),
+    ("r9vx_moe_ffn_fp8_workspace_bytes", [_P], ctypes.c_size_t),
+    ("r9vx_moe_ffn_fp8_status", [_P, _P, _P, _P], ctypes.c_int),
+    ("r9vx_moe_ffn_fp8_expert_bytes", [_P], ctypes.c_uint64),
+    ("r9vx_moe_ffn_fp8_static_bytes", [_P, _U32], ctypes.c_uint64),
+    ("r9vx_moe_ffn_fp8_static_flops", [_P, _U32], ctypes.c_uint64),
     # include/r9vx_probe.h
     ("r9vx_probe_stream_launch", [_P, ctypes.c_uint64, _P, _P], ctypes.c_int),
     ("r9vx_probe_stream_blocks", [ctypes.c_uint64], _U32),
@@ -655,6 +671,62 @@ def matmul_fp8(w, w_scales, x, x_scales=None, out_dtype=F32, bias=None, residual
     _check(load().r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
     _used_on(stream, mine_y, mine_w)
     return y
+
+
+def ffn_fp8_static(t_bucket, e, k, dm, dff, shared=0, out_dtype=F32):
+    return MoeFfnFp8Static(t_bucket, e, k, dm, dff, out_dtype, shared)
+
+
+def ffn_fp8_workspace_bytes(st: MoeFfnFp8Static) -> int:
+    return int(load().r9vx_moe_ffn_fp8_workspace_bytes(ctypes.byref(st)))
+
+
+def moe_ffn_fp8(x, ids, weights, w_gate_up, w_gate_up_scales, w_down, w_down_scales, shared=0, out_dtype=F32, y=None,
+                workspace=None, t_bucket=None, stream=None):
+    """y = moe_ffn over e4m3 experts: bf16 x [t, dm], ids and weights [t, k],
+    w_gate_up [e + shared, 2 dff, dm] with scales [e + shared, 2 dff / 128, dm / 128],
+    w_down [e + shared, dm, dff] with scales [e + shared, dm / 128, dff / 128].
+    ids past the e routed experts refuse the call: y keeps what it held
+    (moe_ffn_fp8_status on a workspace of the caller's tells)."""
+    torch = _fp8_operands({"x": ("bfloat16",), "ids": ("int32", "uint32"), "weights": ("float32",), "w_gate_up": _CODES,
+                           "w_gate_up_scales": ("float32",), "w_down": _CODES, "w_down_scales": ("float32",),
+                           "y": ("float32",) if out_dtype == F32 else ("bfloat16",), "workspace": ("uint8",)},
+                          x=x, ids=ids, weights=weights, w_gate_up=w_gate_up, w_gate_up_scales=w_gate_up_scales,
+                          w_down=w_down, w_down_scales=w_down_scales, y=y, workspace=workspace)
+    t, dm = x.shape
+    k = ids.shape[1]
+    experts, dff = w_down.shape[0], w_down.shape[2]
+    _shape("ids", ids, t, k)
+    _shape("weights", weights, t, k)
+    _shape("w_gate_up", w_gate_up, experts, 2 * dff, dm)
+    _shape("w_gate_up_scales", w_gate_up_scales, experts, 2 * dff // FP8_BLOCK, dm // FP8_BLOCK)
+    _shape("w_down", w_down, experts, dm, dff)
+    _shape("w_down_scales", w_down_scales, experts, dm // FP8_BLOCK, dff // FP8_BLOCK)
+    _shape("y", y, t, dm)
+    if not 0 <= shared < experts:
+        raise R9vxError(-103, f"{shared} shared experts of {experts}")
+    st = ffn_fp8_static(t_bucket or max(t, 1), experts - shared, k, dm, dff, shared, out_dtype)
+    nbytes = ffn_fp8_workspace_bytes(st)
+    mine_y = mine_w = None
+    if workspace is None:
+        workspace = mine_w = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
+    elif workspace.numel() < nbytes:
+        raise R9vxError(-5, f"workspace of {workspace.numel()} bytes: {nbytes} needed")
+    if y is None:
+        y = mine_y = torch.empty((t, dm), dtype=torch.float32 if out_dtype == F32 else torch.bfloat16, device=x.device)
+    args = MoeFfnFp8Args(x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(), w_gate_up_scales.data_ptr(),
+                         w_down.data_ptr(), w_down_scales.data_ptr(), y.data_ptr(), workspace.data_ptr(), t, 0)
+    _check(load().r9vx_moe_ffn_fp8_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
+    _used_on(stream, mine_y, mine_w)
+    return y
+
+
+def moe_ffn_fp8_status(st, workspace, stream=None) -> int:
+    """Status bits of the last moe_ffn_fp8 launch with this workspace."""
+    torch = _need_gpu(workspace)
+    s = ctypes.c_uint32(0)
+    _check(load().r9vx_moe_ffn_fp8_status(ctypes.byref(st), _ptr(workspace), ctypes.byref(s), _stream(torch, stream)))
+    return s.value
 
 
 # ---------------------------------------------------------------- ceilings

@@ -15,7 +15,8 @@ FAKE = 1 << 20  # aligned, never dereferenced: every call below is refused or ha
 INVALID, UNSUPPORTED, NULL, ALIGN, WORKSPACE = -1, -2, -3, -4, -5
 lib = ffi.load()
 
-STRUCTS = {"r9vx_moe_route_group_static": ffi.MoeRouteGroupStatic, "r9vx_quantize_fp8_args": ffi.QuantizeFp8Args, "r9vx_matmul_fp8_static": ffi.MatmulFp8Static,
+STRUCTS = {"r9vx_moe_ffn_fp8_static": ffi.MoeFfnFp8Static, "r9vx_moe_ffn_fp8_args": ffi.MoeFfnFp8Args,
+           "r9vx_moe_route_group_static": ffi.MoeRouteGroupStatic, "r9vx_quantize_fp8_args": ffi.QuantizeFp8Args, "r9vx_matmul_fp8_static": ffi.MatmulFp8Static,
            "r9vx_matmul_fp8_args": ffi.MatmulFp8Args}
 
 
@@ -150,3 +151,41 @@ def test_route_group_other_calls():
     assert lib.r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(a), ctypes.c_void_p(FAKE + 1), None) == ALIGN
     assert lib.r9vx_moe_route_group_static_bytes(ctypes.byref(st), 5) == 5 * 64 * 4 + 5 * 8 * 8
     assert lib.r9vx_moe_route_group_static_flops(ctypes.byref(st), 5) == 5 * (6 * 64 + 3 * 8)
+
+
+def moe(**kw):
+    st = dict(t_bucket=8, e_local=16, k_topk=4, dm=256, dff=384, out_dtype=ffi.F32, shared_experts=1)
+    a = dict(x=FAKE, expert_ids=FAKE, weights=FAKE, w_gate_up=FAKE, w_gate_up_scales=FAKE, w_down=FAKE, w_down_scales=FAKE,
+             y=FAKE, workspace=FAKE, t=5)
+    for k, v in kw.items():
+        (st if k in st else a)[k] = v
+    return ffi.MoeFfnFp8Static(**st), ffi.MoeFfnFp8Args(**a)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(e_local=0), INVALID, "E must be"), (dict(e_local=1025), UNSUPPORTED, "exceeds 1024"), (dict(k_topk=0), INVALID, "top-k"),
+    (dict(k_topk=33), UNSUPPORTED, "top-k 33"), (dict(dm=0), INVALID, "dm=0"), (dict(dm=192), INVALID, "dm=192"),
+    (dict(dff=64), INVALID, "dff=64"), (dict(dff=1 << 17), UNSUPPORTED, "2^16"), (dict(shared_experts=65), UNSUPPORTED, "65 shared"),
+    (dict(t_bucket=1 << 24), UNSUPPORTED, "2^32"), (dict(t_bucket=1 << 23, k_topk=16, dm=128), UNSUPPORTED, "2^26"),
+    (dict(out_dtype=ffi.F16), UNSUPPORTED, "out_dtype"), (dict(t=9), INVALID, "t_bucket"), (dict(x=None), NULL, "required"),
+    (dict(expert_ids=None), NULL, "required"), (dict(weights=None), NULL, "required"), (dict(y=None), NULL, "required"),
+    (dict(w_gate_up=None), NULL, "scales are required"), (dict(w_gate_up_scales=None), NULL, "scales are required"),
+    (dict(w_down=None), NULL, "scales are required"), (dict(w_down_scales=None), NULL, "scales are required"),
+    (dict(workspace=None), WORKSPACE, "workspace"), (dict(workspace=FAKE + 64), ALIGN, "256-byte"), (dict(x=FAKE + 2), ALIGN, "16-byte"),
+    (dict(w_down_scales=FAKE + 2), ALIGN, "4-byte")])
+def test_moe_refusals(kw, code, text):
+    refused(lib.r9vx_moe_ffn_fp8_launch, *moe(**kw), code=code, text=text)
+
+
+def test_moe_other_calls_and_figures():
+    st, a = moe(t=0, x=None, y=None, workspace=None)
+    assert lib.r9vx_moe_ffn_fp8_launch(ctypes.byref(st), ctypes.byref(a), None) == 0
+    assert lib.r9vx_moe_ffn_fp8_launch(None, None, None) == NULL
+    assert lib.r9vx_moe_ffn_fp8_status(ctypes.byref(st), None, None, None) == NULL
+    expert = 3 * 256 * 384 + 12 * 2 * 3
+    assert lib.r9vx_moe_ffn_fp8_expert_bytes(ctypes.byref(st)) == expert
+    assert lib.r9vx_moe_ffn_fp8_static_bytes(ctypes.byref(st), 5) == 17 * expert + 5 * 256 * 6 + 20 * 8
+    assert lib.r9vx_moe_ffn_fp8_static_flops(ctypes.byref(st), 5) == 6 * 25 * 256 * 384
+    assert ffi.ffn_fp8_workspace_bytes(st) > 0
+    st.dm = 100
+    assert ffi.ffn_fp8_workspace_bytes(st) == 0 and lib.r9vx_moe_ffn_fp8_static_bytes(ctypes.byref(st), 5) == 0
