@@ -525,40 +525,67 @@ def moe_sort(ids, e, dm=256, dff=256, workspace=None, stream=None):
 
 # ---------------------------------------------------------------- block-scaled e4m3
 
-# the operators of a checkpoint with e4m3 weights: activations, products, grouped routing, experts
+# The operators of a checkpoint with e4m3 weights: activations, products, grouped
+# routing, experts.  A decode step makes many of these calls and each takes a few
+# microseconds on the GPU, so they check their operands without building
+# anything per call and keep the statics they have filled.
 
 FP8_BLOCK = 128                   # columns of an activation scale, rows and columns of a weight scale
 
 
-def _fp8_operands(dtypes, **tensors):
-    """torch, after checking that every given operand is a dense row-major
-    tensor of one of its dtypes (names of torch dtypes, by operand) on the
-    current device."""
-    import torch
+class _Fp8:
+    """torch, and the dtypes the operands may have (filled on the first call)."""
+    torch = None
 
-    device = None
-    for name, t in tensors.items():
+
+def _fp8():
+    if _Fp8.torch is None:
+        import torch
+
+        _Fp8.f32, _Fp8.bf16, _Fp8.bytes = (torch.float32,), (torch.bfloat16,), (torch.uint8,)
+        _Fp8.floats = (torch.bfloat16, torch.float32)
+        _Fp8.codes = (torch.float8_e4m3fn, torch.uint8)
+        _Fp8.acts = _Fp8.floats + _Fp8.codes
+        _Fp8.ids = (torch.int32, torch.uint32)
+        _Fp8.out = {F32: _Fp8.f32, BF16: _Fp8.bf16}
+        _Fp8.torch = torch
+    return _Fp8
+
+
+def _fp8_operands(*operands):
+    """Checks that every given (name, tensor, dtypes, shape) is a dense row-major
+    tensor of one of the dtypes and that shape, on the current device; returns
+    its index."""
+    device = -1
+    for name, t, dtypes, shape in operands:
         if t is None:
             continue
-        if not t.is_cuda:
-            _need_gpu(t)  # raises: no device at all, or an operand in host memory
-        if device is None:
-            device = t.device
-            if device.index != torch.cuda.current_device():
-                raise R9vxError(-104, f"{name} is on {device}, the current device is cuda:{torch.cuda.current_device()}")
-        elif t.device != device:
-            raise R9vxError(-104, f"{name} is on {t.device}, other operands on {device}")
+        d = t.get_device()
+        if d != device or d < 0:
+            if d < 0:
+                _need_gpu(t)  # raises: no device at all, or an operand in host memory
+            if device >= 0:
+                raise R9vxError(-104, f"{name} is on cuda:{d}, other operands on cuda:{device}")
+            device = d
+            if d != _Fp8.torch.cuda.current_device():
+                raise R9vxError(-104, f"{name} is on cuda:{d}, the current device is cuda:{_Fp8.torch.cuda.current_device()}")
+        if t.dtype not in dtypes:
+            raise R9vxError(-103, f"{name} is {t.dtype}: it must be one of {', '.join(map(str, dtypes))}")
+        if t.shape != shape:
+            raise R9vxError(-103, f"{name} has shape {tuple(t.shape)}: it must be {shape}")
         if not t.is_contiguous():
             raise R9vxError(-103, f"{name} must be contiguous")
-        want = dtypes.get(name)
-        if want and str(t.dtype)[6:] not in want:
-            raise R9vxError(-103, f"{name} is {t.dtype}: it must be one of {', '.join(want)}")
-    return torch
+    return device
 
 
-def _shape(name, t, *want):
-    if t is not None and tuple(t.shape) != want:
-        raise R9vxError(-103, f"{name} has shape {tuple(t.shape)}: it must be {want}")
+def _rows(name, t, dims=2):
+    if t.dim() != dims:
+        raise R9vxError(-103, f"{name} has {t.dim()} dimensions: it must have {dims}")
+    return t.shape
+
+
+def _raw_stream(device, stream):
+    return _Fp8.torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 def _used_on(stream, *tensors):
@@ -570,12 +597,36 @@ def _used_on(stream, *tensors):
                 t.record_stream(stream)
 
 
-_FLOATS, _CODES = ("float32", "bfloat16"), ("float8_e4m3fn", "uint8")
-_ACT = _FLOATS + _CODES
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _fp8_kb(k):
     return -(-k // FP8_BLOCK)
+
+
+_fp8_statics = {}  # key -> (static, its workspace bytes)
+
+
+def _fp8_static(cls, workspace_bytes, *key):
+    got = _fp8_statics.get((cls, key))
+    if got is None:
+        if len(_fp8_statics) >= 4096:  # a caller that never repeats a size
+            _fp8_statics.clear()
+        st = cls(*key)
+        got = _fp8_statics[cls, key] = (st, workspace_bytes(st))
+    return got
+
+
+def _workspace(workspace, nbytes, like):
+    """(workspace, the one allocated here or None)"""
+    if workspace is None:
+        if nbytes:
+            workspace = like.new_empty(nbytes, dtype=_Fp8.torch.uint8)
+        return workspace, workspace
+    if workspace.numel() < nbytes:
+        raise R9vxError(-5, f"workspace of {workspace.numel()} bytes: {nbytes} needed")
+    return workspace, None
 
 
 def moe_route_group(logits, k, n_group, topk_group, bias=None, scoring=SCORING_SIGMOID, group_score=GROUP_TOP2,
@@ -586,22 +637,19 @@ def moe_route_group(logits, k, n_group, topk_group, bias=None, scoring=SCORING_S
     renormalised, times scale.  A row that cannot be routed (non-finite, or a zero
     sum) gets ids -1 and weights 0 and its bits are or-ed into `status`
     (a device int32 of one element, cleared by the caller)."""
-    torch = _fp8_operands({"logits": ("float32",), "bias": ("float32",), "ids": ("int32", "uint32"), "weights": ("float32",),
-                           "status": ("int32", "uint32")},
-                          logits=logits, bias=bias, ids=ids, weights=weights, status=status)
-    t, e = logits.shape
+    T = _fp8()
+    t, e = _rows("logits", logits)
+    device = _fp8_operands(("logits", logits, T.f32, (t, e)), ("bias", bias, T.f32, (e,)), ("ids", ids, T.ids, (t, k)),
+                           ("weights", weights, T.f32, (t, k)), ("status", status, T.ids, (1,)))
     mine_i = mine_w = None
     if ids is None:
-        ids = mine_i = torch.empty((t, k), dtype=torch.int32, device=logits.device)
+        ids = mine_i = logits.new_empty((t, k), dtype=T.torch.int32)
     if weights is None:
-        weights = mine_w = torch.empty((t, k), dtype=torch.float32, device=logits.device)
-    _shape("ids", ids, t, k)
-    _shape("weights", weights, t, k)
-    _shape("bias", bias, e)
-    st = MoeRouteGroupStatic(t_bucket or max(t, 1), e, k, scoring, int(renormalize), n_group, topk_group, group_score,
-                             struct.unpack("<I", struct.pack("<f", scale))[0], int(bias is not None))
-    args = MoeRouteArgs(logits.data_ptr(), _ptr(bias), ids.data_ptr(), weights.data_ptr(), t, 0)
-    _check(load().r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(args), _ptr(status), _stream(torch, stream)))
+        weights = mine_w = logits.new_empty((t, k))
+    st, _ = _fp8_static(MoeRouteGroupStatic, lambda st: 0, t_bucket or max(t, 1), e, k, scoring, int(renormalize), n_group,
+                        topk_group, group_score, struct.unpack("<I", struct.pack("<f", scale))[0], int(bias is not None))
+    args = MoeRouteArgs(logits.data_ptr(), _at(bias), ids.data_ptr(), weights.data_ptr(), t, 0)
+    _check(load().r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(args), _at(status), _raw_stream(device, stream)))
     _used_on(stream, mine_i, mine_w)
     return ids, weights
 
@@ -610,17 +658,17 @@ def quantize_fp8(x, q=None, scales=None, stream=None):
     """f32 or bf16 x [m, k] -> (e4m3 codes [m, k], f32 scales [m, ceil(k / 128)]):
     scale = max(max|x| / 448, 2^-126) over a row's 128 columns, code = the e4m3
     number nearest to x / scale.  k is a multiple of 16."""
-    torch = _fp8_operands({"x": _FLOATS, "q": _CODES, "scales": ("float32",)}, x=x, q=q, scales=scales)
-    m, k = x.shape
+    T = _fp8()
+    m, k = _rows("x", x)
+    kb = _fp8_kb(k)
+    device = _fp8_operands(("x", x, T.floats, (m, k)), ("q", q, T.codes, (m, k)), ("scales", scales, T.f32, (m, kb)))
     mine_q = mine_s = None
     if q is None:
-        q = mine_q = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device)
+        q = mine_q = x.new_empty((m, k), dtype=T.torch.float8_e4m3fn)
     if scales is None:
-        scales = mine_s = torch.empty((m, _fp8_kb(k)), dtype=torch.float32, device=x.device)
-    _shape("q", q, m, k)
-    _shape("scales", scales, m, _fp8_kb(k))
-    args = QuantizeFp8Args(x.data_ptr(), q.data_ptr(), scales.data_ptr(), m, k, _dtype_code(x))
-    _check(load().r9vx_quantize_fp8_launch(ctypes.byref(args), _stream(torch, stream)))
+        scales = mine_s = x.new_empty((m, kb), dtype=T.torch.float32)
+    args = QuantizeFp8Args(x.data_ptr(), q.data_ptr(), scales.data_ptr(), m, k, F32 if x.dtype is T.torch.float32 else BF16)
+    _check(load().r9vx_quantize_fp8_launch(ctypes.byref(args), _raw_stream(device, stream)))
     _used_on(stream, mine_q, mine_s)
     return q, scales
 
@@ -637,38 +685,30 @@ def matmul_fp8(w, w_scales, x, x_scales=None, out_dtype=F32, bias=None, residual
     `quantize_fp8`.  swiglu: w holds 2n rows, gate [0, n) then up [n, 2n), w_scales
     the gate's blocks then the up's; y = silu(gate) * up.  m_bucket (default: m)
     picks the kernels."""
-    torch = _fp8_operands({"w": _CODES, "w_scales": ("float32",), "x": _ACT, "x_scales": ("float32",), "bias": ("float32",),
-                           "residual": ("float32",), "y": ("float32",) if out_dtype == F32 else ("bfloat16",),
-                           "workspace": ("uint8",)},
-                          w=w, w_scales=w_scales, x=x, x_scales=x_scales, bias=bias, residual=residual, y=y, workspace=workspace)
-    m, k = x.shape
+    T = _fp8()
+    m, k = _rows("x", x)
     pair = 2 if swiglu else 1
-    n = w.shape[0] // pair
-    if x_scales is None and x.element_size() == 1:
-        raise R9vxError(-103, "e4m3 activations need x_scales")
-    _shape("w", w, pair * n, k)
-    _shape("w_scales", w_scales, pair * _fp8_kb(n), _fp8_kb(k))
-    _shape("x_scales", x_scales, m, _fp8_kb(k))
-    _shape("bias", bias, n)
-    _shape("residual", residual, m, n)
-    _shape("y", y, m, n)
-    if (bias is not None) + (residual is not None) + swiglu > 1:
-        raise R9vxError(-103, "one epilogue: bias, residual or swiglu")
-    epi = EPILOGUE_BIAS if bias is not None else EPILOGUE_RESIDUAL if residual is not None else \
-        EPILOGUE_SWIGLU if swiglu else EPILOGUE_NONE
-    st = MatmulFp8Static(m_bucket or max(m, 1), n, k, _dtype_code(x) if x_scales is None else E4M3, out_dtype, epi)
-    mine_y = mine_w = None
+    n, kb = _rows("w", w)[0] // pair, _fp8_kb(k)
+    device = _fp8_operands(("w", w, T.codes, (pair * n, k)), ("w_scales", w_scales, T.f32, (pair * _fp8_kb(n), kb)),
+                           ("x", x, T.floats if x_scales is None else T.codes, (m, k)), ("x_scales", x_scales, T.f32, (m, kb)),
+                           ("bias", bias, T.f32, (n,)), ("residual", residual, T.f32, (m, n)),
+                           ("y", y, T.out.get(out_dtype, ()), (m, n)),
+                           ("workspace", workspace, T.bytes, workspace.shape if workspace is not None else ()))
+    if bias is not None or residual is not None:
+        if swiglu or (bias is not None and residual is not None):
+            raise R9vxError(-103, "one epilogue: bias, residual or swiglu")
+        epilogue = EPILOGUE_BIAS if bias is not None else EPILOGUE_RESIDUAL
+    else:
+        epilogue = EPILOGUE_SWIGLU if swiglu else EPILOGUE_NONE
+    in_dtype = E4M3 if x_scales is not None else F32 if x.dtype is T.torch.float32 else BF16
+    st, nbytes = _fp8_static(MatmulFp8Static, matmul_fp8_workspace_bytes, m_bucket or max(m, 1), n, k, in_dtype, out_dtype, epilogue)
+    workspace, mine_w = _workspace(workspace, nbytes, x)
+    mine_y = None
     if y is None:
-        y = mine_y = torch.empty((m, n), dtype=torch.float32 if out_dtype == F32 else torch.bfloat16, device=x.device)
-    nbytes = matmul_fp8_workspace_bytes(st)
-    if workspace is None:
-        if nbytes:
-            workspace = mine_w = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    elif workspace.numel() < nbytes:
-        raise R9vxError(-5, f"workspace of {workspace.numel()} bytes: {nbytes} needed")
-    args = MatmulFp8Args(w.data_ptr(), w_scales.data_ptr(), x.data_ptr(), _ptr(x_scales), _ptr(bias), _ptr(residual),
-                         y.data_ptr(), _ptr(workspace), m, 0)
-    _check(load().r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
+        y = mine_y = x.new_empty((m, n), dtype=T.torch.float32 if out_dtype == F32 else T.torch.bfloat16)
+    args = MatmulFp8Args(w.data_ptr(), w_scales.data_ptr(), x.data_ptr(), _at(x_scales), _at(bias), _at(residual),
+                         y.data_ptr(), _at(workspace), m, 0)
+    _check(load().r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(args), _raw_stream(device, stream)))
     _used_on(stream, mine_y, mine_w)
     return y
 
@@ -688,35 +728,28 @@ def moe_ffn_fp8(x, ids, weights, w_gate_up, w_gate_up_scales, w_down, w_down_sca
     w_down [e + shared, dm, dff] with scales [e + shared, dm / 128, dff / 128].
     ids past the e routed experts refuse the call: y keeps what it held
     (moe_ffn_fp8_status on a workspace of the caller's tells)."""
-    torch = _fp8_operands({"x": ("bfloat16",), "ids": ("int32", "uint32"), "weights": ("float32",), "w_gate_up": _CODES,
-                           "w_gate_up_scales": ("float32",), "w_down": _CODES, "w_down_scales": ("float32",),
-                           "y": ("float32",) if out_dtype == F32 else ("bfloat16",), "workspace": ("uint8",)},
-                          x=x, ids=ids, weights=weights, w_gate_up=w_gate_up, w_gate_up_scales=w_gate_up_scales,
-                          w_down=w_down, w_down_scales=w_down_scales, y=y, workspace=workspace)
-    t, dm = x.shape
-    k = ids.shape[1]
-    experts, dff = w_down.shape[0], w_down.shape[2]
-    _shape("ids", ids, t, k)
-    _shape("weights", weights, t, k)
-    _shape("w_gate_up", w_gate_up, experts, 2 * dff, dm)
-    _shape("w_gate_up_scales", w_gate_up_scales, experts, 2 * dff // FP8_BLOCK, dm // FP8_BLOCK)
-    _shape("w_down", w_down, experts, dm, dff)
-    _shape("w_down_scales", w_down_scales, experts, dm // FP8_BLOCK, dff // FP8_BLOCK)
-    _shape("y", y, t, dm)
+    T = _fp8()
+    t, dm = _rows("x", x)
+    k = _rows("ids", ids)[1]
+    experts, _, dff = _rows("w_down", w_down, 3)
+    kb, fb = dm // FP8_BLOCK, dff // FP8_BLOCK
+    device = _fp8_operands(("x", x, T.bf16, (t, dm)), ("ids", ids, T.ids, (t, k)), ("weights", weights, T.f32, (t, k)),
+                           ("w_gate_up", w_gate_up, T.codes, (experts, 2 * dff, dm)),
+                           ("w_gate_up_scales", w_gate_up_scales, T.f32, (experts, 2 * fb, kb)),
+                           ("w_down", w_down, T.codes, (experts, dm, dff)), ("w_down_scales", w_down_scales, T.f32, (experts, kb, fb)),
+                           ("y", y, T.out.get(out_dtype, ()), (t, dm)),
+                           ("workspace", workspace, T.bytes, workspace.shape if workspace is not None else ()))
     if not 0 <= shared < experts:
         raise R9vxError(-103, f"{shared} shared experts of {experts}")
-    st = ffn_fp8_static(t_bucket or max(t, 1), experts - shared, k, dm, dff, shared, out_dtype)
-    nbytes = ffn_fp8_workspace_bytes(st)
-    mine_y = mine_w = None
-    if workspace is None:
-        workspace = mine_w = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
-    elif workspace.numel() < nbytes:
-        raise R9vxError(-5, f"workspace of {workspace.numel()} bytes: {nbytes} needed")
+    st, nbytes = _fp8_static(MoeFfnFp8Static, ffn_fp8_workspace_bytes, t_bucket or max(t, 1), experts - shared, k, dm, dff,
+                             out_dtype, shared)
+    workspace, mine_w = _workspace(workspace, nbytes, x)
+    mine_y = None
     if y is None:
-        y = mine_y = torch.empty((t, dm), dtype=torch.float32 if out_dtype == F32 else torch.bfloat16, device=x.device)
+        y = mine_y = x.new_empty((t, dm), dtype=T.torch.float32 if out_dtype == F32 else T.torch.bfloat16)
     args = MoeFfnFp8Args(x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(), w_gate_up_scales.data_ptr(),
-                         w_down.data_ptr(), w_down_scales.data_ptr(), y.data_ptr(), workspace.data_ptr(), t, 0)
-    _check(load().r9vx_moe_ffn_fp8_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
+                         w_down.data_ptr(), w_down_scales.data_ptr(), y.data_ptr(), _at(workspace), t, 0)
+    _check(load().r9vx_moe_ffn_fp8_launch(ctypes.byref(st), ctypes.byref(args), _raw_stream(device, stream)))
     _used_on(stream, mine_y, mine_w)
     return y
 
