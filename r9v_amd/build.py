@@ -50,7 +50,8 @@ FLAGS = [
 # spill-free (no scratch at all).  So must those whose registers just fit: the
 # thin tiles with eight chains (127 of 128) and the gated streaming GEMV, which
 # holds two rows' weights, would spill in their loops.
-SPILL_FREE = ("moe_gu_m3_kernel", "moe_dn_m3_kernel", "gemm3_kernel", "gemm_thin_kernel", "gemv_gated_stream_kernel")
+SPILL_FREE = ("moe_gu_m3_kernel", "moe_dn_m3_kernel", "gemm3_kernel", "gemm_thin_kernel", "gemv_gated_stream_kernel",
+              "fp8_tile_kernel", "fp8_thin_kernel", "fp8_moe_tile_kernel")
 RESOURCES = BUILD / "kernel_resources.txt"
 
 _FIELDS = {"VGPRs": "vgpr", "AGPRs": "agpr", "ScratchSize [bytes/lane]": "scratch", "VGPRs Spill": "vgpr_spill",

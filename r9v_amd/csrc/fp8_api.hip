@@ -45,7 +45,7 @@ int r9vx_quantize_fp8_launch(const r9vx_quantize_fp8_args *a, r9vx_stream_t stre
     }
     const int rc = pr.finish("quantize_fp8");
     if (rc || a->m == 0) return rc;
-    return hip_status("quantize_fp8", r9vx_launch_quantize_fp8(a->x, a->in_dtype, a->m, a->k, a->q, a->scales,
+    return hip_status("quantize_fp8", r9vx_launch_quantize_fp8(a->x, a->in_dtype, a->m, a->k, a->k, a->q, a->scales,
                                                                reinterpret_cast<hipStream_t>(stream)));
 }
 
@@ -69,7 +69,7 @@ static bool matmul_fp8_static_ok(const r9vx_matmul_fp8_static *st) {
 }
 
 size_t r9vx_matmul_fp8_workspace_bytes(const r9vx_matmul_fp8_static *st) {
-    return matmul_fp8_static_ok(st) ? r9vx_fp8_workspace_bytes(st->m_bucket, st->k, st->n, st->in_dtype, st->epilogue) : 0;
+    return matmul_fp8_static_ok(st) ? r9vx_fp8_workspace_bytes(st->m_bucket, st->k, st->in_dtype) : 0;
 }
 
 uint64_t r9vx_matmul_fp8_static_bytes(const r9vx_matmul_fp8_static *st, uint32_t m) {

@@ -52,16 +52,29 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(Fp8Args a) {
     r.m0 = mt * BM;
     r.rows = a.m - r.m0 < (uint32_t)BM ? a.m - r.m0 : (uint32_t)BM;
     T t;
-    if (r.rows > BM - 16)
-        t.template run<true>(a, r, nt, lds);
-    else
-        t.template run<false>(a, r, nt, lds);
+    t.run(a, r, nt, lds);
     t.drain(lds, [&](uint32_t t0) {
         for (uint32_t o = threadIdx.x; o < T::kPass * (T::kCols / 4); o += 512) {
             const uint32_t row = o / (T::kCols / 4), quad = o % (T::kCols / 4), n = nt * T::kCols + quad * 4;
             if (t0 + row < r.rows && n < a.n) fp8_store_dense(a, r.m0 + t0 + row, n, *reinterpret_cast<const r9vx_f32x4 *>(lds + T::at(row, quad)));
         }
     });
+}
+
+template <int BM, int BN, int WM, int WN, int KS, bool GATED, bool EXACT>
+__global__ __launch_bounds__(512) void fp8_thin_kernel(Fp8Args a) {
+    typedef Fp8Thin<BM, BN, WM, WN, KS, GATED, EXACT> T;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::kLds];
+    const uint32_t tiles = a.m_tiles * a.n_tiles, x = blockIdx.x & 7u, i = blockIdx.x >> 3, q = tiles >> 3, rem = tiles & 7u;
+    const uint32_t at = x * q + (x < rem ? x : rem) + i, nt = at / a.m_tiles, mt = at - nt * a.m_tiles;
+    Fp8Rows r{};
+    r.w = a.w;
+    r.ws = a.ws;
+    r.m0 = mt * BM;
+    r.rows = a.m - r.m0 < (uint32_t)BM ? a.m - r.m0 : (uint32_t)BM;
+    T t;
+    t.run(a, r, nt, lds);
+    t.drain(a, r, nt, lds, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) { fp8_store_dense(a, r.m0 + row, n, v); });
 }
 
 Fp8Args fp8_args(const r9vx_fp8_problem &p, const uint8_t *xq, const float *xs) {
@@ -108,29 +121,85 @@ int launch_tile(Fp8Args a, bool gated, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
+template <int BM, int BN, int WM, int WN, int KS, bool EXACT>
+int launch_thin(Fp8Args a, bool gated, hipStream_t s) {
+    const uint32_t cols = gated ? BN / 2 : BN;
+    a.m_tiles = (a.m + BM - 1) / BM;
+    a.n_tiles = (a.n + cols - 1) / cols;
+    const dim3 grid(a.m_tiles * a.n_tiles);
+    if (gated)
+        hipLaunchKernelGGL((fp8_thin_kernel<BM, BN, WM, WN, KS, true, EXACT>), grid, dim3(512), 0, s, a);
+    else
+        hipLaunchKernelGGL((fp8_thin_kernel<BM, BN, WM, WN, KS, false, EXACT>), grid, dim3(512), 0, s, a);
+    return (int)hipGetLastError();
+}
+
+/* The kernels for more than 64 rows, each with its time in ns as measured
+ * (n = 2112 .. 14336, K = 2048 .. 8192): a workgroup's start and end, and per K
+ * block; `slots` workgroups run beside each other before a round is full.
+ * EXACT = false / true:
+ *   256 x 256 (EXACT 128 x 256)  4096 x 4096 x 4096  75 / 132 us
+ *   64 x 128                     1024 x 4096 x 4096  33 / 44
+ *   64 x 128, 2 blocks a step     517 x 2112 x 4096  19 / 23
+ *   64 x 64, 4 blocks a step      256 x 4096 x 4096  12 / 15 */
+template <bool EXACT>
+int launch_many(const Fp8Args &a, uint32_t m_bucket, bool gated, hipStream_t s) {
+    static constexpr struct {
+        uint32_t bm, bn, slots, start, block, start_x, block_x;
+    } kShapes[4] = {{EXACT ? 128 : 256, 256, 256, 17000, 1790, 12000, 1900},
+                    {64, 128, 512, 4000, 900, 4000, 1250},
+                    {64, 128, 256, 4000, 440, 4000, 590},
+                    {64, 64, 256, 4000, 260, 4000, 330}};
+    const uint64_t n = gated ? 2ull * a.n : a.n;
+    uint32_t best = 0;
+    uint64_t least = ~0ull;
+    for (uint32_t i = 0; i < 4; ++i) {
+        const auto &k = kShapes[i];
+        const uint64_t tiles = ((m_bucket + k.bm - 1) / k.bm) * ((n + k.bn - 1) / k.bn);
+        const uint64_t block = EXACT ? k.block_x : k.block, start = EXACT ? k.start_x : k.start;
+        /* half a round of the 64 x 128 tiles, which share a CU, is two thirds as long as a whole one */
+        const uint64_t rounds = (tiles + k.slots - 1) / k.slots;
+        const uint64_t ns = rounds * start + (i == 1 && tiles <= k.slots / 2 ? block * 2 / 3 : rounds * block) * a.kb;
+        if (ns < least) least = ns, best = i;
+    }
+    switch (best) {
+    case 0: return launch_tile<EXACT ? 128 : 256, 256, 2, EXACT>(a, gated, s);
+    case 1: return launch_tile<64, 128, 2, EXACT>(a, gated, s);
+    case 2: return launch_thin<64, 128, 2, 2, 2, EXACT>(a, gated, s);
+    default: return launch_thin<64, 64, 2, 1, 4, EXACT>(a, gated, s);
+    }
+}
+
 }  // namespace
 
-/* The codes, then the scales, of in-call quantization. */
-size_t r9vx_fp8_workspace_bytes(uint32_t m_bucket, uint32_t k, uint32_t n, uint32_t x_dtype, uint32_t epilogue) {
-    if (x_dtype == R9VX_DTYPE_E4M3) return 0;
-    return (((size_t)m_bucket * k + 255) & ~(size_t)255) + (size_t)m_bucket * r9vx_fp8_kb(k) * 4;
+/* The activations' codes in rows of whole blocks, then (in-call quantization)
+ * their scales.  Codes that come in such rows are read where they are. */
+static size_t fp8_codes_bytes(uint32_t m_bucket, uint32_t k) {
+    return ((size_t)m_bucket * r9vx_fp8_kb(k) * kFp8Block + 255) & ~(size_t)255;
+}
+size_t r9vx_fp8_workspace_bytes(uint32_t m_bucket, uint32_t k, uint32_t x_dtype) {
+    if (x_dtype == R9VX_DTYPE_E4M3) return k % kFp8Block ? fp8_codes_bytes(m_bucket, k) : 0;
+    return fp8_codes_bytes(m_bucket, k) + (size_t)m_bucket * r9vx_fp8_kb(k) * 4;
 }
 
 int r9vx_launch_matmul_fp8(const r9vx_fp8_problem &p, hipStream_t stream) {
     const uint8_t *xq = static_cast<const uint8_t *>(p.x);
     const float *xs = p.x_scales;
     if (p.x_dtype != R9VX_DTYPE_E4M3) {
-        float *s = reinterpret_cast<float *>(p.workspace + (((size_t)p.m_bucket * p.k + 255) & ~(size_t)255));
-        const int rc = r9vx_launch_quantize_fp8(p.x, p.x_dtype, p.m, p.k, p.workspace, s, stream);
+        float *s = reinterpret_cast<float *>(p.workspace + fp8_codes_bytes(p.m_bucket, p.k));
+        const int rc = r9vx_launch_quantize_fp8(p.x, p.x_dtype, p.m, p.k, r9vx_fp8_kb(p.k) * kFp8Block, p.workspace, s, stream);
         if (rc) return rc;
         xq = p.workspace;
         xs = s;
+    } else if (p.k % kFp8Block) {
+        const int rc = r9vx_launch_pad_fp8(xq, p.m, p.k, p.workspace, stream);
+        if (rc) return rc;
+        xq = p.workspace;
     }
     const Fp8Args a = fp8_args(p, xq, xs);
     const bool gated = p.epilogue == R9VX_EPILOGUE_SWIGLU;
     if (p.m_bucket <= 16) return launch_stream<1, 2, 8>(a, gated, stream);
     if (p.m_bucket <= 32) return launch_stream<2, 2, 8>(a, gated, stream);
     if (p.m_bucket <= 64) return launch_stream<4, 2, 8>(a, gated, stream);
-    if (p.y_dtype == R9VX_DTYPE_F32) return launch_tile<128, 256, 2, true>(a, gated, stream);
-    return launch_tile<256, 256, 2, false>(a, gated, stream);
+    return p.y_dtype == R9VX_DTYPE_F32 ? launch_many<true>(a, p.m_bucket, gated, stream) : launch_many<false>(a, p.m_bucket, gated, stream);
 }

@@ -131,10 +131,7 @@ __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
         r.list = token;
     }
     T t;
-    if (r.rows > 240)
-        t.template run<true>(a.g, r, nt, lds);
-    else
-        t.template run<false>(a.g, r, nt, lds);
+    t.run(a.g, r, nt, lds);
     t.drain(lds, [&](uint32_t t0) {
         if constexpr (UP) {
             /* a row's 128 columns are one block of h: eight lanes, sixteen values each */
@@ -229,7 +226,7 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
     uint8_t *const xq = p.ws + L.xq, *const hq = p.ws + L.hq;
     float *const xs = reinterpret_cast<float *>(p.ws + L.xs), *const hs = reinterpret_cast<float *>(p.ws + L.hs);
     float *const h = reinterpret_cast<float *>(p.ws + L.h), *const o = reinterpret_cast<float *>(p.ws + L.o);
-    int rc = r9vx_launch_quantize_fp8(p.x, R9VX_DTYPE_BF16, p.t, p.dm, xq, xs, stream);
+    int rc = r9vx_launch_quantize_fp8(p.x, R9VX_DTYPE_BF16, p.t, p.dm, p.dm, xq, xs, stream);
     if (rc) return rc;
     r9vx_moe_problem sp{};
     sp.ids = p.ids;
@@ -272,7 +269,7 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
     if (L.stream) {
         hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 8, true>), dim3(p.dff / 16, tiles), dim3(512), 0, stream, up);
         rc = (int)hipGetLastError();
-        if (!rc) rc = r9vx_launch_quantize_fp8(h, R9VX_DTYPE_F32, rows, p.dff, hq, hs, stream);
+        if (!rc) rc = r9vx_launch_quantize_fp8(h, R9VX_DTYPE_F32, rows, p.dff, p.dff, hq, hs, stream);
         if (rc) return rc;
         hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 8, false>), dim3(p.dm / 32, tiles), dim3(512), 0, stream, dn);
     } else {

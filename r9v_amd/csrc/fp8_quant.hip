@@ -17,13 +17,14 @@ namespace {
 
 template <bool F32>
 __global__ __launch_bounds__(256) void quantize_fp8_kernel(const void *__restrict__ x, uint32_t blocks, uint32_t k, uint32_t kb,
-                                                           uint8_t *__restrict__ q, float *__restrict__ scales) {
+                                                           uint32_t ldq, uint8_t *__restrict__ q, float *__restrict__ scales) {
     const uint32_t blk = blockIdx.x * 32 + (threadIdx.x >> 3);
     if (blk >= blocks) return; /* whole groups of eight lanes */
     const uint32_t part = threadIdx.x & 7u;
     const uint32_t row = blk / kb, b = blk - row * kb;
     const uint32_t left = k - b * kFp8Block; /* columns from the block's first; k is a multiple of 16 */
-    const uint64_t at = (uint64_t)row * k + b * kFp8Block;
+    const uint64_t at = (uint64_t)row * k + b * kFp8Block, to = (uint64_t)row * ldq + b * kFp8Block;
+    const uint32_t room = ldq - b * kFp8Block; /* code columns: k's, or with zeros behind them to the end of the block */
     float v[16];
     uint32_t amax = 0;
     /* a lane holds groups of consecutive columns, the lanes' groups side by
@@ -54,18 +55,36 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const void *__restric
         const uint32_t c = (j * 8 + part) * G;
         const uint32_t lo = fp8_code4(v[j * G], v[j * G + 1], v[j * G + 2], v[j * G + 3], s);
         if constexpr (F32) {
-            if (c < left) *reinterpret_cast<uint32_t *>(q + at + c) = lo;
+            if (c < room) *reinterpret_cast<uint32_t *>(q + to + c) = c < left ? lo : 0u;
         } else {
             const uint32_t hi = fp8_code4(v[j * G + 4], v[j * G + 5], v[j * G + 6], v[j * G + 7], s);
-            if (c < left) *reinterpret_cast<r9vx_u32x2 *>(q + at + c) = r9vx_u32x2{lo, hi};
+            if (c < room) *reinterpret_cast<r9vx_u32x2 *>(q + to + c) = c < left ? r9vx_u32x2{lo, hi} : r9vx_u32x2{0u, 0u};
         }
     }
     if (part == 0) scales[blk] = s.s;
 }
 
+/* Rows of k codes to rows of whole blocks, zeros behind them. */
+__global__ __launch_bounds__(256) void pad_fp8_kernel(const r9vx_u32x4 *__restrict__ x, uint64_t n, uint32_t k16, uint32_t ld16,
+                                                      r9vx_u32x4 *__restrict__ q) {
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const uint64_t row = i / ld16;
+    const uint32_t c = (uint32_t)(i - row * ld16);
+    q[i] = c < k16 ? x[row * k16 + c] : r9vx_u32x4{0u, 0u, 0u, 0u};
+}
+
 }  // namespace
 
-int r9vx_launch_quantize_fp8(const void *x, uint32_t x_dtype, uint64_t m, uint32_t k, uint8_t *q, float *scales,
+int r9vx_launch_pad_fp8(const uint8_t *x, uint32_t m, uint32_t k, uint8_t *q, hipStream_t stream) {
+    const uint32_t ld16 = r9vx_fp8_kb(k) * (kFp8Block / 16);
+    const uint64_t n = (uint64_t)m * ld16;
+    hipLaunchKernelGGL(pad_fp8_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, reinterpret_cast<const r9vx_u32x4 *>(x), n,
+                       k / 16, ld16, reinterpret_cast<r9vx_u32x4 *>(q));
+    return (int)hipGetLastError();
+}
+
+int r9vx_launch_quantize_fp8(const void *x, uint32_t x_dtype, uint64_t m, uint32_t k, uint32_t ldq, uint8_t *q, float *scales,
                              hipStream_t stream) {
     const uint32_t kb = r9vx_fp8_kb(k);
     const uint64_t rows = (1u << 31) / kb; /* a launch numbers its blocks in 32 bits */
@@ -73,11 +92,11 @@ int r9vx_launch_quantize_fp8(const void *x, uint32_t x_dtype, uint64_t m, uint32
         const uint32_t n = (uint32_t)((m - r0 < rows ? m - r0 : rows) * kb);
         const dim3 grid((n + 31) / 32);
         if (x_dtype == R9VX_DTYPE_F32)
-            hipLaunchKernelGGL(quantize_fp8_kernel<true>, grid, dim3(256), 0, stream, static_cast<const float *>(x) + r0 * k, n, k, kb,
-                               q + r0 * k, scales + r0 * kb);
+            hipLaunchKernelGGL(quantize_fp8_kernel<true>, grid, dim3(256), 0, stream, static_cast<const float *>(x) + r0 * k, n, k, kb, ldq,
+                               q + r0 * ldq, scales + r0 * kb);
         else
-            hipLaunchKernelGGL(quantize_fp8_kernel<false>, grid, dim3(256), 0, stream, static_cast<const uint16_t *>(x) + r0 * k, n, k, kb,
-                               q + r0 * k, scales + r0 * kb);
+            hipLaunchKernelGGL(quantize_fp8_kernel<false>, grid, dim3(256), 0, stream, static_cast<const uint16_t *>(x) + r0 * k, n, k, kb, ldq,
+                               q + r0 * ldq, scales + r0 * kb);
         const int e = (int)hipGetLastError();
         if (e) return e;
     }

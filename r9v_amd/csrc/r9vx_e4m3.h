@@ -131,8 +131,10 @@ __device__ __forceinline__ i32x8 fp8_frag(r9vx_u32x4 lo, r9vx_u32x4 hi) {
 #endif
 
 /* Internal launchers (return hipError_t as int). */
-int r9vx_launch_quantize_fp8(const void *x, uint32_t x_dtype, uint64_t m, uint32_t k, uint8_t *q, float *scales,
+/* ldq: columns of a row of codes, k or (zeros behind k) whole blocks. */
+int r9vx_launch_quantize_fp8(const void *x, uint32_t x_dtype, uint64_t m, uint32_t k, uint32_t ldq, uint8_t *q, float *scales,
                              hipStream_t stream);
+int r9vx_launch_pad_fp8(const uint8_t *x, uint32_t m, uint32_t k, uint8_t *q, hipStream_t stream);
 
 struct r9vx_fp8_problem {
     const uint8_t *w;
@@ -145,7 +147,7 @@ struct r9vx_fp8_problem {
     uint8_t *workspace;
     uint32_t m, m_bucket, n, k, x_dtype, y_dtype, epilogue;
 };
-size_t r9vx_fp8_workspace_bytes(uint32_t m_bucket, uint32_t k, uint32_t n, uint32_t x_dtype, uint32_t epilogue);
+size_t r9vx_fp8_workspace_bytes(uint32_t m_bucket, uint32_t k, uint32_t x_dtype);
 int r9vx_launch_matmul_fp8(const r9vx_fp8_problem &p, hipStream_t stream);
 
 struct r9vx_moe_fp8_problem {

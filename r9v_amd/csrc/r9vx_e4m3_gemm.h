@@ -11,7 +11,7 @@ struct Fp8Args {
     const uint8_t *w;      /* e4m3 [n or 2n, k] */
     const float *ws;       /* [nb or 2 nb, kb] */
     const void *x;         /* activations as given (in-kernel quantization) */
-    const uint8_t *xq;     /* e4m3 [rows, k] */
+    const uint8_t *xq;     /* e4m3 rows of kb whole blocks, zeros past column k */
     const float *xs;       /* [rows, kb] */
     const float *bias;
     const float *residual;
@@ -32,6 +32,24 @@ struct Fp8Rows {
 
 #ifdef __HIPCC__
 namespace r9vx {
+
+/* f(0), f(1), ... f(N - 1) with the index a constant expression. */
+template <int I>
+struct Fp8Int {
+    static constexpr int v = I;
+};
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void fp8_for(F &&f) {
+    if constexpr (I < N) {
+        f(Fp8Int<I>{});
+        fp8_for<N, I + 1>(f);
+    }
+}
+
+/* o + s d */
+__device__ __forceinline__ r9vx_f32x4 fp8_add_scaled(r9vx_f32x4 o, r9vx_f32x4 d, float s) {
+    return r9vx_f32x4{fmaf(d.x, s, o.x), fmaf(d.y, s, o.y), fmaf(d.z, s, o.z), fmaf(d.w, s, o.w)};
+}
 
 /* Four consecutive outputs of one row with the dense epilogues. */
 __device__ __forceinline__ void fp8_store_dense(const Fp8Args &a, uint32_t m, uint32_t n, r9vx_f32x4 v) {
@@ -112,7 +130,7 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
         uint32_t m = i * 16 + c;
         m = r.m0 + (m < r.rows ? m : r.rows - 1);
         if (r.list) m = r.list[m];
-        xrow[i] = a.xq + (uint64_t)m * a.k;
+        xrow[i] = a.xq + (uint64_t)m * (a.kb * kFp8Block);
         srow[i] = a.xs + (uint64_t)m * a.kb;
     }
     /* a strip lies in one 128-row block of the weight scales: 128 is a multiple of its 16 NC rows */
@@ -123,7 +141,7 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
         for (int j = 0; j < NT; ++j) q.w[j] = fp8_load_frag(wrow[j] + k0, g, left);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            q.x[i] = fp8_load_frag(xrow[i] + k0, g, left);
+            q.x[i] = fp8_load_frag(xrow[i] + k0, g, kFp8Block);
             q.sx[i] = srow[i][kb];
         }
         q.sw[0] = wsg[kb];
@@ -141,8 +159,7 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
             for (int j = 0; j < NT; ++j) {
                 const r9vx_f32x4 d = fp8_mma<true>(q.w[j], q.x[i]);
                 const float s = q.sx[i] * q.sw[GATED && j >= NC ? 1 : 0];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s, acc[i][j][e]);
+                acc[i][j] = fp8_add_scaled(acc[i][j], d, s);
             }
     };
     Fp8StreamRegs<MT, NT> q0, q1;
@@ -177,6 +194,33 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
 
 /* ------------------------------------------------------------------ tile */
 
+/* Copies by the lanes of `mask` (all or none: a branch around them would
+ * cut the step's schedule in pieces). */
+__device__ __forceinline__ void fp8_copy16(uint32_t lds_at, const uint8_t *base, uint32_t off, uint32_t mask) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1" ::"v"(off),
+                 "s"(base), "s"(lds_at), "s"(mask)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void fp8_copy4(uint32_t lds_at, const float *base, uint32_t off, uint32_t mask) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dword %0, %1\n\ts_mov_b64 exec, -1" ::"v"(off),
+                 "s"(base), "s"(lds_at), "s"(mask)
+                 : "memory", "m0");
+}
+
+/* The mask of a copy: all lanes where a < b.  In a scalar register whatever the
+ * compiler makes of the comparison (the value is hidden from it, or it would
+ * take the vector register it knows to be uniform). */
+__device__ __forceinline__ uint32_t fp8_copy_mask(uint32_t a, uint32_t b) {
+    int32_t v = (int32_t)(a - b) >> 31;
+    asm("" : "+v"(v));
+    return (uint32_t)__builtin_amdgcn_readfirstlane(v);
+}
+/* A fragment from LDS rows of 128 bytes whose chunk c stands at slot c ^ (row / 2 % 8). */
+__device__ __forceinline__ i32x8 fp8_read_frag(const uint8_t *p, uint32_t frag) {
+    return fp8_frag(*reinterpret_cast<const r9vx_u32x4 *>(p + frag), *reinterpret_cast<const r9vx_u32x4 *>(p + (frag ^ 64u)));
+}
+
+
 /* BM activation rows x BN weight rows, K steps of 128, 8 waves as WM x 8 / WM:
  * wave (wm, wn) owns the 16-row tiles wm, wm + WM, ... of the activations and
  * BN / WN weight rows (GATED: half of them gate rows, half the up rows beside
@@ -188,42 +232,48 @@ template <int BM, int BN, int WM, bool GATED, bool EXACT>
 struct Fp8Tile {
     static constexpr int WN = 8 / WM, TM = BM / 16 / WM, TN = BN / 16 / WN, NC = GATED ? TN / 2 : TN;
     static constexpr uint32_t kX = BM * 128, kW = BN * 128, kS = BM * 4, kStage = kX + kW + kS, kLds = 2 * kStage;
-    static constexpr int IX = BM / 64, IW = BN / 64; /* copies of 8 rows per wave and step */
-    static_assert(BM % 64 == 0 && BN % 128 == 0 && TM * 16 * WM == BM && TN * 16 * WN == BN, "");
+    static constexpr int IW = BN / 64; /* copies of 8 weight rows per wave and step */
+    static_assert(BM % 64 == 0 && BN % 64 == 0 && TM * 16 * WM == BM && TN * 16 * WN == BN, "");
     static_assert(GATED ? BN / 2 <= 128 : BN / WN <= 128, "a wave's rows share one block of weight scales");
     static_assert(kStage % 16 == 0 && kLds <= 160 * 1024, "");
 
     r9vx_f32x4 acc[TM][TN];
 
-    static __device__ __forceinline__ void copy16(uint32_t lds_at, const uint8_t *base, uint32_t off) {
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_at)
-                     : "memory", "m0");
-    }
-    static __device__ __forceinline__ void copy4(uint32_t lds_at, const float *base, uint32_t off) {
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_at)
-                     : "memory", "m0");
+    /* The products of the tile's rows: of all its row tiles, of half or of a
+     * quarter of them, whatever holds the rows (small tiles: of all). */
+    __device__ __forceinline__ void run(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds) {
+        if (TM % 4 != 0 || r.rows > BM / 2)
+            run_rows<TM>(a, r, nt, lds);
+        else if (r.rows > BM / 4)
+            run_rows<TM % 4 ? TM : TM / 2>(a, r, nt, lds);
+        else
+            run_rows<TM % 4 ? TM : TM / 4>(a, r, nt, lds);
     }
 
-    /* ALL: every row tile of the workgroup holds rows. */
-    template <bool ALL>
-    __device__ __forceinline__ void run(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds) {
+    /* NI row tiles of each wave. */
+    template <int NI>
+    __device__ __forceinline__ void run_rows(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds) {
         const uint32_t lane = threadIdx.x & 63u;
         const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
         const uint32_t wm = wave / WN, wn = wave % WN;
         const uint32_t n0 = nt * (GATED ? BN / 2 : BN);
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
         const uint32_t tail = a.k % kFp8Block; /* columns of a last, ragged block */
-        const uint32_t act = (r.rows + 15) / 16;
 
         /* sources of this lane's copies, from the tile's first row */
+        constexpr int RX = NI * WM * 16, IX = RX >= 64 ? RX / 64 : 1; /* activation rows, copies of 8 per wave and step */
+        static_assert(RX % 64 == 0 || 64 % RX == 0, "");
         uint32_t xo[IX], wo[IW];
-        const uint8_t *xbase = r.list ? a.xq : a.xq + (uint64_t)r.m0 * a.k;
+        /* the 8 rows of copy i (fewer than 64 rows: several waves copy the same ones, so that every wave's count of copies is the same) */
+        auto xr8 = [&](int i) { return RX >= 64 ? (wave * IX + i) * 8 : wave % (RX / 8) * 8; };
+        const uint32_t xk = a.kb * kFp8Block;
+        const uint8_t *xbase = r.list ? a.xq : a.xq + (uint64_t)r.m0 * xk;
         const uint8_t *wg = r.w + (uint64_t)n0 * a.k, *wu = wg + (uint64_t)a.n * a.k;
 #pragma unroll
         for (int i = 0; i < IX; ++i) {
-            const uint32_t row = (wave * IX + i) * 8 + (lane >> 3), c = (lane & 7u) ^ ((row >> 1) & 7u); /* the chunk at this lane's slot */
+            const uint32_t row = xr8(i) + (lane >> 3), c = (lane & 7u) ^ ((row >> 1) & 7u); /* the chunk at this lane's slot */
             const uint32_t in = row < r.rows ? row : r.rows - 1;
-            xo[i] = (r.list ? r.list[r.m0 + in] : in) * a.k + c * 16;
+            xo[i] = (r.list ? r.list[r.m0 + in] : in) * xk + c * 16;
         }
 #pragma unroll
         for (int i = 0; i < IW; ++i) {
@@ -232,45 +282,33 @@ struct Fp8Tile {
             j = n0 + j < a.n ? j : a.n - 1 - n0;
             wo[i] = j * a.k + c * 16;
         }
-        uint32_t so = 0;
         const float *sbase = r.list ? a.xs : a.xs + (uint64_t)r.m0 * a.kb;
-        if (wave < IX) {
-            const uint32_t row = wave * 64 + lane, in = row < r.rows ? row : r.rows - 1;
-            so = (r.list ? r.list[r.m0 + in] : in) * a.kb * 4;
-        }
-        /* this lane's chunk of an even and of an odd copy's row, in bytes */
+        const uint32_t s64 = wave % (BM / 64) * 64, srow = s64 + lane, sin = srow < r.rows ? srow : r.rows - 1;
+        const uint32_t so = (r.list ? r.list[r.m0 + sin] : sin) * a.kb * 4;
+        /* this lane's chunk of an even and of an odd copy's row, in bytes.  Weight
+         * chunks past the last column are filled from the block's first one of the
+         * same row: they meet zeros of the activations, and where they hold a NaN
+         * the row's outputs are NaN already. */
         const uint32_t ce = ((lane & 7u) ^ (lane >> 4)) * 16, co = ce ^ 64u;
-        auto issue = [&](uint32_t kb, uint32_t st) {
-            const uint32_t k0 = kb * kFp8Block, at = lds0 + st * kStage;
+        constexpr int kCopies = IX + IW + 1; /* of one wave and step */
+        /* copies [C0, C1) of step kb into stage kb % 2 */
+        auto issue = [&](uint32_t kb, auto C0, auto C1) {
+            const uint32_t mask = fp8_copy_mask(kb, a.kb);
+            const uint32_t k0 = kb * kFp8Block, at = lds0 + (kb & 1u) * kStage;
             const uint32_t cut = tail && kb + 1 == a.kb ? tail : kFp8Block;
-            const uint32_t de = ce >= cut ? ce : 0u, dd = co >= cut ? co : 0u; /* past the last column: the row's first chunk */
-#pragma unroll
-            for (int i = 0; i < IX; ++i) {
-                const uint32_t r8 = (wave * IX + i) * 8;
-                if (!ALL && r8 >= act * 16) break;
-                copy16(at + r8 * 128, xbase + k0, xo[i] - ((wave * IX + i) & 1u ? dd : de));
-            }
-#pragma unroll
-            for (int i = 0; i < IW; ++i) {
-                const uint32_t r8 = (wave * IW + i) * 8;
-                copy16(at + kX + r8 * 128, (GATED && r8 >= BN / 2 ? wu : wg) + k0, wo[i] - ((wave * IW + i) & 1u ? dd : de));
-            }
-            if (wave < IX) copy4(at + kX + kW + wave * 256, sbase + kb, so);
-        };
-        /* chunks past the last column were filled from the row's start: zeros instead */
-        auto clear = [&](uint32_t st) {
-#pragma unroll
-            for (int i = 0; i < IX; ++i) {
-                const uint32_t r8 = (wave * IX + i) * 8;
-                if (((wave * IX + i) & 1u ? co : ce) >= tail)
-                    *reinterpret_cast<r9vx_u32x4 *>(lds + st * kStage + r8 * 128 + lane * 16) = r9vx_u32x4{0u, 0u, 0u, 0u};
-            }
-#pragma unroll
-            for (int i = 0; i < IW; ++i) {
-                const uint32_t r8 = (wave * IW + i) * 8;
-                if (((wave * IW + i) & 1u ? co : ce) >= tail)
-                    *reinterpret_cast<r9vx_u32x4 *>(lds + st * kStage + kX + r8 * 128 + lane * 16) = r9vx_u32x4{0u, 0u, 0u, 0u};
-            }
+            const uint32_t de = ce >= cut ? ce : 0u, dd = co >= cut ? co : 0u;
+            fp8_for<C1.v - C0.v>([&](auto I) {
+                constexpr int c = C0.v + I.v;
+                if constexpr (c < IW) {
+                    const uint32_t r8 = (wave * IW + c) * 8;
+                    fp8_copy16(at + kX + r8 * 128, (GATED && r8 >= BN / 2 ? wu : wg) + k0, wo[c] - ((wave * IW + c) & 1u ? dd : de), mask);
+                } else if constexpr (c < IW + IX) {
+                    const uint32_t r8 = xr8(c - IW);
+                    fp8_copy16(at + r8 * 128, xbase + k0, xo[c - IW], mask);
+                } else {
+                    fp8_copy4(at + kX + kW + s64 * 4, sbase + kb, so, mask);
+                }
+            });
         };
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -283,89 +321,100 @@ struct Fp8Tile {
         const bool in_n = GATED || n0 + wn * (BN / WN) < a.n; /* else no such scale row; the sums are not stored */
         float swg = 0.f, swu = 0.f; /* lane i: the scale of block 64 (kb / 64) + i */
 
-        issue(0, 0);
+        /* A step's copies go out a few with each row tile's products, from the
+         * barrier that frees their stage on: all at once they would hold the
+         * wave until the address unit has taken them (16 cycles each).  The
+         * barrier stands before a step's last row tile, whose operands are in
+         * registers by then: the next step's first operands are read while its
+         * products run. */
+        constexpr int kPer = (8 * kCopies + 5 * NI - 1) / (5 * NI);
+        auto slot = [&](uint32_t kb, auto I) {
+            constexpr int c0 = I.v * kPer < kCopies ? I.v * kPer : kCopies, c1 = c0 + kPer < kCopies ? c0 + kPer : kCopies;
+            issue(kb, Fp8Int<c0>{}, Fp8Int<c1>{});
+        };
+        issue(0, Fp8Int<0>{}, Fp8Int<kCopies>{});
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        slot(1, Fp8Int<0>{});
+
+        i32x8 w[TN];
+        auto read_w = [&](const uint8_t *stage) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const uint32_t row = GATED ? (j >= NC ? BN / 2 : 0u) + (wn * NC + j % NC) * 16 : (wn * TN + j) * 16;
+                w[j] = fp8_read_frag(stage + kX + row * 128, frag);
+            }
+        };
+        const uint32_t xat = wm * 2048, sat = kX + kW + (wm * 16 + (lane & 15u)) * 4;
+        read_w(lds);
+        i32x8 x = fp8_read_frag(lds + xat, frag);
+        float sx = *reinterpret_cast<const float *>(lds + sat);
+        constexpr bool kCarry = NI % 2 == 0; /* the last row tile's sums are added in the next step */
+        r9vx_f32x4 d[2][TN];
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) d[1][j] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
         for (uint32_t kb = 0; kb < a.kb; ++kb) {
-            const uint32_t st = kb & 1u;
             if ((kb & 63u) == 0) {
                 const uint32_t at = kb + lane < a.kb ? kb + lane : a.kb - 1;
                 swg = in_n ? wsg[at] : 0.f;
                 if constexpr (GATED) swu = wsu[at];
+                /* waited for here: a wait in the step would be one for the copies too */
+                asm volatile("" : "+v"(swg), "+v"(swu));
             }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (tail && kb + 1 == a.kb) clear(st);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (kb + 1 < a.kb) issue(kb + 1, st ^ 1u);
-            const uint8_t *xs = lds + st * kStage, *wl = xs + kX;
-            const float *sl = reinterpret_cast<const float *>(wl + kW);
+            const uint8_t *here = lds + (kb & 1u) * kStage, *there = lds + ((kb & 1u) ^ 1u) * kStage;
             const float sg = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swg), (int)(kb & 63u)));
             const float su = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swu), (int)(kb & 63u)));
-            step<ALL>(xs, wl, sl, sg, su, frag, wm, wn, act, lane);
-        }
-    }
-
-    static __device__ __forceinline__ i32x8 read_frag(const uint8_t *p, uint32_t frag) {
-        return fp8_frag(*reinterpret_cast<const r9vx_u32x4 *>(p + frag), *reinterpret_cast<const r9vx_u32x4 *>(p + (frag ^ 64u)));
-    }
-    __device__ __forceinline__ void fold(r9vx_f32x4 (&o)[TN], const r9vx_f32x4 (&d)[TN], float s0, float s1, int j) {
-        const float s = GATED && j >= NC ? s1 : s0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = fmaf(d[j][e], s, o[j][e]);
-    }
-
-    /* One K step: a row tile's products leave the matrix unit while the row
-     * tile before it is scaled and added, so neither waits for the other. */
-    template <bool ALL>
-    __device__ __forceinline__ void step(const uint8_t *xs, const uint8_t *wl, const float *sl, float sg, float su, uint32_t frag,
-                                         uint32_t wm, uint32_t wn, uint32_t act, uint32_t lane) {
-        i32x8 w[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const uint32_t row = GATED ? (j >= NC ? BN / 2 : 0u) + (wn * NC + j % NC) * 16 : (wn * TN + j) * 16;
-            w[j] = read_frag(wl + row * 128, frag);
-        }
-        xs += wm * 2048;
-        sl += wm * 16 + (lane & 15u);
-        if constexpr (ALL) {
-            i32x8 x = read_frag(xs, frag);
-            float sx = *sl;
-            r9vx_f32x4 d[2][TN];
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                i32x8 xn = x;
-                float sn = sx;
-                if (i + 1 < TM) {
-                    xn = read_frag(xs + (i + 1) * WM * 2048, frag);
-                    sn = sl[(i + 1) * WM * 16];
+            fp8_for<NI>([&](auto Tile) {
+                constexpr int i = Tile.v;
+                i32x8 xn;
+                float sn;
+                if constexpr (i + 1 < NI) {
+                    xn = fp8_read_frag(here + xat + (i + 1) * WM * 2048, frag);
+                    sn = *reinterpret_cast<const float *>(here + sat + (i + 1) * WM * 64);
+                    slot(kb + 1, Fp8Int<i + 1>{});
+                } else {
+                    /* the other stage has its data, and nobody reads this one any more */
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    xn = fp8_read_frag(there + xat, frag); /* after the last step: stale LDS, unused */
+                    sn = *reinterpret_cast<const float *>(there + sat);
+                    slot(kb + 2, Fp8Int<0>{});
                 }
                 const float t0 = sx * sg, t1 = GATED ? sx * su : 0.f;
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
                     d[i & 1][j] = fp8_mma<EXACT>(w[j], x);
-                    if (i > 0) fold(acc[i > 0 ? i - 1 : 0], d[(i & 1) ^ 1], s0, s1, j);
+                    if constexpr (kCarry || i > 0) fold(acc[i > 0 ? i - 1 : NI - 1], d[(i & 1) ^ 1], s0, s1, j);
+                }
+#pragma unroll
+                for (int j = 0; j < TN; ++j) { /* one product, four additions */
+                    __builtin_amdgcn_sched_group_barrier(0x8, EXACT ? 4 : 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
                 }
                 s0 = t0;
                 s1 = t1;
                 x = xn;
                 sx = sn;
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int j = 0; j < TN; ++j) fold(acc[TM - 1], d[(TM - 1) & 1], s0, s1, j);
-        } else {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                if (i * WM + wm < act) {
-                    const i32x8 x = read_frag(xs + i * WM * 2048, frag);
-                    const float sx = sl[i * WM * 16], t0 = sx * sg, t1 = GATED ? sx * su : 0.f;
-                    r9vx_f32x4 d[TN];
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) d[j] = fp8_mma<EXACT>(w[j], x);
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) fold(acc[i], d, t0, t1, j);
+                if constexpr (i + 1 == NI) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    read_w(there);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            if constexpr (!kCarry) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fold(acc[NI - 1], d[(NI - 1) & 1], s0, s1, j);
             }
         }
+        if constexpr (kCarry) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fold(acc[NI - 1], d[1], s0, s1, j);
+        }
+    }
+
+    __device__ __forceinline__ void fold(r9vx_f32x4 (&o)[TN], const r9vx_f32x4 (&d)[TN], float s0, float s1, int j) {
+        o[j] = fp8_add_scaled(o[j], d[j], GATED && j >= NC ? s1 : s0);
     }
 
     /* Output columns of a tile, rows that go through LDS at once. */
@@ -395,6 +444,150 @@ struct Fp8Tile {
                 }
             __syncthreads();
             emit(p * kPass);
+        }
+    }
+};
+
+/* ------------------------------------------------------------------ small tiles */
+
+/* The same product for grids that do not fill the chip with large tiles: there
+ * a step lasts as long as its barrier, LDS reads and copies take, whatever it
+ * computes, so the steps are made fewer.  KS groups of WM x WN waves take one
+ * K block each per step; their sums are joined in group order in LDS. */
+template <int BM, int BN, int WM, int WN, int KS, bool GATED, bool EXACT>
+struct Fp8Thin {
+    static constexpr int TM = BM / 16 / WM, TN = BN / 16 / WN, NC = GATED ? TN / 2 : TN;
+    static constexpr uint32_t kX = BM * 128, kW = BN * 128, kSub = kX + kW + BM * 4, kStage = KS * kSub, kLds = 2 * kStage;
+    static constexpr int RX = BM / 64, RW = BN / 64, RS = KS * BM / 64; /* copies of a wave per block; scale copies of a step */
+    static constexpr uint32_t kCols = GATED ? BN / 2 : BN;
+    static_assert(WM * WN * KS == 8 && BM % 64 == 0 && BN % 64 == 0 && TM * 16 * WM == BM && TN * 16 * WN == BN, "");
+    static_assert(128 % (GATED ? BN / 2 : BN) == 0 && kLds <= 160 * 1024 && KS * BM * BN * 4 <= (int)kLds && RS <= 8, "");
+
+    r9vx_f32x4 acc[TM][TN];
+
+    __device__ __forceinline__ void run(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds) {
+        const uint32_t lane = threadIdx.x & 63u;
+        const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+        const uint32_t kg = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+        const uint32_t n0 = nt * kCols;
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+        const uint32_t tail = a.k % kFp8Block, xk = a.kb * kFp8Block;
+        uint32_t xo[RX], wo[RW];
+        const uint8_t *xbase = r.list ? a.xq : a.xq + (uint64_t)r.m0 * xk;
+        const uint8_t *wg = r.w + (uint64_t)n0 * a.k, *wu = wg + (uint64_t)a.n * a.k;
+        const uint32_t at8 = wave * 8 + (lane >> 3);       /* this lane's row of a copy round of 64 rows */
+        const uint32_t c = (lane & 7u) ^ ((at8 >> 1) & 7u); /* and its chunk */
+#pragma unroll
+        for (int i = 0; i < RX; ++i) {
+            const uint32_t row = i * 64 + at8, in = row < r.rows ? row : r.rows - 1;
+            xo[i] = (r.list ? r.list[r.m0 + in] : in) * xk + c * 16;
+        }
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            const uint32_t row = i * 64 + at8;
+            uint32_t j = GATED && row >= BN / 2 ? row - BN / 2 : row;
+            j = n0 + j < a.n ? j : a.n - 1 - n0;
+            wo[i] = j * a.k + c * 16;
+        }
+        const float *sbase = r.list ? a.xs : a.xs + (uint64_t)r.m0 * a.kb;
+        const uint32_t sq = wave % RS / RX, s64 = wave % RX * 64, srow = s64 + lane, sin = srow < r.rows ? srow : r.rows - 1;
+        const uint32_t so = (r.list ? r.list[r.m0 + sin] : sin) * a.kb * 4;
+        const uint32_t steps = (a.kb + KS - 1) / KS;
+        auto issue = [&](uint32_t step, uint32_t st) {
+            const uint32_t mask = fp8_copy_mask(step, steps);
+            fp8_for<KS>([&](auto Q) {
+                uint32_t kb = step * KS + Q.v;
+                kb = kb < a.kb ? kb : a.kb - 1; /* blocks past the last: the last one, not added */
+                const uint32_t k0 = kb * kFp8Block, at = lds0 + st * kStage + Q.v * kSub + wave * 1024;
+                /* weight chunks past the last column: the block's first one of the row (it meets zeros) */
+                const uint32_t back = tail && kb + 1 == a.kb && c * 16 >= tail ? c * 16 : 0u;
+#pragma unroll
+                for (int i = 0; i < RW; ++i) {
+                    const bool up = GATED && (i * 64 + wave * 8) >= BN / 2;
+                    fp8_copy16(at + kX + i * 8192, (up ? wu : wg) + k0, wo[i] - back, mask);
+                }
+#pragma unroll
+                for (int i = 0; i < RX; ++i) fp8_copy16(at + i * 8192, xbase + k0, xo[i], mask);
+            });
+            uint32_t kb = step * KS + sq;
+            kb = kb < a.kb ? kb : a.kb - 1;
+            fp8_copy4(lds0 + st * kStage + sq * kSub + kX + kW + s64 * 4, sbase, so + kb * 4, mask);
+        };
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
+        const uint32_t frag = (lane & 15u) * 128 + (((lane >> 4) ^ ((lane >> 1) & 7u)) << 4);
+        const float *wsg = r.ws + (uint64_t)(n0 / kFp8Block) * a.kb, *wsu = wsg + (uint64_t)a.nb * a.kb;
+        float swg = 0.f, swu = 0.f; /* lane i: the scales of this group's block in step 64 (step / 64) + i */
+        issue(0, 0);
+        for (uint32_t step = 0; step < steps; ++step) {
+            if ((step & 63u) == 0) {
+                const uint32_t kb = (step + lane) * KS + kg;
+                swg = wsg[kb < a.kb ? kb : a.kb - 1];
+                if constexpr (GATED) swu = wsu[kb < a.kb ? kb : a.kb - 1];
+                asm volatile("" : "+v"(swg), "+v"(swu));
+            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            const uint8_t *sub = lds + (step & 1u) * kStage + kg * kSub;
+            const float sg = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swg), (int)(step & 63u)));
+            const float su = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, swu), (int)(step & 63u)));
+            const bool mine = step * KS + kg < a.kb;
+            i32x8 w[TN], x[TM];
+            float sx[TM];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const uint32_t row = GATED ? (j >= NC ? BN / 2 : 0u) + (wn * NC + j % NC) * 16 : (wn * TN + j) * 16;
+                w[j] = fp8_read_frag(sub + kX + row * 128, frag);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                x[i] = fp8_read_frag(sub + (wm * TM + i) * 2048, frag);
+                sx[i] = *reinterpret_cast<const float *>(sub + kX + kW + ((wm * TM + i) * 16 + (lane & 15u)) * 4);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            issue(step + 1, (step & 1u) ^ 1u);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                r9vx_f32x4 d[TN];
+                const float t0 = mine ? sx[i] * sg : 0.f, t1 = mine ? sx[i] * su : 0.f;
+#pragma unroll
+                for (int j = 0; j < TN; ++j) d[j] = fp8_mma<EXACT>(w[j], x[i]);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = fp8_add_scaled(acc[i][j], d[j], GATED && j >= NC ? t1 : t0);
+            }
+        }
+    }
+
+    /* The groups' sums through LDS: store(tile row, n, four outputs) for every
+     * quad inside the problem. */
+    template <typename Store>
+    __device__ __forceinline__ void drain(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds, Store store) {
+        const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, kg = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN;
+        constexpr uint32_t kQuads = BN / 4, kTile = BM * BN * 4;
+        auto at = [](uint32_t t, uint32_t quad) { return (t * kQuads + (quad ^ (t & 15u))) * 16; };
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const uint32_t col = GATED ? (j >= NC ? BN / 2 : 0u) + (wn * NC + j % NC) * 16 : (wn * TN + j) * 16;
+                *reinterpret_cast<r9vx_f32x4 *>(lds + kg * kTile + at((wm * TM + i) * 16 + (lane & 15u), col / 4 + (lane >> 4))) = acc[i][j];
+            }
+        __syncthreads();
+        auto sum = [&](uint32_t t, uint32_t quad) {
+            r9vx_f32x4 v = *reinterpret_cast<const r9vx_f32x4 *>(lds + at(t, quad));
+#pragma unroll
+            for (int q = 1; q < KS; ++q) v = v + *reinterpret_cast<const r9vx_f32x4 *>(lds + q * kTile + at(t, quad));
+            return v;
+        };
+        for (uint32_t o = threadIdx.x; o < BM * (kCols / 4); o += 512) {
+            const uint32_t t = o / (kCols / 4), quad = o % (kCols / 4), n = nt * kCols + quad * 4;
+            if (t >= r.rows || n >= a.n) continue;
+            r9vx_f32x4 v = sum(t, quad);
+            if constexpr (GATED) v = fp8_swiglu(v, sum(t, quad + BN / 8));
+            store(t, n, v);
         }
     }
 };

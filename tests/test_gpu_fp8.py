@@ -177,9 +177,13 @@ def test_small_whole_numbers_are_exact(m, n, k, out):
     assert np.array_equal(y.float().cpu().numpy(), want)
 
 
-@pytest.mark.parametrize("m,n,k", [(256, 256, 128), (300, 520, 272), (600, 700, 368)])
-def test_matmul_bf16_outputs_of_the_tiles(m, n, k):
-    run(m, n, k, out="bf16")
+@pytest.mark.parametrize("epilogue", ["none", "swiglu"])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(256, 256, 128), (300, 520, 272), (600, 700, 368), (70, 4100, 1040), (130, 2050, 656),
+                                   (520, 2112, 1168), (1100, 2000, 400), (4096, 1030, 272)])
+def test_matmul_tiles(m, n, k, out, epilogue):
+    """Rows and columns that end inside tiles of every kind, K inside a step."""
+    run(m, n, k, out=out, epilogue=epilogue)
 
 
 @pytest.mark.parametrize("bucket", [64, 300])
@@ -198,6 +202,20 @@ def test_nan_codes_past_a_ragged_row_do_not_leak():
         w[1::2, :112] = 0x7F
         y = ffi.matmul_fp8(codes(w), dev(ws), on_gpu(x)).cpu().numpy()
         assert np.isnan(y[:, 1::2]).all() and np.isfinite(y[:, ::2]).all()
+
+
+@pytest.mark.parametrize("m", [4, 40, 200])
+def test_a_rows_bits_do_not_depend_on_its_batch(m):
+    k, n = 528, 300
+    x = acts(13, m, k)
+    w, ws = weights(14, n, k)
+    wg, sg = codes(w), dev(ws)
+    for out in (ffi.F32, ffi.BF16):
+        full = ffi.matmul_fp8(wg, sg, on_gpu(x), out_dtype=out)
+        assert torch.equal(ffi.matmul_fp8(wg, sg, on_gpu(x), out_dtype=out), full)
+        for i in (0, m // 2, m - 1):
+            assert torch.equal(ffi.matmul_fp8(wg, sg, on_gpu(x[i:i + 1]), out_dtype=out, m_bucket=m)[0], full[i])
+        assert torch.equal(ffi.matmul_fp8(wg, sg, on_gpu(x[::-1].copy()), out_dtype=out).flip(0), full)
 
 
 @pytest.mark.parametrize("m", [4, 40, 200])
