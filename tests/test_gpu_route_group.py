@@ -141,3 +141,37 @@ def test_rows_behind_the_last_are_left():
     w = torch.full((6, 4), 7.0, device="cuda")
     ffi.moe_route_group(dev(np.random.default_rng(1).standard_normal((4, 32)).astype(np.float32)), 4, 4, 2, ids=ids[:4], weights=w[:4])
     assert (ids[4:] == 77).all() and (w[4:] == 7.0).all() and (ids[:4] < 32).all()
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("biased", [False, True])
+def test_many_rows(sigmoid, biased):
+    r = np.random.default_rng(12)
+    logits = (3 * r.standard_normal((1531, 192))).astype(np.float32)
+    bias = (0.3 * r.standard_normal(192)).astype(np.float32) if biased else None
+    check(logits, 6, 12, 5, bias, sigmoid)
+    check(logits, 6, 12, 5, bias, sigmoid, top2=False, renormalize=False)
+
+
+def neighbours(start, n, step=1):
+    """n f32 values, `step` representable steps apart."""
+    return (np.float32(start).view(np.int32) + step * np.arange(n, dtype=np.int32)).view(np.float32)
+
+
+@pytest.mark.parametrize("start", [1e-30, 0.1, 3.0, 15.9, 20.0, 25.0, 31.0, 36.0, 40.0, 80.0, -3.0, -15.9, -80.0, -590.0, -700.0])
+def test_neighbouring_logits(start):
+    """Logits that f64 scores tell apart, or round to one value (sigmoid near 1)."""
+    r = np.random.default_rng(13)
+    logits = np.stack([r.permutation(neighbours(start, 64, step)) for step in (1, 1, 2, 5, 40, 300)])
+    for groups, topk_group in ((1, 1), (8, 3)):
+        check(logits, 8, groups, topk_group, None, sigmoid=True, top2=False)
+    check(logits, 8, 1, 1, None, sigmoid=False, top2=False)
+
+
+def test_group_sums_that_cancel():
+    """A group's two keys of a thousand and of opposite signs: their sum is small, its error is not."""
+    r = np.random.default_rng(14)
+    logits = r.standard_normal((200, 16)).astype(np.float32)
+    bias = np.tile(np.array([1000.0, -1000.0], np.float32), 8) + r.standard_normal(16).astype(np.float32) * np.float32(2e-4)
+    check(logits, 4, 8, 3, bias, sigmoid=True)
+    check(logits, 4, 8, 3, bias, sigmoid=False)
