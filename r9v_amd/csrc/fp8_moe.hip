@@ -20,9 +20,12 @@ namespace {
 
 struct Fp8MoeLayout {
     MoeLayout sort; /* the sort's regions */
-    uint64_t xq, xs, h, hq, hs, o, total;
+    uint64_t xq, xs, h, hq, hs, o, os, total;
     bool stream; /* few rows per expert */
+    bool half;   /* o in f16, a power of two per kOutBlock columns beside it */
 };
+
+constexpr uint32_t kOutBlock = 128; /* columns that share a weight scale */
 
 /* Few rows: the streaming form. */
 bool moe_streams(const r9vx_moe_fp8_problem &p) { return p.t_bucket <= 64; }
@@ -55,7 +58,14 @@ Fp8MoeLayout moe_layout(const r9vx_moe_fp8_problem &p) {
     L.h = take(L.stream ? 4 * rows * p.dff : 0);
     L.hq = take(rows * p.dff);
     L.hs = take(4 * rows * (p.dff / kFp8Block));
-    L.o = take(4 * rows * p.dm);
+    /* o is written and read once each, in prompts by far the most bytes of all.
+     * For bf16 outputs the tiles keep it in f16: a row's 128 columns of one
+     * weight scale times the power of two that brings the largest under 4, so
+     * that nothing overflows and an addend is off by half a step, 2^-11 of itself (or 2^-25
+     * of the block's largest): an eighth of the output's own rounding. */
+    L.half = !L.stream && p.y_dtype == R9VX_DTYPE_BF16;
+    L.o = take((L.half ? 2 : 4) * rows * p.dm);
+    L.os = take(L.half ? 4 * rows * (p.dm / kOutBlock) : 0);
     L.total = off;
     return L;
 }
@@ -65,7 +75,8 @@ struct Fp8MoeArgs {
     uint8_t *ws;
     Fp8MoeLayout L;
     uint32_t p, t, topk;
-    float *out;     /* f32 rows of h (streaming gate / up) or o */
+    float *out;     /* f32 rows of h (streaming gate / up) or o (f16: Fp8MoeLayout::half) */
+    float *os;
     uint8_t *hq;
     float *hs;
 };
@@ -146,20 +157,34 @@ __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
                 }
                 const Fp8Scale s = fp8_scale(fp8_max8(amax));
                 r9vx_u32x4 c;
-                c.x = fp8_code4(v[0].x, v[0].y, v[0].z, v[0].w, s);
-                c.y = fp8_code4(v[1].x, v[1].y, v[1].z, v[1].w, s);
-                c.z = fp8_code4(v[2].x, v[2].y, v[2].z, v[2].w, s);
-                c.w = fp8_code4(v[3].x, v[3].y, v[3].z, v[3].w, s);
+                const float inv = 1.0f / s.s;
+                c.x = fp8_near4(v[0].x, v[0].y, v[0].z, v[0].w, s, inv);
+                c.y = fp8_near4(v[1].x, v[1].y, v[1].z, v[1].w, s, inv);
+                c.z = fp8_near4(v[2].x, v[2].y, v[2].z, v[2].w, s, inv);
+                c.w = fp8_near4(v[3].x, v[3].y, v[3].z, v[3].w, s, inv);
                 const uint64_t pos = tile.y + t0 + row;
                 *reinterpret_cast<r9vx_u32x4 *>(a.hq + pos * a.g.n + nt * 128 + part * 16) = c;
                 if (part == 0) a.hs[pos * a.g.nb + nt] = s.s;
             }
         } else {
-            for (uint32_t o = threadIdx.x; o < T::kPass * (T::kCols / 4); o += 512) {
-                const uint32_t row = o / (T::kCols / 4), quad = o % (T::kCols / 4), n = nt * T::kCols + quad * 4;
-                if (t0 + row < r.rows && n < a.g.n)
-                    *reinterpret_cast<r9vx_f32x4 *>(a.out + (uint64_t)(tile.y + t0 + row) * a.g.n + n) =
-                        *reinterpret_cast<const r9vx_f32x4 *>(lds + T::at(row, quad));
+            static_assert(T::kCols == 256 && kOutBlock == 128, "a wave's 64 quads are two blocks of a row");
+            const uint32_t quad = threadIdx.x & 63u, n = nt * T::kCols + quad * 4;
+            for (uint32_t row = threadIdx.x >> 6; row < T::kPass && t0 + row < r.rows; row += 8) {
+                const r9vx_f32x4 v = *reinterpret_cast<const r9vx_f32x4 *>(lds + T::at(row, quad));
+                const uint64_t pos = tile.y + t0 + row;
+                if (a.L.half) {
+                    auto finite = [](float f) { return fp8_absbits(f) < 0x7F800000u ? fp8_absbits(f) : 0u; };
+                    uint32_t top = n < a.g.n ? max(max(finite(v.x), finite(v.y)), max(finite(v.z), finite(v.w))) : 0u;
+                    top = fp8_max32(top) >> 23;
+                    top = top < 27u ? 27u : top > 253u ? 253u : top; /* both powers stay normal numbers */
+                    const float f = __builtin_bit_cast(float, (254u - top) << 23);
+                    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+                    const half4 h = {(_Float16)(v.x * f), (_Float16)(v.y * f), (_Float16)(v.z * f), (_Float16)(v.w * f)};
+                    if (n < a.g.n) *reinterpret_cast<half4 *>(reinterpret_cast<_Float16 *>(a.out) + pos * a.g.n + n) = h;
+                    if (quad % 32 == 0 && n < a.g.n) a.os[pos * (a.g.n / kOutBlock) + n / kOutBlock] = __builtin_bit_cast(float, top << 23);
+                } else if (n < a.g.n) {
+                    *reinterpret_cast<r9vx_f32x4 *>(a.out + pos * a.g.n + n) = v;
+                }
             }
         }
     });
@@ -167,7 +192,7 @@ __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
 
 struct Fp8CombineArgs {
     const float *weights;
-    const float *o;
+    const float *o, *os;
     void *y;
     const uint8_t *ws;
     Fp8MoeLayout L;
@@ -176,7 +201,8 @@ struct Fp8CombineArgs {
 
 /* y[t] = sum over the token's rows in ascending sorted position (= ascending
  * (expert, slot)) of w * o, then the shared experts' rows.  A workgroup takes
- * 1024 columns of one token. */
+ * 256 pieces of one token: 4 columns each, or 8 of an f16 o. */
+template <bool HALF>
 __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) {
     __shared__ uint32_t spos[kMoeMaxK], opos[kMoeMaxK];
     __shared__ float sw[kMoeMaxK], ow[kMoeMaxK];
@@ -195,22 +221,37 @@ __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) 
         ow[rank] = sw[threadIdx.x];
     }
     __syncthreads();
-    const uint32_t d = (blockIdx.y * 256 + threadIdx.x) * 4;
+    constexpr uint32_t kQuads = HALF ? 2 : 1;
+    const uint32_t d = (blockIdx.y * 256 + threadIdx.x) * 4 * kQuads;
     if (d >= a.dm) return;
-    r9vx_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t j = 0; j < kk; ++j) {
-        const r9vx_f32x4 v = *reinterpret_cast<const r9vx_f32x4 *>(a.o + (uint64_t)opos[j] * a.dm + d);
-        acc = acc + ow[j] * v;
+    r9vx_f32x4 acc[kQuads];
+#pragma unroll
+    for (uint32_t i = 0; i < kQuads; ++i) acc[i] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
+    auto add = [&](float w, uint64_t row) {
+        if constexpr (HALF) {
+            typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+            const half8 h = __builtin_bit_cast(half8, __builtin_nontemporal_load(
+                reinterpret_cast<const r9vx_u32x4 *>(reinterpret_cast<const _Float16 *>(a.o) + row * a.dm + d)));
+            const float f = a.os[row * (a.dm / kOutBlock) + d / kOutBlock];
+            acc[0] = acc[0] + w * (f * r9vx_f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]});
+            acc[1] = acc[1] + w * (f * r9vx_f32x4{(float)h[4], (float)h[5], (float)h[6], (float)h[7]});
+        } else {
+            acc[0] = acc[0] + w * __builtin_nontemporal_load(reinterpret_cast<const r9vx_f32x4 *>(a.o + row * a.dm + d));
+        }
+    };
+#pragma unroll 4
+    for (uint32_t j = 0; j < kk; ++j) add(ow[j], opos[j]);
+    for (uint32_t s = 0; s < a.shared; ++s) add(1.0f, (uint64_t)a.p + (uint64_t)s * a.t + t);
+#pragma unroll
+    for (uint32_t i = 0; i < kQuads; ++i) {
+        const uint64_t at = (uint64_t)t * a.dm + d + i * 4;
+        if (a.y_bf16)
+            *reinterpret_cast<r9vx_u32x2 *>(static_cast<uint16_t *>(a.y) + at) =
+                r9vx_u32x2{(uint32_t)r9vx_f32_to_bf16(acc[i].x) | ((uint32_t)r9vx_f32_to_bf16(acc[i].y) << 16),
+                           (uint32_t)r9vx_f32_to_bf16(acc[i].z) | ((uint32_t)r9vx_f32_to_bf16(acc[i].w) << 16)};
+        else
+            *reinterpret_cast<r9vx_f32x4 *>(static_cast<float *>(a.y) + at) = acc[i];
     }
-    for (uint32_t s = 0; s < a.shared; ++s)
-        acc = acc + *reinterpret_cast<const r9vx_f32x4 *>(a.o + ((uint64_t)a.p + (uint64_t)s * a.t + t) * a.dm + d);
-    const uint64_t at = (uint64_t)t * a.dm + d;
-    if (a.y_bf16)
-        *reinterpret_cast<r9vx_u32x2 *>(static_cast<uint16_t *>(a.y) + at) =
-            r9vx_u32x2{(uint32_t)r9vx_f32_to_bf16(acc.x) | ((uint32_t)r9vx_f32_to_bf16(acc.y) << 16),
-                       (uint32_t)r9vx_f32_to_bf16(acc.z) | ((uint32_t)r9vx_f32_to_bf16(acc.w) << 16)};
-    else
-        *reinterpret_cast<r9vx_f32x4 *>(static_cast<float *>(a.y) + at) = acc;
 }
 
 }  // namespace
@@ -264,6 +305,7 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
     dn.g.nb = p.dm / kFp8Block;
     dn.g.kb = p.dff / kFp8Block;
     dn.out = o;
+    dn.os = reinterpret_cast<float *>(p.ws + L.os);
     /* the launch's tiles are at most this many (the list's own count is on the device) */
     const uint32_t tiles = rows / kMoeTileM3 + (pairs < p.e ? pairs : p.e) + p.shared;
     if (L.stream) {
@@ -280,7 +322,10 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
     }
     rc = (int)hipGetLastError();
     if (rc) return rc;
-    const Fp8CombineArgs c{p.weights, o, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16};
-    hipLaunchKernelGGL(fp8_moe_combine_kernel, dim3(p.t, (p.dm / 4 + 255) / 256), dim3(256), 0, stream, c);
+    const Fp8CombineArgs c{p.weights, o, dn.os, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16};
+    if (L.half)
+        hipLaunchKernelGGL(fp8_moe_combine_kernel<true>, dim3(p.t, (p.dm / 8 + 255) / 256), dim3(256), 0, stream, c);
+    else
+        hipLaunchKernelGGL(fp8_moe_combine_kernel<false>, dim3(p.t, (p.dm / 4 + 255) / 256), dim3(256), 0, stream, c);
     return (int)hipGetLastError();
 }

@@ -29,7 +29,7 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t fp8_dpp(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
 }
-/* Largest of 2, 4 and 8 neighbouring lanes. */
+/* Largest of 8, 16 and 32 neighbouring lanes. */
 __device__ __forceinline__ uint32_t fp8_max8(uint32_t x) {
     x = max(x, fp8_dpp<0xB1>(x));  /* quad_perm 1 0 3 2 */
     x = max(x, fp8_dpp<0x4E>(x));  /* quad_perm 2 3 0 1 */
@@ -38,6 +38,12 @@ __device__ __forceinline__ uint32_t fp8_max8(uint32_t x) {
 __device__ __forceinline__ uint32_t fp8_max16(uint32_t x) {
     x = fp8_max8(x);
     return max(x, fp8_dpp<0x140>(x)); /* row_mirror */
+}
+
+__device__ __forceinline__ uint32_t fp8_max32(uint32_t x) {
+    x = fp8_max16(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
 }
 
 /* The scale of a block whose largest |x| has the bit pattern `amax`:
@@ -83,6 +89,14 @@ __device__ __forceinline__ float fp8_quotient(float x, const Fp8Scale &q) {
 __device__ __forceinline__ uint32_t fp8_code4(float a, float b, float c, float d, const Fp8Scale &q) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_quotient(a, q), fp8_quotient(b, q), 0, false);
     w = __builtin_amdgcn_cvt_pk_fp8_f32(fp8_quotient(c, q), fp8_quotient(d, q), w, true);
+    return q.bad ? 0x7F7F7F7Fu : (uint32_t)w;
+}
+
+/* The same for values that carry f32 roundings themselves (h of the experts):
+ * x times 1 / s, within 2^-23 of the quotient. */
+__device__ __forceinline__ uint32_t fp8_near4(float a, float b, float c, float d, const Fp8Scale &q, float inv) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
     return q.bad ? 0x7F7F7F7Fu : (uint32_t)w;
 }
 

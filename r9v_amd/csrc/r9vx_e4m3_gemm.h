@@ -83,7 +83,17 @@ __device__ __forceinline__ void fp8_store_dense(const Fp8Args &a, uint32_t m, ui
     }
 }
 
-__device__ __forceinline__ float fp8_silu(float g) { return g / (1.0f + expf(-g)); }
+/* g / (1 + exp(-g)) by the hardware's exponential and reciprocal, a step each:
+ * with the other roundings under 2^-20 of the value (of a tile's epilogue
+ * the library's exponential and divide took a third of the time of its
+ * products).  The exponential's argument keeps the low half of g log2 e; from
+ * |g| = 128 on silu is g or 0 anyway. */
+__device__ __forceinline__ float fp8_silu(float g) {
+    const float c = __builtin_amdgcn_fmed3f(g, -128.0f, 128.0f);
+    const float t = c * -0x1.715476p+0f;
+    const float low = fmaf(c, -0x1.715476p+0f, -t) + c * -0x1.4ae0cp-26f;
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t) * fmaf(low, 0x1.62e43p-1f, 1.0f));
+}
 
 __device__ __forceinline__ r9vx_f32x4 fp8_swiglu(r9vx_f32x4 g, r9vx_f32x4 u) {
     return r9vx_f32x4{fp8_silu(g.x) * u.x, fp8_silu(g.y) * u.y, fp8_silu(g.z) * u.z, fp8_silu(g.w) * u.w};
@@ -239,11 +249,13 @@ struct Fp8Tile {
 
     r9vx_f32x4 acc[TM][TN];
 
-    /* The products of the tile's rows: of all its row tiles, of half or of a
-     * quarter of them, whatever holds the rows (small tiles: of all). */
+    /* The products of the tile's rows: of all its row tiles, of three, two or
+     * one quarter of them, whatever holds the rows (small tiles: of all). */
     __device__ __forceinline__ void run(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds) {
-        if (TM % 4 != 0 || r.rows > BM / 2)
+        if (TM % 4 != 0 || r.rows > BM / 4 * 3)
             run_rows<TM>(a, r, nt, lds);
+        else if (BM % 256 == 0 && r.rows > BM / 2)
+            run_rows<BM % 256 ? TM : TM / 4 * 3>(a, r, nt, lds);
         else if (r.rows > BM / 4)
             run_rows<TM % 4 ? TM : TM / 2>(a, r, nt, lds);
         else

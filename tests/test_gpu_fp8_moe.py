@@ -48,7 +48,7 @@ def reference(x, ids, wts, gu, gus, dn, dns, shared, exact):
     t, dm = x.shape
     e = gu.shape[0] - shared
     xq, xs = R.quantize(x)
-    y, tol, total = np.zeros((t, dm)), np.zeros((t, dm)), np.zeros((t, dm))
+    y, tol, total, half = np.zeros((t, dm)), np.zeros((t, dm)), np.zeros((t, dm)), np.zeros((t, dm))
     for i in range(e + shared):
         tok, slot = np.nonzero(ids == i) if i < e else (np.arange(t), None)
         if tok.size == 0:
@@ -57,9 +57,21 @@ def reference(x, ids, wts, gu, gus, dn, dns, shared, exact):
         w = wts[tok, slot].astype(np.float64)[:, None] if slot is not None else 1.0
         np.add.at(y, tok, w * o)
         np.add.at(tol, tok, np.abs(w) * d)
-        np.add.at(total, tok, np.abs(w) * (np.abs(o) + d))
-    # o is kept as f32 (or f16 with a scale of its 64 columns: half a step of their largest), weighted and added in f32
-    return y, tol + total * (ids.shape[1] + shared + 3) * 2.0 ** -23
+        size = np.abs(o) + d
+        np.add.at(total, tok, np.abs(w) * size)
+        # bf16 outputs of many tokens keep o in f16, scaled by a power of two that brings the largest
+        # of 128 columns into [1, 2): half a step is 2^-11 of a normal number, 2^-25 below 2^-14
+        top = np.maximum.reduceat(size, np.arange(0, dm, 128), axis=1)
+        top = np.repeat(top, 128, axis=1)
+        np.add.at(half, tok, np.abs(w) * (size * 2.0 ** -11 + top * 2.0 ** -25))
+    # o is weighted and added in f32
+    return y, tol + total * (ids.shape[1] + shared + 3) * 2.0 ** -23, half if t > 64 else 0.0 * half
+
+
+def check_both(x, ids, wts, ex, want, **kw):
+    y, tol, half = want
+    check(call(x, ids, wts, ex, **kw), y, tol, False)
+    check(call(x, ids, wts, ex, out_dtype=ffi.BF16, **kw), y, tol + half, True)
 
 
 def experts(seed, e, dm, dff, whole=False):
@@ -105,9 +117,7 @@ def test_moe_ffn_fp8(t, e, k, dm, dff, shared, whole):
     x = r.integers(-1, 2, (t, dm)).astype(np.float32) if whole else acts(t, t, dm)
     ids, wts = routing(t + 1, t, e, k, 0.7)
     ex = experts(t + 2, e + shared, dm, dff, whole)
-    want, tol = reference(x, ids, wts, *ex, shared, exact=whole or t <= 64)
-    check(call(x, ids, wts, ex, shared=shared), want, tol, False)
-    check(call(x, ids, wts, ex, shared=shared, out_dtype=ffi.BF16), want, tol, True)
+    check_both(x, ids, wts, ex, reference(x, ids, wts, *ex, shared, exact=whole or t <= 64), shared=shared)
 
 
 @pytest.mark.parametrize("t", [20, 300])
@@ -116,8 +126,7 @@ def test_all_tokens_to_one_expert_and_repeated_experts(t):
     ex = experts(4, 7, 256, 128)
     ids = np.full((t, 2), 5, np.int32)
     wts = np.random.default_rng(5).random((t, 2)).astype(np.float32)
-    want, tol = reference(x, ids, wts, *ex, 0, exact=t <= 64)
-    check(call(x, ids, wts, ex), want, tol, False)
+    check_both(x, ids, wts, ex, reference(x, ids, wts, *ex, 0, exact=t <= 64))
 
 
 @pytest.mark.parametrize("bucket", [8, 64, 400])
@@ -161,6 +170,24 @@ def test_bad_token_stays_alone():
         assert torch.isnan(y[2]).all() and torch.equal(y[rest], clean[rest])
 
 
+@pytest.mark.parametrize("t", [6, 150])
+def test_an_outputs_infinity_stays_alone(t):
+    """One weight row of NaN codes and one whose sums pass f32: only their columns lose their values."""
+    x, ids, wts = acts(23, t, 256), *routing(24, t, 3, 2)
+    gu, gus, dn, dns = experts(25, 3, 256, 128)
+    clean = call(x, ids, wts, (gu, gus, dn, dns), out_dtype=ffi.BF16).float()
+    dn, dns = dn.copy(), dns.copy()
+    dn[:, 7] = 0x7F
+    dns[:, 1] = 3e38
+    y = call(x, ids, wts, (gu, gus, dn, dns), out_dtype=ffi.BF16).float()
+    assert torch.isnan(y[:, 7]).all() and not torch.isfinite(y[:, 128:]).all()
+    keep = [i for i in range(128) if i != 7]
+    # the same but for f16's step below 2^-14 of a block's largest, which column 7 may have been:
+    # 2^-25 of it before and after, from two experts, and a bf16 step where that crosses a middle
+    off = 0.0 if t <= 64 else clean[:, keep].abs() * 2.0 ** -7 + clean[:, :128].abs().amax() * 2.0 ** -20
+    assert ((y[:, keep] - clean[:, keep]).abs() <= off).all()
+
+
 def test_rows_behind_the_last_are_left():
     x, ex = acts(15, 9, 128), experts(16, 4, 128, 128)
     ids, wts = routing(17, 9, 4, 2)
@@ -190,9 +217,9 @@ def test_route_experts_and_projection_together(t):
     got = layer(*args)
     # each step's operands from the GPU's own previous step, its arithmetic from the definition
     ids, wts = ffi.moe_route_group(args[1], 4, 4, 2, bias=args[2], scale=2.5)
-    want_y, tol_y = reference(x, ids.cpu().numpy(), wts.cpu().numpy(), *ex, 1, exact=t <= 64)
+    want_y, tol_y, half = reference(x, ids.cpu().numpy(), wts.cpu().numpy(), *ex, 1, exact=t <= 64)
     y = ffi.moe_ffn_fp8(args[0], ids, wts, *gpu_ex, shared=1, out_dtype=ffi.BF16)
-    check(y, want_y, tol_y, True)
+    check(y, want_y, tol_y + half, True)
     q, s = R.quantize(y.float().cpu().numpy())
     p, a = R.product(q, s, w, ws)
     p = p + x
