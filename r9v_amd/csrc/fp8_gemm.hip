@@ -53,7 +53,7 @@ __global__ __launch_bounds__(512) void fp8_tile_kernel(Fp8Args a) {
     r.rows = a.m - r.m0 < (uint32_t)BM ? a.m - r.m0 : (uint32_t)BM;
     T t;
     t.run(a, r, nt, lds);
-    t.drain(lds, [&](uint32_t t0) {
+    t.drain(r.rows, lds, [&](uint32_t t0) {
         for (uint32_t o = threadIdx.x; o < T::kPass * (T::kCols / 4); o += 512) {
             const uint32_t row = o / (T::kCols / 4), quad = o % (T::kCols / 4), n = nt * T::kCols + quad * 4;
             if (t0 + row < r.rows && n < a.n) fp8_store_dense(a, r.m0 + t0 + row, n, *reinterpret_cast<const r9vx_f32x4 *>(lds + T::at(row, quad)));

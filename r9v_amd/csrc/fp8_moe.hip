@@ -143,7 +143,7 @@ __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
     }
     T t;
     t.run(a.g, r, nt, lds);
-    t.drain(lds, [&](uint32_t t0) {
+    t.drain(r.rows, lds, [&](uint32_t t0) {
         if constexpr (UP) {
             /* a row's 128 columns are one block of h: eight lanes, sixteen values each */
             const uint32_t part = threadIdx.x & 7u;

@@ -250,11 +250,12 @@ struct Fp8Tile {
     r9vx_f32x4 acc[TM][TN];
 
     /* The products of the tile's rows: of all its row tiles, of three, two or
-     * one quarter of them, whatever holds the rows (small tiles: of all). */
+     * one quarter of them, whatever holds the rows (tiles of 128 rows have no
+     * three quarters, smaller ones only the whole). */
     __device__ __forceinline__ void run(const Fp8Args &a, const Fp8Rows &r, uint32_t nt, uint8_t *lds) {
         if (TM % 4 != 0 || r.rows > BM / 4 * 3)
             run_rows<TM>(a, r, nt, lds);
-        else if (BM % 256 == 0 && r.rows > BM / 2)
+        else if (r.rows > BM / 2)
             run_rows<BM % 256 ? TM : TM / 4 * 3>(a, r, nt, lds);
         else if (r.rows > BM / 4)
             run_rows<TM % 4 ? TM : TM / 2>(a, r, nt, lds);
@@ -440,11 +441,12 @@ struct Fp8Tile {
      * that a wave writes at a time lie in different banks. */
     static __device__ __forceinline__ uint32_t at(uint32_t t, uint32_t quad) { return (t * (kCols / 4) + (quad ^ (t & 15u))) * 16; }
     template <typename Emit>
-    __device__ __forceinline__ void drain(uint8_t *lds, Emit emit) {
+    __device__ __forceinline__ void drain(uint32_t rows, uint8_t *lds, Emit emit) {
         const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
         constexpr int TP = kPass / (WM * 16);
 #pragma unroll
         for (int p = 0; p < TM / TP; ++p) {
+            if (p * kPass >= rows) return;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < TP; ++i)

@@ -177,6 +177,12 @@ def test_small_whole_numbers_are_exact(m, n, k, out):
     assert np.array_equal(y.float().cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("m,out", [(1800, "f32"), (1878, "f32"), (1900, "f32"), (1800, "bf16"), (1878, "bf16"), (1942, "bf16"), (2020, "bf16")])
+def test_last_tile_of_every_height(m, out):
+    """The large tiles' last rows: up to a quarter, a half, three quarters and all of a tile."""
+    run(m, 4352, 2048, "e4m3", out, "none")
+
+
 @pytest.mark.parametrize("epilogue", ["none", "swiglu"])
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 @pytest.mark.parametrize("m,n,k", [(256, 256, 128), (300, 520, 272), (600, 700, 368), (70, 4100, 1040), (130, 2050, 656),
