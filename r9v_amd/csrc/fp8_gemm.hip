@@ -21,7 +21,7 @@ using namespace r9vx;
 
 namespace {
 
-template <int MT, int NT, int W, int XT, bool GATED>
+template <int MT, int NT, int W, bool GATED>
 __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a) {
     __shared__ __attribute__((aligned(16))) r9vx_f32x4 part[W * NT * MT * 64];
     const uint32_t strip = blockIdx.x, m0 = blockIdx.y * (MT * 16);
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a) {
     r.ws = a.ws;
     r.m0 = m0;
     r.rows = a.m - m0 < MT * 16u ? a.m - m0 : MT * 16u;
-    fp8_stream<MT, NT, W, XT, GATED>(a, r, strip, part, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
+    fp8_stream<MT, NT, W, GATED>(a, r, strip, part, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
         fp8_store_dense(a, m0 + row, n, v);
     });
 }
@@ -81,7 +81,6 @@ Fp8Args fp8_args(const r9vx_fp8_problem &p, const uint8_t *xq, const float *xs) 
     Fp8Args a{};
     a.w = p.w;
     a.ws = p.w_scales;
-    a.x = p.x;
     a.xq = xq;
     a.xs = xs;
     a.bias = p.bias;
@@ -102,9 +101,9 @@ int launch_stream(const Fp8Args &a, bool gated, hipStream_t s) {
     const uint32_t cols = gated ? NT * 8 : NT * 16;
     const dim3 grid((a.n + cols - 1) / cols, (a.m + MT * 16 - 1) / (MT * 16));
     if (gated)
-        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, 0, true>), grid, dim3(W * 64), 0, s, a);
+        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, true>), grid, dim3(W * 64), 0, s, a);
     else
-        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, 0, false>), grid, dim3(W * 64), 0, s, a);
+        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, false>), grid, dim3(W * 64), 0, s, a);
     return (int)hipGetLastError();
 }
 
@@ -134,7 +133,7 @@ int launch_thin(Fp8Args a, bool gated, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
-/* The kernels for more than 64 rows, each with its time in ns as measured
+/* The kernels for more than 32 rows, each with its time in ns as measured
  * (n = 2112 .. 14336, K = 2048 .. 8192): a workgroup's start and end, and per K
  * block; `slots` workgroups run beside each other before a round is full.
  * EXACT = false / true:
@@ -198,8 +197,12 @@ int r9vx_launch_matmul_fp8(const r9vx_fp8_problem &p, hipStream_t stream) {
     }
     const Fp8Args a = fp8_args(p, xq, xs);
     const bool gated = p.epilogue == R9VX_EPILOGUE_SWIGLU;
+    /* Four tiles of 16 rows in the streaming kernel against 64 x 64 tiles, 48 rows,
+     * weights from HBM: 2 x 1408 x 2048 9.8 / 8.0 us, 2112 x 4096 16.8 / 12.8,
+     * 14336 x 4096 34.2 / 20.5, 7168 x 7168 27.0 / 30.1; two tiles, 32 rows:
+     * 7.7 / 7.8, 11.9 / 11.9, 24.9 / 18.8, 20.6 / 27.3; 17 rows: 6.7 / 7.4,
+     * 9.7 / 11.0, 21.0 / 18.8, 16.7 / 25.3. */
     if (p.m_bucket <= 16) return launch_stream<1, 2, 8>(a, gated, stream);
     if (p.m_bucket <= 32) return launch_stream<2, 2, 8>(a, gated, stream);
-    if (p.m_bucket <= 64) return launch_stream<4, 2, 8>(a, gated, stream);
     return p.y_dtype == R9VX_DTYPE_F32 ? launch_many<true>(a, p.m_bucket, gated, stream) : launch_many<false>(a, p.m_bucket, gated, stream);
 }

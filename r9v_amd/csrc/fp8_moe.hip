@@ -112,7 +112,7 @@ __global__ __launch_bounds__(W * 64) void fp8_moe_stream_kernel(Fp8MoeArgs a) {
     for (uint32_t m0 = 0; m0 < tile.z; m0 += MT * 16) {
         r.m0 = (UP ? 0u : tile.y) + m0;
         r.rows = tile.z - m0 < MT * 16u ? tile.z - m0 : MT * 16u;
-        fp8_stream<MT, NT, W, 0, UP>(a.g, r, blockIdx.x, part, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
+        fp8_stream<MT, NT, W, UP>(a.g, r, blockIdx.x, part, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
             *reinterpret_cast<r9vx_f32x4 *>(a.out + (uint64_t)(tile.y + m0 + row) * a.g.n + n) = v;
         });
         __syncthreads(); /* the partial sums have been read */

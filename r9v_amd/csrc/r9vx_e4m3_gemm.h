@@ -10,7 +10,6 @@
 struct Fp8Args {
     const uint8_t *w;      /* e4m3 [n or 2n, k] */
     const float *ws;       /* [nb or 2 nb, kb] */
-    const void *x;         /* activations as given (in-kernel quantization) */
     const uint8_t *xq;     /* e4m3 rows of kb whole blocks, zeros past column k */
     const float *xs;       /* [rows, kb] */
     const float *bias;
@@ -121,7 +120,7 @@ struct Fp8StreamRegs {
  * and the NT / 2 of up rows beside them) times MT tiles of 16 activation rows.
  * Wave v takes the K blocks v, v + W, ...; the W partial sums are joined in
  * wave order in LDS.  store(row, n, four sums) gets each quad once. */
-template <int MT, int NT, int W, int XT, bool GATED, typename Store>
+template <int MT, int NT, int W, bool GATED, typename Store>
 __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, uint32_t strip, r9vx_f32x4 *part, Store store) {
     constexpr int NC = GATED ? NT / 2 : NT; /* output tiles */
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15u;

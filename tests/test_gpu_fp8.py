@@ -125,7 +125,7 @@ def run(m, n, k, dtype="bf16", out="f32", epilogue="none", bucket=None, seed=1):
     res = r.standard_normal((m, n)).astype(np.float32) if epilogue == "residual" else None
     w, ws = weights(seed + 1, n, k)
     p, a = R.product(xq, xs, w, ws)
-    exact = out == "f32" or (bucket or m) <= 64
+    exact = out == "f32" or (bucket or m) <= 32
     tol = R.product_tol(k, a, exact)
     if epilogue == "swiglu":
         w2, ws2 = weights(seed + 3, n, k)
