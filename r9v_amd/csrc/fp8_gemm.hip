@@ -21,16 +21,17 @@ using namespace r9vx;
 
 namespace {
 
-template <int MT, int NT, int W, bool GATED>
+template <int MT, int NT, int W, int XT, bool GATED>
 __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a) {
     __shared__ __attribute__((aligned(16))) r9vx_f32x4 part[W * NT * MT * 64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t quantized[];
     const uint32_t strip = blockIdx.x, m0 = blockIdx.y * (MT * 16);
     Fp8Rows r{};
     r.w = a.w;
     r.ws = a.ws;
     r.m0 = m0;
     r.rows = a.m - m0 < MT * 16u ? a.m - m0 : MT * 16u;
-    fp8_stream<MT, NT, W, GATED>(a, r, strip, part, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
+    fp8_stream<MT, NT, W, XT, GATED>(a, r, strip, part, quantized, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
         fp8_store_dense(a, m0 + row, n, v);
     });
 }
@@ -81,6 +82,7 @@ Fp8Args fp8_args(const r9vx_fp8_problem &p, const uint8_t *xq, const float *xs) 
     Fp8Args a{};
     a.w = p.w;
     a.ws = p.w_scales;
+    a.x = p.x;
     a.xq = xq;
     a.xs = xs;
     a.bias = p.bias;
@@ -96,14 +98,15 @@ Fp8Args fp8_args(const r9vx_fp8_problem &p, const uint8_t *xq, const float *xs) 
     return a;
 }
 
-template <int MT, int NT, int W>
+template <int MT, int NT, int W, int XT>
 int launch_stream(const Fp8Args &a, bool gated, hipStream_t s) {
     const uint32_t cols = gated ? NT * 8 : NT * 16;
     const dim3 grid((a.n + cols - 1) / cols, (a.m + MT * 16 - 1) / (MT * 16));
+    const uint32_t lds = XT == kFp8Codes ? 0 : fp8_lds_rows_bytes(a.m < MT * 16 ? a.m : MT * 16, a.kb);
     if (gated)
-        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, true>), grid, dim3(W * 64), 0, s, a);
+        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, XT, true>), grid, dim3(W * 64), lds, s, a);
     else
-        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, false>), grid, dim3(W * 64), 0, s, a);
+        hipLaunchKernelGGL((fp8_stream_kernel<MT, NT, W, XT, false>), grid, dim3(W * 64), lds, s, a);
     return (int)hipGetLastError();
 }
 
@@ -176,7 +179,14 @@ int launch_many(const Fp8Args &a, uint32_t m_bucket, bool gated, hipStream_t s) 
 static size_t fp8_codes_bytes(uint32_t m_bucket, uint32_t k) {
     return ((size_t)m_bucket * r9vx_fp8_kb(k) * kFp8Block + 255) & ~(size_t)255;
 }
+/* Few activations: each workgroup quantizes them into its LDS beside its first
+ * weights' way from memory, which costs less than a launch of its own for them
+ * (and a workspace): 1 x 4096 x 4096, from Python, 13.0 / 8.7 us. */
+static bool fp8_in_lds(uint32_t m_bucket, uint32_t k, uint32_t x_dtype) {
+    return x_dtype != R9VX_DTYPE_E4M3 && m_bucket <= 16 && fp8_fits_lds(m_bucket, r9vx_fp8_kb(k));
+}
 size_t r9vx_fp8_workspace_bytes(uint32_t m_bucket, uint32_t k, uint32_t x_dtype) {
+    if (fp8_in_lds(m_bucket, k, x_dtype)) return 0;
     if (x_dtype == R9VX_DTYPE_E4M3) return k % kFp8Block ? fp8_codes_bytes(m_bucket, k) : 0;
     return fp8_codes_bytes(m_bucket, k) + (size_t)m_bucket * r9vx_fp8_kb(k) * 4;
 }
@@ -184,6 +194,11 @@ size_t r9vx_fp8_workspace_bytes(uint32_t m_bucket, uint32_t k, uint32_t x_dtype)
 int r9vx_launch_matmul_fp8(const r9vx_fp8_problem &p, hipStream_t stream) {
     const uint8_t *xq = static_cast<const uint8_t *>(p.x);
     const float *xs = p.x_scales;
+    const bool gated = p.epilogue == R9VX_EPILOGUE_SWIGLU;
+    if (fp8_in_lds(p.m_bucket, p.k, p.x_dtype)) {
+        const Fp8Args a = fp8_args(p, nullptr, nullptr);
+        return p.x_dtype == R9VX_DTYPE_F32 ? launch_stream<1, 2, 8, kFp8F32>(a, gated, stream) : launch_stream<1, 2, 8, kFp8Bf16>(a, gated, stream);
+    }
     if (p.x_dtype != R9VX_DTYPE_E4M3) {
         float *s = reinterpret_cast<float *>(p.workspace + fp8_codes_bytes(p.m_bucket, p.k));
         const int rc = r9vx_launch_quantize_fp8(p.x, p.x_dtype, p.m, p.k, r9vx_fp8_kb(p.k) * kFp8Block, p.workspace, s, stream);
@@ -196,13 +211,12 @@ int r9vx_launch_matmul_fp8(const r9vx_fp8_problem &p, hipStream_t stream) {
         xq = p.workspace;
     }
     const Fp8Args a = fp8_args(p, xq, xs);
-    const bool gated = p.epilogue == R9VX_EPILOGUE_SWIGLU;
     /* Four tiles of 16 rows in the streaming kernel against 64 x 64 tiles, 48 rows,
      * weights from HBM: 2 x 1408 x 2048 9.8 / 8.0 us, 2112 x 4096 16.8 / 12.8,
      * 14336 x 4096 34.2 / 20.5, 7168 x 7168 27.0 / 30.1; two tiles, 32 rows:
      * 7.7 / 7.8, 11.9 / 11.9, 24.9 / 18.8, 20.6 / 27.3; 17 rows: 6.7 / 7.4,
      * 9.7 / 11.0, 21.0 / 18.8, 16.7 / 25.3. */
-    if (p.m_bucket <= 16) return launch_stream<1, 2, 8>(a, gated, stream);
-    if (p.m_bucket <= 32) return launch_stream<2, 2, 8>(a, gated, stream);
+    if (p.m_bucket <= 16) return launch_stream<1, 2, 8, kFp8Codes>(a, gated, stream);
+    if (p.m_bucket <= 32) return launch_stream<2, 2, 8, kFp8Codes>(a, gated, stream);
     return p.y_dtype == R9VX_DTYPE_F32 ? launch_many<true>(a, p.m_bucket, gated, stream) : launch_many<false>(a, p.m_bucket, gated, stream);
 }

@@ -94,7 +94,10 @@ __device__ __forceinline__ uint32_t moe_token(const Fp8MoeArgs &a, uint32_t pos)
     return reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.sorted)[pos] / a.topk;
 }
 
-/* UP: gate / up, rows gathered by token, h stored; else down on h's rows. */
+/* UP: gate / up, rows gathered by token, h stored; else down on h's rows.
+ * The rows' codes come from launches of their own: quantized here, in
+ * registers or in LDS, they cost the occupancy that keeps the weights
+ * flowing (5 tokens of 512 experts: 56 us a call, 97 and 89 so). */
 template <int MT, int NT, int W, bool UP>
 __global__ __launch_bounds__(W * 64) void fp8_moe_stream_kernel(Fp8MoeArgs a) {
     __shared__ __attribute__((aligned(16))) r9vx_f32x4 part[W * NT * MT * 64];
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(W * 64) void fp8_moe_stream_kernel(Fp8MoeArgs a) {
     for (uint32_t m0 = 0; m0 < tile.z; m0 += MT * 16) {
         r.m0 = (UP ? 0u : tile.y) + m0;
         r.rows = tile.z - m0 < MT * 16u ? tile.z - m0 : MT * 16u;
-        fp8_stream<MT, NT, W, UP>(a.g, r, blockIdx.x, part, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
+        fp8_stream<MT, NT, W, kFp8Codes, UP>(a.g, r, blockIdx.x, part, nullptr, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
             *reinterpret_cast<r9vx_f32x4 *>(a.out + (uint64_t)(tile.y + m0 + row) * a.g.n + n) = v;
         });
         __syncthreads(); /* the partial sums have been read */

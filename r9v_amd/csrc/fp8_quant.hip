@@ -25,43 +25,20 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const void *__restric
     const uint32_t left = k - b * kFp8Block; /* columns from the block's first; k is a multiple of 16 */
     const uint64_t at = (uint64_t)row * k + b * kFp8Block, to = (uint64_t)row * ldq + b * kFp8Block;
     const uint32_t room = ldq - b * kFp8Block; /* code columns: k's, or with zeros behind them to the end of the block */
-    float v[16];
-    uint32_t amax = 0;
-    /* a lane holds groups of consecutive columns, the lanes' groups side by
-     * side, so that each load instruction reads whole 128-byte lines */
-    constexpr int G = F32 ? 4 : 8, N = 16 / G;
+    Fp8Block<F32> block;
+    block.load(static_cast<const uint8_t *>(x) + at * (F32 ? 4 : 2), left, part);
+    uint32_t code[4];
+    const float s = block.codes(code);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const uint32_t c = (j * 8 + part) * G;
-        r9vx_u32x4 w = {0u, 0u, 0u, 0u};
-        if (c < left)
-            w = __builtin_nontemporal_load(reinterpret_cast<const r9vx_u32x4 *>(static_cast<const uint8_t *>(x) + (at + c) * (F32 ? 4 : 2)));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t u = w[i]; /* a copy: bit_cast of a vector's element takes its first one */
-            if constexpr (F32) {
-                v[j * 4 + i] = __builtin_bit_cast(float, u);
-            } else {
-                v[j * 8 + 2 * i] = __builtin_bit_cast(float, u << 16);
-                v[j * 8 + 2 * i + 1] = __builtin_bit_cast(float, u & 0xFFFF0000u);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) amax = max(amax, fp8_absbits(v[i]));
-    const Fp8Scale s = fp8_scale(fp8_max8(amax));
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const uint32_t c = (j * 8 + part) * G;
-        const uint32_t lo = fp8_code4(v[j * G], v[j * G + 1], v[j * G + 2], v[j * G + 3], s);
+    for (int j = 0; j < block.N; ++j) {
+        const uint32_t c = block.column(j, part);
         if constexpr (F32) {
-            if (c < room) *reinterpret_cast<uint32_t *>(q + to + c) = c < left ? lo : 0u;
+            if (c < room) *reinterpret_cast<uint32_t *>(q + to + c) = c < left ? code[j] : 0u;
         } else {
-            const uint32_t hi = fp8_code4(v[j * G + 4], v[j * G + 5], v[j * G + 6], v[j * G + 7], s);
-            if (c < room) *reinterpret_cast<r9vx_u32x2 *>(q + to + c) = c < left ? r9vx_u32x2{lo, hi} : r9vx_u32x2{0u, 0u};
+            if (c < room) *reinterpret_cast<r9vx_u32x2 *>(q + to + c) = c < left ? r9vx_u32x2{code[2 * j], code[2 * j + 1]} : r9vx_u32x2{0u, 0u};
         }
     }
-    if (part == 0) scales[blk] = s.s;
+    if (part == 0) scales[blk] = s;
 }
 
 /* Rows of k codes to rows of whole blocks, zeros behind them. */

@@ -102,6 +102,47 @@ __device__ __forceinline__ uint32_t fp8_near4(float a, float b, float c, float d
 
 __device__ __forceinline__ uint32_t fp8_absbits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu; }
 
+/* Eight lanes' share of one block to quantize: lane `part` holds groups of G
+ * consecutive columns, the lanes' groups side by side, so that each load
+ * instruction reads whole 128-byte lines. */
+template <bool F32>
+struct Fp8Block {
+    static constexpr int G = F32 ? 4 : 8, N = 16 / G;
+    r9vx_u32x4 w[N];
+
+    static __device__ __forceinline__ uint32_t column(int j, uint32_t part) { return (j * 8 + part) * G; }
+    /* x: the block's first value; `left` columns from there, zeros behind them */
+    __device__ __forceinline__ void load(const uint8_t *x, uint32_t left, uint32_t part) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t c = column(j, part);
+            w[j] = r9vx_u32x4{0u, 0u, 0u, 0u};
+            if (c < left) w[j] = __builtin_nontemporal_load(reinterpret_cast<const r9vx_u32x4 *>(x + c * (F32 ? 4 : 2)));
+        }
+    }
+    /* code: G / 4 words of each group; returns the block's scale */
+    __device__ __forceinline__ float codes(uint32_t (&code)[4]) const {
+        float v[16];
+        uint32_t amax = 0;
+#pragma unroll
+        for (int i = 0; i < 4 * N; ++i) {
+            const uint32_t u = w[i / 4][i % 4]; /* a copy: bit_cast of a vector's element takes its first one */
+            if constexpr (F32) {
+                v[i] = __builtin_bit_cast(float, u);
+            } else {
+                v[2 * i] = __builtin_bit_cast(float, u << 16);
+                v[2 * i + 1] = __builtin_bit_cast(float, u & 0xFFFF0000u);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = max(amax, fp8_absbits(v[i]));
+        const Fp8Scale s = fp8_scale(fp8_max8(amax));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) code[i] = fp8_code4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], s);
+        return s.s;
+    }
+};
+
 typedef _Float16 fp8_half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 fp8_half8 __attribute__((ext_vector_type(8)));
 

@@ -10,6 +10,7 @@
 struct Fp8Args {
     const uint8_t *w;      /* e4m3 [n or 2n, k] */
     const float *ws;       /* [nb or 2 nb, kb] */
+    const void *x;         /* activations as given, where a workgroup quantizes them itself */
     const uint8_t *xq;     /* e4m3 rows of kb whole blocks, zeros past column k */
     const float *xs;       /* [rows, kb] */
     const float *bias;
@@ -110,6 +111,43 @@ __device__ __forceinline__ i32x8 fp8_load_frag(const uint8_t *row, uint32_t g, u
     return fp8_frag(lo, hi);
 }
 
+/* How the activations of a streaming product come. */
+enum Fp8X { kFp8Codes, /* e4m3 rows of whole blocks, and their scales */
+            kFp8F32,   /* rows of K values, which each workgroup quantizes into its LDS */
+            kFp8Bf16 };
+
+/* Quantized rows in LDS: a row's codes, whole blocks with zeros past column k,
+ * 16 bytes between rows so that a chunk of 16 rows lies in all banks; then the
+ * rows' scales. */
+__host__ __device__ inline uint32_t fp8_lds_row(uint32_t kb) { return kb * kFp8Block + 16; }
+__host__ __device__ inline uint32_t fp8_lds_rows_bytes(uint32_t rows, uint32_t kb) { return rows * (fp8_lds_row(kb) + kb * 4); }
+
+/* Whether `rows` of them leave room for two workgroups on a CU. */
+inline bool fp8_fits_lds(uint32_t rows, uint32_t kb) { return fp8_lds_rows_bytes(rows, kb) <= 48 * 1024; }
+
+template <int W, bool F32>
+__device__ __forceinline__ void fp8_quantize_rows(const Fp8Args &a, const Fp8Rows &r, uint8_t *lds) {
+    const uint32_t part = threadIdx.x & 7u, blocks = r.rows * a.kb;
+    float *const scales = reinterpret_cast<float *>(lds + r.rows * fp8_lds_row(a.kb));
+    for (uint32_t i = threadIdx.x >> 3; i < blocks; i += W * 8) {
+        const uint32_t row = i / a.kb, b = i - row * a.kb, left = a.k - b * kFp8Block, m = r.m0 + row;
+        Fp8Block<F32> block;
+        block.load(static_cast<const uint8_t *>(a.x) + ((uint64_t)m * a.k + b * kFp8Block) * (F32 ? 4 : 2), left, part);
+        uint32_t code[4];
+        const float s = block.codes(code);
+        uint8_t *const to = lds + row * fp8_lds_row(a.kb) + b * kFp8Block;
+#pragma unroll
+        for (int j = 0; j < block.N; ++j) {
+            const uint32_t c = block.column(j, part);
+            if constexpr (F32)
+                *reinterpret_cast<uint32_t *>(to + c) = c < left ? code[j] : 0u;
+            else
+                *reinterpret_cast<r9vx_u32x2 *>(to + c) = c < left ? r9vx_u32x2{code[2 * j], code[2 * j + 1]} : r9vx_u32x2{0u, 0u};
+        }
+        if (part == 0) scales[i] = s;
+    }
+}
+
 template <int MT, int NT>
 struct Fp8StreamRegs {
     i32x8 w[NT], x[MT];
@@ -120,8 +158,8 @@ struct Fp8StreamRegs {
  * and the NT / 2 of up rows beside them) times MT tiles of 16 activation rows.
  * Wave v takes the K blocks v, v + W, ...; the W partial sums are joined in
  * wave order in LDS.  store(row, n, four sums) gets each quad once. */
-template <int MT, int NT, int W, bool GATED, typename Store>
-__device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, uint32_t strip, r9vx_f32x4 *part, Store store) {
+template <int MT, int NT, int W, int XT, bool GATED, typename Store>
+__device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, uint32_t strip, r9vx_f32x4 *part, uint8_t *rows, Store store) {
     constexpr int NC = GATED ? NT / 2 : NT; /* output tiles */
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15u;
     const uint32_t n0 = strip * (NC * 16);
@@ -137,6 +175,12 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         uint32_t m = i * 16 + c;
+        if constexpr (XT != kFp8Codes) {
+            m = m < r.rows ? m : r.rows - 1;
+            xrow[i] = rows + m * fp8_lds_row(a.kb);
+            srow[i] = reinterpret_cast<const float *>(rows + r.rows * fp8_lds_row(a.kb)) + m * a.kb;
+            continue;
+        }
         m = r.m0 + (m < r.rows ? m : r.rows - 1);
         if (r.list) m = r.list[m];
         xrow[i] = a.xq + (uint64_t)m * (a.kb * kFp8Block);
@@ -144,17 +188,24 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
     }
     /* a strip lies in one 128-row block of the weight scales: 128 is a multiple of its 16 NC rows */
     const float *wsg = r.ws + (uint64_t)(n0 / kFp8Block) * a.kb, *wsu = wsg + (uint64_t)a.nb * a.kb;
-    auto load = [&](Fp8StreamRegs<MT, NT> &q, uint32_t kb) {
+    auto load_w = [&](Fp8StreamRegs<MT, NT> &q, uint32_t kb) {
         const uint32_t k0 = kb * kFp8Block, left = a.k - k0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) q.w[j] = fp8_load_frag(wrow[j] + k0, g, left);
+        q.sw[0] = wsg[kb];
+        if constexpr (GATED) q.sw[1] = wsu[kb];
+    };
+    auto load_x = [&](Fp8StreamRegs<MT, NT> &q, uint32_t kb) {
+        const uint32_t k0 = kb * kFp8Block;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             q.x[i] = fp8_load_frag(xrow[i] + k0, g, kFp8Block);
             q.sx[i] = srow[i][kb];
         }
-        q.sw[0] = wsg[kb];
-        if constexpr (GATED) q.sw[1] = wsu[kb];
+    };
+    auto load = [&](Fp8StreamRegs<MT, NT> &q, uint32_t kb) {
+        load_w(q, kb);
+        load_x(q, kb);
     };
     r9vx_f32x4 acc[MT][NT];
 #pragma unroll
@@ -173,7 +224,14 @@ __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, u
     };
     Fp8StreamRegs<MT, NT> q0, q1;
     uint32_t kb = wave;
-    if (kb < a.kb) load(q0, kb);
+    if constexpr (XT != kFp8Codes) {
+        if (kb < a.kb) load_w(q0, kb); /* on their way while the rows are quantized */
+        fp8_quantize_rows<W, XT == kFp8F32>(a, r, rows);
+        __syncthreads();
+        if (kb < a.kb) load_x(q0, kb);
+    } else {
+        if (kb < a.kb) load(q0, kb);
+    }
     for (; kb < a.kb; kb += 2 * W) {
         if (kb + W < a.kb) load(q1, kb + W);
         add(q0);

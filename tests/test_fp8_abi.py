@@ -79,8 +79,8 @@ def mm(**kw):
     (dict(y=None), NULL, "y is NULL"), (dict(in_dtype=ffi.E4M3), NULL, "x_scales"), (dict(x_scales=FAKE), INVALID, "x_scales"),
     (dict(epilogue=ffi.EPILOGUE_BIAS), NULL, "bias"), (dict(bias=FAKE), INVALID, "bias given"),
     (dict(epilogue=ffi.EPILOGUE_RESIDUAL), NULL, "residual"), (dict(residual=FAKE), INVALID, "residual given"),
-    (dict(w=FAKE + 4), ALIGN, "16-byte"), (dict(w_scales=FAKE + 1), ALIGN, "4-byte"), (dict(workspace=None), WORKSPACE, "workspace"),
-    (dict(workspace=FAKE + 16), ALIGN, "256-byte")])
+    (dict(w=FAKE + 4), ALIGN, "16-byte"), (dict(w_scales=FAKE + 1), ALIGN, "4-byte"), (dict(m_bucket=17, workspace=None), WORKSPACE, "workspace"),
+    (dict(k=8192, workspace=None), WORKSPACE, "workspace"), (dict(workspace=FAKE + 16), ALIGN, "256-byte")])
 def test_matmul_refusals(kw, code, text):
     refused(lib.r9vx_matmul_fp8_launch, *mm(**kw), code=code, text=text)
 

@@ -234,3 +234,18 @@ def test_bad_rows_stay_alone(m):
     y = ffi.matmul_fp8(codes(w), dev(ws), on_gpu(bad)).cpu().numpy()
     rest = [i for i in range(m) if i not in (1, 3)]
     assert np.isnan(y[[1, 3]]).all() and np.array_equal(y[rest], clean[rest])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,k", [(1, 4096), (5, 272), (16, 2048), (16, 4096), (3, 16)])
+def test_in_call_quantization_is_quantize_fp8s(m, k, dtype):
+    """Few rows are quantized by the workgroups that read them, others by a launch: the same bits."""
+    x = acts(31, m, k, dtype)
+    x[0, :16] = 0.0
+    x[m - 1, k - 1] = np.inf
+    w, ws = weights(32, 200, k)
+    xg = on_gpu(x, dtype)
+    q, s = ffi.quantize_fp8(xg)
+    want = ffi.matmul_fp8(codes(w), dev(ws), q, x_scales=s)
+    got = ffi.matmul_fp8(codes(w), dev(ws), xg)
+    assert torch.isnan(got[m - 1]).all() and torch.equal(got[:m - 1], want[:m - 1])
