@@ -74,6 +74,8 @@ typedef struct r9vx_matmul_fp8_args {
  * silu(gate) * up), then one rounding to out_dtype.  A row's output bits
  * depend on the static and the row alone. */
 int r9vx_matmul_fp8_launch(const r9vx_matmul_fp8_static *st, const r9vx_matmul_fp8_args *args, r9vx_stream_t stream);
+/* 0 where the activations need no place of their own: codes with K a multiple of
+ * 128, and few enough rows (m_bucket <= 16) to be quantized where they are read. */
 size_t r9vx_matmul_fp8_workspace_bytes(const r9vx_matmul_fp8_static *st);
 /* Algorithmic bytes (weights, scales, x, y) and 2 m N K operations (SWIGLU: twice the weights and 4 m N K). */
 uint64_t r9vx_matmul_fp8_static_bytes(const r9vx_matmul_fp8_static *st, uint32_t m);

@@ -10,6 +10,12 @@
  * leaves a list of tiles of up to 256 rows of one expert; both products walk
  * it: few rows per expert through the streaming loop, many through the tiles
  * of r9vx_e4m3_gemm.h.
+ *
+ * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 86 us and down 43, 4.3
+ * TB/s of weights (a 4 GiB copy: 4.7).  8192 tokens, 10 of 512 experts of 2 x
+ * 512 x 2048 (160 rows each): gate / up 376 us (0.91 PFLOP/s, 2.9 TB/s of
+ * weights; of a tile's 68 thousand cycles 55 are products, 10 the drain), down
+ * 320 us, whose K of four steps is as long as its drain, combine 63 us (5.9 TB/s).
  */
 #include "r9vx_e4m3_gemm.h"
 #include "r9vx_moe.h"

@@ -157,7 +157,11 @@ struct Fp8StreamRegs {
 /* Weight strip `strip` (NT tiles of 16 weight rows; GATED: NT / 2 of gate rows
  * and the NT / 2 of up rows beside them) times MT tiles of 16 activation rows.
  * Wave v takes the K blocks v, v + W, ...; the W partial sums are joined in
- * wave order in LDS.  store(row, n, four sums) gets each quad once. */
+ * wave order in LDS.  store(row, n, four sums) gets each quad once.
+ * Weights are read once and used for 16 rows: what bounds it is how many loads
+ * are in flight, so every wave has two blocks' worth, nothing passes through
+ * LDS on the way, and the strips are narrow (32 weight rows) to have many
+ * workgroups.  64 experts' gate and up rows of 2 x 1408 x 2048: 86 us, 4.3 TB/s. */
 template <int MT, int NT, int W, int XT, bool GATED, typename Store>
 __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, uint32_t strip, r9vx_f32x4 *part, uint8_t *rows, Store store) {
     constexpr int NC = GATED ? NT / 2 : NT; /* output tiles */
@@ -294,7 +298,11 @@ __device__ __forceinline__ i32x8 fp8_read_frag(const uint8_t *p, uint32_t frag) 
  * them).  Both operands and the rows' scales of a step are copied straight
  * into LDS one step ahead; rows are 128 bytes of eight 16-byte chunks, chunk
  * c of row r at slot c ^ (r / 2 % 8), which the 16 rows of one LDS read spread
- * over all banks. */
+ * over all banks.
+ * A 256 x 256 step takes 1.8 us: its matrix instructions alone need 0.86 at the
+ * full clock, its LDS reads and copies as much, and under random codes the
+ * clock falls to about 1.6 GHz (all zeros: a tenth faster).  Three to five
+ * stages, a persistent workgroup and lines touched ahead brought nothing. */
 template <int BM, int BN, int WM, bool GATED, bool EXACT>
 struct Fp8Tile {
     static constexpr int WN = 8 / WM, TM = BM / 16 / WM, TN = BN / 16 / WN, NC = GATED ? TN / 2 : TN;

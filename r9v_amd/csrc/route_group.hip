@@ -13,6 +13,11 @@
  * with one too close to call, about one in ten thousand, goes through f64 as
  * a whole.  The K weights are computed in f64 either way.  One wave per row,
  * no workgroup talks to another.
+ *
+ * Bound by instruction issue: 906 vector instructions a row at 512 experts,
+ * K = 10 (a third of them the K + 1 maxima in turn), 8192 rows 17 us against 4
+ * of their bytes; everything in f64 took 59.  5 rows of 256 experts: 6.3 us, a
+ * chain of dependent steps behind a launch.
  */
 #include "r9vx_device.h"
 #include "r9vx_internal.h"
