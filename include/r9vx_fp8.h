@@ -48,7 +48,7 @@ int r9vx_quantize_fp8_launch(const r9vx_quantize_fp8_args *args, r9vx_stream_t s
 
 typedef struct r9vx_matmul_fp8_static {
     uint32_t m_bucket;  /* the launch's m <= m_bucket; it, not m, picks the kernels */
-    uint32_t n;         /* output columns, any positive number */
+    uint32_t n;         /* output columns, 1 .. 2^26 */
     uint32_t k;         /* a positive multiple of 16 */
     uint32_t in_dtype;  /* F32 or BF16 (quantized within the launch) or E4M3 */
     uint32_t out_dtype; /* F32 or BF16 */

@@ -52,7 +52,7 @@ int r9vx_quantize_fp8_launch(const r9vx_quantize_fp8_args *a, r9vx_stream_t stre
 static void check_matmul_fp8_static(const r9vx_matmul_fp8_static *st, Problems &pr) {
     check_k(st->k, pr);
     if (st->n == 0) pr.add(R9VX_ERR_INVALID, "n must be positive");
-    if (st->n > (1u << 30)) pr.add(R9VX_ERR_UNSUPPORTED, "n=%u exceeds 2^30", st->n);
+    if (st->n > (1u << 26)) pr.add(R9VX_ERR_UNSUPPORTED, "n=%u exceeds 2^26", st->n); /* a launch's threads: 32 bits */
     if (st->m_bucket > (1u << 24)) pr.add(R9VX_ERR_UNSUPPORTED, "m_bucket=%u exceeds 2^24", st->m_bucket);
     if (!float_dtype(st->in_dtype) && st->in_dtype != R9VX_DTYPE_E4M3)
         pr.add(R9VX_ERR_UNSUPPORTED, "in_dtype %u: only f32, bf16 and e4m3 activations", st->in_dtype);
@@ -144,6 +144,7 @@ static void check_moe_fp8_static(const r9vx_moe_ffn_fp8_static *st, Problems &pr
     if (st->dm == 0 || st->dm % kFp8Block) pr.add(R9VX_ERR_INVALID, "dm=%u must be a positive multiple of 128", st->dm);
     if (st->dff == 0 || st->dff % kFp8Block) pr.add(R9VX_ERR_INVALID, "dff=%u must be a positive multiple of 128", st->dff);
     if (st->dm > (1u << 16) || st->dff > (1u << 16)) pr.add(R9VX_ERR_UNSUPPORTED, "dm=%u or dff=%u exceeds 2^16", st->dm, st->dff);
+    if (st->t_bucket > (1u << 23)) pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u exceeds 2^23", st->t_bucket); /* a launch's threads: 32 bits */
     if (st->shared_experts > 64) pr.add(R9VX_ERR_UNSUPPORTED, "%u shared experts exceed 64", st->shared_experts);
     /* rows are addressed by 32 bits */
     if ((uint64_t)st->t_bucket * st->dm >= (1ull << 32))

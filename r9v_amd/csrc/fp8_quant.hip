@@ -54,18 +54,28 @@ __global__ __launch_bounds__(256) void pad_fp8_kernel(const r9vx_u32x4 *__restri
 
 }  // namespace
 
+/* A launch's threads are counted in 32 bits: rows beyond this many go through
+ * a further one. */
+static constexpr uint32_t kLaunchThreads = 1u << 31;
+
 int r9vx_launch_pad_fp8(const uint8_t *x, uint32_t m, uint32_t k, uint8_t *q, hipStream_t stream) {
     const uint32_t ld16 = r9vx_fp8_kb(k) * (kFp8Block / 16);
-    const uint64_t n = (uint64_t)m * ld16;
-    hipLaunchKernelGGL(pad_fp8_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, reinterpret_cast<const r9vx_u32x4 *>(x), n,
-                       k / 16, ld16, reinterpret_cast<r9vx_u32x4 *>(q));
-    return (int)hipGetLastError();
+    const uint32_t rows = kLaunchThreads / ld16;
+    for (uint32_t r0 = 0; r0 < m; r0 += rows) {
+        const uint64_t n = (uint64_t)(m - r0 < rows ? m - r0 : rows) * ld16;
+        hipLaunchKernelGGL(pad_fp8_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream,
+                           reinterpret_cast<const r9vx_u32x4 *>(x) + (uint64_t)r0 * (k / 16), n, k / 16, ld16,
+                           reinterpret_cast<r9vx_u32x4 *>(q) + (uint64_t)r0 * ld16);
+        const int e = (int)hipGetLastError();
+        if (e) return e;
+    }
+    return 0;
 }
 
 int r9vx_launch_quantize_fp8(const void *x, uint32_t x_dtype, uint64_t m, uint32_t k, uint32_t ldq, uint8_t *q, float *scales,
                              hipStream_t stream) {
     const uint32_t kb = r9vx_fp8_kb(k);
-    const uint64_t rows = (1u << 31) / kb; /* a launch numbers its blocks in 32 bits */
+    const uint64_t rows = kLaunchThreads / 8 / kb; /* eight threads a block */
     for (uint64_t r0 = 0; r0 < m; r0 += rows) {
         const uint32_t n = (uint32_t)((m - r0 < rows ? m - r0 : rows) * kb);
         const dim3 grid((n + 31) / 32);

@@ -431,6 +431,7 @@ int r9vx_moe_route_group_launch(const r9vx_moe_route_group_static *st, const r9v
     if (st->e_total > 1024) pr.add(R9VX_ERR_UNSUPPORTED, "E=%u exceeds 1024", st->e_total);
     if (st->top_k == 0) pr.add(R9VX_ERR_INVALID, "top_k must be > 0");
     if (st->top_k > 32) pr.add(R9VX_ERR_UNSUPPORTED, "top_k=%u exceeds 32", st->top_k);
+    if (st->t_bucket > (1u << 24)) pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u exceeds 2^24", st->t_bucket); /* a launch's threads: 32 bits */
     if (st->n_group > 64) pr.add(R9VX_ERR_UNSUPPORTED, "n_group=%u exceeds 64", st->n_group);
     if (st->n_group == 0 || st->e_total % st->n_group)
         pr.add(R9VX_ERR_INVALID, "E=%u is no multiple of n_group=%u", st->e_total, st->n_group);

@@ -71,7 +71,7 @@ def mm(**kw):
 
 
 @pytest.mark.parametrize("kw,code,text", [
-    (dict(k=100), INVALID, "multiple of 16"), (dict(n=0), INVALID, "n must be positive"), (dict(n=1 << 31), UNSUPPORTED, "2^30"),
+    (dict(k=100), INVALID, "multiple of 16"), (dict(n=0), INVALID, "n must be positive"), (dict(n=(1 << 26) + 1), UNSUPPORTED, "2^26"),
     (dict(m_bucket=1 << 25), UNSUPPORTED, "m_bucket"), (dict(m=9), INVALID, "exceeds m_bucket"),
     (dict(in_dtype=ffi.F16), UNSUPPORTED, "in_dtype"), (dict(in_dtype=ffi.I8), UNSUPPORTED, "in_dtype"),
     (dict(out_dtype=ffi.E4M3), UNSUPPORTED, "out_dtype"), (dict(epilogue=4), UNSUPPORTED, "epilogue 4"),
@@ -132,7 +132,7 @@ def route(**kw):
     (dict(top_k=33), UNSUPPORTED, "top_k=33"), (dict(n_group=0), INVALID, "multiple of n_group"),
     (dict(n_group=7), INVALID, "multiple of n_group"), (dict(e_total=1024, n_group=128), UNSUPPORTED, "n_group=128"),
     (dict(topk_group=0), INVALID, "topk_group"), (dict(topk_group=9), INVALID, "topk_group"),
-    (dict(top_k=9, topk_group=1), INVALID, "exceeds the 8 experts"), (dict(n_group=64, topk_group=16), INVALID, "at least two"),
+    (dict(t_bucket=(1 << 24) + 1), UNSUPPORTED, "2^24"), (dict(top_k=9, topk_group=1), INVALID, "exceeds the 8 experts"), (dict(n_group=64, topk_group=16), INVALID, "at least two"),
     (dict(group_score=2), UNSUPPORTED, "group_score 2"), (dict(scoring=2), UNSUPPORTED, "scoring 2"), (dict(t=9), INVALID, "t_bucket"),
     (dict(logits=None), NULL, "required"), (dict(expert_ids=None), NULL, "required"), (dict(weights=None), NULL, "required"),
     (dict(has_bias=1), NULL, "bias is NULL"), (dict(bias=FAKE), INVALID, "bias given"), (dict(scale_bits=0), INVALID, "scale"),
@@ -166,7 +166,7 @@ def moe(**kw):
     (dict(e_local=0), INVALID, "E must be"), (dict(e_local=1025), UNSUPPORTED, "exceeds 1024"), (dict(k_topk=0), INVALID, "top-k"),
     (dict(k_topk=33), UNSUPPORTED, "top-k 33"), (dict(dm=0), INVALID, "dm=0"), (dict(dm=192), INVALID, "dm=192"),
     (dict(dff=64), INVALID, "dff=64"), (dict(dff=1 << 17), UNSUPPORTED, "2^16"), (dict(shared_experts=65), UNSUPPORTED, "65 shared"),
-    (dict(t_bucket=1 << 24), UNSUPPORTED, "2^32"), (dict(t_bucket=1 << 23, k_topk=16, dm=128), UNSUPPORTED, "2^26"),
+    (dict(t_bucket=1 << 24), UNSUPPORTED, "2^32"), (dict(t_bucket=(1 << 23) + 1, k_topk=1), UNSUPPORTED, "2^23"), (dict(t_bucket=1 << 23, k_topk=16, dm=128), UNSUPPORTED, "2^26"),
     (dict(out_dtype=ffi.F16), UNSUPPORTED, "out_dtype"), (dict(t=9), INVALID, "t_bucket"), (dict(x=None), NULL, "required"),
     (dict(expert_ids=None), NULL, "required"), (dict(weights=None), NULL, "required"), (dict(y=None), NULL, "required"),
     (dict(w_gate_up=None), NULL, "scales are required"), (dict(w_gate_up_scales=None), NULL, "scales are required"),
