@@ -13,7 +13,15 @@ from r9v_amd import ffi
 ROOT = pathlib.Path(__file__).resolve().parent.parent
 FAKE = 1 << 20  # aligned, never dereferenced: every call below is refused or has no rows
 INVALID, UNSUPPORTED, NULL, ALIGN, WORKSPACE = -1, -2, -3, -4, -5
-lib = ffi.load()
+
+class Lib:
+    """The library, loaded by the first test: at collection it would bind its HIP runtime ahead of torch's."""
+
+    def __getattr__(self, name):
+        return getattr(ffi.load(), name)
+
+
+lib = Lib()
 
 STRUCTS = {"r9vx_moe_ffn_fp8_static": ffi.MoeFfnFp8Static, "r9vx_moe_ffn_fp8_args": ffi.MoeFfnFp8Args,
            "r9vx_moe_route_group_static": ffi.MoeRouteGroupStatic, "r9vx_quantize_fp8_args": ffi.QuantizeFp8Args, "r9vx_matmul_fp8_static": ffi.MatmulFp8Static,
