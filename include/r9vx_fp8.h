@@ -108,7 +108,8 @@ typedef struct r9vx_moe_ffn_fp8_args {
 } r9vx_moe_ffn_fp8_args;
 
 /* moe_ffn of r9vx.h over e4m3 experts: x is quantized once; an expert's gate
- * and up products, h = silu(g) * u in f32, h quantized as activations are, the
+ * and up products, h = silu(g) * u in f32, h quantized as activations are (in
+ * the form for many tokens by a quotient within 2^-23 of the exact one), the
  * down product; y[t] = the token's expert outputs times their weights, added
  * in ascending (expert, slot) order in f32, plus the shared experts' outputs.
  * A row's output bits depend on the static, the row and its experts alone.
