@@ -38,7 +38,7 @@ __global__ __launch_bounds__(W * 64) void fp8_stream_kernel(Fp8Args a) {
     r.ws = a.ws;
     r.m0 = m0;
     r.rows = a.m - m0 < MT * 16u ? a.m - m0 : MT * 16u;
-    fp8_stream<MT, NT, W, XT, GATED>(a, r, strip, part, quantized, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
+    fp8_stream<MT, NT, W, XT, GATED>(a, r, strip, part, quantized, [] {}, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
         fp8_store_dense(a, m0 + row, n, v);
     });
 }

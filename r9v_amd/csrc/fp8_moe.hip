@@ -11,8 +11,8 @@
  * it: few rows per expert through the streaming loop, many through the tiles
  * of r9vx_e4m3_gemm.h.
  *
- * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 86 us and down 43, 4.3
- * TB/s of weights (a 4 GiB copy: 4.7).  8192 tokens, 10 of 512 experts of 2 x
+ * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 69 us and down 39, 5.1
+ * TB/s of weights (a 4 GiB copy: 4.7, reading alone up to 7).  8192 tokens, 10 of 512 experts of 2 x
  * 512 x 2048 (160 rows each): gate / up 376 us (0.91 PFLOP/s, 2.9 TB/s of
  * weights; of a tile's 68 thousand cycles 55 are products, 10 the drain), down
  * 320 us, whose K of four steps is as long as its drain, combine 63 us (5.9 TB/s).
@@ -33,7 +33,10 @@ struct Fp8MoeLayout {
 
 constexpr uint32_t kOutBlock = 128; /* columns that share a weight scale */
 
-/* Few rows: the streaming form. */
+/* Few rows: the streaming form.  A call in it / in tiles, us, at 16, 64 and 150
+ * tokens: 6 of 64 experts of 2 x 1408 x 2048 114 / 137, 141 / 145, 179 / 151;
+ * 10 of 512, 512 x 2048: 123 / 139, 284 / 281, 382 / 378; 2 of 16, 2048 x 4096:
+ * 86 / 101, 110 / 116, 162 / 119. */
 bool moe_streams(const r9vx_moe_fp8_problem &p) { return p.t_bucket <= 64; }
 
 Fp8MoeLayout moe_layout(const r9vx_moe_fp8_problem &p) {
@@ -101,11 +104,13 @@ __device__ __forceinline__ uint32_t moe_token(const Fp8MoeArgs &a, uint32_t pos)
 }
 
 /* UP: gate / up, rows gathered by token, h stored; else down on h's rows.
+ * 128 registers, so that two workgroups share a CU: at 133 gate / up takes 31
+ * us instead of 23 (5 tokens of 512 experts).
  * The rows' codes come from launches of their own: quantized here, in
  * registers or in LDS, they cost the occupancy that keeps the weights
  * flowing (5 tokens of 512 experts: 56 us a call, 97 and 89 so). */
 template <int MT, int NT, int W, bool UP>
-__global__ __launch_bounds__(W * 64) void fp8_moe_stream_kernel(Fp8MoeArgs a) {
+__global__ __launch_bounds__(W * 64, 4) void fp8_moe_stream_kernel(Fp8MoeArgs a) {
     __shared__ __attribute__((aligned(16))) r9vx_f32x4 part[W * NT * MT * 64];
     __shared__ uint32_t token[256];
     if (moe_word(a, 0) != 0u || blockIdx.y >= moe_word(a, 4)) return;
@@ -113,15 +118,17 @@ __global__ __launch_bounds__(W * 64) void fp8_moe_stream_kernel(Fp8MoeArgs a) {
     Fp8Rows r{};
     r.w = a.g.w + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.n * a.g.k;
     r.ws = a.g.ws + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.nb * a.g.kb;
-    if (UP) {
-        for (uint32_t i = threadIdx.x; i < tile.z; i += W * 64) token[i] = moe_token(a, tile.y + i);
-        __syncthreads();
-        r.list = token;
-    }
+    if (UP) r.list = token;
     for (uint32_t m0 = 0; m0 < tile.z; m0 += MT * 16) {
         r.m0 = (UP ? 0u : tile.y) + m0;
         r.rows = tile.z - m0 < MT * 16u ? tile.z - m0 : MT * 16u;
-        fp8_stream<MT, NT, W, kFp8Codes, UP>(a.g, r, blockIdx.x, part, nullptr, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
+        auto tokens = [&] {
+            if (!UP || m0 != 0) return;
+            if (threadIdx.x < tile.z) token[threadIdx.x] = moe_token(a, tile.y + threadIdx.x); /* at most 256 */
+            __syncthreads();
+        };
+        static_assert(W * 64 >= 256, "");
+        fp8_stream<MT, NT, W, kFp8Codes, UP>(a.g, r, blockIdx.x, part, nullptr, tokens, [&](uint32_t row, uint32_t n, r9vx_f32x4 v) {
             *reinterpret_cast<r9vx_f32x4 *>(a.out + (uint64_t)(tile.y + m0 + row) * a.g.n + n) = v;
         });
         __syncthreads(); /* the partial sums have been read */
