@@ -11,7 +11,7 @@
  * it: few rows per expert through the streaming loop, many through the tiles
  * of r9vx_e4m3_gemm.h.
  *
- * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 69 us and down 39, 5.1
+ * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 65 us and down 35, 5.5
  * TB/s of weights (a 4 GiB copy: 4.7, reading alone up to 7).  8192 tokens, 10 of 512 experts of 2 x
  * 512 x 2048 (160 rows each): gate / up 376 us (0.91 PFLOP/s, 2.9 TB/s of
  * weights; of a tile's 68 thousand cycles 55 are products, 10 the drain), down
@@ -104,8 +104,9 @@ __device__ __forceinline__ uint32_t moe_token(const Fp8MoeArgs &a, uint32_t pos)
 }
 
 /* UP: gate / up, rows gathered by token, h stored; else down on h's rows.
- * 128 registers, so that two workgroups share a CU: at 133 gate / up takes 31
- * us instead of 23 (5 tokens of 512 experts).
+ * 128 registers, so that sixteen waves share a CU, in workgroups of four, whose
+ * ends overlap more than those of eight: 5 tokens of 512 experts, gate / up and
+ * down 20.8 + 12.5 us (eight: 23.0 + 15.9, and 31 at 133 registers).
  * The rows' codes come from launches of their own: quantized here, in
  * registers or in LDS, they cost the occupancy that keeps the weights
  * flowing (5 tokens of 512 experts: 56 us a call, 97 and 89 so). */
@@ -325,11 +326,11 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
     /* the launch's tiles are at most this many (the list's own count is on the device) */
     const uint32_t tiles = rows / kMoeTileM3 + (pairs < p.e ? pairs : p.e) + p.shared;
     if (L.stream) {
-        hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 8, true>), dim3(p.dff / 16, tiles), dim3(512), 0, stream, up);
+        hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 4, true>), dim3(p.dff / 16, tiles), dim3(256), 0, stream, up);
         rc = (int)hipGetLastError();
         if (!rc) rc = r9vx_launch_quantize_fp8(h, R9VX_DTYPE_F32, rows, p.dff, p.dff, hq, hs, stream);
         if (rc) return rc;
-        hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 8, false>), dim3(p.dm / 32, tiles), dim3(512), 0, stream, dn);
+        hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 4, false>), dim3(p.dm / 32, tiles), dim3(256), 0, stream, dn);
     } else {
         hipLaunchKernelGGL((fp8_moe_tile_kernel<true>), dim3(tiles * ((p.dff + 127) / 128) + 7), dim3(512), 0, stream, up);
         rc = (int)hipGetLastError();
