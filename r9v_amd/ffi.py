@@ -266,6 +266,35 @@ def _need_gpu(*tensors):
     return torch
 
 
+def _empty(stream, shape, dtype, device, returned=True):
+    """Memory that a call on `stream` (None: the current one) writes.  It comes
+    from that stream's own pool: the current stream's would give blocks whose
+    last kernels there may still be queued, and nothing orders the call's writes
+    behind them.  What is returned is read on the current stream, so once freed
+    it waits for that stream too."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    reader = torch.cuda.current_stream()
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if returned:
+        t.record_stream(reader)
+    return t
+
+
+def _zeros(stream, shape, dtype, device):
+    """The same, cleared on `stream`."""
+    import torch
+
+    t = _empty(stream, shape, dtype, device)
+    if stream is None:
+        return t.zero_()
+    with torch.cuda.stream(stream):
+        return t.zero_()
+
+
 def _dtype_code(t):
     import torch
 
@@ -300,15 +329,14 @@ def matmul(w, w_scheme, n, k, x, out_dtype=F32, bias=None, residual=None, y=None
     torch = _need_gpu(w, x, bias, residual, y, w_scales)
     m = x.shape[0]
     if y is None:
-        y = torch.empty((m, n), dtype=torch.float32 if out_dtype == F32 else torch.bfloat16,
-                        device=x.device)
+        y = _empty(stream, (m, n), torch.float32 if out_dtype == F32 else torch.bfloat16, x.device)
     epi = EPILOGUE_BIAS if bias is not None else (EPILOGUE_RESIDUAL if residual is not None else EPILOGUE_NONE)
     if swiglu:  # w holds 2n rows: gate [0, n) then up [n, 2n); y = silu(gate) * up
         epi = EPILOGUE_SWIGLU
     st = matmul_static(n, k, w_scheme, _dtype_code(x), out_dtype, m_bucket=m_bucket or max(m, 1), epilogue=epi)
     if workspace is None:
         nbytes = matmul_workspace_bytes(st)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        workspace = _empty(stream, nbytes, torch.uint8, x.device, returned=False) if nbytes else None
     args = MatmulArgs(_ptr(w), _ptr(w_scales), None, _ptr(x), None, _ptr(bias), _ptr(residual), _ptr(y),
                       _ptr(workspace), m, 0)
     _check(load().r9vx_matmul_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
@@ -328,7 +356,7 @@ def matmul_static_bytes(st: MatmulStatic, m: int) -> int:
 def dequantize(wire, scheme, n_rows, k, out=None, stream=None):
     torch = _need_gpu(wire, out)
     if out is None:
-        out = torch.empty((n_rows, k), dtype=torch.float32, device=wire.device)
+        out = _empty(stream, (n_rows, k), torch.float32, wire.device)
     _check(load().r9vx_dequantize_launch(scheme, _ptr(wire), n_rows, k, _ptr(out), _stream(torch, stream)))
     return out
 
@@ -339,12 +367,12 @@ def repack(wire, scheme, n_rows, k, stream=None):
     torch = _need_gpu(wire)
     nb = n_rows * (k // BLOCK_LEN[scheme])
     if scheme == IQ3_S:
-        body = torch.empty(nb * IQ3S_DEV_BYTES, dtype=torch.uint8, device=wire.device)
+        body = _empty(stream, nb * IQ3S_DEV_BYTES, torch.uint8, wire.device)
         _check(load().r9vx_repack_launch(scheme, _ptr(wire), n_rows, k, _ptr(body), None,
                                          _stream(torch, stream)))
         return body, None
-    body = torch.empty(nb * (BLOCK_BYTES[scheme] - 2), dtype=torch.uint8, device=wire.device)
-    scales = torch.empty(nb, dtype=torch.int16, device=wire.device)
+    body = _empty(stream, nb * (BLOCK_BYTES[scheme] - 2), torch.uint8, wire.device)
+    scales = _empty(stream, nb, torch.int16, wire.device)
     _check(load().r9vx_repack_launch(scheme, _ptr(wire), n_rows, k, _ptr(body), _ptr(scales),
                                      _stream(torch, stream)))
     return body, scales
@@ -352,10 +380,10 @@ def repack(wire, scheme, n_rows, k, stream=None):
 
 def validate_weights(wire, scheme, n_rows, k, stream=None) -> int:
     torch = _need_gpu(wire)
-    bad = torch.zeros(1, dtype=torch.int32, device=wire.device)
+    bad = _zeros(stream, 1, torch.int32, wire.device)
     _check(load().r9vx_validate_weights_launch(scheme, _ptr(wire), n_rows, k, _ptr(bad),
                                                _stream(torch, stream)))
-    return int(bad.item())
+    return status_read(bad, stream)
 
 
 # ---------------------------------------------------------------- moe_route
@@ -374,9 +402,9 @@ def moe_route(logits, k, bias=None, scoring=SCORING_SOFTMAX, renormalize=True, s
     torch = _need_gpu(logits, bias, status)
     t, e = logits.shape
     if ids is None:
-        ids = torch.empty((t, k), dtype=torch.int32, device=logits.device)
+        ids = _empty(stream, (t, k), torch.int32, logits.device)
     if weights is None:
-        weights = torch.empty((t, k), dtype=torch.float32, device=logits.device)
+        weights = _empty(stream, (t, k), torch.float32, logits.device)
     st = route_static(e, k, max(t, 1), scoring, renormalize, scale, bias is not None)
     args = MoeRouteArgs(_ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights), t, 0)
     if status is not None:
@@ -399,7 +427,7 @@ def router_repack(w, stream=None):
     """f32 router weight [E, dm] -> the k4-interleaved device layout [dm/4][E][4]."""
     torch = _need_gpu(w)
     e, dm = w.shape
-    out = torch.empty(e * dm, dtype=torch.float32, device=w.device)
+    out = _empty(stream, e * dm, torch.float32, w.device)
     _check(load().r9vx_router_repack_launch(_ptr(w), e, dm, _ptr(out), _stream(torch, stream)))
     return out
 
@@ -416,12 +444,12 @@ def moe_route_hidden(x, w_router, k, bias=None, scoring=SCORING_SOFTMAX, renorma
     e = e if e is not None else w_router.numel() // dm
     st = route_static(e, k, t_bucket or max(t, 1), scoring, renormalize, scale, bias is not None)
     if workspace is None:
-        workspace = torch.zeros(int(load().r9vx_moe_route_hidden_workspace_bytes(ctypes.byref(st))),
-                                dtype=torch.uint8, device=x.device)
+        workspace = _zeros(stream, int(load().r9vx_moe_route_hidden_workspace_bytes(ctypes.byref(st))), torch.uint8,
+                           x.device)
     if ids is None:
-        ids = torch.empty((t, k), dtype=torch.int32, device=x.device)
+        ids = _empty(stream, (t, k), torch.int32, x.device)
     if weights is None:
-        weights = torch.empty((t, k), dtype=torch.float32, device=x.device)
+        weights = _empty(stream, (t, k), torch.float32, x.device)
     args = MoeRouteHiddenArgs(_ptr(x), _ptr(w_router), _ptr(bias), _ptr(ids), _ptr(weights), _ptr(workspace),
                               t, dm)
     _check(load().r9vx_moe_route_hidden_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
@@ -472,9 +500,9 @@ def moe_ffn(x, ids, weights, w_gate_up, w_down, e, dff, shared=0, gate_up_scheme
     k = ids.shape[1]
     st = ffn_static(t_bucket or max(t, 1), e, k, dm, dff, shared, gate_up_scheme, down_scheme)
     if workspace is None:
-        workspace = torch.empty(ffn_workspace_bytes(st), dtype=torch.uint8, device=x.device)
+        workspace = _empty(stream, ffn_workspace_bytes(st), torch.uint8, x.device)
     if y is None:
-        y = torch.empty((t, dm), dtype=torch.float32, device=x.device)
+        y = _empty(stream, (t, dm), torch.float32, x.device)
     args = MoeFfnArgs(_ptr(x), _ptr(ids), _ptr(weights), _ptr(w_gate_up), _ptr(w_gate_up_scales), _ptr(w_down),
                       _ptr(w_down_scales), _ptr(y), _ptr(workspace), t, 0)
     _check(load().r9vx_moe_ffn_launch(ctypes.byref(st), ctypes.byref(args), _stream(torch, stream)))
@@ -514,10 +542,10 @@ def moe_sort(ids, e, dm=256, dff=256, workspace=None, stream=None):
     t, k = ids.shape
     st = ffn_static(max(t, 1), e, k, dm, dff)
     if workspace is None:
-        workspace = torch.empty(ffn_workspace_bytes(st), dtype=torch.uint8, device=ids.device)
-    counts = torch.empty(e, dtype=torch.int32, device=ids.device)
-    offsets = torch.empty(e + 1, dtype=torch.int32, device=ids.device)
-    order = torch.empty(t * k, dtype=torch.int32, device=ids.device)
+        workspace = _empty(stream, ffn_workspace_bytes(st), torch.uint8, ids.device)
+    counts = _empty(stream, e, torch.int32, ids.device)
+    offsets = _empty(stream, e + 1, torch.int32, ids.device)
+    order = _empty(stream, t * k, torch.int32, ids.device)
     _check(load().r9vx_moe_sort_launch(ctypes.byref(st), _ptr(ids), t, _ptr(workspace), _ptr(counts),
                                        _ptr(offsets), _ptr(order), _stream(torch, stream)))
     return counts, offsets, order
@@ -588,13 +616,9 @@ def _raw_stream(device, stream):
     return _Fp8.torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
-def _used_on(stream, *tensors):
-    """Memory that was allocated here and is used on a stream of the caller's
-    is not given to others before that stream is through with it."""
-    if stream is not None:
-        for t in tensors:
-            if t is not None:
-                t.record_stream(stream)
+def _new(like, shape, dtype, stream, returned=True):
+    """_empty on a tensor's device, by the shorter way where the stream is the current one."""
+    return like.new_empty(shape, dtype=dtype) if stream is None else _empty(stream, shape, dtype, like.device, returned)
 
 
 def _at(t):
@@ -618,15 +642,12 @@ def _fp8_static(cls, workspace_bytes, *key):
     return got
 
 
-def _workspace(workspace, nbytes, like):
-    """(workspace, the one allocated here or None)"""
+def _workspace(workspace, nbytes, like, stream):
     if workspace is None:
-        if nbytes:
-            workspace = like.new_empty(nbytes, dtype=_Fp8.torch.uint8)
-        return workspace, workspace
+        return _new(like, nbytes, _Fp8.torch.uint8, stream, returned=False) if nbytes else None
     if workspace.numel() < nbytes:
         raise R9vxError(-5, f"workspace of {workspace.numel()} bytes: {nbytes} needed")
-    return workspace, None
+    return workspace
 
 
 def moe_route_group(logits, k, n_group, topk_group, bias=None, scoring=SCORING_SIGMOID, group_score=GROUP_TOP2,
@@ -641,16 +662,14 @@ def moe_route_group(logits, k, n_group, topk_group, bias=None, scoring=SCORING_S
     t, e = _rows("logits", logits)
     device = _fp8_operands(("logits", logits, T.f32, (t, e)), ("bias", bias, T.f32, (e,)), ("ids", ids, T.ids, (t, k)),
                            ("weights", weights, T.f32, (t, k)), ("status", status, T.ids, (1,)))
-    mine_i = mine_w = None
     if ids is None:
-        ids = mine_i = logits.new_empty((t, k), dtype=T.torch.int32)
+        ids = _new(logits, (t, k), T.torch.int32, stream)
     if weights is None:
-        weights = mine_w = logits.new_empty((t, k))
+        weights = _new(logits, (t, k), T.torch.float32, stream)
     st, _ = _fp8_static(MoeRouteGroupStatic, lambda st: 0, t_bucket or max(t, 1), e, k, scoring, int(renormalize), n_group,
                         topk_group, group_score, struct.unpack("<I", struct.pack("<f", scale))[0], int(bias is not None))
     args = MoeRouteArgs(logits.data_ptr(), _at(bias), ids.data_ptr(), weights.data_ptr(), t, 0)
     _check(load().r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(args), _at(status), _raw_stream(device, stream)))
-    _used_on(stream, mine_i, mine_w)
     return ids, weights
 
 
@@ -662,14 +681,12 @@ def quantize_fp8(x, q=None, scales=None, stream=None):
     m, k = _rows("x", x)
     kb = _fp8_kb(k)
     device = _fp8_operands(("x", x, T.floats, (m, k)), ("q", q, T.codes, (m, k)), ("scales", scales, T.f32, (m, kb)))
-    mine_q = mine_s = None
     if q is None:
-        q = mine_q = x.new_empty((m, k), dtype=T.torch.float8_e4m3fn)
+        q = _new(x, (m, k), T.torch.float8_e4m3fn, stream)
     if scales is None:
-        scales = mine_s = x.new_empty((m, kb), dtype=T.torch.float32)
+        scales = _new(x, (m, kb), T.torch.float32, stream)
     args = QuantizeFp8Args(x.data_ptr(), q.data_ptr(), scales.data_ptr(), m, k, F32 if x.dtype is T.torch.float32 else BF16)
     _check(load().r9vx_quantize_fp8_launch(ctypes.byref(args), _raw_stream(device, stream)))
-    _used_on(stream, mine_q, mine_s)
     return q, scales
 
 
@@ -702,14 +719,12 @@ def matmul_fp8(w, w_scales, x, x_scales=None, out_dtype=F32, bias=None, residual
         epilogue = EPILOGUE_SWIGLU if swiglu else EPILOGUE_NONE
     in_dtype = E4M3 if x_scales is not None else F32 if x.dtype is T.torch.float32 else BF16
     st, nbytes = _fp8_static(MatmulFp8Static, matmul_fp8_workspace_bytes, m_bucket or max(m, 1), n, k, in_dtype, out_dtype, epilogue)
-    workspace, mine_w = _workspace(workspace, nbytes, x)
-    mine_y = None
+    workspace = _workspace(workspace, nbytes, x, stream)
     if y is None:
-        y = mine_y = x.new_empty((m, n), dtype=T.torch.float32 if out_dtype == F32 else T.torch.bfloat16)
+        y = _new(x, (m, n), T.torch.float32 if out_dtype == F32 else T.torch.bfloat16, stream)
     args = MatmulFp8Args(w.data_ptr(), w_scales.data_ptr(), x.data_ptr(), _at(x_scales), _at(bias), _at(residual),
                          y.data_ptr(), _at(workspace), m, 0)
     _check(load().r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(args), _raw_stream(device, stream)))
-    _used_on(stream, mine_y, mine_w)
     return y
 
 
@@ -743,14 +758,12 @@ def moe_ffn_fp8(x, ids, weights, w_gate_up, w_gate_up_scales, w_down, w_down_sca
         raise R9vxError(-103, f"{shared} shared experts of {experts}")
     st, nbytes = _fp8_static(MoeFfnFp8Static, ffn_fp8_workspace_bytes, t_bucket or max(t, 1), experts - shared, k, dm, dff,
                              out_dtype, shared)
-    workspace, mine_w = _workspace(workspace, nbytes, x)
-    mine_y = None
+    workspace = _workspace(workspace, nbytes, x, stream)
     if y is None:
-        y = mine_y = x.new_empty((t, dm), dtype=T.torch.float32 if out_dtype == F32 else T.torch.bfloat16)
+        y = _new(x, (t, dm), T.torch.float32 if out_dtype == F32 else T.torch.bfloat16, stream)
     args = MoeFfnFp8Args(x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(), w_gate_up_scales.data_ptr(),
                          w_down.data_ptr(), w_down_scales.data_ptr(), y.data_ptr(), _at(workspace), t, 0)
     _check(load().r9vx_moe_ffn_fp8_launch(ctypes.byref(st), ctypes.byref(args), _raw_stream(device, stream)))
-    _used_on(stream, mine_y, mine_w)
     return y
 
 
@@ -768,7 +781,7 @@ def probe_stream(src, stream=None):
     """Streams src (a device tensor) once; returns the sink tensor."""
     torch = _need_gpu(src)
     nbytes = src.numel() * src.element_size()
-    sink = torch.empty(load().r9vx_probe_stream_blocks(nbytes), dtype=torch.int32, device=src.device)
+    sink = _empty(stream, load().r9vx_probe_stream_blocks(nbytes), torch.int32, src.device)
     _check(load().r9vx_probe_stream_launch(_ptr(src), nbytes, _ptr(sink), _stream(torch, stream)))
     return sink
 
@@ -776,7 +789,7 @@ def probe_stream(src, stream=None):
 def probe_mfma(blocks, iters, sink=None, stream=None):
     torch = _need_gpu(sink)
     if sink is None:
-        sink = torch.empty(blocks * 256, dtype=torch.float32, device="cuda")
+        sink = _empty(stream, blocks * 256, torch.float32, "cuda")
     _check(load().r9vx_probe_mfma_launch(blocks, iters, _ptr(sink), _stream(torch, stream)))
     return sink
 
@@ -788,10 +801,10 @@ def probe_matmul_tiles(w, w_scheme, n, k, x, nr, nc, out_dtype=F32, bias=None, r
     the sizes would choose."""
     torch = _need_gpu(w, x, bias, residual, w_scales)
     m = x.shape[0]
-    y = torch.empty((m, n), dtype=torch.float32 if out_dtype == F32 else torch.bfloat16, device=x.device)
+    y = _empty(stream, (m, n), torch.float32 if out_dtype == F32 else torch.bfloat16, x.device)
     epi = EPILOGUE_BIAS if bias is not None else (EPILOGUE_RESIDUAL if residual is not None else EPILOGUE_NONE)
     st = matmul_static(n, k, w_scheme, _dtype_code(x), out_dtype, m_bucket=max(m, 9), epilogue=epi)
-    workspace = torch.empty(matmul_workspace_bytes(st), dtype=torch.uint8, device=x.device)
+    workspace = _empty(stream, matmul_workspace_bytes(st), torch.uint8, x.device)
     args = MatmulArgs(_ptr(w), _ptr(w_scales), None, _ptr(x), None, _ptr(bias), _ptr(residual), _ptr(y),
                       _ptr(workspace), m, 0)
     _check(load().r9vx_probe_matmul_tiles_launch(ctypes.byref(st), ctypes.byref(args), nr, nc, _stream(torch, stream)))

@@ -359,7 +359,7 @@ def upload(file: GgufFile, data, name: str, out=None, stream=None):
     if info is None:
         raise GgufError(-1, f"no tensor named {name!r}")
     if out is None:
-        out = torch.empty(device_bytes(info), dtype=torch.uint8, device="cuda")
+        out = ffi._empty(stream, device_bytes(info), torch.uint8, "cuda")
     ptr, n, _keep = _buf(data)
     rc = ffi.load().r9vx_gguf_upload(file._h, ptr, n, name.encode(), ctypes.c_void_p(out.data_ptr()),
                                      out.numel() * out.element_size(), ffi._stream(torch, stream))
@@ -378,7 +378,7 @@ def upload_gate_up(gate_file: GgufFile, gate_data, gate: str, up_file: GgufFile,
     if info is None:
         raise GgufError(-1, f"no tensor named {gate!r}")
     if out is None:
-        out = torch.empty(2 * device_bytes(info), dtype=torch.uint8, device="cuda")
+        out = ffi._empty(stream, 2 * device_bytes(info), torch.uint8, "cuda")
     gp, gn, _gk = _buf(gate_data)
     up_, un, _uk = _buf(up_data)
     rc = ffi.load().r9vx_gguf_upload_gate_up(gate_file._h, gp, gn, gate.encode(), up_file._h, up_, un,
@@ -400,8 +400,8 @@ def upload_gate_up_split(gate_file: GgufFile, gate_data, gate: str, up_file: Ggu
     if info is None:
         raise GgufError(-1, f"no tensor named {gate!r}")
     nb = 2 * (info.nbytes // info.block_bytes)
-    body = torch.empty(nb * (info.block_bytes - 2), dtype=torch.uint8, device="cuda")
-    scales = torch.empty(nb, dtype=torch.int16, device="cuda")
+    body = ffi._empty(stream, nb * (info.block_bytes - 2), torch.uint8, "cuda")
+    scales = ffi._empty(stream, nb, torch.int16, "cuda")
     gp, gn, _gk = _buf(gate_data)
     up_, un, _uk = _buf(up_data)
     rc = ffi.load().r9vx_gguf_upload_gate_up_split(gate_file._h, gp, gn, gate.encode(), up_file._h, up_, un,
@@ -422,8 +422,8 @@ def upload_split(file: GgufFile, data, name: str, stream=None):
     if info is None:
         raise GgufError(-1, f"no tensor named {name!r}")
     nb = info.nbytes // info.block_bytes
-    body = torch.empty(nb * (info.block_bytes - 2), dtype=torch.uint8, device="cuda")
-    scales = torch.empty(nb, dtype=torch.int16, device="cuda")
+    body = ffi._empty(stream, nb * (info.block_bytes - 2), torch.uint8, "cuda")
+    scales = ffi._empty(stream, nb, torch.int16, "cuda")
     ptr, n, _keep = _buf(data)
     rc = ffi.load().r9vx_gguf_upload_split(file._h, ptr, n, name.encode(), ctypes.c_void_p(body.data_ptr()),
                                            body.numel(), ctypes.c_void_p(scales.data_ptr()), 2 * scales.numel(),
