@@ -84,7 +84,7 @@ uint64_t r9vx_matmul_fp8_static_flops(const r9vx_matmul_fp8_static *st, uint32_t
 /* ----------------------------------------------------------------- moe_ffn */
 
 typedef struct r9vx_moe_ffn_fp8_static {
-    uint32_t t_bucket;       /* the launch's t <= t_bucket; it, not t, picks the kernels */
+    uint32_t t_bucket;       /* the launch's t <= t_bucket; the static, not t, picks the kernels */
     uint32_t e_local;        /* routed experts E <= 1024 */
     uint32_t k_topk;         /* K <= 32 */
     uint32_t dm;             /* hidden size, a positive multiple of 128 */

@@ -9,7 +9,8 @@
  * then the shared experts' rows), so an expert's rows are one run.  The sort
  * leaves a list of tiles of up to 256 rows of one expert; both products walk
  * it: few rows per expert through the streaming loop, many through the tiles
- * of r9vx_e4m3_gemm.h.
+ * of r9vx_e4m3_gemm.h.  The streaming loop and f32 outputs' tiles keep every
+ * product (EXACT, r9vx_e4m3.h), bf16 outputs' tiles take the 8-bit instruction.
  *
  * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 65 us and down 35, 5.5
  * TB/s of weights (a 4 GiB copy: 4.7, reading alone up to 7).  8192 tokens, 10 of 512 experts of 2 x
@@ -33,11 +34,18 @@ struct Fp8MoeLayout {
 
 constexpr uint32_t kOutBlock = 128; /* columns that share a weight scale */
 
-/* Few rows: the streaming form.  A call in it / in tiles, us, at 16, 64 and 150
- * tokens: 6 of 64 experts of 2 x 1408 x 2048 114 / 137, 141 / 145, 179 / 151;
- * 10 of 512, 512 x 2048: 123 / 139, 284 / 281, 382 / 378; 2 of 16, 2048 x 4096:
- * 86 / 101, 110 / 116, 162 / 119. */
-bool moe_streams(const r9vx_moe_fp8_problem &p) { return p.t_bucket <= 64; }
+/* Few rows: the streaming form.  us of a call in it / in tiles at 16, 64, 96 and
+ * 150 tokens, bf16 outputs: 6 of 64 experts of 2 x 1408 x 2048 83 / 111,
+ * 120 / 142, 149 / 147, 172 / 150; 10 of 512, 512 x 2048: 83 / 108, 165 / 228,
+ * 194 / 247, 233 / 296; 2 of 16, 4096 x 2048: 66 / 102, 104 / 125, 132 / 126,
+ * 162 / 128.  f32 outputs, whose tiles are the slower exact ones, at 64, 150,
+ * 256 and 512 tokens: 120 / 229, 172 / 246, 250 / 280, 424 / 301; 164 / 349,
+ * 233 / 476, 276 / 527, 386 / 614; 104 / 168, 162 / 174, 272 / 206, 423 / 218:
+ * even at 17 to 30 rows an expert. */
+bool moe_streams(const r9vx_moe_fp8_problem &p) {
+    const uint64_t rows = (uint64_t)p.t_bucket * (p.k + p.shared);
+    return p.t_bucket <= 64 || (p.y_dtype == R9VX_DTYPE_F32 && rows <= 16ull * (p.e + p.shared));
+}
 
 Fp8MoeLayout moe_layout(const r9vx_moe_fp8_problem &p) {
     Fp8MoeLayout L{};
@@ -136,25 +144,33 @@ __global__ __launch_bounds__(W * 64, 4) void fp8_moe_stream_kernel(Fp8MoeArgs a)
     }
 }
 
-template <bool UP>
+/* BM rows of a list entry, 256 / BM workgroups for each.  EXACT as in the dense
+ * products: f32 outputs keep their sums in f32 throughout (128 rows: the
+ * widened codes leave no registers for 256); bf16 outputs take the 8-bit
+ * instruction for both products. */
+template <bool UP, int BM, bool EXACT>
 __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
-    typedef Fp8Tile<256, 256, 2, UP, false> T;
+    typedef Fp8Tile<BM, 256, 2, UP, EXACT> T;
+    constexpr uint32_t kParts = kMoeTileM3 / BM;
+    static_assert(kParts * BM == kMoeTileM3, "");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[T::kLds];
-    __shared__ uint32_t token[256];
+    __shared__ uint32_t token[BM];
     if (moe_word(a, 0) != 0u) return;
     /* each XCD takes one run of the list, a tile's column blocks side by side */
-    const uint32_t cols = (a.g.n + T::kCols - 1) / T::kCols, tiles = moe_word(a, 4) * cols;
+    const uint32_t cols = (a.g.n + T::kCols - 1) / T::kCols, tiles = moe_word(a, 4) * cols * kParts;
     const uint32_t x = blockIdx.x & 7u, i = blockIdx.x >> 3, q = tiles >> 3, rem = tiles & 7u;
     if (i >= q + (x < rem ? 1u : 0u)) return;
-    const uint32_t at = x * q + (x < rem ? x : rem) + i, nt = at % cols;
-    const r9vx_u32x4 tile = moe_tile(a, at / cols);
+    const uint32_t at = x * q + (x < rem ? x : rem) + i, nt = at / kParts % cols, r0 = at % kParts * BM;
+    const r9vx_u32x4 tile = moe_tile(a, at / (kParts * cols));
+    if (r0 >= tile.z) return;
+    const uint32_t first = tile.y + r0; /* this workgroup's first sorted position */
     Fp8Rows r{};
     r.w = a.g.w + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.n * a.g.k;
     r.ws = a.g.ws + (uint64_t)tile.x * (UP ? 2u : 1u) * a.g.nb * a.g.kb;
-    r.rows = tile.z;
-    r.m0 = UP ? 0u : tile.y;
+    r.rows = tile.z - r0 < BM ? tile.z - r0 : (uint32_t)BM;
+    r.m0 = UP ? 0u : first;
     if (UP) {
-        for (uint32_t j = threadIdx.x; j < tile.z; j += 512) token[j] = moe_token(a, tile.y + j);
+        for (uint32_t j = threadIdx.x; j < r.rows; j += 512) token[j] = moe_token(a, first + j);
         __syncthreads();
         r.list = token;
     }
@@ -179,7 +195,7 @@ __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
                 c.y = fp8_near4(v[1].x, v[1].y, v[1].z, v[1].w, s, inv);
                 c.z = fp8_near4(v[2].x, v[2].y, v[2].z, v[2].w, s, inv);
                 c.w = fp8_near4(v[3].x, v[3].y, v[3].z, v[3].w, s, inv);
-                const uint64_t pos = tile.y + t0 + row;
+                const uint64_t pos = (uint64_t)first + t0 + row;
                 *reinterpret_cast<r9vx_u32x4 *>(a.hq + pos * a.g.n + nt * 128 + part * 16) = c;
                 if (part == 0) a.hs[pos * a.g.nb + nt] = s.s;
             }
@@ -188,7 +204,7 @@ __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
             const uint32_t quad = threadIdx.x & 63u, n = nt * T::kCols + quad * 4;
             for (uint32_t row = threadIdx.x >> 6; row < T::kPass && t0 + row < r.rows; row += 8) {
                 const r9vx_f32x4 v = *reinterpret_cast<const r9vx_f32x4 *>(lds + T::at(row, quad));
-                const uint64_t pos = tile.y + t0 + row;
+                const uint64_t pos = (uint64_t)first + t0 + row;
                 if (a.L.half) {
                     auto finite = [](float f) { return fp8_absbits(f) < 0x7F800000u ? fp8_absbits(f) : 0u; };
                     uint32_t top = n < a.g.n ? max(max(finite(v.x), finite(v.y)), max(finite(v.z), finite(v.w))) : 0u;
@@ -271,6 +287,16 @@ __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) 
     }
 }
 
+template <int BM, bool EXACT>
+int launch_tiles(const Fp8MoeArgs &up, const Fp8MoeArgs &dn, uint32_t tiles, hipStream_t s) {
+    const uint32_t parts = tiles * (kMoeTileM3 / BM);
+    hipLaunchKernelGGL((fp8_moe_tile_kernel<true, BM, EXACT>), dim3(parts * ((up.g.n + 127) / 128) + 7), dim3(512), 0, s, up);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+    hipLaunchKernelGGL((fp8_moe_tile_kernel<false, BM, EXACT>), dim3(parts * ((dn.g.n + 255) / 256) + 7), dim3(512), 0, s, dn);
+    return (int)hipGetLastError();
+}
+
 }  // namespace
 
 size_t r9vx_moe_fp8_workspace_bytes(const r9vx_moe_fp8_problem &p) { return moe_layout(p).total; }
@@ -331,14 +357,12 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
         if (!rc) rc = r9vx_launch_quantize_fp8(h, R9VX_DTYPE_F32, rows, p.dff, p.dff, hq, hs, stream);
         if (rc) return rc;
         hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 4, false>), dim3(p.dm / 32, tiles), dim3(256), 0, stream, dn);
-    } else {
-        hipLaunchKernelGGL((fp8_moe_tile_kernel<true>), dim3(tiles * ((p.dff + 127) / 128) + 7), dim3(512), 0, stream, up);
         rc = (int)hipGetLastError();
         if (rc) return rc;
-        hipLaunchKernelGGL((fp8_moe_tile_kernel<false>), dim3(tiles * ((p.dm + 255) / 256) + 7), dim3(512), 0, stream, dn);
+    } else {
+        rc = p.y_dtype == R9VX_DTYPE_F32 ? launch_tiles<128, true>(up, dn, tiles, stream) : launch_tiles<256, false>(up, dn, tiles, stream);
+        if (rc) return rc;
     }
-    rc = (int)hipGetLastError();
-    if (rc) return rc;
     const Fp8CombineArgs c{p.weights, o, dn.os, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16};
     if (L.half)
         hipLaunchKernelGGL(fp8_moe_combine_kernel<true>, dim3(p.t, (p.dm / 8 + 255) / 256), dim3(256), 0, stream, c);
