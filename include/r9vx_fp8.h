@@ -116,6 +116,11 @@ typedef struct r9vx_moe_ffn_fp8_args {
  * An expert id >= E refuses the whole call: y is not written and
  * R9VX_STATUS_BAD_EXPERT is set in the workspace. */
 int r9vx_moe_ffn_fp8_launch(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ffn_fp8_args *args, r9vx_stream_t stream);
+/* The same, with a device u32 of the caller's (or NULL) into which a refused
+ * call's bits are or-ed and which no launch clears, as moe_route_group's; and
+ * with nan_refused a refused call fills y's t rows with NaN. */
+int r9vx_moe_ffn_fp8_launch_ex(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ffn_fp8_args *args, uint32_t *status,
+                               uint32_t nan_refused, r9vx_stream_t stream);
 size_t r9vx_moe_ffn_fp8_workspace_bytes(const r9vx_moe_ffn_fp8_static *st);
 /* Synchronises `stream` and returns the status bits the last launch with this
  * workspace left in it. */

@@ -195,6 +195,11 @@ uint64_t r9vx_moe_ffn_fp8_static_flops(const r9vx_moe_ffn_fp8_static *st, uint32
 }
 
 int r9vx_moe_ffn_fp8_launch(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ffn_fp8_args *a, r9vx_stream_t stream) {
+    return r9vx_moe_ffn_fp8_launch_ex(st, a, nullptr, 0, stream);
+}
+
+int r9vx_moe_ffn_fp8_launch_ex(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ffn_fp8_args *a, uint32_t *status, uint32_t nan_refused,
+                               r9vx_stream_t stream) {
     Problems pr;
     if (!st || !a) {
         pr.add(R9VX_ERR_NULL, "static and args must be non-NULL");
@@ -213,6 +218,7 @@ int r9vx_moe_ffn_fp8_launch(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ff
     if (((uintptr_t)a->expert_ids | (uintptr_t)a->weights | (uintptr_t)a->w_gate_up_scales | (uintptr_t)a->w_down_scales) & 3u)
         pr.add(R9VX_ERR_ALIGN, "expert_ids, weights and scales must be 4-byte aligned");
     if ((uintptr_t)a->workspace & 255u) pr.add(R9VX_ERR_ALIGN, "workspace must be 256-byte aligned");
+    if ((uintptr_t)status & 3u) pr.add(R9VX_ERR_ALIGN, "the status word must be 4-byte aligned");
     const int rc = pr.finish("moe_ffn_fp8");
     if (rc || a->t == 0) return rc;
     r9vx_moe_fp8_problem p = moe_fp8_problem(st);
@@ -226,6 +232,8 @@ int r9vx_moe_ffn_fp8_launch(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ff
     p.y = a->y;
     p.ws = a->workspace;
     p.t = a->t;
+    p.status = status;
+    p.nan_refused = nan_refused;
     return hip_status("moe_ffn_fp8", r9vx_launch_moe_fp8(p, reinterpret_cast<hipStream_t>(stream)));
 }
 

@@ -230,7 +230,19 @@ struct Fp8CombineArgs {
     const uint8_t *ws;
     Fp8MoeLayout L;
     uint32_t t, k, dm, shared, p, y_bf16;
+    uint32_t *status; /* the caller's word, or NULL */
+    uint32_t nan_refused;
 };
+
+/* Four outputs of y. */
+__device__ __forceinline__ void moe_store(const Fp8CombineArgs &a, uint64_t at, r9vx_f32x4 v) {
+    if (a.y_bf16)
+        *reinterpret_cast<r9vx_u32x2 *>(static_cast<uint16_t *>(a.y) + at) =
+            r9vx_u32x2{(uint32_t)r9vx_f32_to_bf16(v.x) | ((uint32_t)r9vx_f32_to_bf16(v.y) << 16),
+                       (uint32_t)r9vx_f32_to_bf16(v.z) | ((uint32_t)r9vx_f32_to_bf16(v.w) << 16)};
+    else
+        *reinterpret_cast<r9vx_f32x4 *>(static_cast<float *>(a.y) + at) = v;
+}
 
 /* y[t] = sum over the token's rows in ascending sorted position (= ascending
  * (expert, slot)) of w * o, then the shared experts' rows.  A workgroup takes
@@ -239,8 +251,16 @@ template <bool HALF>
 __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) {
     __shared__ uint32_t spos[kMoeMaxK], opos[kMoeMaxK];
     __shared__ float sw[kMoeMaxK], ow[kMoeMaxK];
-    if (reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.status)[0] != 0u) return; /* a refused call writes no y */
-    const uint32_t t = blockIdx.x, kk = a.k;
+    constexpr uint32_t kQuads = HALF ? 2 : 1;
+    const uint32_t t = blockIdx.x, kk = a.k, d = (blockIdx.y * 256 + threadIdx.x) * 4 * kQuads;
+    const uint32_t refused = reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.status)[0];
+    if (refused != 0u) { /* no y, or NaN */
+        if (a.status && (t | blockIdx.y | threadIdx.x) == 0u) atomicOr(a.status, refused);
+        const float nan = __builtin_nanf("");
+        for (uint32_t i = 0; i < kQuads; ++i)
+            if (a.nan_refused && d < a.dm) moe_store(a, (uint64_t)t * a.dm + d + i * 4, r9vx_f32x4{nan, nan, nan, nan});
+        return;
+    }
     if (threadIdx.x < kk) {
         spos[threadIdx.x] = reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.inv)[(uint64_t)t * kk + threadIdx.x];
         sw[threadIdx.x] = a.weights[(uint64_t)t * kk + threadIdx.x];
@@ -254,8 +274,6 @@ __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) 
         ow[rank] = sw[threadIdx.x];
     }
     __syncthreads();
-    constexpr uint32_t kQuads = HALF ? 2 : 1;
-    const uint32_t d = (blockIdx.y * 256 + threadIdx.x) * 4 * kQuads;
     if (d >= a.dm) return;
     r9vx_f32x4 acc[kQuads];
 #pragma unroll
@@ -276,15 +294,7 @@ __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) 
     for (uint32_t j = 0; j < kk; ++j) add(ow[j], opos[j]);
     for (uint32_t s = 0; s < a.shared; ++s) add(1.0f, (uint64_t)a.p + (uint64_t)s * a.t + t);
 #pragma unroll
-    for (uint32_t i = 0; i < kQuads; ++i) {
-        const uint64_t at = (uint64_t)t * a.dm + d + i * 4;
-        if (a.y_bf16)
-            *reinterpret_cast<r9vx_u32x2 *>(static_cast<uint16_t *>(a.y) + at) =
-                r9vx_u32x2{(uint32_t)r9vx_f32_to_bf16(acc[i].x) | ((uint32_t)r9vx_f32_to_bf16(acc[i].y) << 16),
-                           (uint32_t)r9vx_f32_to_bf16(acc[i].z) | ((uint32_t)r9vx_f32_to_bf16(acc[i].w) << 16)};
-        else
-            *reinterpret_cast<r9vx_f32x4 *>(static_cast<float *>(a.y) + at) = acc[i];
-    }
+    for (uint32_t i = 0; i < kQuads; ++i) moe_store(a, (uint64_t)t * a.dm + d + i * 4, acc[i]);
 }
 
 template <int BM, bool EXACT>
@@ -363,7 +373,8 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
         rc = p.y_dtype == R9VX_DTYPE_F32 ? launch_tiles<128, true>(up, dn, tiles, stream) : launch_tiles<256, false>(up, dn, tiles, stream);
         if (rc) return rc;
     }
-    const Fp8CombineArgs c{p.weights, o, dn.os, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16};
+    const Fp8CombineArgs c{p.weights, o, dn.os, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16,
+                           p.status, p.nan_refused};
     if (L.half)
         hipLaunchKernelGGL(fp8_moe_combine_kernel<true>, dim3(p.t, (p.dm / 8 + 255) / 256), dim3(256), 0, stream, c);
     else

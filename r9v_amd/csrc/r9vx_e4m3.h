@@ -214,6 +214,8 @@ struct r9vx_moe_fp8_problem {
     void *y;
     uint8_t *ws;
     uint32_t t, t_bucket, e, k, dm, dff, shared, y_dtype;
+    uint32_t *status;     /* a refused call's bits are or-ed into it; NULL: none kept */
+    uint32_t nan_refused; /* a refused call's y: NaN, otherwise left */
 };
 size_t r9vx_moe_fp8_workspace_bytes(const r9vx_moe_fp8_problem &p);
 int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream);

@@ -158,6 +158,7 @@ EXPORTS = [
     ("r9vx_matmul_fp8_static_bytes", [_P, _U32], ctypes.c_uint64),
     ("r9vx_matmul_fp8_static_flops", [_P, _U32], ctypes.c_uint64),
     ("r9vx_moe_ffn_fp8_launch", [_P, _P, _P], ctypes.c_int),
+    ("r9vx_moe_ffn_fp8_launch_ex", [_P, _P, _P, _U32, _P], ctypes.c_int),
     ("r9vx_moe_ffn_fp8_workspace_bytes", [_P], ctypes.c_size_t),
     ("r9vx_moe_ffn_fp8_status", [_P, _P, _P, _P], ctypes.c_int),
     ("r9vx_moe_ffn_fp8_expert_bytes", [_P], ctypes.c_uint64),
@@ -737,12 +738,14 @@ def ffn_fp8_workspace_bytes(st: MoeFfnFp8Static) -> int:
 
 
 def moe_ffn_fp8(x, ids, weights, w_gate_up, w_gate_up_scales, w_down, w_down_scales, shared=0, out_dtype=F32, y=None,
-                workspace=None, t_bucket=None, stream=None):
+                workspace=None, t_bucket=None, stream=None, status=None):
     """y = moe_ffn over e4m3 experts: bf16 x [t, dm], ids and weights [t, k],
     w_gate_up [e + shared, 2 dff, dm] with scales [e + shared, 2 dff / 128, dm / 128],
     w_down [e + shared, dm, dff] with scales [e + shared, dm / 128, dff / 128].
-    ids past the e routed experts refuse the call: y keeps what it held
-    (moe_ffn_fp8_status on a workspace of the caller's tells)."""
+    ids past the e routed experts refuse the call: a y that was passed in keeps
+    what it held, a new one is NaN, and STATUS_BAD_EXPERT is or-ed into `status`
+    (a device int32 of one element, cleared by the caller; moe_ffn_fp8_status on
+    a workspace of the caller's tells too)."""
     T = _fp8()
     t, dm = _rows("x", x)
     k = _rows("ids", ids)[1]
@@ -752,18 +755,19 @@ def moe_ffn_fp8(x, ids, weights, w_gate_up, w_gate_up_scales, w_down, w_down_sca
                            ("w_gate_up", w_gate_up, T.codes, (experts, 2 * dff, dm)),
                            ("w_gate_up_scales", w_gate_up_scales, T.f32, (experts, 2 * fb, kb)),
                            ("w_down", w_down, T.codes, (experts, dm, dff)), ("w_down_scales", w_down_scales, T.f32, (experts, kb, fb)),
-                           ("y", y, T.out.get(out_dtype, ()), (t, dm)),
+                           ("y", y, T.out.get(out_dtype, ()), (t, dm)), ("status", status, T.ids, (1,)),
                            ("workspace", workspace, T.bytes, workspace.shape if workspace is not None else ()))
     if not 0 <= shared < experts:
         raise R9vxError(-103, f"{shared} shared experts of {experts}")
     st, nbytes = _fp8_static(MoeFfnFp8Static, ffn_fp8_workspace_bytes, t_bucket or max(t, 1), experts - shared, k, dm, dff,
                              out_dtype, shared)
     workspace = _workspace(workspace, nbytes, x, stream)
+    nan_refused = int(y is None)
     if y is None:
         y = _new(x, (t, dm), T.torch.float32 if out_dtype == F32 else T.torch.bfloat16, stream)
     args = MoeFfnFp8Args(x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(), w_gate_up_scales.data_ptr(),
                          w_down.data_ptr(), w_down_scales.data_ptr(), y.data_ptr(), _at(workspace), t, 0)
-    _check(load().r9vx_moe_ffn_fp8_launch(ctypes.byref(st), ctypes.byref(args), _raw_stream(device, stream)))
+    _check(load().r9vx_moe_ffn_fp8_launch_ex(ctypes.byref(st), ctypes.byref(args), _at(status), nan_refused, _raw_stream(device, stream)))
     return y
 
 
