@@ -113,8 +113,10 @@ typedef struct r9vx_moe_ffn_fp8_args {
  * down product; y[t] = the token's expert outputs times their weights, added
  * in ascending (expert, slot) order in f32, plus the shared experts' outputs.
  * A row's output bits depend on the static, the row and its experts alone.
- * An expert id >= E refuses the whole call: y is not written and
- * R9VX_STATUS_BAD_EXPERT is set in the workspace. */
+ * A token all of whose ids are 0xFFFFFFFF, a row that moe_route_group refused,
+ * gets NaN, the others what they would without it.  Any other expert id >= E
+ * refuses the whole call: y is not written and R9VX_STATUS_BAD_EXPERT is set in
+ * the workspace. */
 int r9vx_moe_ffn_fp8_launch(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe_ffn_fp8_args *args, r9vx_stream_t stream);
 /* The same, with a device u32 of the caller's (or NULL) into which a refused
  * call's bits are or-ed and which no launch clears, as moe_route_group's; and

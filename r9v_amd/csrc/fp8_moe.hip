@@ -230,6 +230,7 @@ struct Fp8CombineArgs {
     const uint8_t *ws;
     Fp8MoeLayout L;
     uint32_t t, k, dm, shared, p, y_bf16;
+    const uint32_t *ids;
     uint32_t *status; /* the caller's word, or NULL */
     uint32_t nan_refused;
 };
@@ -254,11 +255,12 @@ __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) 
     constexpr uint32_t kQuads = HALF ? 2 : 1;
     const uint32_t t = blockIdx.x, kk = a.k, d = (blockIdx.y * 256 + threadIdx.x) * 4 * kQuads;
     const uint32_t refused = reinterpret_cast<const uint32_t *>(a.ws + a.L.sort.status)[0];
-    if (refused != 0u) { /* no y, or NaN */
-        if (a.status && (t | blockIdx.y | threadIdx.x) == 0u) atomicOr(a.status, refused);
+    const bool row = a.ids[(uint64_t)t * kk] == 0xFFFFFFFFu; /* the call was not refused: a row that was */
+    if (refused != 0u || row) { /* no y, or NaN */
+        if (refused != 0u && a.status && (t | blockIdx.y | threadIdx.x) == 0u) atomicOr(a.status, refused);
         const float nan = __builtin_nanf("");
         for (uint32_t i = 0; i < kQuads; ++i)
-            if (a.nan_refused && d < a.dm) moe_store(a, (uint64_t)t * a.dm + d + i * 4, r9vx_f32x4{nan, nan, nan, nan});
+            if ((refused == 0u || a.nan_refused) && d < a.dm) moe_store(a, (uint64_t)t * a.dm + d + i * 4, r9vx_f32x4{nan, nan, nan, nan});
         return;
     }
     if (threadIdx.x < kk) {
@@ -329,6 +331,7 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
     sp.e = p.e;
     sp.k = p.k;
     sp.shared = p.shared;
+    sp.skip_refused = 1;
     rc = r9vx_moe_sort_stage(sp, L.sort, stream, false);
     if (rc) return rc;
     const uint32_t pairs = p.t * p.k, rows = pairs + p.shared * p.t;
@@ -373,7 +376,7 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
         rc = p.y_dtype == R9VX_DTYPE_F32 ? launch_tiles<128, true>(up, dn, tiles, stream) : launch_tiles<256, false>(up, dn, tiles, stream);
         if (rc) return rc;
     }
-    const Fp8CombineArgs c{p.weights, o, dn.os, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16,
+    const Fp8CombineArgs c{p.weights, o, dn.os, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16, p.ids,
                            p.status, p.nan_refused};
     if (L.half)
         hipLaunchKernelGGL(fp8_moe_combine_kernel<true>, dim3(p.t, (p.dm / 8 + 255) / 256), dim3(256), 0, stream, c);

@@ -99,7 +99,18 @@ struct SortArgs {
     _Float16 *x16;
     float *xscale;
     uint32_t dm, xperm;
+    uint32_t skip; /* refused rows are left out (row_refused) */
 };
+
+/* A pair of a row that the router refused, every id 0xFFFFFFFF: in no expert's
+ * rows, and no reason to refuse the call. */
+__device__ __forceinline__ bool row_refused(const SortArgs &a, uint32_t pair, uint32_t id) {
+    if (!a.skip || id != 0xFFFFFFFFu) return false;
+    const uint32_t first = pair / a.k * a.k;
+    for (uint32_t j = 0; j < a.k; ++j)
+        if (a.ids[first + j] != 0xFFFFFFFFu) return false;
+    return true;
+}
 
 /* Workgroups b >= b0 of a sort kernel convert activation rows [r0, r1), one
  * wave per row.  Returns true for them (the caller returns at once). */
@@ -151,7 +162,7 @@ __global__ __launch_bounds__(1024) void sort_small_kernel(SortArgs a) {
     bool in = tid < a.p;
     uint32_t id = in ? a.ids[tid] : 0u;
     bool valid = in && id < a.e;
-    if (in && !valid) atomicOr(&bad_sh, R9VX_STATUS_BAD_EXPERT);
+    if (in && !valid && !row_refused(a, tid, id)) atomicOr(&bad_sh, R9VX_STATUS_BAD_EXPERT);
     uint64_t peers = match_peers(id, valid, id_bits(a.e));
     uint32_t rw = rank_below(peers, lane);
     if (valid && rw == 0) cnt[w][id] = (uint16_t)__popcll(peers);
@@ -206,7 +217,7 @@ __global__ __launch_bounds__(256) void sort_count_kernel(SortArgs a, uint32_t xr
     uint64_t peers = match_peers(id, valid, id_bits(a.e));
     uint32_t rw = rank_below(peers, lane);
     if (valid && rw == 0) cnt[w][id] = (uint16_t)__popcll(peers);
-    const int bad = __syncthreads_or(in && !valid);
+    const int bad = __syncthreads_or(in && !valid && !row_refused(a, pair, id));
     if (tid == 0) reinterpret_cast<uint32_t *>(a.ws + L.cbad)[chunk] = bad ? 1u : 0u;
     if (valid) {
         uint32_t rank = rw;
@@ -1103,6 +1114,7 @@ static uint32_t lpr_for(uint32_t k, uint32_t &nseg) {
 
 int r9vx_moe_sort_stage(const r9vx_moe_problem &p, const MoeLayout &L, hipStream_t s, bool rows) {
     SortArgs a{p.ids, p.ws, L, p.t * p.k, p.e, p.k, p.t, p.shared};
+    a.skip = p.skip_refused;
     if (rows) {
         a.x = p.x;
         a.x16 = reinterpret_cast<_Float16 *>(p.ws + L.x16);

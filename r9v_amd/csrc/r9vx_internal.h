@@ -216,6 +216,7 @@ struct r9vx_moe_problem {
     uint8_t *ws;
     uint32_t t, e, k, dm, dff, shared, t_bucket;
     uint32_t scheme_gu, scheme_dn;
+    uint32_t skip_refused; /* the sort leaves out tokens all of whose ids are 0xFFFFFFFF */
 };
 size_t r9vx_moe_workspace_bytes(uint32_t t_bucket, uint32_t e, uint32_t k, uint32_t dm,
                                 uint32_t dff, uint32_t shared);

@@ -742,7 +742,8 @@ def moe_ffn_fp8(x, ids, weights, w_gate_up, w_gate_up_scales, w_down, w_down_sca
     """y = moe_ffn over e4m3 experts: bf16 x [t, dm], ids and weights [t, k],
     w_gate_up [e + shared, 2 dff, dm] with scales [e + shared, 2 dff / 128, dm / 128],
     w_down [e + shared, dm, dff] with scales [e + shared, dm / 128, dff / 128].
-    ids past the e routed experts refuse the call: a y that was passed in keeps
+    A token all of whose ids are -1 (a row that moe_route_group refused) gets NaN;
+    other ids past the e routed experts refuse the call: a y that was passed in keeps
     what it held, a new one is NaN, and STATUS_BAD_EXPERT is or-ed into `status`
     (a device int32 of one element, cleared by the caller; moe_ffn_fp8_status on
     a workspace of the caller's tells too)."""

@@ -53,3 +53,30 @@ def test_a_captured_call_reports_into_its_word():
         torch.cuda.synchronize()
         assert ffi.status_read(status) == (ffi.STATUS_BAD_EXPERT if bad else 0)
         assert torch.isnan(y).all() if bad else torch.equal(y, want)
+
+
+@pytest.mark.parametrize("out", [ffi.F32, ffi.BF16])
+@pytest.mark.parametrize("t,k,shared", [(6, 2, 0), (5, 1, 1), (150, 2, 1), (700, 3, 0)])
+def test_a_row_that_the_router_refused_stays_alone(t, k, shared, out):
+    from test_gpu_fp8 import codes, dev, on_gpu
+
+    x, ex = acts(15, t, 256), experts(16, 8 + shared, 256, 128)
+    w = (codes(ex[0]), dev(ex[1]), codes(ex[2]), dev(ex[3]))
+    logits = torch.randn(t, 8, generator=torch.Generator().manual_seed(t)).cuda()
+    clean = ffi.moe_ffn_fp8(on_gpu(x), *ffi.moe_route_group(logits, k, 4, 2), *w, shared=shared, out_dtype=out)
+    assert torch.isfinite(clean).all()
+    bad = [0, 3, t - 1]
+    logits[bad, 1] = float("nan")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ids, wts = ffi.moe_route_group(logits, k, 4, 2, status=status)
+    word = torch.zeros(1, dtype=torch.int32, device="cuda")
+    y = ffi.moe_ffn_fp8(on_gpu(x), ids, wts, *w, shared=shared, out_dtype=out, y=torch.empty_like(clean), status=word)
+    rest = [i for i in range(t) if i not in bad]
+    assert ffi.status_read(status) == ffi.STATUS_NONFINITE and ffi.status_read(word) == 0
+    assert torch.isnan(y[bad]).all() and torch.equal(y[rest], clean[rest])
+    assert torch.isnan(ffi.moe_ffn_fp8(on_gpu(x), torch.full_like(ids, -1), wts, *w, shared=shared, out_dtype=out)).all()
+    if k > 1:  # one id of a token is no refused row
+        ids[1, 0] = -1
+        y.fill_(7.0)
+        ffi.moe_ffn_fp8(on_gpu(x), ids, wts, *w, shared=shared, out_dtype=out, y=y, status=word)
+        assert ffi.status_read(word) == ffi.STATUS_BAD_EXPERT and (y == 7.0).all()
