@@ -83,16 +83,20 @@ __device__ __forceinline__ void fp8_store_dense(const Fp8Args &a, uint32_t m, ui
     }
 }
 
-/* g / (1 + exp(-g)) by the hardware's exponential and reciprocal, a step each:
- * with the other roundings under 2^-20 of the value (of a tile's epilogue
- * the library's exponential and divide took a third of the time of its
- * products).  The exponential's argument keeps the low half of g log2 e; from
- * |g| = 128 on silu is g or 0 anyway. */
+/* g / (1 + exp(-g)) by the hardware's exponential and reciprocal, a step each (of a
+ * tile's epilogue the library's exponential and divide took a third of the time
+ * of its products).  e = exp(-|g| / 2) neither overflows nor underflows where the
+ * result is a normal number: silu = g / (1 + e^2) for g >= 0, g e^2 / (1 + e^2)
+ * below.  e is off by 2^-22 of itself (the exponential's step, its correction by
+ * the low half of |g| log2(e) / 2 and their product), its square by 2^-21, and
+ * the other roundings add 6 x 2^-24: under 2^-20 of the value, or 2^-149 where it
+ * is denormal.  From |g| = 256 on e is 0.  -infinity gives NaN, as the formula. */
 __device__ __forceinline__ float fp8_silu(float g) {
-    const float c = __builtin_amdgcn_fmed3f(g, -128.0f, 128.0f);
-    const float t = c * -0x1.715476p+0f;
-    const float low = fmaf(c, -0x1.715476p+0f, -t) + c * -0x1.4ae0cp-26f;
-    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t) * fmaf(low, 0x1.62e43p-1f, 1.0f));
+    const float c = fminf(fabsf(g), 256.0f);
+    const float t = c * -0x1.715476p-1f;
+    const float low = fmaf(c, -0x1.715476p-1f, -t) + c * -0x1.4ae0cp-27f;
+    const float e = __builtin_amdgcn_exp2f(t) * fmaf(low, 0x1.62e43p-1f, 1.0f);
+    return (g < 0.0f ? g * e * e : g) * __builtin_amdgcn_rcpf(fmaf(e, e, 1.0f));
 }
 
 __device__ __forceinline__ r9vx_f32x4 fp8_swiglu(r9vx_f32x4 g, r9vx_f32x4 u) {
