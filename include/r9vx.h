@@ -284,8 +284,8 @@ typedef struct r9vx_moe_route_group_static {
     uint32_t has_bias;    /* 0 / 1 */
 } r9vx_moe_route_group_static;
 
-/* args as for moe_route (logits and bias 4-byte aligned); status: a device u32
- * or NULL.  One launch. */
+/* args as for moe_route (4-byte aligned, none over another); status: a device
+ * u32 or NULL.  One launch. */
 int r9vx_moe_route_group_launch(const r9vx_moe_route_group_static *st, const r9vx_moe_route_args *args,
                                 uint32_t *status, r9vx_stream_t stream);
 uint64_t r9vx_moe_route_group_static_bytes(const r9vx_moe_route_group_static *st, uint32_t t);

@@ -61,8 +61,8 @@ typedef struct r9vx_matmul_fp8_args {
     const void *x;         /* [m, K] of in_dtype, 16-byte aligned */
     const float *x_scales; /* f32 [m, KB] with E4M3 activations, otherwise NULL */
     const float *bias;     /* f32 [N] with the BIAS epilogue */
-    const float *residual; /* f32 [m, N] with the RESIDUAL epilogue; may be y */
-    void *y;               /* [m, N] of out_dtype, 16-byte aligned */
+    const float *residual; /* f32 [m, N] with the RESIDUAL epilogue; may be an f32 y */
+    void *y;               /* [m, N] of out_dtype, 16-byte aligned; overlaps no other operand */
     uint8_t *workspace;    /* r9vx_matmul_fp8_workspace_bytes, 256-byte aligned; NULL when 0 */
     uint32_t m;
     uint32_t _tail_pad;
@@ -101,7 +101,7 @@ typedef struct r9vx_moe_ffn_fp8_args {
     const float *w_gate_up_scales; /* f32 [E + S, 2 Dff / 128, Dm / 128] */
     const uint8_t *w_down;         /* e4m3 [E + S, Dm, Dff], 16-byte aligned */
     const float *w_down_scales;    /* f32 [E + S, Dm / 128, Dff / 128] */
-    void *y;                       /* [t, Dm] of out_dtype, 16-byte aligned */
+    void *y;                       /* [t, Dm] of out_dtype, 16-byte aligned; may overlap x alone */
     uint8_t *workspace;            /* r9vx_moe_ffn_fp8_workspace_bytes, 256-byte aligned */
     uint32_t t;
     uint32_t _tail_pad;

@@ -16,10 +16,7 @@ void check_k(uint32_t k, Problems &pr) {
 
 uint64_t scale_blocks(uint32_t n, uint32_t k) { return (uint64_t)r9vx_fp8_kb(n) * r9vx_fp8_kb(k); }
 
-bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x < y + nb && y < x + na;
-}
+uint64_t float_bytes(uint32_t d) { return d == R9VX_DTYPE_F32 ? 4 : 2; }
 
 }  // namespace
 
@@ -115,6 +112,18 @@ int r9vx_matmul_fp8_launch(const r9vx_matmul_fp8_static *st, const r9vx_matmul_f
     if (ws && a->m > 0 && !a->workspace)
         pr.add(R9VX_ERR_WORKSPACE, "workspace of r9vx_matmul_fp8_workspace_bytes (%zu) required", ws);
     if ((uintptr_t)a->workspace & 255u) pr.add(R9VX_ERR_ALIGN, "workspace must be 256-byte aligned");
+    if (pr.code == R9VX_OK && a->m) {
+        /* workgroups read operands while others store their outputs */
+        const uint64_t m = a->m, ny = m * st->n * float_bytes(st->out_dtype), nx = m * st->k * (codes ? 1 : float_bytes(st->in_dtype)),
+                       nxs = m * r9vx_fp8_kb(st->k) * 4, pair = st->epilogue == R9VX_EPILOGUE_SWIGLU ? 2 : 1;
+        const bool in_place = a->residual == a->y && st->out_dtype == R9VX_DTYPE_F32;
+        if (overlap(a->y, ny, a->x, nx) || overlap(a->y, ny, a->x_scales, nxs) || overlap(a->y, ny, a->w, pair * st->n * st->k) ||
+            overlap(a->y, ny, a->w_scales, pair * scale_blocks(st->n, st->k) * 4) || overlap(a->y, ny, a->bias, 4ull * st->n) ||
+            (!in_place && overlap(a->y, ny, a->residual, m * st->n * 4)))
+            pr.add(R9VX_ERR_INVALID, "y must not overlap an operand (an f32 y may be the residual)");
+        if (overlap(a->workspace, ws, a->x, nx) || overlap(a->workspace, ws, a->x_scales, nxs) || overlap(a->workspace, ws, a->y, ny))
+            pr.add(R9VX_ERR_INVALID, "the workspace must not overlap x, x_scales or y");
+    }
     const int rc = pr.finish("matmul_fp8");
     if (rc || a->m == 0) return rc;
     r9vx_fp8_problem p{};
@@ -219,6 +228,14 @@ int r9vx_moe_ffn_fp8_launch_ex(const r9vx_moe_ffn_fp8_static *st, const r9vx_moe
         pr.add(R9VX_ERR_ALIGN, "expert_ids, weights and scales must be 4-byte aligned");
     if ((uintptr_t)a->workspace & 255u) pr.add(R9VX_ERR_ALIGN, "workspace must be 256-byte aligned");
     if ((uintptr_t)status & 3u) pr.add(R9VX_ERR_ALIGN, "the status word must be 4-byte aligned");
+    if (pr.code == R9VX_OK && a->t) { /* x is read before y is written, the rest beside it */
+        const uint64_t t = a->t, ny = t * st->dm * float_bytes(st->out_dtype), pairs = t * st->k_topk * 4, ws = r9vx_moe_ffn_fp8_workspace_bytes(st);
+        if (overlap(a->y, ny, a->expert_ids, pairs) || overlap(a->y, ny, a->weights, pairs))
+            pr.add(R9VX_ERR_INVALID, "y must not overlap expert_ids or weights");
+        if (overlap(a->workspace, ws, a->y, ny) || overlap(a->workspace, ws, a->x, t * st->dm * 2) ||
+            overlap(a->workspace, ws, a->expert_ids, pairs) || overlap(a->workspace, ws, a->weights, pairs))
+            pr.add(R9VX_ERR_INVALID, "the workspace must not overlap x, expert_ids, weights or y");
+    }
     const int rc = pr.finish("moe_ffn_fp8");
     if (rc || a->t == 0) return rc;
     r9vx_moe_fp8_problem p = moe_fp8_problem(st);

@@ -454,6 +454,12 @@ int r9vx_moe_route_group_launch(const r9vx_moe_route_group_static *st, const r9v
     if (!st->has_bias && a->bias) pr.add(R9VX_ERR_INVALID, "bias given but has_bias is 0");
     if (((uintptr_t)a->logits | (uintptr_t)a->bias | (uintptr_t)a->expert_ids | (uintptr_t)a->weights | (uintptr_t)status) & 3u)
         pr.add(R9VX_ERR_ALIGN, "logits, bias, expert_ids, weights and the status word must be 4-byte aligned");
+    if (pr.code == R9VX_OK && a->t) { /* rows are stored while others are read */
+        const uint64_t nl = (uint64_t)a->t * st->e_total * 4, nk = (uint64_t)a->t * st->top_k * 4, nb = 4ull * st->e_total;
+        if (overlap(a->expert_ids, nk, a->logits, nl) || overlap(a->weights, nk, a->logits, nl) || overlap(a->expert_ids, nk, a->weights, nk) ||
+            overlap(a->expert_ids, nk, a->bias, nb) || overlap(a->weights, nk, a->bias, nb))
+            pr.add(R9VX_ERR_INVALID, "logits, bias, expert_ids and weights must not overlap");
+    }
     const int rc = pr.finish("moe_route_group");
     if (rc || a->t == 0) return rc;
     const r9vx_route_group_problem p{a->logits,     a->bias,         a->expert_ids,  a->weights,                  status,

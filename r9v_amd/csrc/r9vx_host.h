@@ -47,6 +47,12 @@ int hip_status(const char *op, int rc) {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
+/* Whether the two ranges share a byte (NULL: no range). */
+bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && x < y + nb && y < x + na;
+}
+
 }  // namespace
 
 #endif
