@@ -145,6 +145,18 @@ int r9vx_matmul_fp8_launch(const r9vx_matmul_fp8_static *st, const r9vx_matmul_f
     return hip_status("matmul_fp8", r9vx_launch_matmul_fp8(p, reinterpret_cast<hipStream_t>(stream)));
 }
 
+static r9vx_moe_fp8_problem moe_fp8_problem(const r9vx_moe_ffn_fp8_static *st) {
+    r9vx_moe_fp8_problem p{};
+    p.t_bucket = st->t_bucket;
+    p.e = st->e_local;
+    p.k = st->k_topk;
+    p.dm = st->dm;
+    p.dff = st->dff;
+    p.shared = st->shared_experts;
+    p.y_dtype = st->out_dtype;
+    return p;
+}
+
 static void check_moe_fp8_static(const r9vx_moe_ffn_fp8_static *st, Problems &pr) {
     if (st->e_local == 0) pr.add(R9VX_ERR_INVALID, "E must be > 0");
     if (st->e_local > 1024) pr.add(R9VX_ERR_UNSUPPORTED, "E=%u exceeds 1024", st->e_local);
@@ -161,6 +173,9 @@ static void check_moe_fp8_static(const r9vx_moe_ffn_fp8_static *st, Problems &pr
     if ((uint64_t)st->t_bucket * (st->k_topk + (uint64_t)st->shared_experts) >= (1ull << 26))
         pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u rows of %u experts reach 2^26", st->t_bucket, st->k_topk + st->shared_experts);
     if (!float_dtype(st->out_dtype)) pr.add(R9VX_ERR_UNSUPPORTED, "out_dtype %u: only f32 and bf16 outputs", st->out_dtype);
+    if (pr.code == R9VX_OK && !r9vx_moe_fp8_launchable(moe_fp8_problem(st)))
+        pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u rows of %u experts and dff=%u have more tiles than a launch", st->t_bucket,
+               st->k_topk + st->shared_experts, st->dff);
 }
 
 static bool moe_fp8_static_ok(const r9vx_moe_ffn_fp8_static *st) {
@@ -168,18 +183,6 @@ static bool moe_fp8_static_ok(const r9vx_moe_ffn_fp8_static *st) {
     Problems pr;
     check_moe_fp8_static(st, pr);
     return pr.code == R9VX_OK;
-}
-
-static r9vx_moe_fp8_problem moe_fp8_problem(const r9vx_moe_ffn_fp8_static *st) {
-    r9vx_moe_fp8_problem p{};
-    p.t_bucket = st->t_bucket;
-    p.e = st->e_local;
-    p.k = st->k_topk;
-    p.dm = st->dm;
-    p.dff = st->dff;
-    p.shared = st->shared_experts;
-    p.y_dtype = st->out_dtype;
-    return p;
 }
 
 size_t r9vx_moe_ffn_fp8_workspace_bytes(const r9vx_moe_ffn_fp8_static *st) {

@@ -165,6 +165,7 @@ int launch_many(const Fp8Args &a, uint32_t m_bucket, bool gated, hipStream_t s) 
     for (uint32_t i = 0; i < 4; ++i) {
         const auto &k = kShapes[i];
         const uint64_t tiles = ((m_bucket + k.bm - 1) / k.bm) * ((n + k.bn - 1) / k.bn);
+        if (tiles * 512 >> 32) continue; /* a launch's threads: 32 bits; the large tiles' outputs would not fit the card first */
         const uint64_t block = EXACT ? k.block_x : k.block, start = EXACT ? k.start_x : k.start;
         /* half a round of the 64 x 128 tiles, which share a CU, is two thirds as long as a whole one */
         const uint64_t rounds = (tiles + k.slots - 1) / k.slots;

@@ -299,19 +299,34 @@ __global__ __launch_bounds__(256) void fp8_moe_combine_kernel(Fp8CombineArgs a) 
     for (uint32_t i = 0; i < kQuads; ++i) moe_store(a, (uint64_t)t * a.dm + d + i * 4, acc[i]);
 }
 
+/* The launch's list entries are at most this many (their own count is on the device). */
+uint64_t moe_tiles(const r9vx_moe_fp8_problem &p, uint32_t t) {
+    const uint64_t pairs = (uint64_t)t * p.k;
+    return (pairs + (uint64_t)p.shared * t) / kMoeTileM3 + (pairs < p.e ? pairs : p.e) + p.shared;
+}
+/* f32 outputs: the exact tiles of 128 rows */
+uint32_t moe_tile_rows(const r9vx_moe_fp8_problem &p) { return p.y_dtype == R9VX_DTYPE_F32 ? 128 : 256; }
+/* Workgroups of the tiles' launches; seven more, for an even share to each XCD. */
+uint64_t moe_up_tiles(const r9vx_moe_fp8_problem &p, uint64_t tiles) { return tiles * (kMoeTileM3 / moe_tile_rows(p)) * ((p.dff + 127) / 128) + 7; }
+uint64_t moe_down_tiles(const r9vx_moe_fp8_problem &p, uint64_t tiles) { return tiles * (kMoeTileM3 / moe_tile_rows(p)) * ((p.dm + 255) / 256) + 7; }
+
 template <int BM, bool EXACT>
-int launch_tiles(const Fp8MoeArgs &up, const Fp8MoeArgs &dn, uint32_t tiles, hipStream_t s) {
-    const uint32_t parts = tiles * (kMoeTileM3 / BM);
-    hipLaunchKernelGGL((fp8_moe_tile_kernel<true, BM, EXACT>), dim3(parts * ((up.g.n + 127) / 128) + 7), dim3(512), 0, s, up);
+int launch_tiles(const r9vx_moe_fp8_problem &p, const Fp8MoeArgs &up, const Fp8MoeArgs &dn, uint64_t tiles, hipStream_t s) {
+    hipLaunchKernelGGL((fp8_moe_tile_kernel<true, BM, EXACT>), dim3((uint32_t)moe_up_tiles(p, tiles)), dim3(512), 0, s, up);
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    hipLaunchKernelGGL((fp8_moe_tile_kernel<false, BM, EXACT>), dim3(parts * ((dn.g.n + 255) / 256) + 7), dim3(512), 0, s, dn);
+    hipLaunchKernelGGL((fp8_moe_tile_kernel<false, BM, EXACT>), dim3((uint32_t)moe_down_tiles(p, tiles)), dim3(512), 0, s, dn);
     return (int)hipGetLastError();
 }
 
 }  // namespace
 
 size_t r9vx_moe_fp8_workspace_bytes(const r9vx_moe_fp8_problem &p) { return moe_layout(p).total; }
+
+bool r9vx_moe_fp8_launchable(const r9vx_moe_fp8_problem &p) {
+    const uint64_t tiles = moe_tiles(p, p.t_bucket), up = moe_up_tiles(p, tiles), down = moe_down_tiles(p, tiles);
+    return moe_streams(p) || (up > down ? up : down) * 512 < 1ull << 32;
+}
 
 const uint32_t *r9vx_moe_fp8_status_word(const r9vx_moe_fp8_problem &p) {
     return reinterpret_cast<const uint32_t *>(p.ws + moe_layout(p).sort.status);
@@ -362,8 +377,7 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
     dn.g.kb = p.dff / kFp8Block;
     dn.out = o;
     dn.os = reinterpret_cast<float *>(p.ws + L.os);
-    /* the launch's tiles are at most this many (the list's own count is on the device) */
-    const uint32_t tiles = rows / kMoeTileM3 + (pairs < p.e ? pairs : p.e) + p.shared;
+    const uint32_t tiles = (uint32_t)moe_tiles(p, p.t);
     if (L.stream) {
         hipLaunchKernelGGL((fp8_moe_stream_kernel<1, 2, 4, true>), dim3(p.dff / 16, tiles), dim3(256), 0, stream, up);
         rc = (int)hipGetLastError();
@@ -373,7 +387,7 @@ int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream) {
         rc = (int)hipGetLastError();
         if (rc) return rc;
     } else {
-        rc = p.y_dtype == R9VX_DTYPE_F32 ? launch_tiles<128, true>(up, dn, tiles, stream) : launch_tiles<256, false>(up, dn, tiles, stream);
+        rc = moe_tile_rows(p) == 128 ? launch_tiles<128, true>(p, up, dn, tiles, stream) : launch_tiles<256, false>(p, up, dn, tiles, stream);
         if (rc) return rc;
     }
     const Fp8CombineArgs c{p.weights, o, dn.os, p.y, p.ws, L, p.t, p.k, p.dm, p.shared, pairs, p.y_dtype == R9VX_DTYPE_BF16, p.ids,

@@ -218,6 +218,8 @@ struct r9vx_moe_fp8_problem {
     uint32_t nan_refused; /* a refused call's y: NaN, otherwise left */
 };
 size_t r9vx_moe_fp8_workspace_bytes(const r9vx_moe_fp8_problem &p);
+/* Whether t_bucket tokens' launches have no more threads than 32 bits count. */
+bool r9vx_moe_fp8_launchable(const r9vx_moe_fp8_problem &p);
 int r9vx_launch_moe_fp8(const r9vx_moe_fp8_problem &p, hipStream_t stream);
 /* Device address of the status word in a workspace. */
 const uint32_t *r9vx_moe_fp8_status_word(const r9vx_moe_fp8_problem &p);

@@ -46,6 +46,28 @@ def route(t, e, k, scoring=0):
     args = ffi.MoeRouteArgs(FAKE, None, FAKE, FAKE, t, 0)
     return L.r9vx_moe_route_launch_ex(ctypes.byref(st), ctypes.byref(args), FAKE, None)
 
+APART = [ctypes.c_void_p((i + 1) << 44) for i in range(10)]  # operands that share no byte
+
+def matmul_fp8(m, n, k, m_bucket=None, codes=False, bf16_out=False, swiglu=False):
+    st = ffi.MatmulFp8Static(m_bucket or m, n, k, ffi.E4M3 if codes else ffi.BF16, ffi.BF16 if bf16_out else ffi.F32,
+                             ffi.EPILOGUE_SWIGLU if swiglu else ffi.EPILOGUE_NONE)
+    args = ffi.MatmulFp8Args(APART[0], APART[1], APART[2], APART[3] if codes else None, None, None, APART[4], APART[5], m, 0)
+    return L.r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(args), None)
+
+def moe_fp8(t, e, k, dm, dff, shared=0, bf16_out=False, t_bucket=None):
+    st = ffi.ffn_fp8_static(t_bucket or t, e, k, dm, dff, shared, ffi.BF16 if bf16_out else ffi.F32)
+    args = ffi.MoeFfnFp8Args(*APART[:9], t, 0)
+    return L.r9vx_moe_ffn_fp8_launch(ctypes.byref(st), ctypes.byref(args), None)
+
+def quantize_fp8(m, k, x_f32=False):
+    args = ffi.QuantizeFp8Args(APART[0], APART[1], APART[2], m, k, ffi.F32 if x_f32 else ffi.BF16)
+    return L.r9vx_quantize_fp8_launch(ctypes.byref(args), None)
+
+def route_group(t, e, k, n_group=1, topk_group=1):
+    st = ffi.MoeRouteGroupStatic(t, e, k, ffi.SCORING_SIGMOID, 1, n_group, topk_group, ffi.GROUP_MAX, 0x3F800000, 0)
+    args = ffi.MoeRouteArgs(APART[0], None, APART[1], APART[2], t, 0)
+    return L.r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(args), None, None)
+
 out = []
 for f, kw in json.loads(sys.argv[1]):
     rc = globals()[f](**kw)
