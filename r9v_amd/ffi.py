@@ -633,9 +633,18 @@ def _fp8_kb(k):
 _fp8_statics = {}  # key -> (static, its workspace bytes)
 
 
+def _u32(name, v):
+    """v, which a field of 32 bits would otherwise take modulo 2^32."""
+    if not 0 <= v < 1 << 32:
+        raise R9vxError(-2, f"{name}={v} does not fit 32 bits")
+    return v
+
+
 def _fp8_static(cls, workspace_bytes, *key):
     got = _fp8_statics.get((cls, key))
     if got is None:
+        for (name, _), v in zip(cls._fields_, key):
+            _u32(name, v)
         if len(_fp8_statics) >= 4096:  # a caller that never repeats a size
             _fp8_statics.clear()
         st = cls(*key)
@@ -669,7 +678,7 @@ def moe_route_group(logits, k, n_group, topk_group, bias=None, scoring=SCORING_S
         weights = _new(logits, (t, k), T.torch.float32, stream)
     st, _ = _fp8_static(MoeRouteGroupStatic, lambda st: 0, t_bucket or max(t, 1), e, k, scoring, int(renormalize), n_group,
                         topk_group, group_score, struct.unpack("<I", struct.pack("<f", scale))[0], int(bias is not None))
-    args = MoeRouteArgs(logits.data_ptr(), _at(bias), ids.data_ptr(), weights.data_ptr(), t, 0)
+    args = MoeRouteArgs(logits.data_ptr(), _at(bias), ids.data_ptr(), weights.data_ptr(), _u32("t", t), 0)
     _check(load().r9vx_moe_route_group_launch(ctypes.byref(st), ctypes.byref(args), _at(status), _raw_stream(device, stream)))
     return ids, weights
 
@@ -686,7 +695,7 @@ def quantize_fp8(x, q=None, scales=None, stream=None):
         q = _new(x, (m, k), T.torch.float8_e4m3fn, stream)
     if scales is None:
         scales = _new(x, (m, kb), T.torch.float32, stream)
-    args = QuantizeFp8Args(x.data_ptr(), q.data_ptr(), scales.data_ptr(), m, k, F32 if x.dtype is T.torch.float32 else BF16)
+    args = QuantizeFp8Args(x.data_ptr(), q.data_ptr(), scales.data_ptr(), m, _u32("k", k), F32 if x.dtype is T.torch.float32 else BF16)
     _check(load().r9vx_quantize_fp8_launch(ctypes.byref(args), _raw_stream(device, stream)))
     return q, scales
 
@@ -724,7 +733,7 @@ def matmul_fp8(w, w_scales, x, x_scales=None, out_dtype=F32, bias=None, residual
     if y is None:
         y = _new(x, (m, n), T.torch.float32 if out_dtype == F32 else T.torch.bfloat16, stream)
     args = MatmulFp8Args(w.data_ptr(), w_scales.data_ptr(), x.data_ptr(), _at(x_scales), _at(bias), _at(residual),
-                         y.data_ptr(), _at(workspace), m, 0)
+                         y.data_ptr(), _at(workspace), _u32("m", m), 0)
     _check(load().r9vx_matmul_fp8_launch(ctypes.byref(st), ctypes.byref(args), _raw_stream(device, stream)))
     return y
 
@@ -767,7 +776,7 @@ def moe_ffn_fp8(x, ids, weights, w_gate_up, w_gate_up_scales, w_down, w_down_sca
     if y is None:
         y = _new(x, (t, dm), T.torch.float32 if out_dtype == F32 else T.torch.bfloat16, stream)
     args = MoeFfnFp8Args(x.data_ptr(), ids.data_ptr(), weights.data_ptr(), w_gate_up.data_ptr(), w_gate_up_scales.data_ptr(),
-                         w_down.data_ptr(), w_down_scales.data_ptr(), y.data_ptr(), _at(workspace), t, 0)
+                         w_down.data_ptr(), w_down_scales.data_ptr(), y.data_ptr(), _at(workspace), _u32("t", t), 0)
     _check(load().r9vx_moe_ffn_fp8_launch_ex(ctypes.byref(st), ctypes.byref(args), _at(status), nan_refused, _raw_stream(device, stream)))
     return y
 
