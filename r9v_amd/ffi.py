@@ -614,7 +614,11 @@ def _rows(name, t, dims=2):
 
 
 def _raw_stream(device, stream):
-    return _Fp8.torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+    if stream is None:
+        return _Fp8.torch._C._cuda_getCurrentRawStream(device)
+    if stream.device.index != device:
+        raise R9vxError(-104, f"the stream is of cuda:{stream.device.index}, the operands are on cuda:{device}")
+    return stream.cuda_stream
 
 
 def _new(like, shape, dtype, stream, returned=True):

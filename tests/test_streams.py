@@ -19,6 +19,9 @@ def stream(n):
     return types.SimpleNamespace(cuda_stream=n, synchronize=lambda: None)
 
 
+RAW_STREAM = ffi._raw_stream  # the binding's own; the calls below run with a stand-in
+
+
 class Allocations(TorchDispatchMode):
     """(name, stream that is current) of every operator that makes or fills memory."""
 
@@ -116,3 +119,13 @@ def test_every_call_with_a_stream_is_here():
     names = {n for m in (ffi, gguf) for n, f in inspect.getmembers(m, inspect.isfunction)
              if f.__module__ == m.__name__ and not n.startswith("_") and "stream" in inspect.signature(f).parameters}
     assert names == told | {n.split(".")[-1] for n in CALLS if n != "repack_iq3s"}
+
+
+@pytest.mark.parametrize("name", ["moe_route_group", "quantize_fp8", "matmul_fp8", "moe_ffn_fp8"])
+def test_a_stream_of_another_device_is_refused(name, spy, monkeypatch):
+    monkeypatch.setattr(ffi, "_raw_stream", RAW_STREAM)
+    here, other = stream(7), stream(8)
+    here.device, other.device = torch.device("cuda", 0), torch.device("cuda", 1)
+    CALLS[name](stream=here)
+    with pytest.raises(ffi.R9vxError, match="stream is of cuda:1"):
+        CALLS[name](stream=other)
