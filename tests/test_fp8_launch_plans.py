@@ -59,3 +59,14 @@ def test_the_experts_form(runtime, kw, form):
     (rc, msg, launches), = launch_record.record(runtime, [("moe_fp8", kw)])
     assert rc == 0, msg
     assert form in [n for n, _, _ in launches]
+
+
+def test_long_rows_reach_every_kernel(runtime):
+    """The sizes of the tests of long K choose the kernels they are there for."""
+    pytest.importorskip("torch")
+    from test_gpu_fp8_long_k import CASES
+
+    out = launch_record.record(runtime, [("matmul_fp8", dict(m=m, n=n, k=k, codes=True, bf16_out=not f32, swiglu=gated)) for m, n, k, f32, gated, _ in CASES])
+    for case, (rc, msg, launches) in zip(CASES, out):
+        assert rc == 0, msg
+        assert launches[-1][0] == case[5], case
