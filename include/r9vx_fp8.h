@@ -16,7 +16,18 @@
  *     q[m, k] = e4m3(x[m, k] / s[m, k / 128])
  * and a block that holds a NaN or an infinity gets a NaN scale and NaN codes:
  * every output of that row is NaN, the other rows are as they would be.
- * Scales are used as given; they may have any sign and value.
+ * Scales are used as given; they may have any sign and value.  An activation's
+ * and a weight's are multiplied in f32 first.
+ *
+ * Sums.  f32 outputs, and bf16 ones of up to 32 rows (m_bucket) or 64 tokens
+ * (t_bucket), add every product of codes in f32.  bf16 outputs of more take the
+ * 8-bit matrix instruction, which cuts each group of 8 neighbouring columns'
+ * products about 14 bits below the largest of them before it adds them: an
+ * error of up to 2^-10 of the sum of absolute products (about 10^-5 of the
+ * result on ordinary data, a hundredth of the output's own rounding), so that
+ * small products beside large ones that cancel are lost.  In moe_ffn_fp8 it
+ * moves codes of h near a middle by a whole step: with 10 of 512 experts the
+ * outputs are 2.5e-3 from the exact ones, of which 1.7e-3 is their rounding.
  */
 #ifndef R9VX_FP8_H_
 #define R9VX_FP8_H_
@@ -70,7 +81,7 @@ typedef struct r9vx_matmul_fp8_args {
 
 /* y = x . w^T with both operands in e4m3:
  *     a[m, n] = sum_b xs[m, b] * ws[n / 128, b] * sum_{k in block b} xq[m, k] * wq[n, k]
- * accumulated in f32, then the epilogue (bias, residual, or
+ * added as said above, then the epilogue (bias, residual, or
  * silu(gate) * up), then one rounding to out_dtype.  A row's output bits
  * depend on the static and the row alone. */
 int r9vx_matmul_fp8_launch(const r9vx_matmul_fp8_static *st, const r9vx_matmul_fp8_args *args, r9vx_stream_t stream);
@@ -112,6 +123,10 @@ typedef struct r9vx_moe_ffn_fp8_args {
  * the form for many tokens by a quotient within 2^-23 of the exact one), the
  * down product; y[t] = the token's expert outputs times their weights, added
  * in ascending (expert, slot) order in f32, plus the shared experts' outputs.
+ * For bf16 outputs of more than 64 tokens (t_bucket) an expert's output is kept
+ * in f16 with a power of two per row and 128 columns before it is added: off by
+ * 2^-11 of itself and 2^-25 of those columns' largest, which is more than y's
+ * own rounding where experts cancel.  f32 outputs keep f32.
  * A row's output bits depend on the static, the row and its experts alone.
  * A token all of whose ids are 0xFFFFFFFF, a row that moe_route_group refused,
  * gets NaN, the others what they would without it.  Any other expert id >= E

@@ -77,9 +77,12 @@ Fp8MoeLayout moe_layout(const r9vx_moe_fp8_problem &p) {
     L.hs = take(4 * rows * (p.dff / kFp8Block));
     /* o is written and read once each, in prompts by far the most bytes of all.
      * For bf16 outputs the tiles keep it in f16: a row's 128 columns of one
-     * weight scale times the power of two that brings the largest under 4, so
-     * that nothing overflows and an addend is off by half a step, 2^-11 of itself (or 2^-25
-     * of the block's largest): an eighth of the output's own rounding. */
+     * weight scale times the power of two that brings the largest into [1, 2)
+     * (under 4 at f32's upper end), so that nothing overflows and an addend is
+     * off by half a step, 2^-11 of itself or 2^-25 of the block's largest: an
+     * eighth of the output's own rounding where the addends do not cancel.
+     * 8192 tokens of 10 of 512 experts: 778 us a call against 832 with an f32 o,
+     * and 2.516e-3 against 2.507e-3 from the exact outputs. */
     L.half = !L.stream && p.y_dtype == R9VX_DTYPE_BF16;
     L.o = take((L.half ? 2 : 4) * rows * p.dm);
     L.os = take(L.half ? 4 * rows * (p.dm / kOutBlock) : 0);
@@ -146,8 +149,10 @@ __global__ __launch_bounds__(W * 64, 4) void fp8_moe_stream_kernel(Fp8MoeArgs a)
 
 /* BM rows of a list entry, 256 / BM workgroups for each.  EXACT as in the dense
  * products: f32 outputs keep their sums in f32 throughout (128 rows: the
- * widened codes leave no registers for 256); bf16 outputs take the 8-bit
- * instruction for both products. */
+ * widened codes leave no registers for 256).  bf16 outputs take the 8-bit
+ * instruction for both products, 8192 tokens of 10 of 512 experts 778 us a call
+ * against 1280: what it drops moves some codes of h, and the outputs are 2.5e-3
+ * from the exact ones instead of the 1.7e-3 of their own rounding. */
 template <bool UP, int BM, bool EXACT>
 __global__ __launch_bounds__(512) void fp8_moe_tile_kernel(Fp8MoeArgs a) {
     typedef Fp8Tile<BM, 256, 2, UP, EXACT> T;

@@ -4,7 +4,8 @@
  *
  * Numbers: OCP e4m3 (largest 448, smallest 2^-9, NaN 0x7F, no infinity).  A
  * row of activations carries one f32 scale per 128 columns, a weight one per
- * 128 x 128 block; sums and scales are f32 throughout.
+ * 128 x 128 block.  Scaled sums are f32; what a block's 128 products keep
+ * before that is the matrix instruction's matter (fp8_mma).
  */
 #ifndef R9VX_E4M3_H
 #define R9VX_E4M3_H

@@ -7,8 +7,8 @@ import pytest
 
 import fp8_ref as R
 from r9v_amd import ffi
-from test_gpu_fp8 import codes, dev
-from test_gpu_fp8_moe import call, check, reference, routing
+from test_gpu_fp8 import acts, codes, dev
+from test_gpu_fp8_moe import call, check, check_both, reference, routing
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -83,3 +83,32 @@ def test_dense_products_that_cancel(m):
     tol = R.product_tol(k, a)
     assert np.max(tol / np.abs(p)) < 0.9
     check(ffi.matmul_fp8(codes(w), dev(ws), dev(x)), p, tol, False)
+
+
+def cancelling_experts(t):
+    """Two experts whose outputs differ in a hundredth, with weights 1 and -1.  A block of h
+    is one value, so that its codes are 448 whatever the last bits, and the down weights are
+    small whole numbers times a power of two, 2^-14 apart between rows: every sum is exact."""
+    dm, dff = 256, 128
+    r = np.random.default_rng(4)
+    rows = [r.integers(1, 4, (1, dm)).repeat(dff, axis=0) for _ in range(2)]
+    gu, gus = R.encode(np.concatenate(rows)), np.full((2, 2), 2.0 ** -9, np.float32)
+    dn = r.integers(1, 9, (dm, dff)).astype(np.float64)
+    other = dn.copy()
+    other[:, ::16] += 1
+    size = np.where(np.arange(dm) % 2, 2.0 ** -9, 32.0)[:, None]
+    dns = np.full((2, 1), 2.0 ** -7, np.float32)
+    ex = (np.stack([gu, gu]), np.stack([gus, gus]), np.stack([R.encode(dn * size), R.encode(other * size)]), np.stack([dns, dns]))
+    x = np.abs(acts(6, t, dm))
+    ids, wts = np.tile(np.array([0, 1], np.int32), (t, 1)), np.tile(np.array([1, -1], np.float32), (t, 1))
+    return x, ids, wts, ex
+
+
+@pytest.mark.parametrize("t", [40, 150])
+def test_experts_that_cancel(t):
+    """bf16 outputs of many tokens are off by 2^-11 of each |w o| and 2^-25 of its 128
+    columns' largest, not by a share of what is left; f32 ones are not."""
+    x, ids, wts, ex = cancelling_experts(t)
+    y, tol, half = reference(x, ids, wts, *ex, 0, exact=True)
+    assert np.max(tol / np.abs(y)) < 2.0 ** -6 and (t <= 64 or np.min(half / np.abs(y)) > 2.0 ** -5)
+    check_both(x, ids, wts, ex, (y, tol, half))
