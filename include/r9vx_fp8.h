@@ -19,13 +19,14 @@
  * Scales are used as given; they may have any sign and value.  An activation's
  * and a weight's are multiplied in f32 first.
  *
- * Sums.  f32 outputs, and bf16 ones of up to 32 rows (m_bucket) or 64 tokens
- * (t_bucket), add every product of codes in f32.  bf16 outputs of more take the
- * 8-bit matrix instruction, which cuts each group of 8 neighbouring columns'
- * products about 14 bits below the largest of them before it adds them: an
- * error of up to 2^-10 of the sum of absolute products (about 10^-5 of the
- * result on ordinary data, a hundredth of the output's own rounding), so that
- * small products beside large ones that cancel are lost.  In moe_ffn_fp8 it
+ * Sums.  f32 outputs, and bf16 ones of few rows (m_bucket <= 32; in moe_ffn_fp8
+ * t_bucket <= 64, or t_bucket (K + S) <= 8 (E + S) and, with shared experts,
+ * t_bucket <= 128), add every product of codes in f32.  bf16 outputs of more
+ * take the 8-bit matrix instruction, which cuts the products of each group of 8
+ * neighbouring columns about 14 bits below the largest of them before it adds
+ * them: an error of up to 2^-10 of the sum of absolute products (about 10^-5 of
+ * the result on ordinary data, a hundredth of the output's own rounding), so
+ * that small products beside large ones that cancel are lost.  In moe_ffn_fp8 it
  * moves codes of h near a middle by a whole step: with 10 of 512 experts the
  * outputs are 2.5e-3 from the exact ones, of which 1.7e-3 is their rounding.
  */
@@ -123,8 +124,8 @@ typedef struct r9vx_moe_ffn_fp8_args {
  * the form for many tokens by a quotient within 2^-23 of the exact one), the
  * down product; y[t] = the token's expert outputs times their weights, added
  * in ascending (expert, slot) order in f32, plus the shared experts' outputs.
- * For bf16 outputs of more than 64 tokens (t_bucket) an expert's output is kept
- * in f16 with a power of two per row and 128 columns before it is added: off by
+ * For bf16 outputs of many tokens (Sums, above) an expert's output is kept in
+ * f16 with a power of two per row and 128 columns before it is added: off by
  * 2^-11 of itself and 2^-25 of those columns' largest, which is more than y's
  * own rounding where experts cancel.  f32 outputs keep f32.
  * A row's output bits depend on the static, the row and its experts alone.

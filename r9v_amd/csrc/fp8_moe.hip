@@ -34,17 +34,29 @@ struct Fp8MoeLayout {
 
 constexpr uint32_t kOutBlock = 128; /* columns that share a weight scale */
 
-/* Few rows: the streaming form.  us of a call in it / in tiles at 16, 64, 96 and
- * 150 tokens, bf16 outputs: 6 of 64 experts of 2 x 1408 x 2048 83 / 111,
- * 120 / 142, 149 / 147, 172 / 150; 10 of 512, 512 x 2048: 83 / 108, 165 / 228,
- * 194 / 247, 233 / 296; 2 of 16, 4096 x 2048: 66 / 102, 104 / 125, 132 / 126,
- * 162 / 128.  f32 outputs, whose tiles are the slower exact ones, at 64, 150,
- * 256 and 512 tokens: 120 / 229, 172 / 246, 250 / 280, 424 / 301; 164 / 349,
- * 233 / 476, 276 / 527, 386 / 614; 104 / 168, 162 / 174, 272 / 206, 423 / 218:
- * even at 17 to 30 rows an expert. */
+/* Few rows an expert: the streaming form.  us of a call in it / in tiles, rows an
+ * expert in brackets, shared experts counted with the others; bf16 outputs:
+ *   6 of 64 experts of 2 x 1408 x 2048    64 tokens (6) 120 / 142, 96 (9) 149 / 147, 150 (14) 172 / 150
+ *   10 of 512, 512 x 2048                 64 (1) 165 / 228, 256 (5) 275 / 332, 384 (8) 337 / 354, 512 (10) 385 / 375
+ *   2 of 16, 4096 x 2048                  64 (8) 104 / 125, 96 (12) 132 / 126
+ *   8 of 256, 512 x 4096                  64 (2) 208 / 257, 200 (6) 327 / 359, 256 (8) 353 / 345
+ * a shared expert has every token, 16 at a time through each workgroup:
+ *   10 of 512 and one                     128 (3) 260 / 296, 256 (5) 358 / 350
+ *   8 of 256 and one                      128 (5) 322 / 331, 256 (9) 482 / 380
+ *   6 of 64 and two                       64 (8) 157 / 148, 128 (16) 231 / 157
+ * f32 outputs, whose tiles are the slower exact ones:
+ *   6 of 64                               150 (14) 172 / 246, 256 (24) 250 / 280, 512 (48) 424 / 301
+ *   10 of 512                             64 (1) 164 / 349, 512 (10) 386 / 614
+ *   2 of 16                               150 (19) 162 / 174, 256 (32) 272 / 206
+ *   10 of 512 and one                     768 (16) 584 / 675, 1000 (21) 691 / 714
+ *   8 of 256 and one                      384 (13) 576 / 649, 512 (18) 677 / 669
+ * Up to 64 tokens always, whatever the experts' number, so that such calls' sums
+ * are exact for every type. */
 bool moe_streams(const r9vx_moe_fp8_problem &p) {
-    const uint64_t rows = (uint64_t)p.t_bucket * (p.k + p.shared);
-    return p.t_bucket <= 64 || (p.y_dtype == R9VX_DTYPE_F32 && rows <= 16ull * (p.e + p.shared));
+    const uint64_t rows = (uint64_t)p.t_bucket * (p.k + p.shared), experts = p.e + p.shared;
+    if (p.t_bucket <= 64) return true;
+    if (p.y_dtype == R9VX_DTYPE_F32) return rows <= 16 * experts;
+    return rows <= 8 * experts && (p.shared == 0 || p.t_bucket <= 128);
 }
 
 Fp8MoeLayout moe_layout(const r9vx_moe_fp8_problem &p) {

@@ -49,13 +49,17 @@ def test_experts_with_more_tiles_than_a_launch_are_refused(runtime, kw):
 @pytest.mark.parametrize("kw,form", [
     (dict(t=1, e=8, k=2, dm=128, dff=128), "fp8_moe_stream_kernel<1, 2, 4, true>"), (dict(t=64, e=2, k=2, dm=128, dff=128), "fp8_moe_stream_kernel<1, 2, 4, true>"),
     (dict(t=64, e=2, k=2, dm=128, dff=128, bf16_out=True), "fp8_moe_stream_kernel<1, 2, 4, true>"),
-    (dict(t=65, e=64, k=2, dm=128, dff=128, bf16_out=True), "fp8_moe_tile_kernel<true, 256, false>"),
-    (dict(t=5, t_bucket=65, e=64, k=2, dm=128, dff=128, bf16_out=True), "fp8_moe_tile_kernel<true, 256, false>"),
+    (dict(t=65, e=16, k=2, dm=128, dff=128, bf16_out=True), "fp8_moe_tile_kernel<true, 256, false>"),
+    (dict(t=5, t_bucket=65, e=16, k=2, dm=128, dff=128, bf16_out=True), "fp8_moe_tile_kernel<true, 256, false>"),
+    (dict(t=256, e=64, k=2, dm=128, dff=128, bf16_out=True), "fp8_moe_stream_kernel<1, 2, 4, true>"),
+    (dict(t=257, e=64, k=2, dm=128, dff=128, bf16_out=True), "fp8_moe_tile_kernel<true, 256, false>"),
+    (dict(t=128, e=64, k=2, dm=128, dff=128, shared=1, bf16_out=True), "fp8_moe_stream_kernel<1, 2, 4, true>"),
+    (dict(t=129, e=64, k=2, dm=128, dff=128, shared=1, bf16_out=True), "fp8_moe_tile_kernel<true, 256, false>"),
     (dict(t=512, e=64, k=2, dm=128, dff=128), "fp8_moe_stream_kernel<1, 2, 4, true>"), (dict(t=513, e=64, k=2, dm=128, dff=128), "fp8_moe_tile_kernel<true, 128, true>"),
     (dict(t=346, e=64, k=2, dm=128, dff=128, shared=1), "fp8_moe_stream_kernel<1, 2, 4, true>"),
     (dict(t=347, e=64, k=2, dm=128, dff=128, shared=1), "fp8_moe_tile_kernel<true, 128, true>")])
 def test_the_experts_form(runtime, kw, form):
-    """Streaming up to 64 tokens, and for f32 outputs up to 16 rows an expert; f32 outputs never in the 8-bit tiles."""
+    """Streaming up to 64 tokens, and up to 8 rows an expert, 16 for f32 outputs, which never run the 8-bit tiles."""
     (rc, msg, launches), = launch_record.record(runtime, [("moe_fp8", kw)])
     assert rc == 0, msg
     assert form in [n for n, _, _ in launches]
