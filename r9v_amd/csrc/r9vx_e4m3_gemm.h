@@ -94,7 +94,7 @@ __device__ __forceinline__ void fp8_store_dense(const Fp8Args &a, uint32_t m, ui
 __device__ __forceinline__ float fp8_silu(float g) {
     const float c = fminf(fabsf(g), 256.0f);
     const float t = c * -0x1.715476p-1f;
-    const float low = fmaf(c, -0x1.715476p-1f, -t) + c * -0x1.4ae0cp-27f;
+    const float low = fmaf(c, -0x1.4ae0cp-27f, fmaf(c, -0x1.715476p-1f, -t));
     const float e = __builtin_amdgcn_exp2f(t) * fmaf(low, 0x1.62e43p-1f, 1.0f);
     return (g < 0.0f ? g * e * e : g) * __builtin_amdgcn_rcpf(fmaf(e, e, 1.0f));
 }
