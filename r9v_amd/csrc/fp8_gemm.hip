@@ -12,12 +12,14 @@
  * Three kernels, chosen by the variant's bucket and sizes, never by the launch's m:
  *   stream  up to 32 rows: every wave streams weight rows straight into
  *           registers, the waves of a workgroup split K and join their sums in
- *           LDS.  Bound by the weights' way from memory: 1 x 4096 x 4096 f32
- *           7.7 us (2.2 TB/s), 5 x 5120 x 2048 4.8 us, of which the launch is 2.
+ *           LDS.  Bound by the weights' way from memory, n / 32 workgroups of
+ *           it: 1 x 4096 x 4096 f32 7.7 us (2.2 TB/s, 128 workgroups on 256 CUs),
+ *           5 x 5120 x 2048 4.8 us, of which the launch is 2 (160 workgroups).
  *   thin    64-row tiles whose waves split K, for grids that do not fill the
- *           chip: 48 x (2 x 1408) x 2048 8.2 us, 517 x 2112 x 4096 f32 26 us
+ *           chip with large ones: 48 x (2 x 1408) x 2048 8.2 us (44 workgroups),
+ *           517 x 2112 x 4096 f32 26 us (153)
  *   tile    256 x 256 tiles staged through LDS: 2048 x 14336 x 4096 bf16
- *           141 us, 1.70 PFLOP/s (448 tiles on 256 CUs: two rounds, of which an
+ *           144 us, 1.67 PFLOP/s (448 tiles on 256 CUs: two rounds, of which an
  *           eighth is idle); the library's 8-bit product without block scales
  *           reaches 2.6 PFLOP/s at 8192 x 8192 x 8192.
  */
@@ -223,7 +225,9 @@ int r9vx_launch_matmul_fp8(const r9vx_fp8_problem &p, hipStream_t stream) {
      * weights from HBM: 2 x 1408 x 2048 9.8 / 8.0 us, 2112 x 4096 16.8 / 12.8,
      * 14336 x 4096 34.2 / 20.5, 7168 x 7168 27.0 / 30.1; two tiles, 32 rows:
      * 7.7 / 7.8, 11.9 / 11.9, 24.9 / 18.8, 20.6 / 27.3; 17 rows: 6.7 / 7.4,
-     * 9.7 / 11.0, 21.0 / 18.8, 16.7 / 25.3. */
+     * 9.7 / 11.0, 21.0 / 18.8, 16.7 / 25.3.  The line is drawn by rows alone, where
+     * most of these sizes cross; of them it costs 24.9 instead of 18.8 us (32 rows of
+     * the widest) and 30.1 instead of 27.0 (48 of the square one). */
     if (p.m_bucket <= 16) return launch_stream<1, 2, 8, kFp8Codes>(a, gated, stream);
     if (p.m_bucket <= 32) return launch_stream<2, 2, 8, kFp8Codes>(a, gated, stream);
     return p.y_dtype == R9VX_DTYPE_F32 ? launch_many<true>(a, p.m_bucket, gated, stream) : launch_many<false>(a, p.m_bucket, gated, stream);

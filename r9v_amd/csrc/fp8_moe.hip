@@ -12,11 +12,13 @@
  * of r9vx_e4m3_gemm.h.  The streaming loop and f32 outputs' tiles keep every
  * product (EXACT, r9vx_e4m3.h), bf16 outputs' tiles take the 8-bit instruction.
  *
- * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 65 us and down 35, 5.5
- * TB/s of weights (a 4 GiB copy: 4.7, reading alone up to 7).  8192 tokens, 10 of 512 experts of 2 x
- * 512 x 2048 (160 rows each): gate / up 376 us (0.91 PFLOP/s, 2.9 TB/s of
- * weights; of a tile's 68 thousand cycles 55 are products, 10 the drain), down
- * 320 us, whose K of four steps is as long as its drain, combine 63 us (5.9 TB/s).
+ * 48 tokens, 64 experts of 2 x 1408 x 2048: gate / up 65 to 75 us and down 35 to
+ * 39 by the clock, 4.8 to 5.5 TB/s of weights (a 4 GiB copy: 4.7, reading alone
+ * up to 7).  8192 tokens, 10 of 512 experts of 2 x 512 x 2048 (160 rows each),
+ * bf16 outputs: gate / up 377 us (0.91 PFLOP/s, 2.9 TB/s of weights; of a tile's
+ * 68 thousand cycles 55 are products, 10 the drain), down 317 us, whose K of four
+ * steps is as long as its drain, combine 62 us (5.9 TB/s); f32 outputs 671, 505
+ * and 127.
  */
 #include "r9vx_e4m3_gemm.h"
 #include "r9vx_moe.h"

@@ -166,7 +166,8 @@ struct Fp8StreamRegs {
  * Weights are read once and used for 16 rows: what bounds it is how many loads
  * are in flight, so every wave has two blocks' worth, nothing passes through
  * LDS on the way, and the strips are narrow (32 weight rows) to have many
- * workgroups.  64 experts' gate and up rows of 2 x 1408 x 2048: 65 us, 5.7 TB/s. */
+ * workgroups.  64 experts' gate and up rows of 2 x 1408 x 2048: 65 to 75 us, 5.7 to
+ * 4.9 TB/s. */
 template <int MT, int NT, int W, int XT, bool GATED, typename Prepare, typename Store>
 __device__ __forceinline__ void fp8_stream(const Fp8Args &a, const Fp8Rows &r, uint32_t strip, r9vx_f32x4 *part, uint8_t *rows, Prepare prepare,
                                            Store store) {
