@@ -265,10 +265,10 @@ uint64_t r9vx_moe_route_static_flops(const r9vx_moe_route_static *st, uint32_t t
  * Rows are refused one by one, where moe_route refuses the whole batch: a row
  * with a non-finite logit or bias, or whose selected scores sum to zero under
  * renormalize, gets expert ids 0xFFFFFFFF (moe_ffn_fp8 makes that token's
- * output NaN, moe_ffn refuses the call) and weights 0, and its bit is or-ed into the status word; the other rows are
- * routed.  So no launch waits for a check of all rows, and one word can gather
- * a whole step's layers: the caller clears it (zero fill) when it likes and
- * reads it with r9vx_status_read. */
+ * output NaN, moe_ffn refuses the call) and weights 0, and its bit is or-ed into
+ * the status word; the other rows are routed.  So no launch waits for a check of
+ * all rows, and one word can gather a whole step's layers: the caller clears it
+ * (zero fill) when it likes and reads it with r9vx_status_read. */
 enum r9vx_group_score { R9VX_GROUP_MAX = 0, R9VX_GROUP_TOP2 = 1 };
 
 typedef struct r9vx_moe_route_group_static {

@@ -40,7 +40,7 @@ LAUNCHES = {"quantize_fp8_kernel", "sort_small_kernel", "sort_count_kernel", "so
 
 @pytest.mark.parametrize("kw", [dict(t=1 << 16, e=32, k=32, dm=128, dff=1 << 16), dict(t=1 << 17, e=32, k=32, dm=128, dff=1 << 16, bf16_out=True)])
 def test_experts_with_more_tiles_than_a_launch_are_refused(runtime, kw):
-    """Not by the runtime, behind launches that are under way; one token fewer fits."""
+    """Not by the runtime, behind launches that are under way; half the tokens fit."""
     (rc, msg, launches), (_, _, fewer) = launch_record.record(runtime, [("moe_fp8", kw), ("moe_fp8", dict(kw, t=kw["t"] // 2))])
     assert rc == -2 and "more tiles than a launch" in msg and not launches
     assert {n.split("<")[0] for n, _, _ in fewer} <= LAUNCHES and fewer[-1][0].startswith("fp8_moe_combine_kernel")
