@@ -27,8 +27,9 @@
  * them: an error of up to 2^-10 of the sum of absolute products (about 10^-5 of
  * the result on ordinary data, a hundredth of the output's own rounding), so
  * that small products beside large ones that cancel are lost.  In moe_ffn_fp8 it
- * moves codes of h near a middle by a whole step: with 10 of 512 experts the
- * outputs are 2.5e-3 from the exact ones, of which 1.7e-3 is their rounding.
+ * moves codes of h next to a middle to the neighbour on its other side (as near
+ * to h): with 10 of 512 experts the outputs are 2.5e-3 from the definition's, of
+ * which 1.7e-3 is their rounding.
  */
 #ifndef R9VX_FP8_H_
 #define R9VX_FP8_H_
