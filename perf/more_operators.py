@@ -1,0 +1,358 @@
+"""Attention over a paged key-value cache, as cases to be timed.
+
+Between the projections of a layer a serving engine calls three operators:
+
+  rope     rotary positions of the new tokens' q and k, and k and v into the
+           cache's pages (ffi.rope_kv)
+  decode   attention of one new token of each sequence, or of a token and its
+           drafts, over the cache (ffi.attn_decode)
+  prefill  attention of packed prompts or prompt chunks over the cache
+           (ffi.attn_prefill)
+
+`run` in its plain form computes them with elementary torch operations in f32,
+the angles in f64.  `exact` is the definition in f64.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda"
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+SIZE = {"bf16": 2, "f16": 2, "f32": 4}
+
+
+# ------------------------------------------------------------------ the cases
+
+def _rope(name, t, kv, group, dim, rot, start=0, x="bf16", out="bf16", interleaved=False, stretch=1.0, page=64):
+    """t tokens of kv * group query heads, the first at position `start`."""
+    return {"name": name, "kind": "rope", "t": t, "kv": kv, "group": group, "dim": dim, "rot": rot, "start": start, "x": x, "out": out,
+            "interleaved": interleaved, "stretch": stretch, "page": page}
+
+
+def _decode(name, b, longest, kv, group, dim, new=1, shortest=None, idle=0, x="bf16", cap=0.0, bias=False, window=0, page=64):
+    """b sequences of lengths from `shortest` to `longest`, and `idle` empty places of the batch behind them."""
+    return {"name": name, "kind": "decode", "b": b, "longest": longest, "shortest": shortest or longest, "idle": idle, "kv": kv,
+            "group": group, "dim": dim, "new": new, "x": x, "cap": cap, "bias": bias, "window": window, "page": page}
+
+
+def _prefill(name, b, longest, kv, group, dim, shortest=None, before=0, x="bf16", cap=0.0, bias=False, window=0, causal=True,
+             prefix=0.0, docs=0, page=64):
+    """b prompts of `shortest` to `longest` new tokens, each onto `before` cached ones.  prefix: the share of a prompt that all of
+    it sees.  docs: tokens of a document (0: a prompt is one), which sees no other."""
+    return {"name": name, "kind": "prefill", "b": b, "longest": longest, "shortest": shortest or longest, "before": before, "kv": kv,
+            "group": group, "dim": dim, "x": x, "cap": cap, "bias": bias, "window": window, "causal": causal, "prefix": prefix,
+            "docs": docs, "page": page}
+
+
+def listed():
+    return [
+        # the next token of one sequence: wide heads, of which a quarter turns
+        _rope("rope_t1", 1, 2, 8, 256, 64, start=5119),
+        # a token and its four drafts far into a long context, f32 rows as a projection leaves them, neighbouring columns as pairs
+        _rope("rope_t5_f32", 5, 8, 4, 128, 128, start=1000003, x="f32", interleaved=True, stretch=8.0, page=16),
+        # a whole prompt
+        _rope("rope_t8192", 8192, 8, 4, 128, 128),
+        # one sequence, a short context
+        _decode("decode_b1", 1, 517, 2, 8, 256),
+        # a token and its four drafts
+        _decode("decode_drafts", 1, 8191, 2, 8, 256, new=5),
+        # concurrent sequences at every stage, small pages, capped scores, some places of the batch empty
+        _decode("decode_b48_capped", 45, 8192, 8, 4, 128, shortest=100, idle=3, x="f16", cap=50.0, page=16),
+        # small heads, each with keys of its own, a bias by distance, the last thousand tokens only
+        _decode("decode_b8_window_bias", 8, 5000, 12, 1, 64, shortest=300, bias=True, window=1024, page=32),
+        # one very long context
+        _decode("decode_long", 1, 131072, 8, 4, 128),
+        # a short prompt
+        _prefill("prefill_17", 1, 17, 2, 8, 256),
+        # a prompt chunk onto a cached beginning
+        _prefill("prefill_chunk", 1, 300, 2, 8, 256, before=4096),
+        # prompts of many lengths in one call, packed documents, a beginning that is seen as a whole, capped scores, small pages
+        _prefill("prefill_packed", 6, 2048, 4, 4, 96, shortest=130, x="f16", cap=30.0, prefix=0.1, docs=777, page=16),
+        # a whole prompt
+        _prefill("prefill_8192", 1, 8192, 8, 4, 128),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(max(lo, hi))))))
+
+
+def draw(rng):
+    kind = rng.choice(("rope", "decode", "decode", "prefill", "prefill"))
+    kv, dim, page = rng.choice((1, 2, 4, 8)), rng.choice((64, 96, 128, 192, 256)), rng.choice((8, 16, 32, 64, 128, 256))
+    case = {"kind": kind, "kv": kv, "dim": dim, "page": page}
+    if kind == "rope":
+        group = rng.randint(1, 8)
+        x = rng.choice(("bf16", "f16", "f32"))
+        most = min(8192, 8192 * 48 * 128 * 2 // ((group + 2) * kv * dim * SIZE[x]))
+        return {**case, "group": group, "t": _log(rng, 1, most), "rot": 16 * rng.randint(1, dim // 16), "x": x,
+                "out": rng.choice(("bf16", "f16")) if x == "f32" else x, "interleaved": rng.random() < 0.5,
+                "start": rng.choice((0, _log(rng, 1, 1 << 20))), "stretch": rng.choice((1.0, 4.0, 32.0))}
+    case.update({"x": rng.choice(("bf16", "f16")), "cap": rng.choice((0.0, 0.0, 30.0)), "bias": rng.random() < 0.25})
+    if kind == "decode":
+        group, new, b = rng.randint(1, 16), rng.choice((1, 1, 1, rng.randint(2, 8))), _log(rng, 1, 64)
+        longest = _log(rng, 1, min(131072, 131072 * 8 * 128 // (kv * dim * b)))
+        return {**case, "group": group, "new": new, "b": b, "longest": longest, "shortest": _log(rng, max(1, longest // 64), longest),
+                "idle": rng.choice((0, 0, rng.randint(1, 4))), "window": rng.choice((0, 0, 0, _log(rng, 64, 4096)))}
+    group, b = rng.randint(1, 8), _log(rng, 1, 16)
+    square = 8192.0 * 8192 * 32 * 128 / (b * kv * group * dim)  # pairs of one prompt, at the largest listed cost
+    longest = _log(rng, 2, min(8192, int(0.5 * math.sqrt(square))))
+    before = rng.choice((0, 0, _log(rng, 1, max(1, min(32768, int(0.5 * square / longest) - longest)))))
+    causal = rng.random() < 0.85
+    return {**case, "group": group, "b": b, "longest": longest, "shortest": _log(rng, max(1, longest // 32), longest), "before": before,
+            "causal": causal, "window": rng.choice((0, 0, 0, _log(rng, 64, 4096))),
+            "prefix": rng.choice((0.0, 0.0, rng.uniform(0.05, 0.5))) if causal else 0.0,
+            "docs": rng.choice((0, 0, 0, _log(rng, 16, 2048)))}
+
+
+def _spread(case):
+    """The sequences' lengths (decode) or new tokens (prefill), evenly over their logarithm."""
+    b, lo, hi = case["b"], case["shortest"], case["longest"]
+    return [round(hi * (lo / hi) ** (i / max(1, b - 1))) for i in range(b)]
+
+
+# ------------------------------------------------------------------ inputs
+
+def _gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def _freqs(rot, stretch):
+    """Frequencies of base 500000, stretched for a context `stretch` times the trained one: the slow ones by all of it, the fast
+    ones not at all."""
+    i = torch.arange(rot // 2, device=DEV, dtype=torch.float64)
+    f = 500000.0 ** (-2.0 * i / rot)
+    turns = 8192.0 * f / (2.0 * math.pi)
+    keep = ((turns - 1.0) / 31.0).clamp(0.0, 1.0)
+    return f * (keep + (1.0 - keep) / stretch)
+
+
+def _cache(pages, case, kind, g):
+    """Keys and values that stand in every page: an engine's pool is not cleared."""
+    shape = (pages, case["page"], case["kv"], case["dim"])
+    return tuple(torch.randn(shape, generator=g, device=DEV, dtype=torch.bfloat16).to(DTYPES[kind]) for _ in range(2))
+
+
+def prepare(case, seed):
+    g = _gen(seed)
+    st = dict(case)
+    kv, heads, dim, page = case["kv"], case["kv"] * case["group"], case["dim"], case["page"]
+    if case["kind"] == "rope":
+        t = case["t"]
+        rows = torch.randn(t, (heads + 2 * kv) * dim, generator=g, device=DEV).to(DTYPES[case["x"]])  # one projection's rows
+        q, k, v = rows.split((heads * dim, kv * dim, kv * dim), 1)
+        st["q"], st["k"], st["v"] = q.unflatten(1, (heads, dim)), k.unflatten(1, (kv, dim)), v.unflatten(1, (kv, dim))
+        st["positions"] = torch.arange(case["start"], case["start"] + t, device=DEV, dtype=torch.int32)
+        st["freqs"] = _freqs(case["rot"], case["stretch"])
+        st["amplitude"] = 1.0 + 0.1 * math.log(case["stretch"])
+        pages = -(-t // page) + 3
+        st["k_cache"], st["v_cache"] = _cache(pages, case, case["out"], g)
+        at = torch.arange(t, device=DEV) + case["start"] % page  # the first token's place in its page
+        st["slots"] = torch.randperm(pages, generator=g, device=DEV)[at // page] * page + at % page
+        return st
+    sizes = torch.tensor(_spread(case), device=DEV, dtype=torch.int32)[torch.randperm(case["b"], generator=g, device=DEV)]
+    if case["kind"] == "decode":
+        sizes = torch.cat((sizes, sizes.new_zeros(case["idle"])))
+        lengths, most = sizes, case["longest"]
+        q = (len(sizes), case["new"], heads, dim)
+    else:
+        lengths, most = sizes + case["before"], case["longest"] + case["before"]
+        q = (sum(_spread(case)), heads, dim)
+        st["offsets"] = torch.cat((sizes.new_zeros(1), sizes.cumsum(0, dtype=torch.int32)))
+        place = torch.arange(q[0], device=DEV, dtype=torch.int32) - st["offsets"][:-1].repeat_interleave(sizes)
+        st["starts"] = case["before"] + place - place % case["docs"] if case["docs"] else None
+        st["prefix"] = (lengths * case["prefix"]).int() if case["prefix"] else None
+    per = -(-most // page)
+    pages = len(sizes) * per + 1
+    st["lengths"] = lengths
+    st["table"] = torch.randperm(pages, generator=g, device=DEV)[:len(sizes) * per].view(-1, per).int()
+    st["k_cache"], st["v_cache"] = _cache(pages, case, case["x"], g)
+    # a query and its keys agree more than strangers do: scores of standard deviation 1.5
+    st["q"] = (1.5 * torch.randn(q, generator=g, device=DEV)).to(DTYPES[case["x"]])
+    st["slopes"] = 2.0 ** (-8.0 * torch.arange(1, heads + 1, device=DEV) / heads) if case["bias"] else None
+    return st
+
+
+# ------------------------------------------------------------------ the plain form
+
+def _rope_plain(st):
+    half = st["rot"] // 2
+    angle = st["positions"].double()[:, None] * st["freqs"]
+    c, s = ((st["amplitude"] * f(angle)).float()[:, None, :] for f in (torch.cos, torch.sin))
+
+    def turned(x):
+        x = x.float()
+        r = x[:, :, :st["rot"]]
+        a, b = (r[:, :, 0::2], r[:, :, 1::2]) if st["interleaved"] else (r[:, :, :half], r[:, :, half:])
+        a, b = a * c - b * s, a * s + b * c
+        r = torch.stack((a, b), 3).flatten(2) if st["interleaved"] else torch.cat((a, b), 2)
+        return torch.cat((r, x[:, :, st["rot"]:]), 2)
+
+    out = DTYPES[st["out"]]
+    at = (st["slots"] // st["page"], st["slots"] % st["page"])
+    st["k_cache"].index_put_(at, turned(st["k"]).to(out))
+    st["v_cache"].index_put_(at, st["v"].to(out))
+    return turned(st["q"]).to(out), st["k_cache"], st["v_cache"]
+
+
+def _attend(st, q, new, starts, prefix, causal):
+    """q [b, n, heads, dim] f32, of which sequence i has new[i] rows, over the cache: the same shape."""
+    b, n, heads, dim = q.shape
+    kv, group, lengths = st["kv"], st["group"], st["lengths"]
+
+    def gathered(cache):  # [b, kv, length, dim]
+        return cache[st["table"].long()].float().view(b, -1, kv, dim).transpose(1, 2).contiguous()
+
+    k, v = gathered(st["k_cache"]), gathered(st["v_cache"])
+    j = torch.arange(k.shape[2], device=q.device)
+    p = (lengths - new)[:, None] + torch.arange(n, device=q.device)
+    least = torch.zeros_like(p) if starts is None else starts
+    if st["window"]:
+        least = torch.maximum(least, p - st["window"] + 1)
+    last = lengths[:, None].expand(b, n)
+    if causal:
+        last = torch.minimum(last, p + 1 if prefix is None else torch.maximum(p + 1, prefix[:, None]))
+    seen = ((j >= least[:, :, None]) & (j < last[:, :, None]))[:, None, None]  # [b, 1, 1, n, length]
+    rows = q.view(b, n, kv, group, dim).permute(0, 2, 3, 1, 4).reshape(b, kv, group * n, dim)
+    s = torch.matmul(rows, k.transpose(2, 3).contiguous()) * dim ** -0.5
+    if st["cap"]:
+        s = st["cap"] * torch.tanh(s / st["cap"])
+    s = s.view(b, kv, group, n, -1)
+    if st["slopes"] is not None:
+        s = s - st["slopes"].view(kv, group, 1, 1) * (p[:, :, None] - j).abs()[:, None, None]
+    s = torch.where(seen, s, -math.inf)
+    top = s.amax(4, keepdim=True)
+    e = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
+    total = e.sum(4, keepdim=True)
+    e = e / torch.where(total == 0.0, 1.0, total)
+    o = torch.matmul(e.view(b, kv, group * n, -1), v)
+    return o.view(b, kv, group, n, dim).permute(0, 3, 1, 2, 4).reshape(b, n, heads, dim)
+
+
+def _prefill_plain(st):
+    lengths, offsets = st["lengths"], st["offsets"]
+    new = offsets[1:] - offsets[:-1]
+    row = torch.arange(st["longest"], device=DEV)
+    packed = (offsets[:-1, None] + torch.minimum(row, new[:, None] - 1)).long()  # a short prompt repeats its last row
+    starts = None if st["starts"] is None else st["starts"][packed]
+    o = _attend(st, st["q"][packed].float(), new, starts, st["prefix"], st["causal"])
+    token = torch.arange(st["q"].shape[0], device=DEV)
+    owner = torch.bucketize(token, offsets[1:], right=True)
+    return o[owner, token - offsets[owner]].to(st["q"].dtype)
+
+
+def run(state):
+    kind = state["kind"]
+    if own:
+        from r9v_amd import ffi
+
+        if kind == "rope":
+            q = ffi.rope_kv(state["q"], state["k"], state["v"], state["positions"], state["freqs"], state["k_cache"], state["v_cache"],
+                            state["slots"], interleaved=state["interleaved"], amplitude=state["amplitude"])
+            return q, state["k_cache"], state["v_cache"]
+        if kind == "decode":
+            return ffi.attn_decode(state["q"], state["k_cache"], state["v_cache"], state["table"], state["lengths"], softcap=state["cap"],
+                                   slopes=state["slopes"], window=state["window"])
+        return ffi.attn_prefill(state["q"], state["k_cache"], state["v_cache"], state["table"], state["lengths"], state["offsets"],
+                                softcap=state["cap"], slopes=state["slopes"], window=state["window"], causal=state["causal"],
+                                prefix=state["prefix"], starts=state["starts"])
+    if kind == "rope":
+        return _rope_plain(state)
+    if kind == "decode":
+        return _attend(state, state["q"].float(), torch.full_like(state["lengths"], state["new"]), None, None, True).to(state["q"].dtype)
+    return _prefill_plain(state)
+
+
+# ------------------------------------------------------------------ what a pass cannot do without
+
+def work(case):
+    kv, heads, dim = case["kv"], case["kv"] * case["group"], case["dim"]
+    if case["kind"] == "rope":
+        n = case["t"] * (heads + 2 * kv) * dim
+        return {"bytes": n * (SIZE[case["x"]] + SIZE[case["out"]]) + case["t"] * 12 + case["rot"] * 4, "flops": 3 * case["t"] * (heads + kv) * case["rot"]}
+    size, window = SIZE[case["x"]], case["window"]
+    if case["kind"] == "decode":
+        n = case["new"]
+        keys = sum(min(x, window + n - 1) if window else x for x in _spread(case))
+        pairs = sum(min(x - n + 1 + i, window or x) for x in _spread(case) for i in range(n) if x - n + 1 + i > 0)
+        rows = (case["b"] + case["idle"]) * n
+        return {"bytes": 2 * size * (keys * kv + rows * heads) * dim + 4 * (keys // case["page"] + rows), "flops": 4 * pairs * heads * dim}
+    keys = pairs = rows = 0
+    for new in _spread(case):
+        length, first = case["before"] + new, case["before"] + new
+        prefix = int(length * case["prefix"])
+        for i in range(new):
+            p = case["before"] + i
+            lo = max(p - window + 1 if window else 0, p - i % case["docs"] if case["docs"] else 0, 0)
+            hi = min(length, max(p + 1, prefix)) if case["causal"] else length
+            pairs += max(0, hi - lo)
+            first = min(first, lo)
+        keys += length - first
+        rows += new
+    return {"bytes": 2 * size * (keys * kv + rows * heads) * dim + 4 * (keys // case["page"] + 2 * case["b"]), "flops": 4 * pairs * heads * dim}
+
+
+# ------------------------------------------------------------------ the definition in 64 bits
+
+def _exact_rope(st):
+    rot = st["rot"]
+    z = torch.polar(torch.full((st["t"], rot // 2), st["amplitude"], device=DEV, dtype=torch.float64),
+                    st["positions"].double()[:, None] * st["freqs"])[:, None, :]
+
+    def turned(x):
+        y = x.double().clone()
+        first, second = (slice(0, rot, 2), slice(1, rot, 2)) if st["interleaved"] else (slice(0, rot // 2), slice(rot // 2, rot))
+        w = torch.complex(y[:, :, first].clone(), y[:, :, second].clone()) * z
+        y[:, :, first], y[:, :, second] = w.real, w.imag
+        return y
+
+    k, v = (c.double().flatten(0, 1) for c in (st["k_cache"], st["v_cache"]))
+    k[st["slots"]], v[st["slots"]] = turned(st["k"]), st["v"].double()
+    return turned(st["q"]), k.view(st["k_cache"].shape), v.view(st["v_cache"].shape)
+
+
+def _exact_sequence(st, b, q, starts, prefix, causal):
+    """The new tokens q [n, heads, dim] of sequence b in f64, a head at a time."""
+    n, heads, dim = q.shape
+    length = int(st["lengths"][b])
+    o = torch.zeros(n, heads, dim, dtype=torch.float64, device=DEV)
+    if length == 0 or n == 0:
+        return o
+    token = torch.arange(length, device=DEV)
+    at = (st["table"][b].long()[token // st["page"]], token % st["page"])
+    p = length - n + torch.arange(n, device=DEV)[:, None]
+    seen = (token <= p) | (token < prefix) if causal else torch.ones(n, length, dtype=torch.bool, device=DEV)
+    if st["window"]:
+        seen &= p - token < st["window"]
+    if starts is not None:
+        seen &= token >= starts[:, None]
+    some = seen.any(1)
+    for h in range(heads):
+        k, v = (st[c][at[0], at[1], h // st["group"]].double() for c in ("k_cache", "v_cache"))
+        s = q[:, h].double() @ k.T / math.sqrt(dim)
+        if st["cap"]:
+            s = st["cap"] * torch.tanh(s / st["cap"])
+        if st["slopes"] is not None:
+            s -= st["slopes"][h].double() * (p - token).abs()
+        s[~seen] = -math.inf
+        o[some, h] = torch.softmax(s[some], 1) @ v
+    return o
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    if case["kind"] == "rope":
+        return _exact_rope(st)
+    if case["kind"] == "decode":
+        return torch.stack([_exact_sequence(st, b, q, None, 0, True) for b, q in enumerate(st["q"])])
+    offsets, out = st["offsets"].tolist(), []
+    for b, (lo, hi) in enumerate(zip(offsets, offsets[1:])):
+        out.append(_exact_sequence(st, b, st["q"][lo:hi], None if st["starts"] is None else st["starts"][lo:hi],
+                                   0 if st["prefix"] is None else int(st["prefix"][b]), case["causal"]))
+    return torch.cat(out)
