@@ -3,11 +3,11 @@
 Between the projections of a layer a serving engine calls three operators:
 
   rope     rotary positions of the new tokens' q and k, and k and v into the
-           cache's pages (ffi.rope_kv)
+           cache's pages (attn.rope_kv)
   decode   attention of one new token of each sequence, or of a token and its
-           drafts, over the cache (ffi.attn_decode)
+           drafts, over the cache (attn.decode)
   prefill  attention of packed prompts or prompt chunks over the cache
-           (ffi.attn_prefill)
+           (attn.prefill)
 
 `run` in its plain form computes them with elementary torch operations in f32,
 the angles in f64.  `exact` is the definition in f64.
@@ -250,18 +250,18 @@ def _prefill_plain(st):
 def run(state):
     kind = state["kind"]
     if own:
-        from r9v_amd import ffi
+        from r9v_amd import attn
 
         if kind == "rope":
-            q = ffi.rope_kv(state["q"], state["k"], state["v"], state["positions"], state["freqs"], state["k_cache"], state["v_cache"],
-                            state["slots"], interleaved=state["interleaved"], amplitude=state["amplitude"])
+            q = attn.rope_kv(state["q"], state["k"], state["v"], state["positions"], state["freqs"], state["k_cache"], state["v_cache"],
+                             state["slots"], interleaved=state["interleaved"], amplitude=state["amplitude"])
             return q, state["k_cache"], state["v_cache"]
         if kind == "decode":
-            return ffi.attn_decode(state["q"], state["k_cache"], state["v_cache"], state["table"], state["lengths"], softcap=state["cap"],
-                                   slopes=state["slopes"], window=state["window"])
-        return ffi.attn_prefill(state["q"], state["k_cache"], state["v_cache"], state["table"], state["lengths"], state["offsets"],
-                                softcap=state["cap"], slopes=state["slopes"], window=state["window"], causal=state["causal"],
-                                prefix=state["prefix"], starts=state["starts"])
+            return attn.decode(state["q"], state["k_cache"], state["v_cache"], state["table"], state["lengths"], softcap=state["cap"],
+                               slopes=state["slopes"], window=state["window"])
+        return attn.prefill(state["q"], state["k_cache"], state["v_cache"], state["table"], state["lengths"], state["offsets"],
+                            softcap=state["cap"], slopes=state["slopes"], window=state["window"], causal=state["causal"],
+                            prefix=state["prefix"], starts=state["starts"])
     if kind == "rope":
         return _rope_plain(state)
     if kind == "decode":
