@@ -1,0 +1,476 @@
+/*
+ * attn_decode.hip -- attention of the next 1 to 8 tokens of each sequence over
+ * the paged cache.
+ *
+ * A workgroup of four waves takes a sequence, a kv head, 16 or 32 of the rows
+ * that share it (tokens x query heads of the group) and a part of the keys; the
+ * waves take blocks of 32 keys in turn, each with a softmax of its own (running
+ * maximum and sum), and are joined through LDS; parts are joined by a further
+ * launch (r9vx_launch_attn_join).
+ *
+ * Scores are taken transposed, S^T = K Q^T by 16 x 16 x 32 products, with a
+ * block's keys dealt to the two tiles so that what a lane holds of S^T, 8
+ * neighbouring keys of one row, is what the second product O^T = V^T P^T
+ * takes from it: probabilities never leave their lane.  Values are loaded as they
+ * stand, a lane 8 keys x head_dim / 16 columns, and turned in registers
+ * (half a v_perm an element).  Nothing but the joins goes through LDS.
+ *
+ * Bound by the keys' and values' bytes: a wave keeps a block's keys or values on
+ * their way while it works on the others.
+ */
+#include "r9vx_attn_kernels.h"
+
+using namespace r9vx;
+
+namespace {
+
+constexpr int kBlock = 32; /* keys of a wave's step */
+constexpr int kWaves = 4;
+
+template <int D>
+struct DecodeShape {
+    static constexpr int VC = D > 128 ? 2 : 1;   /* column pieces of a value row */
+    static constexpr int CW = D / VC;            /* columns of a piece */
+    static constexpr int DL = CW / 16;           /* of them a lane's: 4, 6 or 8 */
+    static constexpr int DW = DL / 2;            /* in words */
+    static constexpr int KS = D / 32;            /* steps of a score's product */
+};
+
+template <int DW>
+__device__ __forceinline__ void load_words(const uint16_t *p, uint32_t (&w)[DW]) {
+    static_assert(DW >= 2 && DW <= 4);
+    if constexpr (DW == 2) {
+        const r9vx_u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const r9vx_u32x2 *>(p));
+        w[0] = v.x, w[1] = v.y;
+    } else if constexpr (DW == 3) { /* 12 bytes: dword alignment */
+        typedef attn_u32x3 vec __attribute__((aligned(4)));
+        const attn_u32x3 v = *reinterpret_cast<const vec *>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z;
+    } else {
+        const r9vx_u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const r9vx_u32x4 *>(p));
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
+}
+
+template <class T, int D, int RT>
+__global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_problem a, uint32_t row_tiles) {
+    using S = DecodeShape<D>;
+    typedef typename T::x8 x8;
+    __shared__ float jm[kWaves][RT * 16], jl[kWaves][RT * 16];
+    __shared__ float jo[2][16][D + 4]; /* two waves' sums of 16 rows */
+    __shared__ uint32_t redo;
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int col = lane & 15, g4 = lane >> 4;
+    uint32_t id = blockIdx.x;
+    const uint32_t split = id % a.splits;
+    id /= a.splits;
+    const uint32_t tile = id % row_tiles;
+    id /= row_tiles;
+    const uint32_t kvh = id % a.kv_heads, b = id / a.kv_heads;
+    const int rows = (int)(a.t_bucket * a.group);
+    const int row0 = (int)tile * RT * 16;
+    const int length = a.lengths[b];
+    const bool bad_length = length < 0 || length > (int)a.len_bucket;
+    if (bad_length && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
+
+    /* a lane's row of each tile */
+    const int start = a.starts ? a.starts[b] : 0;
+    int lo[RT], hi[RT], pos[RT], token[RT];
+    float slope[RT];
+    x8 q[RT][S::KS];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = row0 + r * 16 + col;
+        token[r] = row / (int)a.group;
+        const uint32_t h = kvh * a.group + (row - token[r] * (int)a.group);
+        pos[r] = length - (int)a.t_bucket + token[r];
+        attn_seen(a.window, a.causal, pos[r], length, start, 0, lo[r], hi[r]);
+        const bool there = row < rows && !bad_length;
+        if (!there) lo[r] = hi[r] = 0;
+        slope[r] = a.slopes && row < rows ? a.slopes[h] * kLog2e : 0.0f;
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) {
+            q[r][s] = x8{};
+            if (there) q[r][s] = *reinterpret_cast<const x8 *>(a.q + b * a.q_stride[0] + token[r] * a.q_stride[1] + h * a.q_stride[2] + s * 32 + g4 * 8);
+        }
+    }
+    const int first = row0 / (int)a.group, last = ((row0 + RT * 16 < rows ? row0 + RT * 16 : rows) - 1) / (int)a.group; /* tokens */
+    /* keys that some row sees, and those that all of them do */
+    int ulo, uhi, flo, fhi;
+    attn_seen(a.window, a.causal, length - (int)a.t_bucket + first, length, start, 0, ulo, fhi);
+    attn_seen(a.window, a.causal, length - (int)a.t_bucket + last, length, start, 0, flo, uhi);
+    if (bad_length) uhi = ulo = 0;
+
+    const AttnScore score(a);
+    const uint16_t *kbase = a.k + kvh * a.k_stride[2], *vbase = a.v + kvh * a.v_stride[2];
+    const int32_t *table = a.table + b * a.table_stride;
+    const uint32_t mask = (1u << a.page_shift) - 1;
+
+    /* this part's blocks */
+    const int b0 = ulo / kBlock, b1 = uhi > ulo ? (uhi + kBlock - 1) / kBlock : b0;
+    int begin, end;
+    attn_part(b0, b1, kWaves, (int)a.splits, (int)split, begin, end);
+
+    float m[RT], l[RT];
+    r9vx_f32x4 o[RT][S::VC][S::DL];
+
+    /* Keys [vlo, vhi) have values; a second pass for each token follows only where
+     * the first gave a NaN or an infinity, which a key that another token alone
+     * sees may have brought in through a probability of zero. */
+    int vlo = ulo, vhi = uhi;
+    for (int pass = -1; pass < (int)a.t_bucket; ++pass) {
+        if (pass >= 0) {
+            if (pass < first || pass > last) continue;
+            attn_seen(a.window, a.causal, length - (int)a.t_bucket + pass, length, start, 0, vlo, vhi);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            m[r] = -INFINITY, l[r] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                for (int j = 0; j < S::DL; ++j) o[r][c][j] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
+        const int kgroup = 8 * (col >> 2); /* the eight keys this lane's key rows are among */
+        auto page_of = [&](int key) -> uint32_t { return key < uhi ? (uint32_t)table[key >> a.page_shift] : 0u; };
+        x8 k[2][S::KS];
+        uint32_t v[8][S::VC][S::DW];
+        auto load_k = [&](int key0, uint32_t page) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int key = key0 + kgroup + 4 * t + (col & 3);
+                const uint16_t *p = attn_row<T>(attn_place(page, a.pages, key, ulo, uhi), kbase, a.k_stride, page, (uint32_t)key & mask);
+#pragma unroll
+                for (int s = 0; s < S::KS; ++s) k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const x8 *>(p + s * 32 + g4 * 8));
+            }
+        };
+        auto load_v = [&](int key0, uint32_t page) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = key0 + 8 * g4 + i;
+                const uint16_t *p = attn_row<T>(attn_place(page, a.pages, key, vlo, vhi), vbase, a.v_stride, page, (uint32_t)key & mask);
+#pragma unroll
+                for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW + S::DL * col, v[i][c]);
+            }
+        };
+
+        int blk = begin + wave;
+        uint32_t kpage = 0, vpage = 0;
+        if (blk < end) {
+            kpage = page_of(blk * kBlock + kgroup);
+            vpage = page_of(blk * kBlock + 8 * g4);
+            load_k(blk * kBlock, kpage);
+        }
+        for (; blk < end; blk += kWaves) {
+            const int key0 = blk * kBlock;
+            load_v(key0, vpage);
+            if (vpage >= a.pages && a.status) { /* of keys that are seen: page 0 stands for the others */
+                if (key0 + 8 * g4 + 7 >= ulo) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+            }
+            const int next = key0 + kWaves * kBlock;
+            const bool more = blk + kWaves < end;
+            if (more) {
+                kpage = page_of(next + kgroup);
+                vpage = page_of(next + 8 * g4);
+            }
+            r9vx_f32x4 sc[RT][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    sc[r][t] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < S::KS; ++s) sc[r][t] = T::mma16(k[t][s], q[r][s], sc[r][t]);
+                }
+            if (more) load_k(next, kpage);
+            const bool edge = key0 < flo || key0 + kBlock > fhi;
+            x8 ph[RT], pl[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = sc[r][e >> 2][e & 3];
+                if (a.softcap > 0.0f) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = score.capped(x[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] *= score.factor;
+                }
+                const int k8 = key0 + 8 * g4;
+                if (a.slopes) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int d = pos[r] - (k8 + e);
+                        x[e] = fmaf(-slope[r], (float)(d < 0 ? -d : d), x[e]);
+                    }
+                }
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (k8 + e < lo[r] || k8 + e >= hi[r]) x[e] = -INFINITY;
+                }
+                float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                top = fmaxf(top, __shfl_xor(top, 16, R9VX_WAVE));
+                top = fmaxf(top, __shfl_xor(top, 32, R9VX_WAVE));
+                if (__any(top > m[r])) {
+                    const float now = fmaxf(m[r], top);
+                    const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - now);
+                    m[r] = now;
+                    l[r] *= f;
+#pragma unroll
+                    for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                        for (int j = 0; j < S::DL; ++j) o[r][c][j] *= f;
+                }
+                const float ref = (m[r] == -INFINITY ? 0.0f : m[r]) - T::kBits;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float pe = __builtin_amdgcn_exp2f(x[e] - ref);
+                    l[r] += pe;
+                    ph[r][e] = (typename T::elem)pe;
+                    if constexpr (T::kBits == 0.0f) pl[r][e] = (typename T::elem)(pe - (float)ph[r][e]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                for (int j = 0; j < S::DL; ++j) {
+                    r9vx_u32x4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = __builtin_amdgcn_perm(v[2 * i + 1][c][j >> 1], v[2 * i][c][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+                    const x8 vt = __builtin_bit_cast(x8, w);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        o[r][c][j] = T::mma16(vt, ph[r], o[r][c][j]);
+                        if constexpr (T::kBits == 0.0f) o[r][c][j] = T::mma16(vt, pl[r], o[r][c][j]);
+                    }
+                }
+        }
+
+        /* the waves' sums: 2 and 3 to 0 and 1, then 1 to 0 */
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            l[r] += __shfl_xor(l[r], 16, R9VX_WAVE);
+            l[r] += __shfl_xor(l[r], 32, R9VX_WAVE);
+            if (lane < 16) jm[wave][r * 16 + col] = m[r], jl[wave][r * 16 + col] = l[r];
+        }
+        if (pass < 0 && threadIdx.x == 0) redo = 0;
+        __syncthreads();
+        bool odd = false; /* a value that is not finite */
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float all = -INFINITY, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) all = fmaxf(all, jm[w][r * 16 + col]);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float mw = jm[w][r * 16 + col];
+                /* a wave that saw nothing (or scores of -infinity alone) has no part; its sum is zero, unless NaN scores made it one */
+                sum += jl[w][r * 16 + col] * (mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - all));
+            }
+            const float f = m[r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - all);
+#pragma unroll
+            for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                for (int j = 0; j < S::DL; ++j) o[r][c][j] *= f;
+#pragma unroll
+            for (int half = 2; half >= 1; half >>= 1) {
+                if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                    for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                        for (int j = 0; j < S::DL; ++j) *reinterpret_cast<r9vx_f32x4 *>(&jo[wave - half][col][((c * S::DL + j) * 4 + g4) * 4]) = o[r][c][j];
+                }
+                __syncthreads();
+                if (wave < half) {
+#pragma unroll
+                    for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                        for (int j = 0; j < S::DL; ++j) o[r][c][j] += *reinterpret_cast<const r9vx_f32x4 *>(&jo[wave][col][((c * S::DL + j) * 4 + g4) * 4]);
+                }
+                __syncthreads();
+            }
+            m[r] = all, l[r] = sum;
+            if (wave == 0) {
+                odd |= !(fabsf(sum) < INFINITY);
+#pragma unroll
+                for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < S::DL; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) odd |= !(fabsf(o[r][c][j][e]) < INFINITY);
+            }
+        }
+        if (pass < 0 && first != last) {
+            if (wave == 0 && __any(odd) && lane == 0) redo = 1;
+            __syncthreads();
+            if (redo) continue; /* the tokens one by one */
+        }
+        if (wave == 0) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const int row = row0 + r * 16 + col;
+                if (row >= rows || (pass >= 0 && token[r] != pass)) continue;
+                const uint32_t h = kvh * a.group + (row - token[r] * (int)a.group);
+                /* scores of -infinity alone are no softmax; no score at all is zeros */
+                float sum = l[r], top = m[r];
+                if (bad_length || (sum != sum && top == -INFINITY)) top = 0.0f; /* a NaN that counts beside any other part */
+                if (bad_length || (sum == 0.0f && top == -INFINITY && (lo[r] > begin * kBlock ? lo[r] : begin * kBlock) < (hi[r] < end * kBlock ? hi[r] : end * kBlock)))
+                    sum = __builtin_nanf("");
+                if (a.splits == 1) {
+                    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    uint16_t *y = a.out + b * a.out_stride[0] + token[r] * a.out_stride[1] + h * a.out_stride[2];
+#pragma unroll
+                    for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int j = 0; j < S::DL; j += 2) {
+                                typedef typename T::elem pair __attribute__((ext_vector_type(2)));
+                                const pair w = {(typename T::elem)(o[r][c][j][e] * f), (typename T::elem)(o[r][c][j + 1][e] * f)};
+                                *reinterpret_cast<pair *>(y + c * S::CW + S::DL * (4 * g4 + e) + j) = w;
+                            }
+                } else {
+                    const uint64_t at = (((uint64_t)b * a.t_bucket + token[r]) * a.heads + h) * a.splits + split;
+                    float *y = a.partial + at * D;
+#pragma unroll
+                    for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int j = 0; j < S::DL; j += 2)
+                                *reinterpret_cast<float2 *>(y + c * S::CW + S::DL * (4 * g4 + e) + j) = make_float2(o[r][c][j][e], o[r][c][j + 1][e]);
+                    if (g4 == 0) {
+                        float2 *ml = reinterpret_cast<float2 *>(a.partial + (uint64_t)a.b_bucket * a.t_bucket * a.heads * a.splits * D);
+                        ml[at] = make_float2(top, sum);
+                    }
+                }
+            }
+        }
+        if (pass < 0) break;
+    }
+}
+
+/* A row's parts: a wave, its lanes over the columns.  Bound by a launch and the
+ * parts' bytes, head_dim f32 each. */
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, uint64_t rows, const float2 *ml) {
+    const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t tok = row / a.heads;
+    const uint32_t h = (uint32_t)(row - tok * a.heads);
+    uint64_t seq = 0, t = tok;
+    if (a.offsets) { /* prefill: rows of no sequence are left */
+        if ((int64_t)tok < a.offsets[0] || (int64_t)tok >= a.offsets[a.b]) return;
+    } else {
+        seq = tok / a.t_bucket;
+        t = tok - seq * a.t_bucket;
+    }
+    const uint64_t at = row * a.splits;
+    float m = -INFINITY, sum = 0.0f;
+    for (uint32_t s = lane; s < a.splits; s += 64) {
+        const float2 x = ml[at + s];
+        const float now = fmaxf(m, x.x);
+        /* beside parts that saw something, one of -infinity alone has no weight, but a NaN sum that NaN scores made has */
+        sum = (m == -INFINITY ? 0.0f : sum * __builtin_amdgcn_exp2f(m - now)) + (x.x == -INFINITY ? 0.0f : x.y * __builtin_amdgcn_exp2f(x.x - now));
+        m = now;
+    }
+    for (int off = 1; off < 64; off <<= 1) {
+        const float om = __shfl_xor(m, off, R9VX_WAVE), os = __shfl_xor(sum, off, R9VX_WAVE);
+        const float now = fmaxf(m, om);
+        sum = (m == -INFINITY ? 0.0f : sum * __builtin_amdgcn_exp2f(m - now)) + (om == -INFINITY ? 0.0f : os * __builtin_amdgcn_exp2f(om - now));
+        m = now;
+    }
+    bool none = m == -INFINITY;
+    if (none) { /* zeros, or NaN where a part saw scores of -infinity */
+        bool odd = false;
+        for (uint32_t s = lane; s < a.splits; s += 64) odd |= ml[at + s].y != 0.0f;
+        sum = __any(odd) ? __builtin_nanf("") : 0.0f;
+    }
+    const float f = none ? sum : 1.0f / sum; /* NaN or 0 where there is nothing */
+    uint16_t *y = a.out + seq * a.out_stride[0] + t * a.out_stride[1] + h * a.out_stride[2];
+    for (uint32_t c = lane * 2; c < a.head_dim; c += 128) {
+        float x0 = 0.0f, x1 = 0.0f;
+        if (!none) {
+            for (uint32_t s = 0; s < a.splits; ++s) {
+                const float mw = ml[at + s].x;
+                if (mw == -INFINITY) continue;
+                const float w = __builtin_amdgcn_exp2f(mw - m);
+                const float2 v = *reinterpret_cast<const float2 *>(a.partial + (at + s) * a.head_dim + c);
+                x0 = fmaf(w, v.x, x0), x1 = fmaf(w, v.y, x1);
+            }
+        }
+        typedef typename T::elem pair __attribute__((ext_vector_type(2)));
+        const pair w = {(typename T::elem)(none ? f : x0 * f), (typename T::elem)(none ? f : x1 * f)};
+        *reinterpret_cast<pair *>(y + c) = w;
+    }
+}
+
+uint32_t decode_row_tiles(const r9vx_attn_problem &p, uint32_t &rt) {
+    const uint32_t rows = p.t_bucket * p.group;
+    rt = rows > 16 && p.head_dim <= 128 ? 2 : 1;
+    return (rows + 16 * rt - 1) / (16 * rt);
+}
+
+template <class T, int D>
+int launch_decode(const r9vx_attn_problem &p, hipStream_t stream) {
+    uint32_t rt;
+    const uint32_t tiles = decode_row_tiles(p, rt);
+    const dim3 grid((unsigned)r9vx_attn_decode_groups(p));
+    if constexpr (D <= 128) {
+        if (rt == 2) {
+            hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+            return (int)hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+    return (int)hipGetLastError();
+}
+
+template <class T>
+int launch_decode_type(const r9vx_attn_problem &p, hipStream_t stream) {
+    switch (p.head_dim) {
+    case 64: return launch_decode<T, 64>(p, stream);
+    case 96: return launch_decode<T, 96>(p, stream);
+    case 128: return launch_decode<T, 128>(p, stream);
+    case 192: return launch_decode<T, 192>(p, stream);
+    default: return launch_decode<T, 256>(p, stream);
+    }
+}
+
+}  // namespace
+
+uint64_t r9vx_attn_decode_groups(const r9vx_attn_problem &p) {
+    uint32_t rt;
+    return (uint64_t)p.b * p.kv_heads * decode_row_tiles(p, rt) * p.splits;
+}
+
+uint32_t r9vx_attn_decode_splits(const r9vx_attn_problem &p) {
+    uint32_t rt;
+    const uint64_t groups = (uint64_t)p.b_bucket * p.kv_heads * decode_row_tiles(p, rt);
+    const uint64_t fill = 3ull * r9vx_device_cus();
+    const uint64_t most = ((uint64_t)p.len_bucket + kWaves * kBlock - 1) / (kWaves * kBlock);
+    uint64_t s = groups ? fill / groups : 1;
+    if (s > most) s = most;
+    if (s > 256) s = 256;
+    return s > 1 ? (uint32_t)s : 1u;
+}
+
+int r9vx_launch_attn_join(const r9vx_attn_problem &p, uint64_t rows, hipStream_t stream) {
+    const float2 *ml = reinterpret_cast<const float2 *>(p.partial + (p.offsets ? (uint64_t)p.t_bucket : (uint64_t)p.b_bucket * p.t_bucket) * p.heads * p.splits * p.head_dim);
+    const dim3 grid((unsigned)((rows + 3) / 4));
+    if (p.dtype == R9VX_DTYPE_BF16) hipLaunchKernelGGL(attn_join_kernel<AttnBf16>, grid, dim3(256), 0, stream, p, rows, ml);
+    else hipLaunchKernelGGL(attn_join_kernel<AttnF16>, grid, dim3(256), 0, stream, p, rows, ml);
+    return (int)hipGetLastError();
+}
+
+int r9vx_launch_attn_decode(const r9vx_attn_problem &p, hipStream_t stream) {
+    const int rc = p.dtype == R9VX_DTYPE_BF16 ? launch_decode_type<AttnBf16>(p, stream) : launch_decode_type<AttnF16>(p, stream);
+    if (rc || p.splits == 1) return rc;
+    return r9vx_launch_attn_join(p, (uint64_t)p.b * p.t_bucket * p.heads, stream);
+}

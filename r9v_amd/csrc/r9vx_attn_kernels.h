@@ -1,0 +1,124 @@
+/*
+ * r9vx_attn_kernels.h -- what the attention kernels share: the problem as the
+ * launchers take it, the two element types, the score and its mask.
+ */
+#ifndef R9VX_ATTN_KERNELS_H
+#define R9VX_ATTN_KERNELS_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "r9vx_attn.h"
+#include "r9vx_attn_index.h"
+#include "r9vx_device.h"
+#include "r9vx_internal.h"
+
+struct r9vx_rope_problem {
+    const void *q, *k, *v;
+    const int32_t *positions;
+    const double *freqs;
+    void *q_out, *k_cache, *v_cache;
+    const int64_t *slots;
+    uint32_t *status;
+    uint64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2], k_cache_stride[3], v_cache_stride[3];
+    uint32_t pages, t, heads, kv_heads, head_dim, rot, interleaved, page_shift, in_dtype, out_dtype;
+    float amplitude;
+};
+int r9vx_launch_rope_kv(const r9vx_rope_problem &p, hipStream_t stream);
+
+struct r9vx_attn_problem {
+    const uint16_t *q, *k, *v;
+    const int32_t *table, *lengths, *offsets, *starts, *prefix;
+    const float *slopes;
+    uint16_t *out;
+    float *partial;   /* f32 [rows][splits][head_dim], then (m, l) [rows][splits] */
+    uint32_t *status;
+    uint64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3], table_stride;
+    uint32_t pages, b, t, b_bucket, t_bucket, len_bucket, heads, kv_heads, group, head_dim, page_shift, dtype, causal, window, splits;
+    float scale, softcap;
+};
+/* Parts a row's keys are cut into: by the static alone. */
+uint32_t r9vx_attn_decode_splits(const r9vx_attn_problem &p);
+uint32_t r9vx_attn_prefill_splits(const r9vx_attn_problem &p);
+int r9vx_launch_attn_decode(const r9vx_attn_problem &p, hipStream_t stream);
+int r9vx_launch_attn_prefill(const r9vx_attn_problem &p, hipStream_t stream);
+/* out from the parts of rows [0, rows): row r is token r / heads, head r % heads. */
+int r9vx_launch_attn_join(const r9vx_attn_problem &p, uint64_t rows, hipStream_t stream);
+/* Workgroups a launch of these sizes has (the API refuses more than 32 bits of threads). */
+uint64_t r9vx_attn_decode_groups(const r9vx_attn_problem &p);
+uint64_t r9vx_attn_prefill_groups(const r9vx_attn_problem &p);
+
+/* A part that saw nothing has the maximum -infinity and the sum 0; one that saw
+ * scores of -infinity alone the sum NaN, which the join gives out where no part
+ * saw more. */
+#ifdef __HIPCC__
+namespace r9vx {
+
+typedef _Float16 attn_f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t attn_u32x3 __attribute__((ext_vector_type(3)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+/* The two element types.  kBits is added to every exponent of a probability:
+ * f16 holds 2^-24 at the least, so the largest is made 2^15 there. */
+struct AttnBf16 {
+    typedef r9vx_bf16x8 x8;
+    typedef __bf16 elem;
+    static constexpr float kBits = 0.0f;
+    static constexpr uint32_t kNan = 0x7FC07FC0u;
+    static __device__ __forceinline__ r9vx_f32x4 mma16(x8 a, x8 b, r9vx_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ r9vx_f32x16 mma32(x8 a, x8 b, r9vx_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+struct AttnF16 {
+    typedef attn_f16x8 x8;
+    typedef _Float16 elem;
+    static constexpr float kBits = 15.0f;
+    static constexpr uint32_t kNan = 0x7E007E00u;
+    static __device__ __forceinline__ r9vx_f32x4 mma16(x8 a, x8 b, r9vx_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ r9vx_f32x16 mma32(x8 a, x8 b, r9vx_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+/* A key's row where there is none (zeros: a value nobody sees must not be a NaN
+ * beside a probability of zero), and that of a page outside the cache (NaN: a
+ * score that sees it is one). */
+static __device__ const uint32_t kAttnZeroRow[128] = {};
+template <class T>
+__device__ __forceinline__ const uint16_t *attn_nan_row();
+#define R9VX_ROW16(x) x, x, x, x, x, x, x, x, x, x, x, x, x, x, x, x
+#define R9VX_ROW128(x) R9VX_ROW16(x), R9VX_ROW16(x), R9VX_ROW16(x), R9VX_ROW16(x), R9VX_ROW16(x), R9VX_ROW16(x), R9VX_ROW16(x), R9VX_ROW16(x)
+static __device__ const uint32_t kAttnNanBf16[128] = {R9VX_ROW128(AttnBf16::kNan)};
+static __device__ const uint32_t kAttnNanF16[128] = {R9VX_ROW128(AttnF16::kNan)};
+template <>
+__device__ __forceinline__ const uint16_t *attn_nan_row<AttnBf16>() { return reinterpret_cast<const uint16_t *>(kAttnNanBf16); }
+template <>
+__device__ __forceinline__ const uint16_t *attn_nan_row<AttnF16>() { return reinterpret_cast<const uint16_t *>(kAttnNanF16); }
+
+/* What turns products into exponents of two: x = score * log2(e). */
+struct AttnScore {
+    float factor; /* scale * log2 e, or with a cap 2 log2(e) scale / cap */
+    float cap;    /* cap * log2 e; 0: none */
+    __device__ __forceinline__ explicit AttnScore(const r9vx_attn_problem &a) {
+        cap = a.softcap * kLog2e;
+        factor = a.softcap > 0.0f ? 2.0f * kLog2e * a.scale / a.softcap : a.scale * kLog2e;
+    }
+    /* cap tanh(y): 1 - 2 / (e^2y + 1), whose error 2^-23 is absolute, times the
+     * cap: 10^-5 of a probability at a cap of 50.  e^2y = infinity gives the cap. */
+    __device__ __forceinline__ float capped(float product) const {
+        const float e = __builtin_amdgcn_exp2f(product * factor);
+        return fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(e + 1.0f), cap);
+    }
+};
+
+/* A key's row of keys or values. */
+template <class T>
+__device__ __forceinline__ const uint16_t *attn_row(AttnPlace where, const uint16_t *base, const uint64_t *stride, uint32_t page, uint32_t place) {
+    const uint16_t *p = base + page * stride[0] + place * stride[1];
+    return where == kAttnKept ? p : where == kAttnBad ? attn_nan_row<T>() : reinterpret_cast<const uint16_t *>(kAttnZeroRow);
+}
+
+/* The other half wave's value. */
+__device__ __forceinline__ float attn_swap32(float x) { return __shfl_xor(x, 32, R9VX_WAVE); }
+
+}  // namespace r9vx
+#endif
+#endif

@@ -33,6 +33,7 @@ SCORING_SOFTMAX, SCORING_SIGMOID = 0, 1
 GROUP_MAX, GROUP_TOP2 = 0, 1
 ACT_SILU = 0
 STATUS_NONFINITE, STATUS_DEGENERATE, STATUS_BAD_EXPERT = 1, 2, 4
+STATUS_BAD_PAGE, STATUS_BAD_LENGTH, STATUS_BAD_SLOT = 8, 16, 32
 BLOCK_BYTES = {Q4_K: 144, IQ4_XS: 136, Q6_K: 210, Q8_0: 34, IQ3_S: 110}
 BLOCK_LEN = {Q4_K: 256, IQ4_XS: 256, Q6_K: 256, Q8_0: 32, IQ3_S: 256}
 SPLIT_SCHEMES = (Q6_K, Q8_0)      # read in the split device layout (body + f16 d array)
@@ -78,6 +79,31 @@ class MoeFfnFp8Static(ctypes.Structure):
 class MoeFfnFp8Args(ctypes.Structure):
     _fields_ = [("x", _P), ("expert_ids", _P), ("weights", _P), ("w_gate_up", _P), ("w_gate_up_scales", _P), ("w_down", _P),
                 ("w_down_scales", _P), ("y", _P), ("workspace", _P), ("t", _U32), ("_tail_pad", _U32)]
+
+
+class RopeKvStatic(ctypes.Structure):
+    _fields_ = [("heads", _U32), ("kv_heads", _U32), ("head_dim", _U32), ("rot", _U32), ("interleaved", _U32),
+                ("page_size", _U32), ("in_dtype", _U32), ("out_dtype", _U32), ("amplitude_bits", _U32)]
+
+
+class RopeKvArgs(ctypes.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("positions", _P), ("freqs", _P), ("q_out", _P), ("k_cache", _P),
+                ("v_cache", _P), ("slots", _P), ("status", _P), ("q_stride", _U64 * 2), ("k_stride", _U64 * 2),
+                ("v_stride", _U64 * 2), ("q_out_stride", _U64 * 2), ("k_cache_stride", _U64 * 3),
+                ("v_cache_stride", _U64 * 3), ("pages", _U32), ("t", _U32)]
+
+
+class AttnStatic(ctypes.Structure):
+    _fields_ = [("b_bucket", _U32), ("t_bucket", _U32), ("len_bucket", _U32), ("heads", _U32), ("kv_heads", _U32),
+                ("head_dim", _U32), ("page_size", _U32), ("dtype", _U32), ("causal", _U32), ("window", _U32),
+                ("scale_bits", _U32), ("softcap_bits", _U32)]
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [("q", _P), ("k_cache", _P), ("v_cache", _P), ("table", _P), ("lengths", _P), ("offsets", _P),
+                ("starts", _P), ("prefix", _P), ("slopes", _P), ("out", _P), ("workspace", _P), ("status", _P),
+                ("q_stride", _U64 * 3), ("out_stride", _U64 * 3), ("k_stride", _U64 * 3), ("v_stride", _U64 * 3),
+                ("table_stride", _U64), ("pages", _U32), ("b", _U32), ("t", _U32), ("_tail_pad", _U32)]
 
 
 class MoeRouteStatic(ctypes.Structure):
@@ -164,6 +190,12 @@ EXPORTS = [
     ("r9vx_moe_ffn_fp8_expert_bytes", [_P], ctypes.c_uint64),
     ("r9vx_moe_ffn_fp8_static_bytes", [_P, _U32], ctypes.c_uint64),
     ("r9vx_moe_ffn_fp8_static_flops", [_P, _U32], ctypes.c_uint64),
+    # include/r9vx_attn.h
+    ("r9vx_rope_kv_launch", [_P, _P, _P], ctypes.c_int),
+    ("r9vx_attn_decode_launch", [_P, _P, _P], ctypes.c_int),
+    ("r9vx_attn_decode_workspace_bytes", [_P], ctypes.c_size_t),
+    ("r9vx_attn_prefill_launch", [_P, _P, _P], ctypes.c_int),
+    ("r9vx_attn_prefill_workspace_bytes", [_P], ctypes.c_size_t),
     # include/r9vx_probe.h
     ("r9vx_probe_stream_launch", [_P, ctypes.c_uint64, _P, _P], ctypes.c_int),
     ("r9vx_probe_stream_blocks", [ctypes.c_uint64], _U32),
