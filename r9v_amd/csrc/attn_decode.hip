@@ -92,7 +92,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
 #pragma unroll
         for (int s = 0; s < S::KS; ++s) {
             q[r][s] = x8{};
-            if (there) q[r][s] = *reinterpret_cast<const x8 *>(a.q + b * a.q_stride[0] + token[r] * a.q_stride[1] + h * a.q_stride[2] + s * 32 + g4 * 8);
+            if (there) q[r][s] = attn_query<T>(a, a.q + b * a.q_stride[0] + token[r] * a.q_stride[1] + h * a.q_stride[2] + s * 32 + g4 * 8);
         }
     }
     const int first = row0 / (int)a.group, last = ((row0 + RT * 16 < rows ? row0 + RT * 16 : rows) - 1) / (int)a.group; /* tokens */
@@ -195,17 +195,12 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
                 if (a.softcap > 0.0f) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = score.capped(x[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] *= score.factor;
                 }
                 const int k8 = key0 + 8 * g4;
                 if (a.slopes) {
+                    const float far = (float)(pos[r] - k8);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int d = pos[r] - (k8 + e);
-                        x[e] = fmaf(-slope[r], (float)(d < 0 ? -d : d), x[e]);
-                    }
+                    for (int e = 0; e < 8; ++e) x[e] = fmaf(-slope[r], fabsf(far - (float)e), x[e] * score.before);
                 }
                 if (edge) {
 #pragma unroll
@@ -214,7 +209,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
                 }
                 float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
                 top = fmaxf(top, __shfl_xor(top, 16, R9VX_WAVE));
-                top = fmaxf(top, __shfl_xor(top, 32, R9VX_WAVE));
+                top = fmaxf(top, __shfl_xor(top, 32, R9VX_WAVE)) * score.factor;
                 if (__any(top > m[r])) {
                     const float now = fmaxf(m[r], top);
                     const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - now);
@@ -228,7 +223,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
                 const float ref = (m[r] == -INFINITY ? 0.0f : m[r]) - T::kBits;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float pe = __builtin_amdgcn_exp2f(x[e] - ref);
+                    const float pe = __builtin_amdgcn_exp2f(fmaf(x[e], score.factor, -ref));
                     l[r] += pe;
                     ph[r][e] = (typename T::elem)pe;
                     if constexpr (T::kBits == 0.0f) pl[r][e] = (typename T::elem)(pe - (float)ph[r][e]);

@@ -5,13 +5,13 @@
  * A workgroup of four waves takes a sequence, a kv head and 128 of the rows that
  * share it (row = token * group + query head, so that a tile of few tokens still
  * fills the matrix unit and what a causal tile masks is a few tokens wide), and
- * runs over the keys that some of them sees, a tile at a time: keys and values
- * through registers into LDS, two buffers, one barrier a tile.  Scores are taken
- * transposed by 32 x 32 x 16 products, S^T = K Q^T: a lane then holds 16 keys
- * of one row in the order that the second product O^T = V^T P^T takes, so that
- * probabilities stay in registers; V^T comes from LDS by the transposing read.
- * Where the rows are too few to fill the card the keys are cut into parts,
- * joined by a further launch.
+ * runs over the keys that some of them sees, a tile at a time: keys and values go
+ * from the pages straight into LDS, the next tile's while this one is worked on,
+ * one barrier a tile.  Scores are taken transposed by 32 x 32 x 16 products,
+ * S^T = K Q^T: a lane then holds 16 keys of one row in the order that the second
+ * product O^T = V^T P^T takes, so that probabilities stay in registers; V^T
+ * comes from LDS by the transposing read.  Where the rows are too few to fill the
+ * card the keys are cut into parts, joined by a further launch.
  */
 #include "r9vx_attn_kernels.h"
 
@@ -19,7 +19,7 @@ using namespace r9vx;
 
 namespace {
 
-constexpr int kRows = 128;  /* of a workgroup */
+constexpr int kRows = 128; /* of a workgroup */
 constexpr int kWaves = 4;
 
 typedef short attn_s4 __attribute__((ext_vector_type(4)));
@@ -27,22 +27,42 @@ typedef __attribute__((address_space(3))) attn_s4 attn_lds_s4;
 
 template <int D>
 struct PrefillShape {
-    static constexpr int KT = D > 128 ? 32 : 64;  /* keys of a tile */
-    static constexpr int KP = D + 8;              /* a key's elements in LDS: 16 bytes more, so that rows start in other banks */
-    static constexpr int VP = D + 32;
-    static constexpr int N = KT * D / 8 / 256;    /* 16-byte pieces of a tile each thread moves */
+    static constexpr int KT = D > 128 ? 32 : 64; /* keys of a tile */
+    static constexpr int CH = D / 8;             /* 16-byte pieces of a key's row */
+    static constexpr int N = KT * CH / 256;      /* of a tile, each thread's */
+    /* A row stands in LDS with its pieces' numbers xor-ed by swizzle(row), so that
+     * both a score's reads (16 rows, the same piece) and the transposing ones (4
+     * rows, 4 neighbouring pieces) meet each of the 64 banks once: rows of 256
+     * bytes and their multiples start in one bank, of 128 in two, of 192 in four. */
+    static __device__ __forceinline__ int swizzle(int r) {
+        if constexpr (D == 96) return (r >> 2) & 3;
+        else if constexpr (D % 128) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
+        else return (r & 3) << 2 | ((r >> 2) & 3);
+    }
 };
 
+/* 16 bytes a lane from global memory to LDS at `at` + 16 * lane (uniform `at`). */
+__device__ __forceinline__ void attn_copy16(uint32_t at, const uint16_t *p) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory", "m0");
+}
+
+/* Bits of a pair of elements whose exponent is that of an infinity or a NaN. */
+template <class T>
+__device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
+    constexpr uint32_t e = T::kBits == 0.0f ? 0x7F80u : 0x7C00u;
+    return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
+}
+
 template <class T, int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_prefill_kernel(r9vx_attn_problem a, uint32_t tiles) {
+__global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem a, uint32_t tiles) {
     using S = PrefillShape<D>;
     typedef typename T::x8 x8;
     constexpr int KT = S::KT, NK = KT / 32;
-    __shared__ __attribute__((aligned(16))) uint16_t ks[2][KT * S::KP], vs[2][KT * S::VP];
-    __shared__ int bounds[kWaves][4];
-    __shared__ uint32_t redo;
+    __shared__ __attribute__((aligned(1024))) uint16_t kv[2][2][KT * D]; /* buffer, keys and values */
+    __shared__ int bounds[kWaves][2];
+    __shared__ uint32_t redo, odds[2]; /* odds: keys of a tile with values that are not finite */
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c32 = lane & 31, h2 = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h2 = lane >> 5;
     uint32_t id = blockIdx.x;
     const uint32_t kvh = id % a.kv_heads;
     id /= a.kv_heads;
@@ -77,7 +97,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_prefill_kernel(r9v
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
         q[s] = x8{};
-        if (there) q[s] = *reinterpret_cast<const x8 *>(a.q + at * a.q_stride[1] + head * a.q_stride[2] + s * 16 + h2 * 8);
+        if (there) q[s] = attn_query<T>(a, a.q + at * a.q_stride[1] + head * a.q_stride[2] + s * 16 + h2 * 8);
     }
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
 
@@ -108,41 +128,40 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_prefill_kernel(r9v
 
     float m, l;
     r9vx_f32x16 o[D / 32];
-    r9vx_u32x4 kr[S::N], vr[S::N];
     uint32_t pages[S::N];
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)kv;
 
     auto look_up = [&](int t) {
 #pragma unroll
         for (int i = 0; i < S::N; ++i) {
-            const int key = t * KT + (int)(threadIdx.x + 256 * i) / (D / 8);
+            const int key = t * KT + (int)(threadIdx.x + 256 * i) / S::CH;
             pages[i] = key >= ulo && key < uhi ? (uint32_t)table[key >> a.page_shift] : 0u;
         }
     };
-    auto load = [&](int t) {
+    auto load = [&](int t, int buf) {
+        bool bad = false;
 #pragma unroll
         for (int i = 0; i < S::N; ++i) {
-            const int c = (int)threadIdx.x + 256 * i, key = t * KT + c / (D / 8), e = c % (D / 8) * 8;
+            const int c = (int)threadIdx.x + 256 * i, r = c / S::CH, key = t * KT + r, e = 8 * ((c - r * S::CH) ^ S::swizzle(r));
             const AttnPlace where = attn_place(pages[i], a.pages, key, ulo, uhi);
-            const uint16_t *kp = attn_row<T>(where, kbase, a.k_stride, pages[i], (uint32_t)key & mask);
-            const uint16_t *vp = attn_row<T>(where, vbase, a.v_stride, pages[i], (uint32_t)key & mask);
-            kr[i] = *reinterpret_cast<const r9vx_u32x4 *>(kp + e);
-            vr[i] = *reinterpret_cast<const r9vx_u32x4 *>(vp + e);
-            if (where == kAttnBad && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+            bad |= where == kAttnBad;
+            const uint32_t to = lds + (uint32_t)(buf * 2 * KT * D * 2 + (wave * 64 + 256 * i) * 16);
+            attn_copy16(to, attn_row<T>(where, kbase, a.k_stride, pages[i], (uint32_t)key & mask) + e);
+            attn_copy16(to + KT * D * 2, attn_row<T>(where, vbase, a.v_stride, pages[i], (uint32_t)key & mask) + e);
         }
+        if (bad && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
     };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < S::N; ++i) {
-            const int c = (int)threadIdx.x + 256 * i, key = c / (D / 8), e = c % (D / 8) * 8;
-            *reinterpret_cast<r9vx_u32x4 *>(&ks[buf][key * S::KP + e]) = kr[i];
-            *reinterpret_cast<r9vx_u32x4 *>(&vs[buf][key * S::VP + e]) = vr[i];
-        }
-    };
+
+    /* where this lane's pieces are: of key c32 for a score, of keys 4 h2 + lane / 4 % 4 for the values */
+    const int krow = c32 * D, kpiece = h2 ^ S::swizzle(c32);
+    const int vkey = 4 * h2 + (lane & 15) / 4, vpiece = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ S::swizzle(vkey);
+    const int vrow = vkey * D + 4 * (lane & 1);
 
     /* A first pass; a second one follows only where it gave a NaN or an infinity,
      * which a value that a row does not see may have brought into it through a
-     * probability of zero.  The second pass then leaves out, token by token, the
-     * values of each tile that not all rows see. */
+     * probability of zero.  The second pass takes such values out of LDS, and
+     * adds each to the rows that see its key (times a probability, a NaN or an
+     * infinity is itself). */
     for (int pass = 0; pass < 2; ++pass) {
         m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -151,58 +170,75 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_prefill_kernel(r9v
             for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
         if (begin < end) {
             look_up(begin);
-            load(begin);
+            load(begin, 0);
             if (begin + 1 < end) look_up(begin + 1);
-            store(0);
         }
-        __syncthreads();
         for (int t = begin; t < end; ++t) {
             const int buf = (t - begin) & 1;
             const int key0 = t * KT;
+            /* this tile has landed, and every wave is done with the other buffer */
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
             if (t + 1 < end) {
-                load(t + 1);
+                load(t + 1, buf ^ 1);
                 if (t + 2 < end) look_up(t + 2);
+            }
+            const uint16_t *ks = kv[buf][0];
+            uint16_t *vs = kv[buf][1];
+            if (pass) {
+                if (threadIdx.x == 0) odds[0] = odds[1] = 0;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < S::N; ++i) {
+                    const int c = (int)threadIdx.x + 256 * i, r = c / S::CH;
+                    r9vx_u32x4 w = *reinterpret_cast<const r9vx_u32x4 *>(vs + 8 * c);
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t x = attn_odd<T>(w[j]);
+                        any |= x;
+                        w[j] &= ~x;
+                    }
+                    if (any) {
+                        *reinterpret_cast<r9vx_u32x4 *>(vs + 8 * c) = w;
+                        atomicOr(&odds[r / 32], 1u << (r % 32));
+                    }
+                }
+                __syncthreads();
             }
             if (key0 < whi && key0 + KT > wlo) {
                 r9vx_f32x16 sc[NK];
 #pragma unroll
-                for (int k = 0; k < NK; ++k) {
+                for (int k = 0; k < NK; ++k)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) sc[k][e] = 0.0f;
 #pragma unroll
-                    for (int s = 0; s < D / 16; ++s) {
-                        const x8 kf = *reinterpret_cast<const x8 *>(&ks[buf][(32 * k + c32) * S::KP + s * 16 + h2 * 8]);
-                        sc[k] = T::mma32(kf, q[s], sc[k]);
-                    }
-                }
-                const bool edge = key0 < wfl || key0 + KT > wfh;
+                for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                    for (int k = 0; k < NK; ++k)
+                        sc[k] = T::mma32(*reinterpret_cast<const x8 *>(ks + 32 * k * D + krow + 8 * (kpiece ^ (2 * s))), q[s], sc[k]);
                 if (a.softcap > 0.0f) {
 #pragma unroll
                     for (int k = 0; k < NK; ++k)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) sc[k][e] = score.capped(sc[k][e]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < NK; ++k)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) sc[k][e] *= score.factor;
                 }
                 if (a.slopes) {
+                    const float far = (float)(pos - key0 - 4 * h2);
 #pragma unroll
                     for (int k = 0; k < NK; ++k)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int d = pos - (key0 + 32 * k + 8 * (e >> 2) + 4 * h2 + (e & 3));
-                            sc[k][e] = fmaf(-slope, (float)(d < 0 ? -d : d), sc[k][e]);
-                        }
+                        for (int e = 0; e < 16; ++e)
+                            sc[k][e] = fmaf(-slope, fabsf(far - (float)(32 * k + 8 * (e >> 2) + (e & 3))), sc[k][e] * score.before);
                 }
-                if (edge) {
+                if (key0 < wfl || key0 + KT > wfh) {
+                    const int from = lo - key0 - 4 * h2, to = hi - key0 - 4 * h2;
 #pragma unroll
                     for (int k = 0; k < NK; ++k)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const int key = key0 + 32 * k + 8 * (e >> 2) + 4 * h2 + (e & 3);
-                            if (key < lo || key >= hi) sc[k][e] = -INFINITY;
+                            const int key = 32 * k + 8 * (e >> 2) + (e & 3);
+                            if (key < from || key >= to) sc[k][e] = -INFINITY;
                         }
                 }
                 float top = -INFINITY;
@@ -210,7 +246,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_prefill_kernel(r9v
                 for (int k = 0; k < NK; ++k)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[k][e]);
-                top = fmaxf(top, attn_swap32(top));
+                top = fmaxf(top, attn_swap32(top)) * score.factor;
                 if (__any(top > m)) {
                     const float now = fmaxf(m, top);
                     const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
@@ -227,49 +263,34 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attn_prefill_kernel(r9v
                 for (int s = 0; s < KT / 16; ++s)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float x = __builtin_amdgcn_exp2f(sc[s >> 1][8 * (s & 1) + e] - ref);
+                        const float x = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], score.factor, -ref));
                         l += x;
                         p[s][e] = (typename T::elem)x;
                     }
-                auto value = [&](int s, int d) -> x8 { /* 8 keys of column 32 d + c32: 16 s + 4 h2 .. + 3 and 8 further */
-                    const uint16_t *v = &vs[buf][(16 * s + 4 * h2 + (lane & 15) / 4) * S::VP + 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
-                    const attn_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)v);
-                    const attn_s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)(v + 8 * S::VP));
-                    return __builtin_bit_cast(x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-                };
-                if (pass == 0 || !edge) {
 #pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
+                for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                        for (int s = 0; s < KT / 16; ++s) o[d] = T::mma32(value(s, d), p[s], o[d]);
-                } else {
-                    int done = -1;
-                    for (int r = 0; r < 32; ++r) {
-                        const int tok = __shfl(there ? token : -1, r, R9VX_WAVE);
-                        if (tok == done || tok < 0) continue;
-                        done = tok;
-                        const int from = __shfl(lo, r, R9VX_WAVE), to = __shfl(hi, r, R9VX_WAVE);
+                    for (int s = 0; s < KT / 16; ++s) { /* 8 keys of column 32 d + c32: 16 s + 4 h2 .. + 3 and 8 further */
+                        uint16_t *v = vs + 16 * s * D + vrow + 8 * (vpiece ^ (4 * d)), *w = vs + (16 * s + 8) * D + vrow + 8 * (vpiece ^ (4 * d) ^ 2);
+                        const attn_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)v), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)w);
+                        o[d] = T::mma32(__builtin_bit_cast(x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), p[s], o[d]);
+                    }
+                if (pass) {
+                    for (int r = 0; r < KT; ++r) {
+                        const int key = key0 + r;
+                        if (!(odds[r / 32] >> (r % 32) & 1u) || key < lo || key >= hi) continue;
+                        const uint32_t page = (uint32_t)table[key >> a.page_shift];
+                        const uint16_t *v = attn_row<T>(attn_place(page, a.pages, key, ulo, uhi), vbase, a.v_stride, page, (uint32_t)key & mask);
 #pragma unroll
-                        for (int d = 0; d < D / 32; ++d) {
-                            r9vx_f32x16 sum = o[d]; /* the same sum as the first pass's, for the rows whose keys these are */
+                        for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                            for (int s = 0; s < KT / 16; ++s) {
-                                typedef short s8 __attribute__((ext_vector_type(8)));
-                                s8 v = __builtin_bit_cast(s8, value(s, d));
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const int key = key0 + 16 * s + 8 * (e >> 2) + 4 * h2 + (e & 3);
-                                    v[e] = key >= from && key < to ? v[e] : (short)0;
-                                }
-                                sum = T::mma32(__builtin_bit_cast(x8, v), p[s], sum);
+                            for (int e = 0; e < 16; ++e) {
+                                const uint16_t x = v[32 * d + 8 * (e >> 2) + 4 * h2 + (e & 3)];
+                                if (attn_odd<T>(x)) o[d][e] += (float)__builtin_bit_cast(typename T::elem, x);
                             }
-                            if (there && token == tok) o[d] = sum;
-                        }
                     }
                 }
             }
-            if (t + 1 < end) store(buf ^ 1);
-            __syncthreads();
         }
         l += attn_swap32(l);
         bool odd = !(fabsf(l) < INFINITY);

@@ -93,21 +93,40 @@ __device__ __forceinline__ const uint16_t *attn_nan_row<AttnBf16>() { return rei
 template <>
 __device__ __forceinline__ const uint16_t *attn_nan_row<AttnF16>() { return reinterpret_cast<const uint16_t *>(kAttnNanF16); }
 
-/* What turns products into exponents of two: x = score * log2(e). */
+/* What turns products into exponents of two, x = score * log2(e).  The query's sign
+ * is the scale's (attn_query), so that the largest product is the largest score;
+ * a scale of zero makes it zeros.  A cap and a bias are applied to the
+ * products first and leave them in units of 1 / log2(e): factor 1. */
 struct AttnScore {
-    float factor; /* scale * log2 e, or with a cap 2 log2(e) scale / cap */
-    float cap;    /* cap * log2 e; 0: none */
+    float factor; /* of what is left of a product */
+    float before; /* of a product before a bias */
+    float inner;  /* 2 log2(e) scale / cap */
+    float cap;    /* cap * log2(e) */
     __device__ __forceinline__ explicit AttnScore(const r9vx_attn_problem &a) {
+        const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+        const bool capped = a.softcap > 0.0f, bias = a.slopes != nullptr;
         cap = a.softcap * kLog2e;
-        factor = a.softcap > 0.0f ? 2.0f * kLog2e * a.scale / a.softcap : a.scale * kLog2e;
+        inner = capped ? 2.0f * kLog2e * scale / a.softcap : 0.0f;
+        before = capped ? 1.0f : scale * kLog2e;
+        factor = capped || bias ? 1.0f : scale * kLog2e;
     }
     /* cap tanh(y): 1 - 2 / (e^2y + 1), whose error 2^-23 is absolute, times the
      * cap: 10^-5 of a probability at a cap of 50.  e^2y = infinity gives the cap. */
     __device__ __forceinline__ float capped(float product) const {
-        const float e = __builtin_amdgcn_exp2f(product * factor);
+        const float e = __builtin_amdgcn_exp2f(product * inner);
         return fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(e + 1.0f), cap);
     }
 };
+
+/* Eight elements of a query, with the scale's sign. */
+template <class T>
+__device__ __forceinline__ typename T::x8 attn_query(const r9vx_attn_problem &a, const uint16_t *p) {
+    r9vx_u32x4 w = *reinterpret_cast<const r9vx_u32x4 *>(p);
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
+    return __builtin_bit_cast(typename T::x8, w);
+}
 
 /* A key's row of keys or values. */
 template <class T>
