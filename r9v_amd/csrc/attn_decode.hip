@@ -350,13 +350,16 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
     }
 }
 
-/* A row's parts: a wave, its lanes over the columns.  Bound by a launch and the
- * parts' bytes, head_dim f32 each. */
+constexpr uint32_t kMostParts = 256;
+
+/* A row's parts, by a workgroup: each wave takes the parts' maxima and sums, then
+ * head_dim / 4 threads a part add them up, several parts side by side, and are
+ * added through LDS.  Bound by a launch and two loads in turn. */
 template <class T>
-__global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, uint64_t rows, const float2 *ml) {
-    const uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const uint32_t lane = threadIdx.x & 63;
+__global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, const float2 *ml) {
+    __shared__ float weight[kMostParts];
+    __shared__ r9vx_f32x4 sums[256];
+    const uint64_t row = blockIdx.x;
     const uint64_t tok = row / a.heads;
     const uint32_t h = (uint32_t)(row - tok * a.heads);
     uint64_t seq = 0, t = tok;
@@ -367,42 +370,48 @@ __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, uin
         t = tok - seq * a.t_bucket;
     }
     const uint64_t at = row * a.splits;
-    float m = -INFINITY, sum = 0.0f;
-    for (uint32_t s = lane; s < a.splits; s += 64) {
-        const float2 x = ml[at + s];
-        const float now = fmaxf(m, x.x);
-        /* beside parts that saw something, one of -infinity alone has no weight, but a NaN sum that NaN scores made has */
-        sum = (m == -INFINITY ? 0.0f : sum * __builtin_amdgcn_exp2f(m - now)) + (x.x == -INFINITY ? 0.0f : x.y * __builtin_amdgcn_exp2f(x.x - now));
-        m = now;
+    const uint32_t lane = threadIdx.x & 63;
+    constexpr int N = kMostParts / 64;
+    float2 x[N];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        x[i] = make_float2(-INFINITY, 0.0f);
+        if (lane + 64 * i < a.splits) x[i] = ml[at + lane + 64 * i];
+        m = fmaxf(m, x[i].x);
     }
-    for (int off = 1; off < 64; off <<= 1) {
-        const float om = __shfl_xor(m, off, R9VX_WAVE), os = __shfl_xor(sum, off, R9VX_WAVE);
-        const float now = fmaxf(m, om);
-        sum = (m == -INFINITY ? 0.0f : sum * __builtin_amdgcn_exp2f(m - now)) + (om == -INFINITY ? 0.0f : os * __builtin_amdgcn_exp2f(om - now));
-        m = now;
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, R9VX_WAVE));
+    /* a part that saw nothing, or scores of -infinity alone, has no weight beside
+     * others; where no part saw more, one with a sum (a NaN) makes the row NaN */
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float w = x[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[i].x - m);
+        if (x[i].x != -INFINITY || m == -INFINITY) sum += x[i].y * (m == -INFINITY ? 1.0f : w);
+        if (threadIdx.x < 64) weight[lane + 64 * i] = w;
     }
-    bool none = m == -INFINITY;
-    if (none) { /* zeros, or NaN where a part saw scores of -infinity */
-        bool odd = false;
-        for (uint32_t s = lane; s < a.splits; s += 64) odd |= ml[at + s].y != 0.0f;
-        sum = __any(odd) ? __builtin_nanf("") : 0.0f;
-    }
-    const float f = none ? sum : 1.0f / sum; /* NaN or 0 where there is nothing */
-    uint16_t *y = a.out + seq * a.out_stride[0] + t * a.out_stride[1] + h * a.out_stride[2];
-    for (uint32_t c = lane * 2; c < a.head_dim; c += 128) {
-        float x0 = 0.0f, x1 = 0.0f;
-        if (!none) {
-            for (uint32_t s = 0; s < a.splits; ++s) {
-                const float mw = ml[at + s].x;
-                if (mw == -INFINITY) continue;
-                const float w = __builtin_amdgcn_exp2f(mw - m);
-                const float2 v = *reinterpret_cast<const float2 *>(a.partial + (at + s) * a.head_dim + c);
-                x0 = fmaf(w, v.x, x0), x1 = fmaf(w, v.y, x1);
-            }
+    for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, R9VX_WAVE);
+    __syncthreads();
+    const uint32_t width = a.head_dim / 4, side = 256 / width;
+    const uint32_t part = threadIdx.x / width, c = threadIdx.x - part * width;
+    r9vx_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (part < side) {
+        const float *p = a.partial + at * a.head_dim + 4 * c;
+#pragma unroll 4
+        for (uint32_t s = part; s < a.splits; s += side) {
+            const r9vx_f32x4 v = *reinterpret_cast<const r9vx_f32x4 *>(p + (uint64_t)s * a.head_dim);
+            const float w = weight[s];
+            if (w != 0.0f || w != w) o += v * w; /* not 0 times what a part without weight left */
         }
-        typedef typename T::elem pair __attribute__((ext_vector_type(2)));
-        const pair w = {(typename T::elem)(none ? f : x0 * f), (typename T::elem)(none ? f : x1 * f)};
-        *reinterpret_cast<pair *>(y + c) = w;
+    }
+    sums[threadIdx.x] = o;
+    __syncthreads();
+    if (threadIdx.x < width) {
+        for (uint32_t s = 1; s < side; ++s) o += sums[s * width + c];
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        typedef typename T::elem four __attribute__((ext_vector_type(4)));
+        const four w = {(typename T::elem)(o[0] * f), (typename T::elem)(o[1] * f), (typename T::elem)(o[2] * f), (typename T::elem)(o[3] * f)};
+        *reinterpret_cast<four *>(a.out + seq * a.out_stride[0] + t * a.out_stride[1] + h * a.out_stride[2] + 4 * c) = w;
     }
 }
 
@@ -452,15 +461,15 @@ uint32_t r9vx_attn_decode_splits(const r9vx_attn_problem &p) {
     const uint64_t most = ((uint64_t)p.len_bucket + kWaves * kBlock - 1) / (kWaves * kBlock);
     uint64_t s = groups ? fill / groups : 1;
     if (s > most) s = most;
-    if (s > 256) s = 256;
+    if (s > kMostParts) s = kMostParts;
     return s > 1 ? (uint32_t)s : 1u;
 }
 
 int r9vx_launch_attn_join(const r9vx_attn_problem &p, uint64_t rows, hipStream_t stream) {
     const float2 *ml = reinterpret_cast<const float2 *>(p.partial + (p.offsets ? (uint64_t)p.t_bucket : (uint64_t)p.b_bucket * p.t_bucket) * p.heads * p.splits * p.head_dim);
-    const dim3 grid((unsigned)((rows + 3) / 4));
-    if (p.dtype == R9VX_DTYPE_BF16) hipLaunchKernelGGL(attn_join_kernel<AttnBf16>, grid, dim3(256), 0, stream, p, rows, ml);
-    else hipLaunchKernelGGL(attn_join_kernel<AttnF16>, grid, dim3(256), 0, stream, p, rows, ml);
+    const dim3 grid((unsigned)rows);
+    if (p.dtype == R9VX_DTYPE_BF16) hipLaunchKernelGGL(attn_join_kernel<AttnBf16>, grid, dim3(256), 0, stream, p, ml);
+    else hipLaunchKernelGGL(attn_join_kernel<AttnF16>, grid, dim3(256), 0, stream, p, ml);
     return (int)hipGetLastError();
 }
 
