@@ -34,6 +34,8 @@ struct DecodeShape {
     static constexpr int DL = CW / 16;           /* of them a lane's: 4, 6 or 8 */
     static constexpr int DW = DL / 2;            /* in words */
     static constexpr int KS = D / 32;            /* steps of a score's product */
+    /* waves a SIMD that the registers are to leave room for */
+    static constexpr int kWavesASimd(int rt) { return D * rt > 256 ? 1 : D * rt > 128 ? 2 : 3; }
 };
 
 template <int DW>
@@ -53,14 +55,14 @@ __device__ __forceinline__ void load_words(const uint16_t *p, uint32_t (&w)[DW])
 }
 
 template <class T, int D, int RT>
-__global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_problem a, uint32_t row_tiles) {
+__global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void attn_decode_kernel(r9vx_attn_problem a, uint32_t row_tiles) {
     using S = DecodeShape<D>;
     typedef typename T::x8 x8;
-    __shared__ float jm[kWaves][RT * 16], jl[kWaves][RT * 16];
-    __shared__ float jo[2][16][D + 4]; /* two waves' sums of 16 rows */
+    __shared__ float jm[kWaves][16], jl[kWaves][16];
+    __shared__ __attribute__((aligned(16))) float jo[kWaves][16][D + 4];
     __shared__ uint32_t redo;
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = lane >> 4;
     uint32_t id = blockIdx.x;
     const uint32_t split = id % a.splits;
@@ -73,9 +75,65 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
     const int length = a.lengths[b];
     const bool bad_length = length < 0 || length > (int)a.len_bucket;
     if (bad_length && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
+    const int start = a.starts ? a.starts[b] : 0;
+    const int p0 = length - (int)a.t_bucket; /* of token 0 */
+
+    /* tokens of the rows; keys that some row sees, and those that all of them do */
+    const int first = row0 / (int)a.group, last = ((row0 + RT * 16 < rows ? row0 + RT * 16 : rows) - 1) / (int)a.group;
+    int ulo, uhi, flo, fhi;
+    attn_seen(a.window, a.causal, p0 + first, length, start, 0, ulo, fhi);
+    attn_seen(a.window, a.causal, p0 + last, length, start, 0, flo, uhi);
+    if (bad_length) uhi = ulo = 0;
+
+    /* this part's blocks */
+    const int b0 = ulo / kBlock, b1 = uhi > ulo ? (uhi + kBlock - 1) / kBlock : b0;
+    int begin, end;
+    attn_part(b0, b1, kWaves, (int)a.splits, (int)split, begin, end);
+
+    const uint16_t *kbase = a.k + kvh * a.k_stride[2], *vbase = a.v + kvh * a.v_stride[2];
+    const int32_t *table = a.table + b * a.table_stride;
+    const uint32_t mask = (1u << a.page_shift) - 1;
+
+    /* Eight keys from a multiple of eight stand in one page: a lane's key rows (of
+     * both tiles) are among those from `kgroup` on, its value rows those from 8 g4
+     * on.  A group of which nothing is seen has no page. */
+    const int kgroup = 8 * (col >> 2);
+    auto page_of = [&](int key) -> uint32_t { return key < uhi && key + 8 > ulo ? (uint32_t)table[key >> a.page_shift] : 0u; };
+    struct Rows {
+        const uint16_t *p;
+        uint64_t step; /* from a row to the next; 0: one row stands for all */
+    };
+    auto rows_of = [&](const uint16_t *base, const uint64_t *stride, uint32_t page, int key) -> Rows {
+        const bool seen = key < uhi && key + 8 > ulo;
+        const AttnPlace where = attn_place(page, a.pages, seen ? ulo : -1, ulo, uhi);
+        return {attn_row<T>(where, base, stride, page, (uint32_t)key & mask), where == kAttnKept ? stride[1] : 0};
+    };
+    x8 k[2][S::KS];
+    uint32_t v[8][S::VC][S::DW];
+    auto load_k = [&](int key0, uint32_t page) {
+        const Rows r = rows_of(kbase, a.k_stride, page, key0 + kgroup);
+        const uint16_t *p = r.p + (col & 3) * r.step + g4 * 8;
+#pragma unroll
+        for (int t = 0; t < 2; ++t, p += 4 * r.step)
+#pragma unroll
+            for (int s = 0; s < S::KS; ++s) k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const x8 *>(p + s * 32));
+    };
+    auto load_v = [&](int key0, uint32_t page) {
+        const Rows r = rows_of(vbase, a.v_stride, page, key0 + 8 * g4);
+        const uint16_t *p = r.p + S::DL * col;
+#pragma unroll
+        for (int i = 0; i < 8; ++i, p += r.step)
+#pragma unroll
+            for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW, v[i][c]);
+    };
+    int blk = begin + wave;
+    uint32_t kpage = 0, vpage = 0;
+    if (blk < end) {
+        kpage = page_of(blk * kBlock + kgroup);
+        vpage = page_of(blk * kBlock + 8 * g4);
+    }
 
     /* a lane's row of each tile */
-    const int start = a.starts ? a.starts[b] : 0;
     int lo[RT], hi[RT], pos[RT], token[RT];
     float slope[RT];
     x8 q[RT][S::KS];
@@ -84,7 +142,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
         const int row = row0 + r * 16 + col;
         token[r] = row / (int)a.group;
         const uint32_t h = kvh * a.group + (row - token[r] * (int)a.group);
-        pos[r] = length - (int)a.t_bucket + token[r];
+        pos[r] = p0 + token[r];
         attn_seen(a.window, a.causal, pos[r], length, start, 0, lo[r], hi[r]);
         const bool there = row < rows && !bad_length;
         if (!there) lo[r] = hi[r] = 0;
@@ -95,22 +153,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
             if (there) q[r][s] = attn_query<T>(a, a.q + b * a.q_stride[0] + token[r] * a.q_stride[1] + h * a.q_stride[2] + s * 32 + g4 * 8);
         }
     }
-    const int first = row0 / (int)a.group, last = ((row0 + RT * 16 < rows ? row0 + RT * 16 : rows) - 1) / (int)a.group; /* tokens */
-    /* keys that some row sees, and those that all of them do */
-    int ulo, uhi, flo, fhi;
-    attn_seen(a.window, a.causal, length - (int)a.t_bucket + first, length, start, 0, ulo, fhi);
-    attn_seen(a.window, a.causal, length - (int)a.t_bucket + last, length, start, 0, flo, uhi);
-    if (bad_length) uhi = ulo = 0;
-
     const AttnScore score(a);
-    const uint16_t *kbase = a.k + kvh * a.k_stride[2], *vbase = a.v + kvh * a.v_stride[2];
-    const int32_t *table = a.table + b * a.table_stride;
-    const uint32_t mask = (1u << a.page_shift) - 1;
-
-    /* this part's blocks */
-    const int b0 = ulo / kBlock, b1 = uhi > ulo ? (uhi + kBlock - 1) / kBlock : b0;
-    int begin, end;
-    attn_part(b0, b1, kWaves, (int)a.splits, (int)split, begin, end);
 
     float m[RT], l[RT];
     r9vx_f32x4 o[RT][S::VC][S::DL];
@@ -119,10 +162,16 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
      * the first gave a NaN or an infinity, which a key that another token alone
      * sees may have brought in through a probability of zero. */
     int vlo = ulo, vhi = uhi;
-    for (int pass = -1; pass < (int)a.t_bucket; ++pass) {
+    if (threadIdx.x == 0) redo = 0;
+    for (int pass = -1; pass <= last; ++pass) {
         if (pass >= 0) {
-            if (pass < first || pass > last) continue;
-            attn_seen(a.window, a.causal, length - (int)a.t_bucket + pass, length, start, 0, vlo, vhi);
+            if (pass < first) continue;
+            attn_seen(a.window, a.causal, p0 + pass, length, start, 0, vlo, vhi);
+            blk = begin + wave;
+            if (blk < end) {
+                kpage = page_of(blk * kBlock + kgroup);
+                vpage = page_of(blk * kBlock + 8 * g4);
+            }
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -132,43 +181,11 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
 #pragma unroll
                 for (int j = 0; j < S::DL; ++j) o[r][c][j] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
         }
-
-        const int kgroup = 8 * (col >> 2); /* the eight keys this lane's key rows are among */
-        auto page_of = [&](int key) -> uint32_t { return key < uhi ? (uint32_t)table[key >> a.page_shift] : 0u; };
-        x8 k[2][S::KS];
-        uint32_t v[8][S::VC][S::DW];
-        auto load_k = [&](int key0, uint32_t page) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int key = key0 + kgroup + 4 * t + (col & 3);
-                const uint16_t *p = attn_row<T>(attn_place(page, a.pages, key, ulo, uhi), kbase, a.k_stride, page, (uint32_t)key & mask);
-#pragma unroll
-                for (int s = 0; s < S::KS; ++s) k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const x8 *>(p + s * 32 + g4 * 8));
-            }
-        };
-        auto load_v = [&](int key0, uint32_t page) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int key = key0 + 8 * g4 + i;
-                const uint16_t *p = attn_row<T>(attn_place(page, a.pages, key, vlo, vhi), vbase, a.v_stride, page, (uint32_t)key & mask);
-#pragma unroll
-                for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW + S::DL * col, v[i][c]);
-            }
-        };
-
-        int blk = begin + wave;
-        uint32_t kpage = 0, vpage = 0;
-        if (blk < end) {
-            kpage = page_of(blk * kBlock + kgroup);
-            vpage = page_of(blk * kBlock + 8 * g4);
-            load_k(blk * kBlock, kpage);
-        }
+        if (blk < end) load_k(blk * kBlock, kpage);
         for (; blk < end; blk += kWaves) {
             const int key0 = blk * kBlock;
             load_v(key0, vpage);
-            if (vpage >= a.pages && a.status) { /* of keys that are seen: page 0 stands for the others */
-                if (key0 + 8 * g4 + 7 >= ulo) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
-            }
+            if (vpage >= a.pages && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
             const int next = key0 + kWaves * kBlock;
             const bool more = blk + kWaves < end;
             if (more) {
@@ -185,7 +202,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
                     for (int s = 0; s < S::KS; ++s) sc[r][t] = T::mma16(k[t][s], q[r][s], sc[r][t]);
                 }
             if (more) load_k(next, kpage);
-            const bool edge = key0 < flo || key0 + kBlock > fhi;
+            const int k8 = key0 + 8 * g4; /* of this lane's scores and values */
             x8 ph[RT], pl[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
@@ -196,16 +213,16 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = score.capped(x[e]);
                 }
-                const int k8 = key0 + 8 * g4;
                 if (a.slopes) {
                     const float far = (float)(pos[r] - k8);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = fmaf(-slope[r], fabsf(far - (float)e), x[e] * score.before);
                 }
-                if (edge) {
+                if (key0 < flo || key0 + kBlock > fhi) {
+                    const int from = lo[r] - k8, to = hi[r] - k8;
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (k8 + e < lo[r] || k8 + e >= hi[r]) x[e] = -INFINITY;
+                        if (e < from || e >= to) x[e] = -INFINITY;
                 }
                 float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
                 top = fmaxf(top, __shfl_xor(top, 16, R9VX_WAVE));
@@ -229,6 +246,15 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
                     if constexpr (T::kBits == 0.0f) pl[r][e] = (typename T::elem)(pe - (float)ph[r][e]);
                 }
             }
+            if (key0 < vlo || key0 + kBlock > vhi) { /* what stands behind the last key, or is not to be seen */
+                const int from = vlo - k8, to = vhi - k8;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int c = 0; c < S::VC; ++c)
+#pragma unroll
+                        for (int w = 0; w < S::DW; ++w) v[i][c][w] = i >= from && i < to ? v[i][c][w] : 0u;
+            }
 #pragma unroll
             for (int c = 0; c < S::VC; ++c)
 #pragma unroll
@@ -246,107 +272,64 @@ __global__ __launch_bounds__(64 * kWaves) void attn_decode_kernel(r9vx_attn_prob
                 }
         }
 
-        /* the waves' sums: 2 and 3 to 0 and 1, then 1 to 0 */
+        /* the waves' sums, through LDS; then a thread has four columns of a row at a time */
+        bool odd = false; /* a value that is not finite */
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             l[r] += __shfl_xor(l[r], 16, R9VX_WAVE);
             l[r] += __shfl_xor(l[r], 32, R9VX_WAVE);
-            if (lane < 16) jm[wave][r * 16 + col] = m[r], jl[wave][r * 16 + col] = l[r];
-        }
-        if (pass < 0 && threadIdx.x == 0) redo = 0;
-        __syncthreads();
-        bool odd = false; /* a value that is not finite */
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            float all = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) all = fmaxf(all, jm[w][r * 16 + col]);
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float mw = jm[w][r * 16 + col];
-                /* a wave that saw nothing (or scores of -infinity alone) has no part; its sum is zero, unless NaN scores made it one */
-                sum += jl[w][r * 16 + col] * (mw == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mw - all));
-            }
-            const float f = m[r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - all);
+            if (r > 0 || pass >= 0) __syncthreads();
+            if (lane < 16) jm[wave][col] = m[r], jl[wave][col] = l[r];
 #pragma unroll
             for (int c = 0; c < S::VC; ++c)
 #pragma unroll
-                for (int j = 0; j < S::DL; ++j) o[r][c][j] *= f;
+                for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int half = 2; half >= 1; half >>= 1) {
-                if (wave >= half && wave < 2 * half) {
-#pragma unroll
-                    for (int c = 0; c < S::VC; ++c)
-#pragma unroll
-                        for (int j = 0; j < S::DL; ++j) *reinterpret_cast<r9vx_f32x4 *>(&jo[wave - half][col][((c * S::DL + j) * 4 + g4) * 4]) = o[r][c][j];
-                }
-                __syncthreads();
-                if (wave < half) {
-#pragma unroll
-                    for (int c = 0; c < S::VC; ++c)
-#pragma unroll
-                        for (int j = 0; j < S::DL; ++j) o[r][c][j] += *reinterpret_cast<const r9vx_f32x4 *>(&jo[wave][col][((c * S::DL + j) * 4 + g4) * 4]);
-                }
-                __syncthreads();
-            }
-            m[r] = all, l[r] = sum;
-            if (wave == 0) {
-                odd |= !(fabsf(sum) < INFINITY);
-#pragma unroll
-                for (int c = 0; c < S::VC; ++c)
-#pragma unroll
-                    for (int j = 0; j < S::DL; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) odd |= !(fabsf(o[r][c][j][e]) < INFINITY);
-            }
-        }
-        if (pass < 0 && first != last) {
-            if (wave == 0 && __any(odd) && lane == 0) redo = 1;
+                    for (int j = 0; j < S::DL; j += 2)
+                        *reinterpret_cast<float2 *>(&jo[wave][col][c * S::CW + S::DL * (4 * g4 + e) + j]) = make_float2(o[r][c][j][e], o[r][c][j + 1][e]);
             __syncthreads();
-            if (redo) continue; /* the tokens one by one */
-        }
-        if (wave == 0) {
+            for (int i = threadIdx.x; i < 16 * D / 4; i += 64 * kWaves) {
+                const int in = i / (D / 4), c = i % (D / 4) * 4, row = row0 + r * 16 + in;
+                const int tok = row / (int)a.group;
+                if (row >= rows || (pass >= 0 && tok != pass)) continue;
+                float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const int row = row0 + r * 16 + col;
-                if (row >= rows || (pass >= 0 && token[r] != pass)) continue;
-                const uint32_t h = kvh * a.group + (row - token[r] * (int)a.group);
-                /* scores of -infinity alone are no softmax; no score at all is zeros */
-                float sum = l[r], top = m[r];
+                for (int w = 0; w < kWaves; ++w) top = fmaxf(top, jm[w][in]);
+                r9vx_f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    /* a wave that saw nothing (or scores of -infinity alone) has zeros, or a NaN of NaN scores */
+                    const float f = jm[w][in] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(jm[w][in] - top);
+                    sum += jl[w][in] * f;
+                    y += *reinterpret_cast<const r9vx_f32x4 *>(&jo[w][in][c]) * f;
+                }
+                odd |= !(fabsf(sum) < INFINITY) || !(fabsf(y[0]) < INFINITY) || !(fabsf(y[1]) < INFINITY) || !(fabsf(y[2]) < INFINITY) || !(fabsf(y[3]) < INFINITY);
                 if (bad_length || (sum != sum && top == -INFINITY)) top = 0.0f; /* a NaN that counts beside any other part */
-                if (bad_length || (sum == 0.0f && top == -INFINITY && (lo[r] > begin * kBlock ? lo[r] : begin * kBlock) < (hi[r] < end * kBlock ? hi[r] : end * kBlock)))
-                    sum = __builtin_nanf("");
+                if (bad_length) sum = __builtin_nanf("");
+                if (sum == 0.0f && top == -INFINITY) { /* scores of -infinity alone are no softmax; no score at all is zeros */
+                    int from, to;
+                    attn_seen(a.window, a.causal, p0 + tok, length, start, 0, from, to);
+                    if ((from > begin * kBlock ? from : begin * kBlock) < (to < end * kBlock ? to : end * kBlock)) sum = __builtin_nanf("");
+                }
+                const uint32_t h = kvh * a.group + (row - tok * (int)a.group);
                 if (a.splits == 1) {
                     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    uint16_t *y = a.out + b * a.out_stride[0] + token[r] * a.out_stride[1] + h * a.out_stride[2];
-#pragma unroll
-                    for (int c = 0; c < S::VC; ++c)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int j = 0; j < S::DL; j += 2) {
-                                typedef typename T::elem pair __attribute__((ext_vector_type(2)));
-                                const pair w = {(typename T::elem)(o[r][c][j][e] * f), (typename T::elem)(o[r][c][j + 1][e] * f)};
-                                *reinterpret_cast<pair *>(y + c * S::CW + S::DL * (4 * g4 + e) + j) = w;
-                            }
+                    typedef typename T::elem four __attribute__((ext_vector_type(4)));
+                    const four w = {(typename T::elem)(y[0] * f), (typename T::elem)(y[1] * f), (typename T::elem)(y[2] * f), (typename T::elem)(y[3] * f)};
+                    *reinterpret_cast<four *>(a.out + b * a.out_stride[0] + tok * a.out_stride[1] + h * a.out_stride[2] + c) = w;
                 } else {
-                    const uint64_t at = (((uint64_t)b * a.t_bucket + token[r]) * a.heads + h) * a.splits + split;
-                    float *y = a.partial + at * D;
-#pragma unroll
-                    for (int c = 0; c < S::VC; ++c)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int j = 0; j < S::DL; j += 2)
-                                *reinterpret_cast<float2 *>(y + c * S::CW + S::DL * (4 * g4 + e) + j) = make_float2(o[r][c][j][e], o[r][c][j + 1][e]);
-                    if (g4 == 0) {
-                        float2 *ml = reinterpret_cast<float2 *>(a.partial + (uint64_t)a.b_bucket * a.t_bucket * a.heads * a.splits * D);
-                        ml[at] = make_float2(top, sum);
-                    }
+                    const uint64_t at = (((uint64_t)b * a.t_bucket + tok) * a.heads + h) * a.splits + split;
+                    *reinterpret_cast<r9vx_f32x4 *>(a.partial + at * D + c) = y;
+                    if (c == 0) reinterpret_cast<float2 *>(a.partial + (uint64_t)a.b_bucket * a.t_bucket * a.heads * a.splits * D)[at] = make_float2(top, sum);
                 }
             }
         }
-        if (pass < 0) break;
+        if (pass < 0) {
+            if (first == last) break;
+            if (odd) redo = 1;
+            __syncthreads();
+            if (!redo) break;
+        }
     }
 }
 
