@@ -8,6 +8,8 @@
 #include "r9vx_attn_kernels.h"
 #include "r9vx_host.h"
 
+using namespace r9vx;
+
 namespace {
 
 float as_float(uint32_t bits) {
@@ -78,7 +80,7 @@ void check_attn_static(const r9vx_attn_static *st, bool decode, Problems &pr) {
     if (!(cap >= 0.0f && cap < INFINITY)) pr.add(R9VX_ERR_INVALID, "the softcap must be finite and not negative");
     else if (cap > 0.0f && !isfinite(as_float(st->scale_bits) / cap * 2.885390f)) pr.add(R9VX_ERR_INVALID, "scale / softcap must be finite");
     if (st->len_bucket > (1u << 30)) pr.add(R9VX_ERR_UNSUPPORTED, "len_bucket=%u exceeds 2^30", st->len_bucket);
-    if (st->b_bucket > (1u << 20)) pr.add(R9VX_ERR_UNSUPPORTED, "b_bucket=%u exceeds 2^20", st->b_bucket);
+    if (st->b_bucket >= (1u << 16)) pr.add(R9VX_ERR_UNSUPPORTED, "b_bucket=%u reaches 2^16", st->b_bucket); /* a grid's third extent */
     if (decode && (st->t_bucket == 0 || st->t_bucket > 8)) pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u: 1 to 8 new tokens a sequence", st->t_bucket);
     if (!decode && st->t_bucket > (1u << 24)) pr.add(R9VX_ERR_UNSUPPORTED, "t_bucket=%u exceeds 2^24", st->t_bucket);
 }
@@ -91,6 +93,7 @@ r9vx_attn_problem attn_problem(const r9vx_attn_static *st, bool decode) {
     p.heads = st->heads;
     p.kv_heads = st->kv_heads;
     p.group = st->heads / st->kv_heads;
+    p.group_magic = attn_group_magic(p.group);
     p.head_dim = st->head_dim;
     p.page_shift = log2_of(st->page_size);
     p.dtype = st->dtype;

@@ -34,9 +34,24 @@ struct DecodeShape {
     static constexpr int DL = CW / 16;           /* of them a lane's: 4, 6 or 8 */
     static constexpr int DW = DL / 2;            /* in words */
     static constexpr int KS = D / 32;            /* steps of a score's product */
+    /* A key's (or query's) elements in LDS, 16 bytes more than it has: the 16 rows
+     * whose same piece an operand's read takes start in different banks. */
+    static constexpr int KP = D + 8;
+    static constexpr int kArea = kBlock * KP * 2; /* bytes of a wave: a block's keys, or after them its sums of 16 rows */
+    static_assert(16 * (D + 4) * 4 <= kArea);
     /* waves a SIMD that the registers are to leave room for */
     static constexpr int kWavesASimd(int rt) { return D * rt > 256 ? 1 : D * rt > 128 ? 2 : 3; }
 };
+
+/* DW words in LDS. */
+template <int DW>
+__device__ __forceinline__ void store_words(uint16_t *p, const uint32_t (&w)[DW]) {
+    if constexpr (DW == 2) *reinterpret_cast<r9vx_u32x2 *>(p) = r9vx_u32x2{w[0], w[1]};
+    else if constexpr (DW == 3) {
+        typedef attn_u32x3 vec __attribute__((aligned(4)));
+        *reinterpret_cast<vec *>(p) = attn_u32x3{w[0], w[1], w[2]};
+    } else *reinterpret_cast<r9vx_u32x4 *>(p) = r9vx_u32x4{w[0], w[1], w[2], w[3]};
+}
 
 template <int DW>
 __device__ __forceinline__ void load_words(const uint16_t *p, uint32_t (&w)[DW]) {
@@ -59,17 +74,14 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     using S = DecodeShape<D>;
     typedef typename T::x8 x8;
     __shared__ float jm[kWaves][16], jl[kWaves][16];
-    __shared__ __attribute__((aligned(16))) float jo[kWaves][16][D + 4];
+    __shared__ __attribute__((aligned(16))) uint8_t area[kWaves][S::kArea];
     __shared__ uint32_t redo;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = lane >> 4;
-    uint32_t id = blockIdx.x;
-    const uint32_t split = id % a.splits;
-    id /= a.splits;
-    const uint32_t tile = id % row_tiles;
-    id /= row_tiles;
-    const uint32_t kvh = id % a.kv_heads, b = id / a.kv_heads;
+    const uint32_t split = blockIdx.x, b = blockIdx.z;
+    uint32_t kvh = blockIdx.y, tile = 0;
+    if (row_tiles > 1) kvh = blockIdx.y / row_tiles, tile = blockIdx.y - kvh * row_tiles;
     const int rows = (int)(a.t_bucket * a.group);
     const int row0 = (int)tile * RT * 16;
     const int length = a.lengths[b];
@@ -79,10 +91,10 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     const int p0 = length - (int)a.t_bucket; /* of token 0 */
 
     /* tokens of the rows; keys that some row sees, and those that all of them do */
-    const int first = row0 / (int)a.group, last = ((row0 + RT * 16 < rows ? row0 + RT * 16 : rows) - 1) / (int)a.group;
+    const int first = attn_token(row0, a.group_magic), last = attn_token((row0 + RT * 16 < rows ? row0 + RT * 16 : rows) - 1, a.group_magic);
     int ulo, uhi, flo, fhi;
-    attn_seen(a.window, a.causal, p0 + first, length, start, 0, ulo, fhi);
-    attn_seen(a.window, a.causal, p0 + last, length, start, 0, flo, uhi);
+    attn_seen(a.window, 1, p0 + first, length, start, 0, ulo, fhi);
+    attn_seen(a.window, 1, p0 + last, length, start, 0, flo, uhi);
     if (bad_length) uhi = ulo = 0;
 
     /* this part's blocks */
@@ -94,64 +106,53 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     const int32_t *table = a.table + b * a.table_stride;
     const uint32_t mask = (1u << a.page_shift) - 1;
 
-    /* Eight keys from a multiple of eight stand in one page: a lane's key rows (of
-     * both tiles) are among those from `kgroup` on, its value rows those from 8 g4
-     * on.  A group of which nothing is seen has no page. */
-    const int kgroup = 8 * (col >> 2);
+    /* A lane loads columns DL col .. of eight neighbouring keys, which stand in one
+     * page: whole lines are read.  Keys go through the wave's part of LDS into the
+     * operand's order, values are turned in registers.  A group of eight of which
+     * nothing is seen has no page. */
     auto page_of = [&](int key) -> uint32_t { return key < uhi && key + 8 > ulo ? (uint32_t)table[key >> a.page_shift] : 0u; };
-    struct Rows {
-        const uint16_t *p;
-        uint64_t step; /* from a row to the next; 0: one row stands for all */
-    };
-    auto rows_of = [&](const uint16_t *base, const uint64_t *stride, uint32_t page, int key) -> Rows {
+    auto load = [&](uint32_t (&w)[8][S::VC][S::DW], const uint16_t *base, const uint64_t *stride, uint32_t page, int key) {
         const bool seen = key < uhi && key + 8 > ulo;
         const AttnPlace where = attn_place(page, a.pages, seen ? ulo : -1, ulo, uhi);
-        return {attn_row<T>(where, base, stride, page, (uint32_t)key & mask), where == kAttnKept ? stride[1] : 0};
+        const uint16_t *p = attn_row<T>(where, base, stride, page, (uint32_t)key & mask) + S::DL * col;
+        const uint64_t step = where == kAttnKept ? stride[1] : 0; /* zeros and NaN: one row for all */
+#pragma unroll
+        for (int i = 0; i < 8; ++i, p += step)
+#pragma unroll
+            for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW, w[i][c]);
     };
-    x8 k[2][S::KS];
-    uint32_t v[8][S::VC][S::DW];
-    auto load_k = [&](int key0, uint32_t page) {
-        const Rows r = rows_of(kbase, a.k_stride, page, key0 + kgroup);
-        const uint16_t *p = r.p + (col & 3) * r.step + g4 * 8;
-#pragma unroll
-        for (int t = 0; t < 2; ++t, p += 4 * r.step)
-#pragma unroll
-            for (int s = 0; s < S::KS; ++s) k[t][s] = __builtin_nontemporal_load(reinterpret_cast<const x8 *>(p + s * 32));
-    };
-    auto load_v = [&](int key0, uint32_t page) {
-        const Rows r = rows_of(vbase, a.v_stride, page, key0 + 8 * g4);
-        const uint16_t *p = r.p + S::DL * col;
-#pragma unroll
-        for (int i = 0; i < 8; ++i, p += r.step)
-#pragma unroll
-            for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW, v[i][c]);
-    };
+    uint16_t *mine = reinterpret_cast<uint16_t *>(area[wave]);
+    uint32_t k[8][S::VC][S::DW], v[8][S::VC][S::DW];
     int blk = begin + wave;
-    uint32_t kpage = 0, vpage = 0;
-    if (blk < end) {
-        kpage = page_of(blk * kBlock + kgroup);
-        vpage = page_of(blk * kBlock + 8 * g4);
-    }
+    uint32_t page = 0;
+    if (blk < end) page = page_of(blk * kBlock + 8 * g4);
 
-    /* a lane's row of each tile */
-    int lo[RT], hi[RT], pos[RT], token[RT];
+    /* the queries: 16 rows at a time through LDS; a lane's row of each tile */
+    int lo[RT], hi[RT], pos[RT];
     float slope[RT];
     x8 q[RT][S::KS];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-        const int row = row0 + r * 16 + col;
-        token[r] = row / (int)a.group;
-        const uint32_t h = kvh * a.group + (row - token[r] * (int)a.group);
-        pos[r] = p0 + token[r];
-        attn_seen(a.window, a.causal, pos[r], length, start, 0, lo[r], hi[r]);
-        const bool there = row < rows && !bad_length;
-        if (!there) lo[r] = hi[r] = 0;
-        slope[r] = a.slopes && row < rows ? a.slopes[h] * kLog2e : 0.0f;
+        uint32_t w[4][S::VC][S::DW];
 #pragma unroll
-        for (int s = 0; s < S::KS; ++s) {
-            q[r][s] = x8{};
-            if (there) q[r][s] = attn_query<T>(a, a.q + b * a.q_stride[0] + token[r] * a.q_stride[1] + h * a.q_stride[2] + s * 32 + g4 * 8);
+        for (int i = 0; i < 4; ++i) {
+            const int row = row0 + r * 16 + 4 * g4 + i, tok = attn_token(row, a.group_magic);
+            const uint32_t h = kvh * a.group + (row - tok * (int)a.group);
+            const uint16_t *p = row < rows ? a.q + b * a.q_stride[0] + tok * a.q_stride[1] + h * a.q_stride[2] : reinterpret_cast<const uint16_t *>(kAttnZeroRow);
+#pragma unroll
+            for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW + S::DL * col, w[i][c]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < S::VC; ++c) store_words<S::DW>(mine + (4 * g4 + i) * S::KP + c * S::CW + S::DL * col, w[i][c]);
+        const int row = row0 + r * 16 + col, tok = attn_token(row, a.group_magic);
+        pos[r] = p0 + tok;
+        attn_seen(a.window, 1, pos[r], length, start, 0, lo[r], hi[r]);
+        if (row >= rows || bad_length) lo[r] = hi[r] = 0;
+        slope[r] = a.slopes && row < rows ? a.slopes[kvh * a.group + (row - tok * (int)a.group)] * kLog2e : 0.0f;
+#pragma unroll
+        for (int s = 0; s < S::KS; ++s) q[r][s] = attn_query<T>(a, mine + col * S::KP + s * 32 + g4 * 8);
     }
     const AttnScore score(a);
 
@@ -166,12 +167,10 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     for (int pass = -1; pass <= last; ++pass) {
         if (pass >= 0) {
             if (pass < first) continue;
-            attn_seen(a.window, a.causal, p0 + pass, length, start, 0, vlo, vhi);
+            attn_seen(a.window, 1, p0 + pass, length, start, 0, vlo, vhi);
+            __syncthreads(); /* the sums of the pass before have been read */
             blk = begin + wave;
-            if (blk < end) {
-                kpage = page_of(blk * kBlock + kgroup);
-                vpage = page_of(blk * kBlock + 8 * g4);
-            }
+            if (blk < end) page = page_of(blk * kBlock + 8 * g4);
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -181,27 +180,32 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 #pragma unroll
                 for (int j = 0; j < S::DL; ++j) o[r][c][j] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        if (blk < end) load_k(blk * kBlock, kpage);
+        if (blk < end) load(k, kbase, a.k_stride, page, blk * kBlock + 8 * g4);
         for (; blk < end; blk += kWaves) {
             const int key0 = blk * kBlock;
-            load_v(key0, vpage);
-            if (vpage >= a.pages && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+            load(v, vbase, a.v_stride, page, key0 + 8 * g4);
+            if (page >= a.pages && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
             const int next = key0 + kWaves * kBlock;
             const bool more = blk + kWaves < end;
-            if (more) {
-                kpage = page_of(next + kgroup);
-                vpage = page_of(next + 8 * g4);
-            }
+            if (more) page = page_of(next + 8 * g4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < S::VC; ++c) store_words<S::DW>(mine + (8 * g4 + i) * S::KP + c * S::CW + S::DL * col, k[i][c]);
+            if (more) load(k, kbase, a.k_stride, page, next + 8 * g4);
+            /* tile t has keys 4 t .. 4 t + 3 of each eight: what a lane gets of both is its own eight */
             r9vx_f32x4 sc[RT][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t) {
 #pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    sc[r][t] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int r = 0; r < RT; ++r) sc[r][t] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int s = 0; s < S::KS; ++s) sc[r][t] = T::mma16(k[t][s], q[r][s], sc[r][t]);
+                for (int s = 0; s < S::KS; ++s) {
+                    const x8 kf = *reinterpret_cast<const x8 *>(mine + (8 * (col >> 2) + 4 * t + (col & 3)) * S::KP + s * 32 + g4 * 8);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) sc[r][t] = T::mma16(kf, q[r][s], sc[r][t]);
                 }
-            if (more) load_k(next, kpage);
+            }
             const int k8 = key0 + 8 * g4; /* of this lane's scores and values */
             x8 ph[RT], pl[RT];
 #pragma unroll
@@ -278,7 +282,8 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
         for (int r = 0; r < RT; ++r) {
             l[r] += __shfl_xor(l[r], 16, R9VX_WAVE);
             l[r] += __shfl_xor(l[r], 32, R9VX_WAVE);
-            if (r > 0 || pass >= 0) __syncthreads();
+            if (r > 0) __syncthreads();
+            float *sums = reinterpret_cast<float *>(mine);
             if (lane < 16) jm[wave][col] = m[r], jl[wave][col] = l[r];
 #pragma unroll
             for (int c = 0; c < S::VC; ++c)
@@ -286,11 +291,11 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int j = 0; j < S::DL; j += 2)
-                        *reinterpret_cast<float2 *>(&jo[wave][col][c * S::CW + S::DL * (4 * g4 + e) + j]) = make_float2(o[r][c][j][e], o[r][c][j + 1][e]);
+                        *reinterpret_cast<float2 *>(sums + col * (D + 4) + c * S::CW + S::DL * (4 * g4 + e) + j) = make_float2(o[r][c][j][e], o[r][c][j + 1][e]);
             __syncthreads();
             for (int i = threadIdx.x; i < 16 * D / 4; i += 64 * kWaves) {
                 const int in = i / (D / 4), c = i % (D / 4) * 4, row = row0 + r * 16 + in;
-                const int tok = row / (int)a.group;
+                const int tok = attn_token(row, a.group_magic);
                 if (row >= rows || (pass >= 0 && tok != pass)) continue;
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -301,14 +306,14 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
                     /* a wave that saw nothing (or scores of -infinity alone) has zeros, or a NaN of NaN scores */
                     const float f = jm[w][in] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(jm[w][in] - top);
                     sum += jl[w][in] * f;
-                    y += *reinterpret_cast<const r9vx_f32x4 *>(&jo[w][in][c]) * f;
+                    y += *reinterpret_cast<const r9vx_f32x4 *>(reinterpret_cast<const float *>(area[w]) + in * (D + 4) + c) * f;
                 }
                 odd |= !(fabsf(sum) < INFINITY) || !(fabsf(y[0]) < INFINITY) || !(fabsf(y[1]) < INFINITY) || !(fabsf(y[2]) < INFINITY) || !(fabsf(y[3]) < INFINITY);
                 if (bad_length || (sum != sum && top == -INFINITY)) top = 0.0f; /* a NaN that counts beside any other part */
                 if (bad_length) sum = __builtin_nanf("");
                 if (sum == 0.0f && top == -INFINITY) { /* scores of -infinity alone are no softmax; no score at all is zeros */
                     int from, to;
-                    attn_seen(a.window, a.causal, p0 + tok, length, start, 0, from, to);
+                    attn_seen(a.window, 1, p0 + tok, length, start, 0, from, to);
                     if ((from > begin * kBlock ? from : begin * kBlock) < (to < end * kBlock ? to : end * kBlock)) sum = __builtin_nanf("");
                 }
                 const uint32_t h = kvh * a.group + (row - tok * (int)a.group);
@@ -408,7 +413,7 @@ template <class T, int D>
 int launch_decode(const r9vx_attn_problem &p, hipStream_t stream) {
     uint32_t rt;
     const uint32_t tiles = decode_row_tiles(p, rt);
-    const dim3 grid((unsigned)r9vx_attn_decode_groups(p));
+    const dim3 grid(p.splits, p.kv_heads * tiles, p.b);
     if constexpr (D <= 128) {
         if (rt == 2) {
             hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);

@@ -32,6 +32,10 @@ R9VX_HD void attn_seen(uint32_t window, uint32_t causal, int p, int length, int 
     if (p < 0 || hi < 0) hi = 0; /* p < 0: more new tokens than the sequence holds */
 }
 
+/* row / group as a product: magic = ceil(2^31 / group), exact while row * group < 2^31. */
+R9VX_HD uint32_t attn_group_magic(uint32_t group) { return (uint32_t)(((1ull << 31) + group - 1) / group); }
+R9VX_HD int attn_token(int row, uint32_t magic) { return (int)((uint64_t)(uint32_t)row * magic >> 31); }
+
 /* Where a key's row is: in the cache, nowhere (zeros; not in [from, to)), or in a
  * page that the cache does not have (NaN). */
 enum AttnPlace { kAttnKept, kAttnNone, kAttnBad };

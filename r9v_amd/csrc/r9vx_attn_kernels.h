@@ -34,7 +34,7 @@ struct r9vx_attn_problem {
     float *partial;   /* f32 [rows][splits][head_dim], then (m, l) [rows][splits] */
     uint32_t *status;
     uint64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3], table_stride;
-    uint32_t pages, b, t, b_bucket, t_bucket, len_bucket, heads, kv_heads, group, head_dim, page_shift, dtype, causal, window, splits;
+    uint32_t pages, b, t, b_bucket, t_bucket, len_bucket, heads, kv_heads, group, group_magic, head_dim, page_shift, dtype, causal, window, splits;
     float scale, softcap;
 };
 /* Parts a row's keys are cut into: by the static alone. */
@@ -122,9 +122,11 @@ struct AttnScore {
 template <class T>
 __device__ __forceinline__ typename T::x8 attn_query(const r9vx_attn_problem &a, const uint16_t *p) {
     r9vx_u32x4 w = *reinterpret_cast<const r9vx_u32x4 *>(p);
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
+    if (a.scale <= 0.0f) { /* (nothing waits for the load where the scale is positive) */
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
+        for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
+    }
     return __builtin_bit_cast(typename T::x8, w);
 }
 

@@ -46,6 +46,10 @@ int main() {
                             CHECK(lo >= 0 && hi >= 0 && hi <= length);
                         }
 
+    // tokens of decode's rows: 8 tokens of up to 1024 heads
+    for (int group = 1; group <= 1024; ++group)
+        for (int row = 0; row < 8 * group + 32; ++row) CHECK(attn_token(row, attn_group_magic(group)) == row / group);
+
     // places: a key outside [from, to) or a page outside the cache is never kept
     for (uint32_t page : {0u, 1u, 9u, 10u, 0x7FFFFFFFu, 0x80000000u, 0xFFFFFFFFu})
         for (int key : kHostile)

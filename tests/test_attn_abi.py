@@ -112,7 +112,7 @@ BOTH = [
     (dict(page_size=4), UNSUPPORTED, "page_size"), (dict(dtype=ffi.F32), UNSUPPORTED, "dtype"), (dict(causal=2), INVALID, "causal"),
     (dict(scale_bits=attn._bits(math.nan)), INVALID, "scale"), (dict(softcap_bits=attn._bits(-1.0)), INVALID, "softcap"),
     (dict(softcap_bits=attn._bits(math.inf)), INVALID, "softcap"), (dict(softcap_bits=attn._bits(1e-45)), INVALID, "scale / softcap"),
-    (dict(len_bucket=(1 << 30) + 1), UNSUPPORTED, "2^30"), (dict(b_bucket=(1 << 20) + 1), UNSUPPORTED, "2^20"), (dict(b=5), INVALID, "b=5"),
+    (dict(len_bucket=(1 << 30) + 1), UNSUPPORTED, "2^30"), (dict(b_bucket=1 << 16), UNSUPPORTED, "2^16"), (dict(b=5), INVALID, "b=5"),
     (dict(q=None), NULL, "q, k_cache"), (dict(out=None), NULL, "out"), (dict(table=None), NULL, "table"), (dict(lengths=None), NULL, "lengths"),
     (dict(pages=0), INVALID, "no page"), (dict(pages=(1 << 31) + 1), UNSUPPORTED, "2^31"), (dict(k_cache=ATTN["k_cache"] + 8), ALIGN, "16-byte"),
     (dict(table=ATTN["table"] + 1), ALIGN, "4-byte"), (dict(status=ATTN["status"] + 2), ALIGN, "4-byte"),
@@ -124,7 +124,7 @@ BOTH = [
     (dict(workspace=ATTN["table"], len_bucket=600), INVALID, "workspace must not overlap")]
 DECODE = [(dict(t_bucket=0), UNSUPPORTED, "1 to 8"), (dict(t_bucket=9), UNSUPPORTED, "1 to 8"), (dict(causal=0), INVALID, "causal"), (dict(t=2), INVALID, "t=2"),
           (dict(offsets=ATTN["offsets"]), INVALID, "prefill's"), (dict(prefix=ATTN["prefix"]), INVALID, "prefill's"),
-          (dict(b_bucket=1 << 20, heads=1024, kv_heads=64), UNSUPPORTED, "more tiles than a launch")]
+          (dict(b_bucket=65535, heads=1024, kv_heads=512), UNSUPPORTED, "more tiles than a launch")]
 PREFILL = [(dict(t_bucket=(1 << 24) + 1), UNSUPPORTED, "2^24"), (dict(t=101), INVALID, "t=101"), (dict(offsets=None), NULL, "offsets"),
            (dict(causal=0, prefix=ATTN["prefix"]), INVALID, "prefix without"), (dict(t_bucket=1 << 24, heads=1024, kv_heads=4), UNSUPPORTED, "more tiles")]
 
@@ -284,7 +284,7 @@ def test_launches(tmp_path, monkeypatch):
     runtime = launch_record.build(tmp_path)
     calls = [("attn", dict(decode=True)), ("attn", dict(decode=True, b_bucket=2000)), ("attn", dict(decode=True, len_bucket=100)), ("attn", dict(decode=False)),
              ("attn", dict(decode=False, t_bucket=100000)), ("attn", dict(decode=True, t_bucket=8)), ("attn", dict(decode=False, t_bucket=1 << 23, heads=128, kv_heads=8)),
-             ("attn", dict(decode=True, b_bucket=1 << 20, heads=14, kv_heads=14))]
+             ("attn", dict(decode=True, b_bucket=65535, heads=224, kv_heads=224))]
     out = launch_record.record(runtime, calls)
     names = [[n.split("<")[0] for n, _, _ in ls] for _, _, ls in out]
     assert all(rc == 0 for rc, _, _ in out), [(rc, msg) for rc, msg, _ in out]
@@ -292,4 +292,4 @@ def test_launches(tmp_path, monkeypatch):
     assert names == [[d, j], [d], [d], [p, j], [p], [d, j], [p], [d]]
     for _, _, ls in out:
         for _, grid, block in ls:
-            assert grid[0] * block[0] < 1 << 32
+            assert grid[0] * grid[1] * grid[2] * block[0] < 1 << 32 and grid[1] < 1 << 16 and grid[2] < 1 << 16
