@@ -98,12 +98,13 @@ r9vx_attn_problem attn_problem(const r9vx_attn_static *st, bool decode) {
     p.page_shift = log2_of(st->page_size);
     p.dtype = st->dtype;
     p.causal = st->causal;
-    p.window = st->window;
+    p.window = st->window && st->window < kAttnNoWindow ? st->window : kAttnNoWindow;
     p.scale = as_float(st->scale_bits);
     p.softcap = as_float(st->softcap_bits);
     p.b = st->b_bucket;
     p.t = st->t_bucket;
-    p.splits = decode ? r9vx_attn_decode_splits(p) : r9vx_attn_prefill_splits(p);
+    if (decode) r9vx_attn_decode_plan(p);
+    else r9vx_attn_prefill_plan(p);
     return p;
 }
 

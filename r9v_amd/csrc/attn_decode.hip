@@ -40,7 +40,7 @@ struct DecodeShape {
     static constexpr int kArea = kBlock * KP * 2; /* bytes of a wave: a block's keys, or after them its sums of 16 rows */
     static_assert(16 * (D + 4) * 4 <= kArea);
     /* waves a SIMD that the registers are to leave room for */
-    static constexpr int kWavesASimd(int rt) { return D * rt > 256 ? 1 : D * rt > 128 ? 2 : 3; }
+    static constexpr int kWavesASimd(int rt) { return D > 192 ? 1 : D * rt > 96 ? 2 : 3; }
 };
 
 /* DW words in LDS. */
@@ -79,9 +79,11 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = lane >> 4;
-    const uint32_t split = blockIdx.x, b = blockIdx.z;
-    uint32_t kvh = blockIdx.y, tile = 0;
-    if (row_tiles > 1) kvh = blockIdx.y / row_tiles, tile = blockIdx.y - kvh * row_tiles;
+    /* Consecutive workgroups go to the eight dies in turn: heads, then sequences,
+     * then parts, so that dies whose sequences end early are not the same ones. */
+    const uint32_t b = blockIdx.y, split = blockIdx.z;
+    uint32_t kvh = blockIdx.x, tile = 0;
+    if (row_tiles > 1) kvh = blockIdx.x / row_tiles, tile = blockIdx.x - kvh * row_tiles;
     const int rows = (int)(a.t_bucket * a.group);
     const int row0 = (int)tile * RT * 16;
     const int length = a.lengths[b];
@@ -100,7 +102,7 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     /* this part's blocks */
     const int b0 = ulo / kBlock, b1 = uhi > ulo ? (uhi + kBlock - 1) / kBlock : b0;
     int begin, end;
-    attn_part(b0, b1, kWaves, (int)a.splits, (int)split, begin, end);
+    attn_part(b0, b1, kWaves, a.parts, a.part_blocks, split, begin, end);
 
     const uint16_t *kbase = a.k + kvh * a.k_stride[2], *vbase = a.v + kvh * a.v_stride[2];
     const int32_t *table = a.table + b * a.table_stride;
@@ -123,29 +125,44 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     };
     uint16_t *mine = reinterpret_cast<uint16_t *>(area[wave]);
     uint32_t k[8][S::VC][S::DW], v[8][S::VC][S::DW];
-    int blk = begin + wave;
-    uint32_t page = 0;
-    if (blk < end) page = page_of(blk * kBlock + 8 * g4);
+    /* The first block's page, the queries' rows, then the block: each load goes out
+     * before anything waits for the one before it. */
+    uint32_t page = 0, after = 0; /* of the next block, and of the one after it */
+    auto first_page = [&]() {
+        if (begin + wave < end) page = page_of((begin + wave) * kBlock + 8 * g4);
+    };
+    auto first_block = [&]() {
+        const int blk = begin + wave;
+        if (blk >= end) return;
+        load(k, kbase, a.k_stride, page, blk * kBlock + 8 * g4);
+        load(v, vbase, a.v_stride, page, blk * kBlock + 8 * g4);
+        if (page >= a.pages && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+        if (blk + kWaves < end) page = page_of((blk + kWaves) * kBlock + 8 * g4);
+    };
+    first_page();
 
     /* the queries: 16 rows at a time through LDS; a lane's row of each tile */
+    uint32_t qw[RT][4][S::VC][S::DW];
     int lo[RT], hi[RT], pos[RT];
     float slope[RT];
     x8 q[RT][S::KS];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        uint32_t w[4][S::VC][S::DW];
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = row0 + r * 16 + 4 * g4 + i, tok = attn_token(row, a.group_magic);
             const uint32_t h = kvh * a.group + (row - tok * (int)a.group);
             const uint16_t *p = row < rows ? a.q + b * a.q_stride[0] + tok * a.q_stride[1] + h * a.q_stride[2] : reinterpret_cast<const uint16_t *>(kAttnZeroRow);
 #pragma unroll
-            for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW + S::DL * col, w[i][c]);
+            for (int c = 0; c < S::VC; ++c) load_words<S::DW>(p + c * S::CW + S::DL * col, qw[r][i][c]);
         }
+    first_block();
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < S::VC; ++c) store_words<S::DW>(mine + (4 * g4 + i) * S::KP + c * S::CW + S::DL * col, w[i][c]);
+            for (int c = 0; c < S::VC; ++c) store_words<S::DW>(mine + (4 * g4 + i) * S::KP + c * S::CW + S::DL * col, qw[r][i][c]);
         const int row = row0 + r * 16 + col, tok = attn_token(row, a.group_magic);
         pos[r] = p0 + tok;
         attn_seen(a.window, 1, pos[r], length, start, 0, lo[r], hi[r]);
@@ -169,8 +186,8 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
             if (pass < first) continue;
             attn_seen(a.window, 1, p0 + pass, length, start, 0, vlo, vhi);
             __syncthreads(); /* the sums of the pass before have been read */
-            blk = begin + wave;
-            if (blk < end) page = page_of(blk * kBlock + 8 * g4);
+            first_page();
+            first_block();
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -180,19 +197,18 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 #pragma unroll
                 for (int j = 0; j < S::DL; ++j) o[r][c][j] = r9vx_f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        if (blk < end) load(k, kbase, a.k_stride, page, blk * kBlock + 8 * g4);
-        for (; blk < end; blk += kWaves) {
-            const int key0 = blk * kBlock;
-            load(v, vbase, a.v_stride, page, key0 + 8 * g4);
-            if (page >= a.pages && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
-            const int next = key0 + kWaves * kBlock;
+        for (int blk = begin + wave; blk < end; blk += kWaves) {
+            const int key0 = blk * kBlock, next = key0 + kWaves * kBlock;
             const bool more = blk + kWaves < end;
-            if (more) page = page_of(next + 8 * g4);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int c = 0; c < S::VC; ++c) store_words<S::DW>(mine + (8 * g4 + i) * S::KP + c * S::CW + S::DL * col, k[i][c]);
-            if (more) load(k, kbase, a.k_stride, page, next + 8 * g4);
+            if (more) {
+                load(k, kbase, a.k_stride, page, next + 8 * g4);
+                if (page >= a.pages && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+                if (blk + 2 * kWaves < end) after = page_of(next + kWaves * kBlock + 8 * g4);
+            }
             /* tile t has keys 4 t .. 4 t + 3 of each eight: what a lane gets of both is its own eight */
             r9vx_f32x4 sc[RT][2];
 #pragma unroll
@@ -274,6 +290,10 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
                         if constexpr (T::kBits == 0.0f) o[r][c][j] = T::mma16(vt, pl[r], o[r][c][j]);
                     }
                 }
+            if (more) {
+                load(v, vbase, a.v_stride, page, next + 8 * g4);
+                page = after;
+            }
         }
 
         /* the waves' sums, through LDS; then a thread has four columns of a row at a time */
@@ -339,10 +359,12 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 }
 
 constexpr uint32_t kMostParts = 256;
+constexpr uint32_t kPartBlocks = 64; /* a part's blocks at most */
 
-/* A row's parts, by a workgroup: each wave takes the parts' maxima and sums, then
- * head_dim / 4 threads a part add them up, several parts side by side, and are
- * added through LDS.  Bound by a launch and two loads in turn. */
+/* A row's parts, by a workgroup (or where they are many one for each 32 columns):
+ * each wave takes the parts' maxima and sums, then four columns a thread are added
+ * up, several parts side by side, and those through LDS.  Bound by a launch and
+ * two loads in turn. */
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, const float2 *ml) {
     __shared__ float weight[kMostParts];
@@ -380,11 +402,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, con
     }
     for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, R9VX_WAVE);
     __syncthreads();
-    const uint32_t width = a.head_dim / 4, side = 256 / width;
-    const uint32_t part = threadIdx.x / width, c = threadIdx.x - part * width;
+    const uint32_t width = a.head_dim / 4 / gridDim.y, side = 256 / width;
+    const uint32_t part = threadIdx.x / width, c = threadIdx.x - part * width, column = 4 * (blockIdx.y * width + c);
     r9vx_f32x4 o = {0.f, 0.f, 0.f, 0.f};
     if (part < side) {
-        const float *p = a.partial + at * a.head_dim + 4 * c;
+        const float *p = a.partial + at * a.head_dim + column;
 #pragma unroll 4
         for (uint32_t s = part; s < a.splits; s += side) {
             const r9vx_f32x4 v = *reinterpret_cast<const r9vx_f32x4 *>(p + (uint64_t)s * a.head_dim);
@@ -399,7 +421,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, con
         const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
         typedef typename T::elem four __attribute__((ext_vector_type(4)));
         const four w = {(typename T::elem)(o[0] * f), (typename T::elem)(o[1] * f), (typename T::elem)(o[2] * f), (typename T::elem)(o[3] * f)};
-        *reinterpret_cast<four *>(a.out + seq * a.out_stride[0] + t * a.out_stride[1] + h * a.out_stride[2] + 4 * c) = w;
+        *reinterpret_cast<four *>(a.out + seq * a.out_stride[0] + t * a.out_stride[1] + h * a.out_stride[2] + column) = w;
     }
 }
 
@@ -413,7 +435,7 @@ template <class T, int D>
 int launch_decode(const r9vx_attn_problem &p, hipStream_t stream) {
     uint32_t rt;
     const uint32_t tiles = decode_row_tiles(p, rt);
-    const dim3 grid(p.splits, p.kv_heads * tiles, p.b);
+    const dim3 grid(p.kv_heads * tiles, p.b, p.splits);
     if constexpr (D <= 128) {
         if (rt == 2) {
             hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
@@ -442,20 +464,30 @@ uint64_t r9vx_attn_decode_groups(const r9vx_attn_problem &p) {
     return (uint64_t)p.b * p.kv_heads * decode_row_tiles(p, rt) * p.splits;
 }
 
-uint32_t r9vx_attn_decode_splits(const r9vx_attn_problem &p) {
+void r9vx_attn_decode_plan(r9vx_attn_problem &p) {
     uint32_t rt;
     const uint64_t groups = (uint64_t)p.b_bucket * p.kv_heads * decode_row_tiles(p, rt);
-    const uint64_t fill = 3ull * r9vx_device_cus();
-    const uint64_t most = ((uint64_t)p.len_bucket + kWaves * kBlock - 1) / (kWaves * kBlock);
-    uint64_t s = groups ? fill / groups : 1;
-    if (s > most) s = most;
-    if (s > kMostParts) s = kMostParts;
-    return s > 1 ? (uint32_t)s : 1u;
+    const uint64_t fill = (p.head_dim > 192 ? 1ull : p.head_dim * rt > 96 ? 2ull : 3ull) * r9vx_device_cus();
+    /* blocks of the longest row */
+    const uint32_t whole = (p.len_bucket + kBlock - 1) / kBlock, seen = (p.window + p.t_bucket - 1) / kBlock + 2;
+    const uint32_t most = seen < whole ? seen : whole > 0 ? whole : 1;
+    uint64_t parts = groups ? fill / groups : 1;
+    if (parts > (most + kWaves - 1) / kWaves) parts = (most + kWaves - 1) / kWaves;
+    if (parts > kMostParts) parts = kMostParts;
+    if (parts < 1) parts = 1;
+    uint32_t per = (uint32_t)((most + parts - 1) / parts);
+    if (per > kPartBlocks) per = kPartBlocks;
+    if (per < (most + kMostParts - 1) / kMostParts) per = (most + kMostParts - 1) / kMostParts;
+    per = (per + kWaves - 1) / kWaves * kWaves;
+    p.parts = (uint32_t)parts;
+    p.part_blocks = per;
+    p.splits = (most + per - 1) / per;
+    if (p.splits < p.parts) p.splits = p.parts;
 }
 
 int r9vx_launch_attn_join(const r9vx_attn_problem &p, uint64_t rows, hipStream_t stream) {
     const float2 *ml = reinterpret_cast<const float2 *>(p.partial + (p.offsets ? (uint64_t)p.t_bucket : (uint64_t)p.b_bucket * p.t_bucket) * p.heads * p.splits * p.head_dim);
-    const dim3 grid((unsigned)rows);
+    const dim3 grid((unsigned)rows, p.splits > 16 ? p.head_dim / 32 : 1);
     if (p.dtype == R9VX_DTYPE_BF16) hipLaunchKernelGGL(attn_join_kernel<AttnBf16>, grid, dim3(256), 0, stream, p, ml);
     else hipLaunchKernelGGL(attn_join_kernel<AttnF16>, grid, dim3(256), 0, stream, p, ml);
     return (int)hipGetLastError();

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
     /* this part's tiles */
     const int t0 = ulo < uhi ? ulo / KT : 0, t1 = ulo < uhi ? (uhi + KT - 1) / KT : 0;
     int begin, end;
-    attn_part(t0, t1, 1, (int)a.splits, (int)split, begin, end);
+    attn_part(t0, t1, 1, a.parts, a.part_blocks, split, begin, end);
 
     const AttnScore score(a);
     const uint16_t *kbase = a.k + kvh * a.k_stride[2], *vbase = a.v + kvh * a.v_stride[2];
@@ -351,14 +351,15 @@ int launch_prefill(const r9vx_attn_problem &p, hipStream_t stream) {
 
 uint64_t r9vx_attn_prefill_groups(const r9vx_attn_problem &p) { return (uint64_t)attn_tiles(p.t, p.b, p.group, kRows) * p.kv_heads * p.splits; }
 
-uint32_t r9vx_attn_prefill_splits(const r9vx_attn_problem &p) {
+void r9vx_attn_prefill_plan(r9vx_attn_problem &p) {
     const uint64_t groups = (uint64_t)attn_tiles(p.t_bucket, p.b_bucket, p.group, kRows) * p.kv_heads;
     const uint64_t fill = 2ull * r9vx_device_cus();
     const uint64_t most = ((uint64_t)p.len_bucket + 255) / 256; /* keys of a part: 256 or more */
     uint64_t s = groups ? fill / groups : 1;
     if (s > most) s = most;
     if (s > 64) s = 64;
-    return s > 1 ? (uint32_t)s : 1u;
+    p.splits = p.parts = s > 1 ? (uint32_t)s : 1u;
+    p.part_blocks = 1u << 27; /* no limit */
 }
 
 int r9vx_launch_attn_prefill(const r9vx_attn_problem &p, hipStream_t stream) {

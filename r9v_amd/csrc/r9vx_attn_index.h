@@ -16,14 +16,15 @@
 
 namespace r9vx {
 
-/* The keys [lo, hi) that the token at position p of a sequence of `length`
- * tokens sees: 0 <= lo, hi <= length; none where lo >= hi. */
+constexpr uint32_t kAttnNoWindow = 1u << 30; /* no sequence is longer */
+
+/* The keys [lo, hi) that the token at position p < 2^30 of a sequence of `length`
+ * tokens sees through a window of 1 .. 2^30: 0 <= lo, 0 <= hi <= length; none where
+ * lo >= hi. */
 R9VX_HD void attn_seen(uint32_t window, uint32_t causal, int p, int length, int start, int prefix, int &lo, int &hi) {
     lo = start > 0 ? start : 0;
-    if (window) {
-        const int64_t w = (int64_t)p - window + 1; /* a window may pass 2^31 */
-        if (w > lo) lo = (int)w;
-    }
+    const int w = (int)((uint32_t)p - window + 1u);
+    if (p >= 0 && w > lo) lo = w;
     hi = length;
     if (causal) {
         const int last = prefix > p + 1 ? prefix : p + 1;
@@ -44,12 +45,15 @@ R9VX_HD AttnPlace attn_place(uint32_t page, uint32_t pages, int key, int from, i
     return page < pages ? kAttnKept : kAttnBad;
 }
 
-/* Part `split` of the blocks [b0, b1) of a row's keys, `unit` blocks at a time. */
-R9VX_HD void attn_part(int b0, int b1, int unit, int splits, int split, int &begin, int &end) {
-    const int64_t per = ((int64_t)(b1 - b0) + (int64_t)unit * splits - 1) / ((int64_t)unit * splits) * unit;
-    const int64_t first = b0 + split * per, last = first + per;
-    begin = (int)(first < b1 ? first : b1);
-    end = (int)(last < b1 ? last : b1);
+/* Part `split` of the blocks [b0, b1) (of 0 .. 2^26) of a row's keys: the blocks over
+ * `parts`, in whole `unit`s, at most `most` (whole units) of them.  Enough of them
+ * cover every block: ceil((b1 - b0) / most) and at least `parts`. */
+R9VX_HD void attn_part(int b0, int b1, uint32_t unit, uint32_t parts, uint32_t most, uint32_t split, int &begin, int &end) {
+    const uint32_t n = (uint32_t)(b1 - b0), share = parts == 1 ? n : (n + parts - 1) / parts;
+    const uint32_t whole = (share + unit - 1) / unit * unit, per = whole < most ? whole : most;
+    const uint64_t first = (uint64_t)split * per, last = first + per;
+    begin = b0 + (int)(first < n ? first : n);
+    end = b0 + (int)(last < n ? last : n);
 }
 
 /* Prefill's rows of a sequence are cut into tiles of `rows`; sequence i's tiles

@@ -34,12 +34,13 @@ struct r9vx_attn_problem {
     float *partial;   /* f32 [rows][splits][head_dim], then (m, l) [rows][splits] */
     uint32_t *status;
     uint64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3], table_stride;
-    uint32_t pages, b, t, b_bucket, t_bucket, len_bucket, heads, kv_heads, group, group_magic, head_dim, page_shift, dtype, causal, window, splits;
+    uint32_t pages, b, t, b_bucket, t_bucket, len_bucket, heads, kv_heads, group, group_magic, head_dim, page_shift, dtype, causal, window;
+    uint32_t splits, parts, part_blocks; /* parts of a row's keys in the grid; those a row is cut into, of at most part_blocks blocks (attn_part) */
     float scale, softcap;
 };
-/* Parts a row's keys are cut into: by the static alone. */
-uint32_t r9vx_attn_decode_splits(const r9vx_attn_problem &p);
-uint32_t r9vx_attn_prefill_splits(const r9vx_attn_problem &p);
+/* Sets splits, parts and part_blocks: by the static alone. */
+void r9vx_attn_decode_plan(r9vx_attn_problem &p);
+void r9vx_attn_prefill_plan(r9vx_attn_problem &p);
 int r9vx_launch_attn_decode(const r9vx_attn_problem &p, hipStream_t stream);
 int r9vx_launch_attn_prefill(const r9vx_attn_problem &p, hipStream_t stream);
 /* out from the parts of rows [0, rows): row r is token r / heads, head r % heads. */

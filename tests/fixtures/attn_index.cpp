@@ -27,19 +27,19 @@ int main() {
 
     // seen: against the definition, and inside [0, length) whatever the data
     for (int i = 0; i < 400000; ++i) {
-        const int length = any(0, 40), p = any(-3, 45), start = any(-5, 50), prefix = any(-5, 50), window = any(0, 1) ? any(0, 45) : 0, causal = any(0, 1);
+        const int length = any(0, 40), p = any(-3, 45), start = any(-5, 50), prefix = any(-5, 50), window = any(0, 1) ? any(1, 45) : (int)kAttnNoWindow, causal = any(0, 1);
         int lo, hi;
         attn_seen(window, causal, p, length, start, prefix, lo, hi);
         for (int j = -2; j < 60; ++j) {
-            const bool want = p >= 0 && j >= 0 && j < length && j >= start && (!window || j > p - window) && (!causal || j <= p || j < prefix);
+            const bool want = p >= 0 && j >= 0 && j < length && j >= start && j > p - window && (!causal || j <= p || j < prefix);
             CHECK((j >= lo && j < hi) == want);
         }
     }
     for (int start : kHostile)
         for (int prefix : kHostile)
-            for (uint32_t window : {0u, 1u, 100u, 1u << 31, 0xFFFFFFFFu})
+            for (uint32_t window : {1u, 100u, 1u << 29, (1u << 30) - 1, kAttnNoWindow})
                 for (int length : {0, 1, 1 << 20, 1 << 30})
-                    for (int back : {0, 1, 7, 1 << 24})
+                    for (int back : {1, 2, 7, 1 << 24})
                         for (uint32_t causal : {0u, 1u}) {
                             int lo, hi;
                             attn_seen(window, causal, length - back, length, start, prefix, lo, hi);
@@ -60,14 +60,18 @@ int main() {
                     CHECK(x != kAttnKept || page < 10);
                 }
 
-    // parts: every block once, in order, whole units
+    // parts: every block once, in order, whole units, none over the most
     for (int i = 0; i < 200000; ++i) {
-        const int b0 = any(0, 1 << 24), b1 = b0 + (any(0, 3) ? any(0, 300) : any(0, 1 << 25)), unit = any(0, 1) ? 1 : 4, splits = any(1, 256);
+        const int b0 = any(0, 1 << 25), b1 = b0 + (any(0, 3) ? any(0, 300) : any(0, 1 << 25)), unit = any(0, 1) ? 1 : 4;
+        const int parts = any(0, 2) ? any(1, 8) : any(1, 256), n = b1 - b0;
+        int most = unit * any(1, 64);
+        if ((n + most - 1) / most > 1000) most = (n / 900 + 1) * unit;
+        const int splits = std::max(parts, (n + most - 1) / most);
         int at = b0;
         for (int s = 0; s < splits; ++s) {
             int begin, end;
-            attn_part(b0, b1, unit, splits, s, begin, end);
-            CHECK(begin <= end && begin >= b0 && end <= b1 && begin == at);
+            attn_part(b0, b1, unit, parts, most, s, begin, end);
+            CHECK(begin <= end && begin >= b0 && end <= b1 && begin == at && end - begin <= most);
             CHECK((begin - b0) % unit == 0 || begin == b1);
             at = end;
         }
