@@ -22,9 +22,9 @@ from .ffi import BF16, F16, F32, R9vxError
 
 HEAD_DIMS = (64, 96, 128, 192, 256)
 
-# RopeKvArgs and AttnArgs as bytes: a decode step makes these calls in every layer
-_ROPE_ARGS = struct.Struct("10P14Q2I")
-_ATTN_ARGS = struct.Struct("12P13Q4I")
+# RopeKvArgs and AttnArgs as bytes: the pointers of a call, and what its operands' shapes and strides give
+_ROPE_POINTERS, _ROPE_REST = struct.Struct("10P"), struct.Struct("14Q2I")
+_ATTN_POINTERS, _ATTN_REST = struct.Struct("12P"), struct.Struct("13Q4I")
 
 
 def rope_freqs(rot, base=10000.0, scaling="none", factor=1.0, original_length=0, factors=None, beta_fast=32.0, beta_slow=1.0,
@@ -90,6 +90,32 @@ def _bits(x):
         raise R9vxError(-103, f"{x!r} is no f32 number") from None
 
 
+# A decode step makes these calls in every layer and each takes a few microseconds
+# on the GPU.  What a call checks and fills in goes by its operands' shapes, strides,
+# types and devices and by its numbers alone: it is kept by those (ffi._fp8_statics,
+# beside the statics), and a further call of the same ones packs its pointers.
+
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _plan(key, make, *args):
+    plans = ffi._fp8_statics
+    got = plans.get(key)
+    if got is None:
+        got = make(*args)
+        if len(plans) >= 4096:  # a caller that never repeats a size
+            plans.clear()
+        plans[key] = got
+    return got
+
+
+def _number(name, x):
+    if type(x) not in (int, float):
+        raise R9vxError(-103, f"{name}={x!r} is no number")
+    return _bits(x)
+
+
 def _strides(name, t, dims):
     """A tensor's strides but for the last axis, which must be dense; 0 along an axis of one."""
     shape, stride = t.shape, t.stride()
@@ -120,6 +146,32 @@ def _cache(k_cache, v_cache, dtypes, device):
     return page, kv, dim, ffi._u32("pages", pages), ks, _strides("v_cache", v_cache, 4)
 
 
+def _rope_plan(q, k, v, positions, freqs, k_cache, v_cache, slots, interleaved, amplitude, q_out, status):
+    """(static, the rest of the arguments, device, shape and type of q_out)."""
+    T = _types()
+    t, heads, dim = ffi._rows("q" if k is not None else "x", q, 3)
+    device = ffi._fp8_operands(("positions", positions, T.i32, (t,)), ("freqs", freqs, T.f64, freqs.shape[:1]), ("slots", slots, T.i64, (t,)),
+                               ("status", status, T.i32, (1,)))
+    name, out_name = ("x", "out") if k is None else ("q", "q_out")
+    _like(name, q, T.rows, (t, heads, dim), device)
+    page, kv, pages, out, strides = 0, 0, 0, q.dtype, [0] * 10
+    if k is not None:
+        page, kv, cdim, pages, ks, vs = _cache(k_cache, v_cache, T.halves, device)
+        if cdim != dim:
+            raise R9vxError(-103, f"the cache's head_dim is {cdim}, q's {dim}")
+        _like("k", k, (q.dtype,), (t, kv, dim), device)
+        _like("v", v, (q.dtype,), (t, kv, dim), device)
+        strides, out = _strides("k", k, 3) + _strides("v", v, 3) + ks + vs, k_cache.dtype
+    if q_out is not None:
+        _like(out_name, q_out, (out,), (t, heads, dim), device)
+    to = _strides(out_name, q_out, 3) if q_out is not None else [heads * dim if t > 1 else 0, dim if heads > 1 else 0]
+    st = ffi.RopeKvStatic(*(ffi._u32(n, x) for n, x in (
+        ("heads", heads), ("kv_heads", kv), ("head_dim", dim), ("rot", 2 * freqs.shape[0]), ("interleaved", int(interleaved)), ("page_size", page),
+        ("in_dtype", T.code[q.dtype]), ("out_dtype", T.code[out]), ("amplitude", _number("amplitude", amplitude)))))
+    rest = _ROPE_REST.pack(*_strides(name, q, 3), *strides[:4], *to, *strides[4:], pages, ffi._u32("t", t))
+    return st, ffi.ctypes.byref(st), rest, device, (t, heads, dim), out
+
+
 def rope_kv(q, k, v, positions, freqs, k_cache, v_cache, slots, interleaved=False, amplitude=1.0, q_out=None, status=None,
             stream=None):
     """Turns q [t, heads, head_dim] and k [t, kv_heads, head_dim] by positions
@@ -129,44 +181,25 @@ def rope_kv(q, k, v, positions, freqs, k_cache, v_cache, slots, interleaved=Fals
     on are copied.  q, k and v are f32 or of the cache's type, with strides
     of their own (views of one projection's rows).  Returns q_out, of the cache's
     type; q_out may be q where q has that type."""
-    T = _types()
-    t, heads, dim = ffi._rows("q", q, 3)
-    device = ffi._fp8_operands(("positions", positions, T.i32, (t,)), ("freqs", freqs, T.f64, freqs.shape[:1]), ("slots", slots, T.i64, (t,)),
-                               ("status", status, T.i32, (1,)))
-    page, kv, _, pages, ks, vs = _cache(k_cache, v_cache, T.halves, device)
-    _like("q", q, T.rows, (t, heads, dim), device)
-    _like("k", k, (q.dtype,), (t, kv, dim), device)
-    _like("v", v, (q.dtype,), (t, kv, dim), device)
-    if k_cache.shape[3] != dim:
-        raise R9vxError(-103, f"the cache's head_dim is {k_cache.shape[3]}, q's {dim}")
+    key = ("rope_kv", q.shape, q.stride(), q.dtype, q.get_device(), _meta(k), _meta(v), _meta(positions), _meta(freqs), _meta(k_cache),
+           _meta(v_cache), _meta(slots), interleaved, amplitude, _meta(q_out), _meta(status), ffi._current())
+    _, st, rest, device, shape, out = _plan(key, _rope_plan, q, k, v, positions, freqs, k_cache, v_cache, slots, interleaved, amplitude, q_out, status)
     if q_out is None:
-        q_out = ffi._new(q, (t, heads, dim), k_cache.dtype, stream)
-    else:
-        _like("q_out", q_out, (k_cache.dtype,), (t, heads, dim), device)
-    st, _ = ffi._fp8_static(ffi.RopeKvStatic, lambda st: 0, heads, kv, dim, 2 * freqs.shape[0], int(interleaved), page, T.code[q.dtype],
-                            T.code[k_cache.dtype], _bits(amplitude))
-    args = _ROPE_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), freqs.data_ptr(), q_out.data_ptr(),
-                           k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), ffi._at(status) or 0, *_strides("q", q, 3),
-                           *_strides("k", k, 3), *_strides("v", v, 3), *_strides("q_out", q_out, 3), *ks, *vs, pages, ffi._u32("t", t))
-    ffi._check(ffi.load().r9vx_rope_kv_launch(ffi.ctypes.byref(st), args, ffi._raw_stream(device, stream)))
+        q_out = ffi._new(q, shape, out, stream)
+    args = _ROPE_POINTERS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), freqs.data_ptr(), q_out.data_ptr(),
+                               k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr(), 0 if status is None else status.data_ptr())
+    ffi._check(ffi.load().r9vx_rope_kv_launch(st, args + rest, ffi._raw_stream(device, stream)))
     return q_out
 
 
 def rope(x, positions, freqs, interleaved=False, amplitude=1.0, out=None, stream=None):
     """rope_kv's turn alone: x [t, heads, head_dim] of f32, bf16 or f16; out has x's type and may be x."""
-    T = _types()
-    t, heads, dim = ffi._rows("x", x, 3)
-    device = ffi._fp8_operands(("positions", positions, T.i32, (t,)), ("freqs", freqs, T.f64, freqs.shape[:1]))
-    _like("x", x, T.rows, (t, heads, dim), device)
+    key = ("rope", _meta(x), _meta(positions), _meta(freqs), interleaved, amplitude, _meta(out), ffi._current())
+    _, st, rest, device, shape, dtype = _plan(key, _rope_plan, x, None, None, positions, freqs, None, None, None, interleaved, amplitude, out, None)
     if out is None:
-        out = ffi._new(x, (t, heads, dim), x.dtype, stream)
-    else:
-        _like("out", out, (x.dtype,), (t, heads, dim), device)
-    code = T.code[x.dtype]
-    st, _ = ffi._fp8_static(ffi.RopeKvStatic, lambda st: 0, heads, 0, dim, 2 * freqs.shape[0], int(interleaved), 0, code, code, _bits(amplitude))
-    args = _ROPE_ARGS.pack(x.data_ptr(), 0, 0, positions.data_ptr(), freqs.data_ptr(), out.data_ptr(), 0, 0, 0, 0, *_strides("x", x, 3),
-                           0, 0, 0, 0, *_strides("out", out, 3), 0, 0, 0, 0, 0, 0, 0, ffi._u32("t", t))
-    ffi._check(ffi.load().r9vx_rope_kv_launch(ffi.ctypes.byref(st), args, ffi._raw_stream(device, stream)))
+        out = ffi._new(x, shape, dtype, stream)
+    args = _ROPE_POINTERS.pack(x.data_ptr(), 0, 0, positions.data_ptr(), freqs.data_ptr(), out.data_ptr(), 0, 0, 0, 0)
+    ffi._check(ffi.load().r9vx_rope_kv_launch(st, args + rest, ffi._raw_stream(device, stream)))
     return out
 
 
@@ -178,9 +211,22 @@ def prefill_workspace_bytes(st: ffi.AttnStatic) -> int:
     return int(ffi.load().r9vx_attn_prefill_workspace_bytes(ffi.ctypes.byref(st)))
 
 
-def _pages_of(table, b, page, len_bucket):
-    """(the table's stride, len_bucket)."""
-    stride = _strides("table", table, 2)[0]
+def _attn_plan(q, k_cache, v_cache, table, lengths, offsets, scale, softcap, slopes, causal, window, starts, prefix, out, workspace, status,
+               b_bucket, t_bucket, len_bucket):
+    """(static, its workspace bytes, the rest of the arguments, device); offsets None: decode."""
+    T = _types()
+    F = ffi._Fp8
+    shape = ffi._rows("q", q, 4 if offsets is None else 3)
+    heads, dim = shape[-2:]
+    b = ffi._rows("lengths", lengths, 1)[0]
+    t = shape[0]  # prefill: rows; decode: sequences
+    device = ffi._fp8_operands(("lengths", lengths, T.i32, (t,) if offsets is None else (b,)), ("offsets", offsets, T.i32, (b + 1,)),
+                               ("starts", starts, T.i32, (t,)), ("prefix", prefix, T.i32, (b,)), ("slopes", slopes, F.f32, (heads,)),
+                               ("status", status, T.i32, (1,)), ("workspace", workspace, F.bytes, workspace.shape if workspace is not None else ()))
+    page, kv, cdim, pages, ks, vs = _cache(k_cache, v_cache, T.halves, device)
+    _like("q", q, (k_cache.dtype,), (*shape[:-1], cdim), device)
+    _like("table", table, T.i32, table.shape, device)
+    columns = _strides("table", table, 2)[0]
     if table.shape[0] != b:
         raise R9vxError(-103, f"table has {table.shape[0]} rows: {b} sequences")
     room = table.shape[1] * page
@@ -188,14 +234,20 @@ def _pages_of(table, b, page, len_bucket):
         len_bucket = min(room, 1 << 30)
     elif len_bucket > room:
         raise R9vxError(-103, f"len_bucket={len_bucket}: the table's {table.shape[1]} columns hold {room}")
-    return stride, len_bucket
-
-
-def _check_out(q, out, device, stream):
-    if out is None:
-        return ffi._new(q, q.shape, q.dtype, stream)
-    _like("out", out, (q.dtype,), q.shape, device)
-    return out
+    if out is not None:
+        _like("out", out, (q.dtype,), shape, device)
+        to = _strides("out", out, len(shape))
+    else:
+        to = [math.prod(shape[i + 1:]) if n > 1 else 0 for i, n in enumerate(shape[:-1])]
+    pad = [] if offsets is None else [0]
+    st = ffi.AttnStatic(*(ffi._u32(n, x) for n, x in (
+        ("b_bucket", b_bucket or b), ("t_bucket", shape[1] if offsets is None else t_bucket or t), ("len_bucket", len_bucket), ("heads", heads),
+        ("kv_heads", kv), ("head_dim", dim), ("page_size", page), ("dtype", T.code[q.dtype]), ("causal", int(causal)), ("window", window),
+        ("scale", _number("scale", dim ** -0.5 if scale is None else scale)), ("softcap", _number("softcap", softcap)))))
+    nbytes = (decode_workspace_bytes if offsets is None else prefill_workspace_bytes)(st)
+    rest = _ATTN_REST.pack(*pad, *_strides("q", q, len(shape)), *pad, *to, *ks, *vs, columns, pages, ffi._u32("b", b),
+                           0 if offsets is None else ffi._u32("t", t), 0)
+    return st, ffi.ctypes.byref(st), nbytes, rest, device
 
 
 def decode(q, k_cache, v_cache, table, lengths, scale=None, softcap=0.0, slopes=None, window=0, starts=None, out=None, workspace=None,
@@ -208,22 +260,18 @@ def decode(q, k_cache, v_cache, table, lengths, scale=None, softcap=0.0, slopes=
     distance; window: that many last keys; starts (int32 [b]): no key before it.
     A length of 0 gives zeros.  b_bucket and len_bucket (by default b and what the
     table holds) pick the kernels."""
-    T = _types()
-    b, new, heads, dim = ffi._rows("q", q, 4)
-    device = ffi._fp8_operands(("lengths", lengths, T.i32, (b,)), ("starts", starts, T.i32, (b,)), ("slopes", slopes, ffi._Fp8.f32, (heads,)),
-                               ("status", status, T.i32, (1,)), ("workspace", workspace, ffi._Fp8.bytes, workspace.shape if workspace is not None else ()))
-    page, kv, cdim, pages, ks, vs = _cache(k_cache, v_cache, T.halves, device)
-    _like("q", q, (k_cache.dtype,), (b, new, heads, cdim), device)
-    _like("table", table, T.i32, table.shape, device)
-    stride, len_bucket = _pages_of(table, b, page, len_bucket)
-    st, nbytes = ffi._fp8_static(ffi.AttnStatic, decode_workspace_bytes, b_bucket or b, new, len_bucket, heads, kv, dim, page,
-                                 T.code[q.dtype], 1, window, _bits(dim ** -0.5 if scale is None else scale), _bits(softcap))
-    workspace = ffi._workspace(workspace, nbytes, q, stream)
-    out = _check_out(q, out, device, stream)
-    args = _ATTN_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0, ffi._at(starts) or 0, 0,
-                           ffi._at(slopes) or 0, out.data_ptr(), ffi._at(workspace) or 0, ffi._at(status) or 0, *_strides("q", q, 4),
-                           *_strides("out", out, 4), *ks, *vs, stride, pages, ffi._u32("b", b), 0, 0)
-    ffi._check(ffi.load().r9vx_attn_decode_launch(ffi.ctypes.byref(st), args, ffi._raw_stream(device, stream)))
+    key = ("decode", q.shape, q.stride(), q.dtype, q.get_device(), _meta(k_cache), _meta(v_cache), _meta(table), _meta(lengths), scale, softcap,
+           _meta(slopes), window, _meta(starts), _meta(out), _meta(workspace), _meta(status), b_bucket, len_bucket, ffi._current())
+    _, st, nbytes, rest, device = _plan(key, _attn_plan, q, k_cache, v_cache, table, lengths, None, scale, softcap, slopes, True, window, starts,
+                                        None, out, workspace, status, b_bucket, None, len_bucket)
+    if workspace is not None or nbytes:
+        workspace = ffi._workspace(workspace, nbytes, q, stream)
+    if out is None:
+        out = ffi._new(q, q.shape, q.dtype, stream)
+    args = _ATTN_POINTERS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), 0,
+                               0 if starts is None else starts.data_ptr(), 0, 0 if slopes is None else slopes.data_ptr(), out.data_ptr(),
+                               0 if workspace is None else workspace.data_ptr(), 0 if status is None else status.data_ptr())
+    ffi._check(ffi.load().r9vx_attn_decode_launch(st, args + rest, ffi._raw_stream(device, stream)))
     return out
 
 
@@ -236,23 +284,20 @@ def prefill(q, k_cache, v_cache, table, lengths, offsets, scale=None, softcap=0.
     before its own (the document it is in); prefix (int32 [b]): keys before it are
     seen by all of the sequence's rows.  Rows outside every sequence are left as
     they were.  b_bucket, t_bucket and len_bucket pick the kernels."""
-    T = _types()
-    t, heads, dim = ffi._rows("q", q, 3)
-    b = ffi._rows("lengths", lengths, 1)[0]
-    device = ffi._fp8_operands(("lengths", lengths, T.i32, (b,)), ("offsets", offsets, T.i32, (b + 1,)), ("starts", starts, T.i32, (t,)),
-                               ("prefix", prefix, T.i32, (b,)), ("slopes", slopes, ffi._Fp8.f32, (heads,)), ("status", status, T.i32, (1,)),
-                               ("workspace", workspace, ffi._Fp8.bytes, workspace.shape if workspace is not None else ()))
-    page, kv, cdim, pages, ks, vs = _cache(k_cache, v_cache, T.halves, device)
-    _like("q", q, (k_cache.dtype,), (t, heads, cdim), device)
-    _like("table", table, T.i32, table.shape, device)
-    stride, len_bucket = _pages_of(table, b, page, len_bucket)
-    st, nbytes = ffi._fp8_static(ffi.AttnStatic, prefill_workspace_bytes, b_bucket or b, t_bucket or t, len_bucket, heads, kv, dim, page,
-                                 T.code[q.dtype], int(causal), window, _bits(dim ** -0.5 if scale is None else scale), _bits(softcap))
-    workspace = ffi._workspace(workspace, nbytes, q, stream)
-    out = _check_out(q, out, device, stream)
-    args = _ATTN_ARGS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(),
-                           ffi._at(starts) or 0, ffi._at(prefix) or 0, ffi._at(slopes) or 0, out.data_ptr(), ffi._at(workspace) or 0,
-                           ffi._at(status) or 0, 0, *_strides("q", q, 3), 0, *_strides("out", out, 3), *ks, *vs, stride, pages,
-                           ffi._u32("b", b), ffi._u32("t", t), 0)
-    ffi._check(ffi.load().r9vx_attn_prefill_launch(ffi.ctypes.byref(st), args, ffi._raw_stream(device, stream)))
+    if offsets is None:
+        raise R9vxError(-103, "offsets are required")
+    key = ("prefill", q.shape, q.stride(), q.dtype, q.get_device(), _meta(k_cache), _meta(v_cache), _meta(table), _meta(lengths), _meta(offsets),
+           scale, softcap, _meta(slopes), causal, window, _meta(starts), _meta(prefix), _meta(out), _meta(workspace), _meta(status), b_bucket,
+           t_bucket, len_bucket, ffi._current())
+    _, st, nbytes, rest, device = _plan(key, _attn_plan, q, k_cache, v_cache, table, lengths, offsets, scale, softcap, slopes, causal, window, starts,
+                                        prefix, out, workspace, status, b_bucket, t_bucket, len_bucket)
+    if workspace is not None or nbytes:
+        workspace = ffi._workspace(workspace, nbytes, q, stream)
+    if out is None:
+        out = ffi._new(q, q.shape, q.dtype, stream)
+    args = _ATTN_POINTERS.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), lengths.data_ptr(), offsets.data_ptr(),
+                               0 if starts is None else starts.data_ptr(), 0 if prefix is None else prefix.data_ptr(),
+                               0 if slopes is None else slopes.data_ptr(), out.data_ptr(), 0 if workspace is None else workspace.data_ptr(),
+                               0 if status is None else status.data_ptr())
+    ffi._check(ffi.load().r9vx_attn_prefill_launch(st, args + rest, ffi._raw_stream(device, stream)))
     return out

@@ -476,7 +476,10 @@ void r9vx_attn_decode_plan(r9vx_attn_problem &p) {
     if (parts > kMostParts) parts = kMostParts;
     if (parts < 1) parts = 1;
     uint32_t per = (uint32_t)((most + parts - 1) / parts);
-    if (per > kPartBlocks) per = kPartBlocks;
+    /* a long sequence among short ones ends late in one piece; the more workgroups
+     * there are, the longer its pieces may be */
+    const uint64_t piece = kPartBlocks * (groups > 4 * fill ? groups / (4 * fill) : 1);
+    if (per > piece) per = (uint32_t)piece;
     if (per < (most + kMostParts - 1) / kMostParts) per = (most + kMostParts - 1) / kMostParts;
     per = (per + kWaves - 1) / kWaves * kWaves;
     p.parts = (uint32_t)parts;

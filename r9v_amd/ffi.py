@@ -645,6 +645,12 @@ def _rows(name, t, dims=2):
     return t.shape
 
 
+def _current():
+    """The current device's index."""
+    T = _Fp8.torch or _fp8().torch
+    return T._C._cuda_getDevice() if T.cuda.is_initialized() else -1
+
+
 def _raw_stream(device, stream):
     if stream is None:
         return _Fp8.torch._C._cuda_getCurrentRawStream(device)

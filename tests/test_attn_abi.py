@@ -40,10 +40,13 @@ def test_struct_layouts(tmp_path):
     assert got == want
 
 
-@pytest.mark.parametrize("cls,packed", [(ffi.RopeKvArgs, attn._ROPE_ARGS), (ffi.AttnArgs, attn._ATTN_ARGS)])
-def test_packed_arguments_are_the_struct(cls, packed):
+@pytest.mark.parametrize("cls,pointers,rest", [(ffi.RopeKvArgs, attn._ROPE_POINTERS, attn._ROPE_REST), (ffi.AttnArgs, attn._ATTN_POINTERS, attn._ATTN_REST)])
+def test_packed_arguments_are_the_struct(cls, pointers, rest):
     values = list(range(1, 1 + sum(getattr(t, "_length_", 1) for _, t in cls._fields_)))
-    s = cls.from_buffer_copy(packed.pack(*values))
+    n = len(pointers.unpack(bytes(pointers.size)))
+    data = pointers.pack(*values[:n]) + rest.pack(*values[n:])
+    assert len(data) == ctypes.sizeof(cls)
+    s = cls.from_buffer_copy(data)
     got = []
     for name, _ in cls._fields_:
         v = getattr(s, name)
@@ -207,9 +210,9 @@ def meta(*shape, dtype=torch.float32):
     ("decode", {3: z(2, 4, dtype=I)}, {}, "2 rows"), ("decode", {3: z(3, 4, dtype=L)}, {}, "table is"), ("decode", {}, dict(len_bucket=65), "len_bucket=65"),
     ("decode", {}, dict(out=z(3, 1, 8, 64)), "out is"), ("decode", {}, dict(out=z(3, 2, 8, 64, dtype=B)), "out has shape"),
     ("decode", {}, dict(workspace=z(16, dtype=torch.uint8)), "workspace of 16"), ("decode", {}, dict(window=1 << 32), "32 bits"), ("decode", {}, dict(window=-1), "32 bits"),
-    ("decode", {}, dict(b_bucket=1 << 32), "32 bits"), ("decode", {}, dict(scale=1e300), "no f32"),
-    ("prefill", {0: z(30, 8, 64)}, {}, "q is"), ("prefill", {}, dict(t_bucket=1 << 32), "32 bits"), ("prefill", {}, dict(softcap="a"), "no f32"),
-    ("rope_kv", {1: z(4, 2, 64)}, {}, "k is torch.float32"), ("rope_kv", {2: z(4, 3, 64, dtype=B)}, {}, "v has shape"), ("rope_kv", {0: z(4, 8, 96, dtype=B)}, {}, "k has shape"),
+    ("decode", {}, dict(b_bucket=1 << 32), "32 bits"), ("decode", {}, dict(scale=1e300), "no f32"), ("decode", {}, dict(scale=z(1)), "no number"),
+    ("prefill", {0: z(30, 8, 64)}, {}, "q is"), ("prefill", {}, dict(t_bucket=1 << 32), "32 bits"), ("prefill", {}, dict(softcap="a"), "no number"), ("prefill", {5: None}, {}, "offsets are required"),
+    ("rope_kv", {1: z(4, 2, 64)}, {}, "k is torch.float32"), ("rope_kv", {2: z(4, 3, 64, dtype=B)}, {}, "v has shape"), ("rope_kv", {0: z(4, 8, 96, dtype=B)}, {}, "head_dim is 64"), ("rope_kv", {1: z(4, 3, 64, dtype=B)}, {}, "k has shape"),
     ("rope_kv", {}, dict(q_out=z(4, 8, 64)), "q_out is"), ("rope", {0: z(4, 8, 64, dtype=D)}, {}, "x is torch.float64"), ("rope", {}, dict(out=z(4, 8, 64, dtype=B)), "out is")])
 def test_binding_refusals(name, args, kw, text, on_cpu, monkeypatch):
     monkeypatch.setattr(attn.ffi, "_fp8_operands", lambda *o: 0)
@@ -282,12 +285,12 @@ def test_launches(tmp_path, monkeypatch):
     """Parts and their join where the rows are few; a grid whose threads 32 bits count."""
     monkeypatch.setattr(launch_record, "CHILD", launch_record.CHILD.replace("out = []\n", CHILD + "out = []\n", 1))
     runtime = launch_record.build(tmp_path)
-    calls = [("attn", dict(decode=True)), ("attn", dict(decode=True, b_bucket=2000)), ("attn", dict(decode=True, len_bucket=100)), ("attn", dict(decode=False)),
+    calls = [("attn", dict(decode=True)), ("attn", dict(decode=True, b_bucket=20000)), ("attn", dict(decode=True, len_bucket=100)), ("attn", dict(decode=False)),
              ("attn", dict(decode=False, t_bucket=100000)), ("attn", dict(decode=True, t_bucket=8)), ("attn", dict(decode=False, t_bucket=1 << 23, heads=128, kv_heads=8)),
              ("attn", dict(decode=True, b_bucket=65535, heads=224, kv_heads=224))]
     out = launch_record.record(runtime, calls)
     names = [[n.split("<")[0] for n, _, _ in ls] for _, _, ls in out]
-    assert all(rc == 0 for rc, _, _ in out), [(rc, msg) for rc, msg, _ in out]
+    assert all(rc == 0 for rc, _, _ in out), [msg for rc, msg, _ in out if rc]
     d, p, j = "attn_decode_kernel", "attn_prefill_kernel", "attn_join_kernel"
     assert names == [[d, j], [d], [d], [p, j], [p], [d, j], [p], [d]]
     for _, _, ls in out:
