@@ -159,6 +159,7 @@ int attn_launch(const char *op, bool decode, const r9vx_attn_static *st, const r
     check_strides("out", a->out_stride, 2, pr);
     check_strides("k_cache", a->k_stride, 2, pr);
     check_strides("v_cache", a->v_stride, 2, pr);
+    if (a->k_stride[1] >> 27 || a->v_stride[1] >> 27) pr.add(R9VX_ERR_UNSUPPORTED, "a cache's tokens are 2^27 elements or more apart"); /* 8 rows: 32 bits */
     const size_t ws = pr.code == R9VX_OK ? attn_workspace_bytes(st, decode) : 0;
     if (ws && work && !a->workspace) pr.add(R9VX_ERR_WORKSPACE, "workspace of r9vx_attn_%s_workspace_bytes (%zu) required", decode ? "decode" : "prefill", ws);
     if ((uintptr_t)a->workspace & 255u) pr.add(R9VX_ERR_ALIGN, "workspace must be 256-byte aligned");

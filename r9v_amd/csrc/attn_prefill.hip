@@ -27,23 +27,28 @@ typedef __attribute__((address_space(3))) attn_s4 attn_lds_s4;
 
 template <int D>
 struct PrefillShape {
-    static constexpr int KT = D > 128 ? 32 : 64; /* keys of a tile */
-    static constexpr int CH = D / 8;             /* 16-byte pieces of a key's row */
-    static constexpr int N = KT * CH / 256;      /* of a tile, each thread's */
+    static constexpr int KT = D > 128 ? 32 : 64;             /* keys of a tile */
+    static constexpr int CH = D / 8;                         /* 16-byte pieces of a key's row */
+    static constexpr int R = CH <= 8 ? 8 : CH <= 16 ? 4 : 2; /* rows a wave copies at once, into 1 KiB: neighbours in one page */
+    static constexpr int LANES = R * CH;                     /* of 64: all, or 48 for 96 and 192 columns */
+    static constexpr int N = KT / R / kWaves;                /* copies of a tile's keys each wave makes */
+    static constexpr int TILE = KT / R * 512;                /* elements of a tile's keys (of its values) in LDS */
     /* A row stands in LDS with its pieces' numbers xor-ed by swizzle(row), so that
      * both a score's reads (16 rows, the same piece) and the transposing ones (4
      * rows, 4 neighbouring pieces) meet each of the 64 banks once: rows of 256
-     * bytes and their multiples start in one bank, of 128 in two, of 192 in four. */
+     * bytes and their multiples start in one bank, of 128 and 384 in two, of 192
+     * in four. */
     static __device__ __forceinline__ int swizzle(int r) {
         if constexpr (D == 96) return (r >> 2) & 3;
         else if constexpr (D % 128) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
         else return (r & 3) << 2 | ((r >> 2) & 3);
     }
+    static __device__ __forceinline__ constexpr int row(int r) { return r / R * 512 + r % R * D; } /* its first element in LDS */
 };
 
-/* 16 bytes a lane from global memory to LDS at `at` + 16 * lane (uniform `at`). */
-__device__ __forceinline__ void attn_copy16(uint32_t at, const uint16_t *p) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(at) : "memory", "m0");
+/* 16 bytes a lane from `base` + `off` (bytes) in global memory to LDS at `at` + 16 * lane. */
+__device__ __forceinline__ void attn_copy16(uint32_t at, const uint16_t *base, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory", "m0");
 }
 
 /* Bits of a pair of elements whose exponent is that of an infinity or a NaN. */
@@ -58,7 +63,7 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
     using S = PrefillShape<D>;
     typedef typename T::x8 x8;
     constexpr int KT = S::KT, NK = KT / 32;
-    __shared__ __attribute__((aligned(1024))) uint16_t kv[2][2][KT * D]; /* buffer, keys and values */
+    __shared__ __attribute__((aligned(1024))) uint16_t kv[2][2][S::TILE]; /* buffer, keys and values */
     __shared__ int bounds[kWaves][2];
     __shared__ uint32_t redo, odds[2]; /* odds: keys of a tile with values that are not finite */
 
@@ -128,34 +133,43 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
 
     float m, l;
     r9vx_f32x16 o[D / 32];
-    uint32_t pages[S::N];
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)kv;
 
+    /* Lane j of every wave has the page of the tile's j-th eight keys (page 0 where
+     * nothing of them is seen or the cache has no such page: something has to be
+     * copied, and is replaced in LDS).  Copy i of a wave has rows R (wave + 4 i) ..
+     * of the tile, all in one eight and at the same place in it for every i. */
+    uint32_t page = 0, lacking = 0; /* lacking: eights of the next tile whose page the cache does not have */
+    const int lrow = lane / S::CH, lpiece = lane % S::CH; /* (beyond the rows for lanes that copy nothing) */
+    const int inside = S::R * wave % 8 + lrow;
+    const uint32_t kstep = (uint32_t)(inside * a.k_stride[1] * 2), vstep = (uint32_t)(inside * a.v_stride[1] * 2);
     auto look_up = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < S::N; ++i) {
-            const int key = t * KT + (int)(threadIdx.x + 256 * i) / S::CH;
-            pages[i] = key >= ulo && key < uhi ? (uint32_t)table[key >> a.page_shift] : 0u;
-        }
+        const int key = t * KT + 8 * lane;
+        if (lane < KT / 8) page = key < uhi && key + 8 > ulo ? (uint32_t)table[key >> a.page_shift] : 0u;
     };
     auto load = [&](int t, int buf) {
-        bool bad = false;
+        const bool there = page < a.pages;
+        const uint32_t place = (uint32_t)(t * KT + 8 * lane) & mask, from = there ? page : 0u;
+        lacking = (uint32_t)__ballot(!there);
+        const uint64_t kp = (uint64_t)(kbase + from * a.k_stride[0] + place * a.k_stride[1]), vp = (uint64_t)(vbase + from * a.v_stride[0] + place * a.v_stride[1]);
 #pragma unroll
         for (int i = 0; i < S::N; ++i) {
-            const int c = (int)threadIdx.x + 256 * i, r = c / S::CH, key = t * KT + r, e = 8 * ((c - r * S::CH) ^ S::swizzle(r));
-            const AttnPlace where = attn_place(pages[i], a.pages, key, ulo, uhi);
-            bad |= where == kAttnBad;
-            const uint32_t to = lds + (uint32_t)(buf * 2 * KT * D * 2 + (wave * 64 + 256 * i) * 16);
-            attn_copy16(to, attn_row<T>(where, kbase, a.k_stride, pages[i], (uint32_t)key & mask) + e);
-            attn_copy16(to + KT * D * 2, attn_row<T>(where, vbase, a.v_stride, pages[i], (uint32_t)key & mask) + e);
+            const int c = wave + kWaves * i, eight = S::R * c / 8;
+            const uint32_t e = 16 * (lpiece ^ S::swizzle(S::R * c + lrow)), to = lds + (uint32_t)(buf * 4 * S::TILE + c * 1024);
+            const uint64_t k8 = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(kp >> 32), eight) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)kp, eight);
+            const uint64_t v8 = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(vp >> 32), eight) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)vp, eight);
+            if (S::LANES == 64 || lane < S::LANES) {
+                attn_copy16(to, (const uint16_t *)k8, kstep + e);
+                attn_copy16(to + 2 * S::TILE, (const uint16_t *)v8, vstep + e);
+            }
         }
-        if (bad && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+        if (lacking && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
     };
 
     /* where this lane's pieces are: of key c32 for a score, of keys 4 h2 + lane / 4 % 4 for the values */
-    const int krow = c32 * D, kpiece = h2 ^ S::swizzle(c32);
+    const int krow = S::row(c32), kpiece = h2 ^ S::swizzle(c32);
     const int vkey = 4 * h2 + (lane & 15) / 4, vpiece = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ S::swizzle(vkey);
-    const int vrow = vkey * D + 4 * (lane & 1);
+    const int vrow = S::row(vkey) + 4 * (lane & 1);
 
     /* A first pass; a second one follows only where it gave a NaN or an infinity,
      * which a value that a row does not see may have brought into it through a
@@ -179,29 +193,38 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
             /* this tile has landed, and every wave is done with the other buffer */
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
+            const uint32_t gone = lacking;
             if (t + 1 < end) {
                 load(t + 1, buf ^ 1);
                 if (t + 2 < end) look_up(t + 2);
             }
-            const uint16_t *ks = kv[buf][0];
-            uint16_t *vs = kv[buf][1];
-            if (pass) {
+            uint16_t *ks = kv[buf][0], *vs = kv[buf][1];
+            if (pass || gone || key0 < ulo || key0 + KT > uhi) { /* what stands beside the keys that are seen is no value */
                 if (threadIdx.x == 0) odds[0] = odds[1] = 0;
                 __syncthreads();
+                if (S::LANES == 64 || lane < S::LANES) {
+#pragma unroll 1
+                    for (int i = 0; i < S::N; ++i) {
+                        const int r = S::R * (wave + kWaves * i) + lrow;
+                        r9vx_u32x4 *at = reinterpret_cast<r9vx_u32x4 *>(vs + (wave + kWaves * i) * 512 + 8 * lane);
+                        const bool lost = gone >> (r / 8) & 1u; /* a key that makes NaN of the scores that see it */
+                        if (lost) at[-S::TILE / 8] = r9vx_u32x4{T::kNan, T::kNan, T::kNan, T::kNan};
+                        if (lost || key0 + r < ulo || key0 + r >= uhi) {
+                            *at = r9vx_u32x4{0u, 0u, 0u, 0u};
+                        } else if (pass) {
+                            r9vx_u32x4 w = *at;
+                            uint32_t any = 0;
 #pragma unroll
-                for (int i = 0; i < S::N; ++i) {
-                    const int c = (int)threadIdx.x + 256 * i, r = c / S::CH;
-                    r9vx_u32x4 w = *reinterpret_cast<const r9vx_u32x4 *>(vs + 8 * c);
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t x = attn_odd<T>(w[j]);
-                        any |= x;
-                        w[j] &= ~x;
-                    }
-                    if (any) {
-                        *reinterpret_cast<r9vx_u32x4 *>(vs + 8 * c) = w;
-                        atomicOr(&odds[r / 32], 1u << (r % 32));
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t x = attn_odd<T>(w[j]);
+                                any |= x;
+                                w[j] &= ~x;
+                            }
+                            if (any) {
+                                *at = w;
+                                atomicOr(&odds[r / 32], 1u << (r % 32));
+                            }
+                        }
                     }
                 }
                 __syncthreads();
@@ -216,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
                 for (int s = 0; s < D / 16; ++s)
 #pragma unroll
                     for (int k = 0; k < NK; ++k)
-                        sc[k] = T::mma32(*reinterpret_cast<const x8 *>(ks + 32 * k * D + krow + 8 * (kpiece ^ (2 * s))), q[s], sc[k]);
+                        sc[k] = T::mma32(*reinterpret_cast<const x8 *>(ks + S::row(32 * k) + krow + 8 * (kpiece ^ (2 * s))), q[s], sc[k]);
                 if (a.softcap > 0.0f) {
 #pragma unroll
                     for (int k = 0; k < NK; ++k)
@@ -247,10 +270,12 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
 #pragma unroll
                     for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[k][e]);
                 top = fmaxf(top, attn_swap32(top)) * score.factor;
-                if (__any(top > m)) {
-                    const float now = fmaxf(m, top);
-                    const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - now);
-                    m = now;
+                /* a row's reference moves only where its largest score has grown by 2^8:
+                 * probabilities are then up to 2^8, and sums are rescaled seldom */
+                const bool grown = top > m + kAttnSlack;
+                if (__any(grown)) {
+                    const float f = grown ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+                    m = grown ? top : m;
                     l *= f;
 #pragma unroll
                     for (int d = 0; d < D / 32; ++d)
@@ -260,18 +285,17 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
                 const float ref = (m == -INFINITY ? 0.0f : m) - T::kBits;
                 x8 p[KT / 16];
 #pragma unroll
-                for (int s = 0; s < KT / 16; ++s)
+                for (int s = 0; s < KT / 16; ++s) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], score.factor, -ref));
-                        l += x;
-                        p[s][e] = (typename T::elem)x;
-                    }
+                    for (int e = 0; e < 8; ++e)
+                        p[s][e] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], score.factor, -ref));
+                    l = T::add8(p[s], l); /* of what is multiplied, in f32 */
+                }
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d)
 #pragma unroll
                     for (int s = 0; s < KT / 16; ++s) { /* 8 keys of column 32 d + c32: 16 s + 4 h2 .. + 3 and 8 further */
-                        uint16_t *v = vs + 16 * s * D + vrow + 8 * (vpiece ^ (4 * d)), *w = vs + (16 * s + 8) * D + vrow + 8 * (vpiece ^ (4 * d) ^ 2);
+                        uint16_t *v = vs + S::row(16 * s) + vrow + 8 * (vpiece ^ (4 * d)), *w = vs + S::row(16 * s + 8) + vrow + 8 * (vpiece ^ (4 * d) ^ 2);
                         const attn_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)v), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)w);
                         o[d] = T::mma32(__builtin_bit_cast(x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), p[s], o[d]);
                     }
@@ -279,8 +303,8 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
                     for (int r = 0; r < KT; ++r) {
                         const int key = key0 + r;
                         if (!(odds[r / 32] >> (r % 32) & 1u) || key < lo || key >= hi) continue;
-                        const uint32_t page = (uint32_t)table[key >> a.page_shift];
-                        const uint16_t *v = attn_row<T>(attn_place(page, a.pages, key, ulo, uhi), vbase, a.v_stride, page, (uint32_t)key & mask);
+                        const uint32_t own = (uint32_t)table[key >> a.page_shift];
+                        const uint16_t *v = attn_row<T>(attn_place(own, a.pages, key, ulo, uhi), vbase, a.v_stride, own, (uint32_t)key & mask);
 #pragma unroll
                         for (int d = 0; d < D / 32; ++d)
 #pragma unroll

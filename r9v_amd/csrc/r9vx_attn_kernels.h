@@ -60,21 +60,37 @@ typedef uint32_t attn_u32x3 __attribute__((ext_vector_type(3)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+/* How far (in powers of two) a row's largest score may be above its reference. */
+constexpr float kAttnSlack = 8.0f;
+
 /* The two element types.  kBits is added to every exponent of a probability:
- * f16 holds 2^-24 at the least, so the largest is made 2^15 there. */
+ * f16 holds 2^-24 at the least, so they are made up to 2^15 there. */
 struct AttnBf16 {
     typedef r9vx_bf16x8 x8;
     typedef __bf16 elem;
     static constexpr float kBits = 0.0f;
     static constexpr uint32_t kNan = 0x7FC07FC0u;
+    /* c and the eight elements, in f32 */
+    static __device__ __forceinline__ float add8(x8 x, float c) {
+        const r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = r9vx_dot2_bf16(w[i], 0x3F803F80u, c);
+        return c;
+    }
     static __device__ __forceinline__ r9vx_f32x4 mma16(x8 a, x8 b, r9vx_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ r9vx_f32x16 mma32(x8 a, x8 b, r9vx_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 struct AttnF16 {
     typedef attn_f16x8 x8;
     typedef _Float16 elem;
-    static constexpr float kBits = 15.0f;
+    static constexpr float kBits = 15.0f - kAttnSlack;
     static constexpr uint32_t kNan = 0x7E007E00u;
+    static __device__ __forceinline__ float add8(x8 x, float c) {
+        const r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = r9vx_dot2_f16(w[i], 0x3C003C00u, c);
+        return c;
+    }
     static __device__ __forceinline__ r9vx_f32x4 mma16(x8 a, x8 b, r9vx_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ r9vx_f32x16 mma32(x8 a, x8 b, r9vx_f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };

@@ -120,7 +120,7 @@ BOTH = [
     (dict(pages=0), INVALID, "no page"), (dict(pages=(1 << 31) + 1), UNSUPPORTED, "2^31"), (dict(k_cache=ATTN["k_cache"] + 8), ALIGN, "16-byte"),
     (dict(table=ATTN["table"] + 1), ALIGN, "4-byte"), (dict(status=ATTN["status"] + 2), ALIGN, "4-byte"),
     (dict(q_stride=(2048, 1028, 128)), ALIGN, "q: a stride"), (dict(out_stride=(2048, 1024, 1)), ALIGN, "out: a stride"),
-    (dict(v_stride=(4097, 256, 128)), ALIGN, "v_cache: a stride"), (dict(workspace=None, len_bucket=4096, table_stride=256), WORKSPACE, "workspace"),
+    (dict(v_stride=(4097, 256, 128)), ALIGN, "v_cache: a stride"), (dict(k_stride=(4096, 1 << 27, 128)), UNSUPPORTED, "2^27 elements"), (dict(workspace=None, len_bucket=4096, table_stride=256), WORKSPACE, "workspace"),
     (dict(workspace=ATTN["workspace"] + 16), ALIGN, "256-byte"), (dict(table_stride=31), INVALID, "columns apart"),
     (dict(out=ATTN["q"]), INVALID, "out must not overlap"), (dict(out=ATTN["v_cache"] + 4096), INVALID, "out must not overlap"),
     (dict(out=ATTN["lengths"]), INVALID, "out must not overlap"), (dict(workspace=ATTN["out"], len_bucket=600), INVALID, "workspace must not overlap"),
