@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kRows = 128; /* of a workgroup */
 constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
 
 typedef short attn_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) attn_s4 attn_lds_s4;
@@ -46,9 +47,23 @@ struct PrefillShape {
     static __device__ __forceinline__ constexpr int row(int r) { return r / R * 512 + r % R * D; } /* its first element in LDS */
 };
 
-/* 16 bytes a lane from `base` + `off` (bytes) in global memory to LDS at `at` + 16 * lane. */
-__device__ __forceinline__ void attn_copy16(uint32_t at, const uint16_t *base, uint32_t off) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory", "m0");
+/* 16 bytes of each lane of `lanes` from `base` + `off` (bytes) in global memory to LDS at
+ * `at` + 16 * lane.  Within straight-line code: a branch around it would cut the
+ * schedule in pieces.  (No "memory": it writes a buffer that is read behind the next
+ * barrier alone, and may stand among reads of the other.) */
+__device__ __forceinline__ void attn_copy16(uint32_t at, const uint16_t *base, uint32_t off, uint64_t lanes) {
+    uint64_t all;
+    asm volatile("s_mov_b32 m0, %3\n\ts_and_saveexec_b64 %0, %4\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, %0"
+                 : "=&s"(all) : "v"(off), "s"(base), "s"(at), "s"(lanes) : "m0", "scc");
+}
+
+/* Holds what makes x before what follows: pure arithmetic is otherwise moved to its use,
+ * behind the barriers that part the phases. */
+template <class X>
+__device__ __forceinline__ void attn_pin(X &x) {
+    r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, x);
+    asm volatile("" : "+v"(w));
+    x = __builtin_bit_cast(X, w);
 }
 
 /* Bits of a pair of elements whose exponent is that of an infinity or a NaN. */
@@ -58,14 +73,26 @@ __device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
     return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
 }
 
-template <class T, int D>
-__global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem a, uint32_t tiles) {
+template <int D>
+struct PrefillShared {
+    __attribute__((aligned(1024))) uint16_t kv[4][PrefillShape<D>::TILE]; /* keys of two tiles, values of two */
+    int bounds[kWaves][2];
+    uint32_t redo, odds[2]; /* odds: keys of a tile with values that are not finite */
+};
+
+/* A workgroup's rows.  CAREFUL: the second way through, which a workgroup takes where
+ * the first one gave a NaN or an infinity: a value that a row does not see may have
+ * brought it in through a probability of zero.  It takes such values out of LDS, and
+ * adds each to the rows that see its key (times a probability, a NaN or an infinity is
+ * itself).  Returns whether the second way has to be taken (nothing is written then). */
+template <class T, int D, bool CAREFUL>
+__device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, uint32_t tiles, PrefillShared<D> &sh) {
     using S = PrefillShape<D>;
     typedef typename T::x8 x8;
     constexpr int KT = S::KT, NK = KT / 32;
-    __shared__ __attribute__((aligned(1024))) uint16_t kv[2][2][S::TILE]; /* buffer, keys and values */
-    __shared__ int bounds[kWaves][2];
-    __shared__ uint32_t redo, odds[2]; /* odds: keys of a tile with values that are not finite */
+    auto &kv = sh.kv;
+    auto &bounds = sh.bounds;
+    auto &odds = sh.odds;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h2 = lane >> 5;
     uint32_t id = blockIdx.x;
@@ -76,24 +103,24 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
 
     if (tile == 0 && kvh == 0 && split == 0 && a.status) {
         bool odd = false;
-        for (uint32_t i = threadIdx.x; i < a.b; i += 256) odd |= a.offsets[i] < 0 || a.offsets[i] > a.offsets[i + 1] || (int64_t)a.offsets[i + 1] > a.t;
+        for (uint32_t i = threadIdx.x; i < a.b; i += kThreads) odd |= a.offsets[i] < 0 || a.offsets[i] > a.offsets[i + 1] || (int64_t)a.offsets[i + 1] > a.t;
         if (odd) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
     }
     AttnTile part;
-    if (!attn_tile(a.offsets, a.b, a.t, a.group, kRows, tile, part)) return;
+    if (!attn_tile(a.offsets, a.b, a.t, a.group, kRows, tile, part)) return false;
     const uint32_t b = part.b, r0 = part.row;
-    const int off = part.offset, n = part.n;
+    const int off = part.offset, news = part.n;
     const int length = a.lengths[b];
     const bool bad_length = length < 0 || length > (int)a.len_bucket;
     if (bad_length && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
 
     /* this lane's row */
     const uint32_t row = r0 + wave * 32 + c32;
-    const bool there = row < (uint64_t)n * a.group;
+    const bool there = row < (uint64_t)news * a.group;
     const int token = there ? (int)(row / a.group) : 0;
     const uint32_t head = kvh * a.group + (there ? row - token * a.group : 0);
     const uint64_t at = (uint64_t)off + token;
-    const int pos = length - n + token;
+    const int pos = length - news + token;
     int lo, hi;
     attn_seen(a.window, a.causal, pos, length, a.starts ? a.starts[at] : 0, a.prefix ? a.prefix[b] : 0, lo, hi);
     if (!there || bad_length) lo = hi = 0;
@@ -116,10 +143,12 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
     wlo = __builtin_amdgcn_readfirstlane(wlo), whi = __builtin_amdgcn_readfirstlane(whi);
     wfl = __builtin_amdgcn_readfirstlane(wfl), wfh = __builtin_amdgcn_readfirstlane(wfh);
     if (lane == 0) bounds[wave][0] = wlo, bounds[wave][1] = whi;
-    if (threadIdx.x == 0) redo = 0;
+    if (!CAREFUL && threadIdx.x == 0) sh.redo = 0; /* (the second way is on while other waves read it) */
     __syncthreads();
-    const int ulo = min(min(bounds[0][0], bounds[1][0]), min(bounds[2][0], bounds[3][0]));
-    const int uhi = max(max(bounds[0][1], bounds[1][1]), max(bounds[2][1], bounds[3][1]));
+    int ulo = INT32_MAX, uhi = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) ulo = min(ulo, bounds[i][0]), uhi = max(uhi, bounds[i][1]);
+    ulo = __builtin_amdgcn_readfirstlane(ulo), uhi = __builtin_amdgcn_readfirstlane(uhi);
 
     /* this part's tiles */
     const int t0 = ulo < uhi ? ulo / KT : 0, t1 = ulo < uhi ? (uhi + KT - 1) / KT : 0;
@@ -133,37 +162,36 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
 
     float m, l;
     r9vx_f32x16 o[D / 32];
+    constexpr uint32_t kTileBytes = 2 * S::TILE;
+    constexpr uint64_t kLanes = ~0ull >> (64 - S::LANES);
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)kv;
 
     /* Lane j of every wave has the page of the tile's j-th eight keys (page 0 where
      * nothing of them is seen or the cache has no such page: something has to be
      * copied, and is replaced in LDS).  Copy i of a wave has rows R (wave + 4 i) ..
      * of the tile, all in one eight and at the same place in it for every i. */
-    uint32_t page = 0, lacking = 0; /* lacking: eights of the next tile whose page the cache does not have */
     const int lrow = lane / S::CH, lpiece = lane % S::CH; /* (beyond the rows for lanes that copy nothing) */
     const int inside = S::R * wave % 8 + lrow;
     const uint32_t kstep = (uint32_t)(inside * a.k_stride[1] * 2), vstep = (uint32_t)(inside * a.v_stride[1] * 2);
-    auto look_up = [&](int t) {
+    /* (nothing is done with what is loaded until the tile is copied: a wait here would be
+     * one for the copies under way) */
+    auto page_of = [&](int t) -> uint32_t {
         const int key = t * KT + 8 * lane;
-        if (lane < KT / 8) page = key < uhi && key + 8 > ulo ? (uint32_t)table[key >> a.page_shift] : 0u;
+        return (uint32_t)table[(lane < KT / 8 && key < uhi && key + 8 > ulo ? key : ulo) >> a.page_shift];
     };
-    auto load = [&](int t, int buf) {
-        const bool there = page < a.pages;
-        const uint32_t place = (uint32_t)(t * KT + 8 * lane) & mask, from = there ? page : 0u;
-        lacking = (uint32_t)__ballot(!there);
-        const uint64_t kp = (uint64_t)(kbase + from * a.k_stride[0] + place * a.k_stride[1]), vp = (uint64_t)(vbase + from * a.v_stride[0] + place * a.v_stride[1]);
-#pragma unroll
-        for (int i = 0; i < S::N; ++i) {
-            const int c = wave + kWaves * i, eight = S::R * c / 8;
-            const uint32_t e = 16 * (lpiece ^ S::swizzle(S::R * c + lrow)), to = lds + (uint32_t)(buf * 4 * S::TILE + c * 1024);
-            const uint64_t k8 = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(kp >> 32), eight) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)kp, eight);
-            const uint64_t v8 = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(vp >> 32), eight) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)vp, eight);
-            if (S::LANES == 64 || lane < S::LANES) {
-                attn_copy16(to, (const uint16_t *)k8, kstep + e);
-                attn_copy16(to + 2 * S::TILE, (const uint16_t *)v8, vstep + e);
-            }
-        }
-        if (lacking && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+    auto no_page = [&](int t, uint32_t page) -> bool {
+        const int key = t * KT + 8 * lane;
+        return lane < KT / 8 && key < uhi && key + 8 > ulo && page >= a.pages;
+    };
+    /* where tile t's eights begin, in lane j's registers; copy i of them into a buffer */
+    auto source = [&](int t, uint32_t page, const uint16_t *base, const uint64_t *stride) -> uint64_t {
+        const uint32_t place = (uint32_t)(t * KT + 8 * lane) & mask, from = page < a.pages ? page : 0u;
+        return (uint64_t)(base + from * stride[0] + place * stride[1]);
+    };
+    auto copy = [&](int i, uint64_t p, uint32_t step, uint32_t at, uint64_t on) {
+        const int c = wave + kWaves * i, eight = S::R * c / 8;
+        const uint64_t p8 = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), eight) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)p, eight);
+        attn_copy16(__builtin_amdgcn_readfirstlane(lds + at + c * 1024), (const uint16_t *)p8, step + 16 * (lpiece ^ S::swizzle(S::R * c + lrow)), on);
     };
 
     /* where this lane's pieces are: of key c32 for a score, of keys 4 h2 + lane / 4 % 4 for the values */
@@ -171,164 +199,193 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
     const int vkey = 4 * h2 + (lane & 15) / 4, vpiece = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ S::swizzle(vkey);
     const int vrow = S::row(vkey) + 4 * (lane & 1);
 
-    /* A first pass; a second one follows only where it gave a NaN or an infinity,
-     * which a value that a row does not see may have brought into it through a
-     * probability of zero.  The second pass takes such values out of LDS, and
-     * adds each to the rows that see its key (times a probability, a NaN or an
-     * infinity is itself). */
-    for (int pass = 0; pass < 2; ++pass) {
-        m = -INFINITY, l = 0.0f;
+    const int n = end - begin;
+    constexpr int kEach = (2 * S::N + D / 16 - 1) / (D / 16); /* copies beside a score's step */
+    static_assert(kEach * (D / 16) >= 2 * S::N);
+
+    m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < D / 32; ++d)
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
-        if (begin < end) {
-            look_up(begin);
-            load(begin, 0);
-            if (begin + 1 < end) look_up(begin + 1);
-        }
-        for (int t = begin; t < end; ++t) {
-            const int buf = (t - begin) & 1;
-            const int key0 = t * KT;
-            /* this tile has landed, and every wave is done with the other buffer */
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            const uint32_t gone = lacking;
-            if (t + 1 < end) {
-                load(t + 1, buf ^ 1);
-                if (t + 2 < end) look_up(t + 2);
-            }
-            uint16_t *ks = kv[buf][0], *vs = kv[buf][1];
-            if (pass || gone || key0 < ulo || key0 + KT > uhi) { /* what stands beside the keys that are seen is no value */
-                if (threadIdx.x == 0) odds[0] = odds[1] = 0;
-                __syncthreads();
-                if (S::LANES == 64 || lane < S::LANES) {
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+    r9vx_f32x16 sc[NK];
+    x8 p[KT / 16];
+
+    /* Tile t (of n) has landed.  What stands beside the keys that are seen is no value, a
+     * key of a page that is not there makes NaN of the scores that see it. */
+    auto landed = [&](int t, uint32_t no) {
+        const int key0 = (begin + t) * KT;
+        if (!(CAREFUL || no || key0 < ulo || key0 + KT > uhi)) return;
+        if (CAREFUL && threadIdx.x == 0) odds[0] = odds[1] = 0;
+        if (no && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+        if (CAREFUL) __syncthreads();
+        if (S::LANES == 64 || lane < S::LANES) {
 #pragma unroll 1
-                    for (int i = 0; i < S::N; ++i) {
-                        const int r = S::R * (wave + kWaves * i) + lrow;
-                        r9vx_u32x4 *at = reinterpret_cast<r9vx_u32x4 *>(vs + (wave + kWaves * i) * 512 + 8 * lane);
-                        const bool lost = gone >> (r / 8) & 1u; /* a key that makes NaN of the scores that see it */
-                        if (lost) at[-S::TILE / 8] = r9vx_u32x4{T::kNan, T::kNan, T::kNan, T::kNan};
-                        if (lost || key0 + r < ulo || key0 + r >= uhi) {
-                            *at = r9vx_u32x4{0u, 0u, 0u, 0u};
-                        } else if (pass) {
-                            r9vx_u32x4 w = *at;
-                            uint32_t any = 0;
+            for (int i = 0; i < S::N; ++i) {
+                const int c = wave + kWaves * i, r = S::R * c + lrow;
+                r9vx_u32x4 *at = reinterpret_cast<r9vx_u32x4 *>(kv[2 + (t & 1)] + c * 512 + 8 * lane);
+                const bool lost = no >> (r / 8) & 1u;
+                if (lost) *reinterpret_cast<r9vx_u32x4 *>(kv[t & 1] + c * 512 + 8 * lane) = r9vx_u32x4{T::kNan, T::kNan, T::kNan, T::kNan};
+                if (lost || key0 + r < ulo || key0 + r >= uhi) {
+                    *at = r9vx_u32x4{0u, 0u, 0u, 0u};
+                } else if (CAREFUL) {
+                    r9vx_u32x4 w = *at;
+                    uint32_t any = 0;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint32_t x = attn_odd<T>(w[j]);
-                                any |= x;
-                                w[j] &= ~x;
-                            }
-                            if (any) {
-                                *at = w;
-                                atomicOr(&odds[r / 32], 1u << (r % 32));
-                            }
-                        }
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t x = attn_odd<T>(w[j]);
+                        any |= x;
+                        w[j] &= ~x;
+                    }
+                    if (any) {
+                        *at = w;
+                        atomicOr(&odds[r / 32], 1u << (r % 32));
                     }
                 }
-                __syncthreads();
             }
-            if (key0 < whi && key0 + KT > wlo) {
-                r9vx_f32x16 sc[NK];
+        }
+        __syncthreads();
+    };
+
+    if (n > 0) {
+        uint32_t page = page_of(begin);
+        uint64_t kp = source(begin, page, kbase, a.k_stride), vp = source(begin, page, vbase, a.v_stride);
+        uint32_t no = (uint32_t)__ballot(no_page(begin, page));
+#pragma unroll
+        for (int i = 0; i < S::N; ++i) copy(i, kp, kstep, 0, kLanes), copy(i, vp, vstep, 2 * kTileBytes, kLanes);
+        page = page_of(begin + 1);
+        for (int t = 0; t < n; ++t) {
+            const int buf = t & 1, key0 = (begin + t) * KT;
+            /* this tile has landed, and every wave is done with the other buffers */
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            asm volatile("" : "+v"(page)); /* used before the copies go out: a wait for it behind would be one for the copies */
+            __syncthreads();
+            landed(t, no);
+            const bool more = t + 1 < n;
+            no = more ? (uint32_t)__ballot(no_page(begin + t + 1, page)) : 0u;
+            const uint32_t to = (buf ^ 1) * kTileBytes;
+            const uint64_t lanes = (uint64_t)__builtin_amdgcn_readfirstlane(more ? (uint32_t)(kLanes >> 32) : 0u) << 32 | __builtin_amdgcn_readfirstlane(more ? ~0u : 0u);
+            kp = source(begin + t + 1, page, kbase, a.k_stride), vp = source(begin + t + 1, page, vbase, a.v_stride);
+            page = page_of(begin + t + 2);
+            const uint16_t *ks = kv[buf];
+            uint16_t *vs = kv[2 + buf];
+#pragma unroll
+            for (int k = 0; k < NK; ++k)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[k][e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+#pragma unroll
+                for (int k = 0; k < NK; ++k)
+                    sc[k] = T::mma32(*reinterpret_cast<const x8 *>(ks + S::row(32 * k) + krow + 8 * (kpiece ^ (2 * s))), q[s], sc[k]);
+#pragma unroll
+                for (int i = s * kEach; i < (s + 1) * kEach && i < 2 * S::N; ++i)
+                    if (i < S::N) copy(i, kp, kstep, to, lanes);
+                    else copy(i - S::N, vp, vstep, to + 2 * kTileBytes, lanes);
+            }
+            /* two steps' keys are on their way while a step's are multiplied */
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * NK, 0);
+#pragma unroll
+            for (int s = 0; s < D / 16 - 2; ++s) {
+                __builtin_amdgcn_sched_group_barrier(0x8, NK, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, NK, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, 2 * NK, 0);
+            if (a.softcap > 0.0f) {
 #pragma unroll
                 for (int k = 0; k < NK; ++k)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) sc[k][e] = 0.0f;
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-                    for (int k = 0; k < NK; ++k)
-                        sc[k] = T::mma32(*reinterpret_cast<const x8 *>(ks + S::row(32 * k) + krow + 8 * (kpiece ^ (2 * s))), q[s], sc[k]);
-                if (a.softcap > 0.0f) {
-#pragma unroll
-                    for (int k = 0; k < NK; ++k)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) sc[k][e] = score.capped(sc[k][e]);
-                }
-                if (a.slopes) {
-                    const float far = (float)(pos - key0 - 4 * h2);
-#pragma unroll
-                    for (int k = 0; k < NK; ++k)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            sc[k][e] = fmaf(-slope, fabsf(far - (float)(32 * k + 8 * (e >> 2) + (e & 3))), sc[k][e] * score.before);
-                }
-                if (key0 < wfl || key0 + KT > wfh) {
-                    const int from = lo - key0 - 4 * h2, to = hi - key0 - 4 * h2;
-#pragma unroll
-                    for (int k = 0; k < NK; ++k)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int key = 32 * k + 8 * (e >> 2) + (e & 3);
-                            if (key < from || key >= to) sc[k][e] = -INFINITY;
-                        }
-                }
-                float top = -INFINITY;
+                    for (int e = 0; e < 16; ++e) sc[k][e] = score.capped(sc[k][e]);
+            }
+            if (a.slopes) {
+                const float far = (float)(pos - key0 - 4 * h2);
 #pragma unroll
                 for (int k = 0; k < NK; ++k)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[k][e]);
-                top = fmaxf(top, attn_swap32(top)) * score.factor;
-                /* a row's reference moves only where its largest score has grown by 2^8:
-                 * probabilities are then up to 2^8, and sums are rescaled seldom */
-                const bool grown = top > m + kAttnSlack;
-                if (__any(grown)) {
-                    const float f = grown ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-                    m = grown ? top : m;
-                    l *= f;
+                    for (int e = 0; e < 16; ++e)
+                        sc[k][e] = fmaf(-slope, fabsf(far - (float)(32 * k + 8 * (e >> 2) + (e & 3))), sc[k][e] * score.before);
+            }
+            if (key0 < wfl || key0 + KT > wfh) {
+                const int from = lo - key0 - 4 * h2, to = hi - key0 - 4 * h2;
 #pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
+                for (int k = 0; k < NK; ++k)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[d][e] *= f;
-                }
-                const float ref = (m == -INFINITY ? 0.0f : m) - T::kBits;
-                x8 p[KT / 16];
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = 32 * k + 8 * (e >> 2) + (e & 3);
+                        if (key < from || key >= to) sc[k][e] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
 #pragma unroll
-                for (int s = 0; s < KT / 16; ++s) {
+            for (int k = 0; k < NK; ++k)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        p[s][e] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], score.factor, -ref));
-                    l = T::add8(p[s], l); /* of what is multiplied, in f32 */
-                }
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[k][e]);
+            top = attn_max32(top) * score.factor;
+            /* a row's reference moves only where its largest score has grown by 2^8:
+             * probabilities are then up to 2^8, and sums are rescaled seldom */
+            const bool grown = top > m + kAttnSlack;
+            if (__any(grown)) {
+                const float f = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 1.0f; /* (sums before the first score: zeros, or what is no number) */
+                m = grown ? top : m;
+                l *= f;
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-                    for (int s = 0; s < KT / 16; ++s) { /* 8 keys of column 32 d + c32: 16 s + 4 h2 .. + 3 and 8 further */
-                        uint16_t *v = vs + S::row(16 * s) + vrow + 8 * (vpiece ^ (4 * d)), *w = vs + S::row(16 * s + 8) + vrow + 8 * (vpiece ^ (4 * d) ^ 2);
-                        const attn_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)v), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)w);
-                        o[d] = T::mma32(__builtin_bit_cast(x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), p[s], o[d]);
-                    }
-                if (pass) {
-                    for (int r = 0; r < KT; ++r) {
-                        const int key = key0 + r;
-                        if (!(odds[r / 32] >> (r % 32) & 1u) || key < lo || key >= hi) continue;
-                        const uint32_t own = (uint32_t)table[key >> a.page_shift];
-                        const uint16_t *v = attn_row<T>(attn_place(own, a.pages, key, ulo, uhi), vbase, a.v_stride, own, (uint32_t)key & mask);
+                    for (int e = 0; e < 16; ++e) o[d][e] *= f;
+            }
+            const float ref = (m == -INFINITY ? 0.0f : m) - T::kBits;
 #pragma unroll
-                        for (int d = 0; d < D / 32; ++d)
+            for (int s = 0; s < KT / 16; ++s) {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const uint16_t x = v[32 * d + 8 * (e >> 2) + 4 * h2 + (e & 3)];
-                                if (attn_odd<T>(x)) o[d][e] += (float)__builtin_bit_cast(typename T::elem, x);
-                            }
-                    }
+                for (int e = 0; e < 8; ++e)
+                    p[s][e] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], score.factor, -ref));
+                l = T::add8(p[s], l); /* of what is multiplied, in f32 */
+            }
+#pragma unroll
+            for (int s = 0; s < KT / 16; ++s)
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) { /* 8 keys of column 32 d + c32: 16 s + 4 h2 .. + 3 and 8 further */
+                    uint16_t *v = vs + S::row(16 * s) + vrow + 8 * (vpiece ^ (4 * d)), *w = vs + S::row(16 * s + 8) + vrow + 8 * (vpiece ^ (4 * d) ^ 2);
+                    const attn_s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)v), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((attn_lds_s4 *)w);
+                    o[d] = T::mma32(__builtin_bit_cast(x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), p[s], o[d]);
+                }
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * 4, 0);
+#pragma unroll
+            for (int s = 0; s < KT / 16 * (D / 32) - 4; ++s) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+            if (CAREFUL) {
+#pragma unroll 1
+                for (int r = 0; r < KT; ++r) {
+                    const int key = key0 + r;
+                    if (!(odds[r / 32] >> (r % 32) & 1u) || key < lo || key >= hi) continue;
+                    const uint32_t own = (uint32_t)table[key >> a.page_shift];
+                    const uint16_t *v = vbase + own * a.v_stride[0] + ((uint32_t)key & mask) * a.v_stride[1]; /* (a page that is not there has no odd value) */
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint16_t x = v[32 * d + 8 * (e >> 2) + 4 * h2 + (e & 3)];
+                            if (attn_odd<T>(x)) o[d][e] += (float)__builtin_bit_cast(typename T::elem, x);
+                        }
                 }
             }
         }
-        l += attn_swap32(l);
-        bool odd = !(fabsf(l) < INFINITY);
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) odd |= !(fabsf(o[d][e]) < INFINITY);
-        if (pass == 0) {
-            if (__any(odd && there) && lane == 0) redo = 1;
-            __syncthreads();
-            if (!redo) break;
-        }
     }
-    if (!there) return;
+    l += attn_swap32(l);
+    bool odd = !(fabsf(l) < INFINITY);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) odd |= !(fabsf(o[d][e]) < INFINITY);
+    if (!CAREFUL) {
+        if (__any(odd && there) && lane == 0) sh.redo = 1;
+        __syncthreads();
+        if (sh.redo) return true;
+    }
+    if (!there) return false;
     float sum = l, top = m;
     if (bad_length || (sum != sum && top == -INFINITY)) top = 0.0f; /* a NaN that counts beside any other part */
     if (bad_length || (sum == 0.0f && top == -INFINITY && max(lo, begin * KT) < min(hi, end * KT))) sum = __builtin_nanf("");
@@ -355,12 +412,29 @@ __global__ __launch_bounds__(256, 2) void attn_prefill_kernel(r9vx_attn_problem 
             ml[r] = make_float2(top, sum);
         }
     }
+    return false;
+}
+
+typedef __attribute__((address_space(4))) const r9vx_attn_problem attn_kernel_args;
+
+/* Out of line: nothing of it takes registers of the first way's loop. */
+template <class T, int D>
+__device__ __attribute__((noinline)) void attn_prefill_careful(attn_kernel_args *args, uint32_t tiles, __attribute__((address_space(3))) PrefillShared<D> *sh) {
+    const r9vx_attn_problem a = *(const r9vx_attn_problem *)args;
+    attn_prefill_rows<T, D, true>(a, tiles, *(PrefillShared<D> *)sh);
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, 2) void attn_prefill_kernel(r9vx_attn_problem a, uint32_t tiles) {
+    __shared__ PrefillShared<D> sh;
+    if (attn_prefill_rows<T, D, false>(a, tiles, sh))
+        attn_prefill_careful<T, D>((attn_kernel_args *)__builtin_amdgcn_kernarg_segment_ptr(), tiles, (__attribute__((address_space(3))) PrefillShared<D> *)&sh);
 }
 
 template <class T>
 int launch_prefill(const r9vx_attn_problem &p, hipStream_t stream) {
     const uint32_t tiles = attn_tiles(p.t, p.b, p.group, kRows);
-    const dim3 grid((unsigned)r9vx_attn_prefill_groups(p)), block(256);
+    const dim3 grid((unsigned)r9vx_attn_prefill_groups(p)), block(kThreads);
     switch (p.head_dim) {
     case 64: hipLaunchKernelGGL((attn_prefill_kernel<T, 64>), grid, block, 0, stream, p, tiles); break;
     case 96: hipLaunchKernelGGL((attn_prefill_kernel<T, 96>), grid, block, 0, stream, p, tiles); break;

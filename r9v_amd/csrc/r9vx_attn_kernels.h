@@ -154,6 +154,14 @@ __device__ __forceinline__ const uint16_t *attn_row(AttnPlace where, const uint1
     return where == kAttnKept ? p : where == kAttnBad ? attn_nan_row<T>() : reinterpret_cast<const uint16_t *>(kAttnZeroRow);
 }
 
+/* The larger of the two half waves' values. */
+__device__ __forceinline__ float attn_max32(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+
 /* The other half wave's value. */
 __device__ __forceinline__ float attn_swap32(float x) { return __shfl_xor(x, 32, R9VX_WAVE); }
 
