@@ -169,7 +169,11 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
         if (row >= rows || bad_length) lo[r] = hi[r] = 0;
         slope[r] = a.slopes && row < rows ? a.slopes[kvh * a.group + (row - tok * (int)a.group)] * kLog2e : 0.0f;
 #pragma unroll
-        for (int s = 0; s < S::KS; ++s) q[r][s] = attn_query<T>(a, mine + col * S::KP + s * 32 + g4 * 8);
+        for (int s = 0; s < S::KS; ++s) q[r][s] = *reinterpret_cast<const x8 *>(mine + col * S::KP + s * 32 + g4 * 8);
+        if (a.scale <= 0.0f) {
+#pragma unroll
+            for (int s = 0; s < S::KS; ++s) q[r][s] = attn_signed<T>(a, q[r][s]);
+        }
     }
     const AttnScore score(a);
 

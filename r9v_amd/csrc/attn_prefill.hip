@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
 template <int D>
 struct PrefillShared {
     __attribute__((aligned(1024))) uint16_t kv[4][PrefillShape<D>::TILE]; /* keys of two tiles, values of two */
-    int bounds[kWaves][2];
+    int bounds[kWaves];
     uint32_t redo, odds[2]; /* odds: keys of a tile with values that are not finite */
 };
 
@@ -126,29 +126,38 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     if (!there || bad_length) lo = hi = 0;
     const bool some = lo < hi;
     x8 q[D / 16];
+    const uint16_t *qrow = (there ? a.q + at * a.q_stride[1] + head * a.q_stride[2] : reinterpret_cast<const uint16_t *>(kAttnZeroRow)) + h2 * 8;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-        q[s] = x8{};
-        if (there) q[s] = attn_query<T>(a, a.q + at * a.q_stride[1] + head * a.q_stride[2] + s * 16 + h2 * 8);
+    for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const x8 *>(qrow + s * 16);
+    if (a.scale <= 0.0f) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) q[s] = attn_signed<T>(a, q[s]);
     }
     const float slope = a.slopes ? a.slopes[head] * kLog2e : 0.0f;
 
-    /* keys that some row of the wave (of the workgroup) sees, and those that all of them do */
-    int wlo = some ? lo : INT32_MAX, whi = some ? hi : 0, wfl = there ? (some ? lo : INT32_MAX) : 0, wfh = there ? hi : INT32_MAX;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-        wlo = min(wlo, __shfl_xor(wlo, s, R9VX_WAVE)), whi = max(whi, __shfl_xor(whi, s, R9VX_WAVE));
-        wfl = max(wfl, __shfl_xor(wfl, s, R9VX_WAVE)), wfh = min(wfh, __shfl_xor(wfh, s, R9VX_WAVE));
-    }
-    wlo = __builtin_amdgcn_readfirstlane(wlo), whi = __builtin_amdgcn_readfirstlane(whi);
-    wfl = __builtin_amdgcn_readfirstlane(wfl), wfh = __builtin_amdgcn_readfirstlane(wfh);
-    if (lane == 0) bounds[wave][0] = wlo, bounds[wave][1] = whi;
+    /* keys that all rows of the wave see, and those that some of the workgroup do: where
+     * they begin and end grows with the token, but for the tokens' own starts */
+    const uint32_t rows = (uint32_t)news * a.group, w0 = r0 + wave * 32, w1 = (w0 + 32 < rows ? w0 + 32 : rows) - 1; /* (w0 >= rows: nothing is there) */
+    int ulo, uhi, wfl, wfh, any;
+    auto seen_by = [&](uint32_t r, int &from, int &to) {
+        attn_seen(a.window, a.causal, length - news + (int)(r / a.group), length, 0, a.prefix ? a.prefix[b] : 0, from, to);
+    };
+    seen_by(r0, ulo, any);
+    seen_by((r0 + kRows < rows ? r0 + kRows : rows) - 1, any, uhi);
+    seen_by(w0 < rows ? w0 : 0, any, wfh);
+    seen_by(w0 < rows ? w1 : 0, wfl, any);
     if (!CAREFUL && threadIdx.x == 0) sh.redo = 0; /* (the second way is on while other waves read it) */
-    __syncthreads();
-    int ulo = INT32_MAX, uhi = 0;
+    if (a.starts) {
+        int most = there ? lo : 0, least = some ? lo : INT32_MAX;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) ulo = min(ulo, bounds[i][0]), uhi = max(uhi, bounds[i][1]);
-    ulo = __builtin_amdgcn_readfirstlane(ulo), uhi = __builtin_amdgcn_readfirstlane(uhi);
+        for (int s = 1; s < 32; s <<= 1) most = max(most, __shfl_xor(most, s, R9VX_WAVE)), least = min(least, __shfl_xor(least, s, R9VX_WAVE));
+        wfl = max(wfl, __builtin_amdgcn_readfirstlane(most));
+        if (lane == 0) bounds[wave] = least;
+        __syncthreads();
+        least = min(min(bounds[0], bounds[1]), min(bounds[2], bounds[3]));
+        ulo = max(ulo, __builtin_amdgcn_readfirstlane(least));
+    }
+    if (bad_length) ulo = uhi = 0;
 
     /* this part's tiles */
     const int t0 = ulo < uhi ? ulo / KT : 0, t1 = ulo < uhi ? (uhi + KT - 1) / KT : 0;
@@ -375,13 +384,13 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
         }
     }
     l += attn_swap32(l);
-    bool odd = !(fabsf(l) < INFINITY);
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) odd |= !(fabsf(o[d][e]) < INFINITY);
     if (!CAREFUL) {
-        if (__any(odd && there) && lane == 0) sh.redo = 1;
+        float zero = l * 0.0f; /* or a NaN where something is not finite */
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) zero = fmaf(o[d][e], 0.0f, zero);
+        if (__any(zero != 0.0f && there) && lane == 0) sh.redo = 1;
         __syncthreads();
         if (sh.redo) return true;
     }

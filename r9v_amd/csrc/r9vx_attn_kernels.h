@@ -111,7 +111,7 @@ template <>
 __device__ __forceinline__ const uint16_t *attn_nan_row<AttnF16>() { return reinterpret_cast<const uint16_t *>(kAttnNanF16); }
 
 /* What turns products into exponents of two, x = score * log2(e).  The query's sign
- * is the scale's (attn_query), so that the largest product is the largest score;
+ * is the scale's (attn_signed), so that the largest product is the largest score;
  * a scale of zero makes it zeros.  A cap and a bias are applied to the
  * products first and leave them in units of 1 / log2(e): factor 1. */
 struct AttnScore {
@@ -135,15 +135,13 @@ struct AttnScore {
     }
 };
 
-/* Eight elements of a query, with the scale's sign. */
+/* Eight elements of a query, with a scale's sign (zeros for one of zero). */
 template <class T>
-__device__ __forceinline__ typename T::x8 attn_query(const r9vx_attn_problem &a, const uint16_t *p) {
-    r9vx_u32x4 w = *reinterpret_cast<const r9vx_u32x4 *>(p);
-    if (a.scale <= 0.0f) { /* (nothing waits for the load where the scale is positive) */
-        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
+__device__ __forceinline__ typename T::x8 attn_signed(const r9vx_attn_problem &a, typename T::x8 q) {
+    r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, q);
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, keep = a.scale == 0.0f ? 0u : ~0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
-    }
+    for (int i = 0; i < 4; ++i) w[i] = (w[i] ^ flip) & keep;
     return __builtin_bit_cast(typename T::x8, w);
 }
 
