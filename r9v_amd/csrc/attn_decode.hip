@@ -40,7 +40,7 @@ struct DecodeShape {
     static constexpr int kArea = kBlock * KP * 2; /* bytes of a wave: a block's keys, or after them its sums of 16 rows */
     static_assert(16 * (D + 4) * 4 <= kArea);
     /* waves a SIMD that the registers are to leave room for */
-    static constexpr int kWavesASimd(int rt) { return D > 192 ? 1 : D * rt > 96 ? 2 : 3; }
+    static constexpr int kWavesASimd(int rt) { return D > 192 || D * rt > 256 ? 1 : D * rt > 96 ? 2 : 3; }
 };
 
 /* DW words in LDS. */
@@ -429,9 +429,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, con
     }
 }
 
+/* blocks of the longest row */
+uint32_t decode_blocks(const r9vx_attn_problem &p) {
+    const uint32_t whole = (p.len_bucket + kBlock - 1) / kBlock, seen = (p.window + p.t_bucket - 1) / kBlock + 2;
+    return seen < whole ? seen : whole > 0 ? whole : 1;
+}
+
+/* 32 rows a workgroup halve what is read through the caches, but beyond 128 columns
+ * they take all registers of a SIMD and longer to begin: only where every wave has
+ * several blocks (256 columns, 2 kv heads at 8192 keys, 32 rows: one sequence 25 us
+ * with 16 rows and 30 with 32, four 34 and 37, eight 54 and 50; 65536 keys and 64
+ * rows 94 and 74; 192 columns, 40 rows, one sequence 19 and 22, eight with 4 kv
+ * heads and 32 rows 67 and 53). */
 uint32_t decode_row_tiles(const r9vx_attn_problem &p, uint32_t &rt) {
     const uint32_t rows = p.t_bucket * p.group;
-    rt = rows > 16 && p.head_dim <= 128 ? 2 : 1;
+    rt = rows > 16 && (p.head_dim <= 128 || (uint64_t)p.b_bucket * p.kv_heads * decode_blocks(p) >= 16ull * r9vx_device_cus()) ? 2 : 1;
     return (rows + 16 * rt - 1) / (16 * rt);
 }
 
@@ -440,13 +452,8 @@ int launch_decode(const r9vx_attn_problem &p, hipStream_t stream) {
     uint32_t rt;
     const uint32_t tiles = decode_row_tiles(p, rt);
     const dim3 grid(p.kv_heads * tiles, p.b, p.splits);
-    if constexpr (D <= 128) {
-        if (rt == 2) {
-            hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
-            return (int)hipGetLastError();
-        }
-    }
-    hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+    if (rt == 2) hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+    else hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
     return (int)hipGetLastError();
 }
 
@@ -471,10 +478,8 @@ uint64_t r9vx_attn_decode_groups(const r9vx_attn_problem &p) {
 void r9vx_attn_decode_plan(r9vx_attn_problem &p) {
     uint32_t rt;
     const uint64_t groups = (uint64_t)p.b_bucket * p.kv_heads * decode_row_tiles(p, rt);
-    const uint64_t fill = (p.head_dim > 192 ? 1ull : p.head_dim * rt > 96 ? 2ull : 3ull) * r9vx_device_cus();
-    /* blocks of the longest row */
-    const uint32_t whole = (p.len_bucket + kBlock - 1) / kBlock, seen = (p.window + p.t_bucket - 1) / kBlock + 2;
-    const uint32_t most = seen < whole ? seen : whole > 0 ? whole : 1;
+    const uint64_t fill = (p.head_dim > 192 || p.head_dim * rt > 256 ? 1ull : p.head_dim * rt > 96 ? 2ull : 3ull) * r9vx_device_cus();
+    const uint32_t most = decode_blocks(p);
     uint64_t parts = groups ? fill / groups : 1;
     if (parts > (most + kWaves - 1) / kWaves) parts = (most + kWaves - 1) / kWaves;
     if (parts > kMostParts) parts = kMostParts;

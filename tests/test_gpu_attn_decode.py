@@ -212,3 +212,29 @@ def test_on_a_stream_of_its_own():
     out = attn.decode(q, k, v, table, n, stream=s)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("lengths,new,kv,group,dim,kind", [([900, 33, 2100, 0], 4, 2, 8, 256, "bf16"), ([1, 1500, 64, 310], 6, 2, 6, 192, "f16"),
+                                                           ([520, 17, 6, 95], 8, 2, 7, 256, "f16"), ([40, 2000, 31, 33], 3, 2, 6, 192, "bf16")])
+def test_wide_heads_of_many_rows_with_room_for_long_sequences(lengths, new, kv, group, dim, kind):
+    """A table of 16384 places: what picks the kernel is the room, not the lengths."""
+    k, v, table = pool(lengths, 64, kv, dim, DT[kind], 121)
+    wide = torch.full((len(lengths), 256), -9, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q = queries((len(lengths), new, kv * group, dim), DT[kind], 122)
+    out = attn.decode(q, k, v, wide, ints(lengths))
+    check(out, q, k, v, table, lengths)
+    out = attn.decode(q, k, v, wide, ints(lengths), scale=-0.1, starts=ints([20, 0, 64, 3]), softcap=9.0)
+    check(out, q, k, v, table, lengths, scale=-0.1, starts=[20, 0, 64, 3], softcap=9.0)
+
+
+def test_a_long_tail_of_small_probabilities():
+    """One key far above 3000 that weigh 2^-16 of it each: below the steps of an f16 probability of 1, a twentieth of the sum."""
+    for kind, new in (("f16", 1), ("bf16", 1), ("f16", 3)):
+        k, v, table = pool([3001], 16, 1, 64, DT[kind], 131)
+        k.mul_(0.0), k.nan_to_num_(0.0)
+        k[table[0, 5].long(), 7, 0, 0] = 1.0
+        q = torch.zeros(1, new, 2, 64, dtype=DT[kind], device="cuda")
+        q[..., 0] = 11.0
+        out = attn.decode(q, k, v, table, ints([3001]), scale=1.0)
+        check(out, q, k, v, table, [3001], scale=1.0)

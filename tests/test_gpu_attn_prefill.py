@@ -227,3 +227,16 @@ def test_on_a_stream_of_its_own():
     out = attn.prefill(q, k, v, table, n, off, stream=s)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("score", [11.0, 17.0])
+def test_a_long_tail_of_small_probabilities(kind, score):
+    """One key far above 3000 that weigh 2^-16 (2^-24) of it each, which an f16 probability of 1 would not resolve."""
+    k, v, table = pool([3001], 16, 1, 64, DT[kind], 131)
+    k.mul_(0.0), k.nan_to_num_(0.0)
+    k[table[0, 5].long(), 7, 0, 0] = 1.0
+    q = torch.zeros(4, 2, 64, dtype=DT[kind], device="cuda")
+    q[..., 0] = score
+    out = attn.prefill(q, k, v, table, ints([3001]), offsets_of([4]), scale=1.0)
+    check(out, q, k, v, table, [3001], [4], scale=1.0)
