@@ -287,12 +287,13 @@ def test_launches(tmp_path, monkeypatch):
     runtime = launch_record.build(tmp_path)
     calls = [("attn", dict(decode=True)), ("attn", dict(decode=True, b_bucket=20000)), ("attn", dict(decode=True, len_bucket=100)), ("attn", dict(decode=False)),
              ("attn", dict(decode=False, t_bucket=100000)), ("attn", dict(decode=True, t_bucket=8)), ("attn", dict(decode=False, t_bucket=1 << 23, heads=128, kv_heads=8)),
-             ("attn", dict(decode=True, b_bucket=65535, heads=224, kv_heads=224))]
+             ("attn", dict(decode=True, b_bucket=65535, heads=224, kv_heads=224)), ("attn", dict(decode=True, b_bucket=1, len_bucket=131072)),
+             ("attn", dict(decode=True, t_bucket=5, b_bucket=8, head_dim=256, len_bucket=16384))]
     out = launch_record.record(runtime, calls)
     names = [[n.split("<")[0] for n, _, _ in ls] for _, _, ls in out]
     assert all(rc == 0 for rc, _, _ in out), [msg for rc, msg, _ in out if rc]
-    d, p, j = "attn_decode_kernel", "attn_prefill_kernel", "attn_join_kernel"
-    assert names == [[d, j], [d], [d], [p, j], [p], [d, j], [p], [d]]
+    d, p, j, few = "attn_decode_kernel", "attn_prefill_kernel", "attn_join_kernel", "attn_join_few_kernel"
+    assert names == [[d, j], [d], [d], [p, few], [p], [d, j], [p], [d], [d, j], [d, few]]
     for _, _, ls in out:
         for _, grid, block in ls:
             assert grid[0] * grid[1] * grid[2] * block[0] < 1 << 32 and grid[1] < 1 << 16 and grid[2] < 1 << 16
