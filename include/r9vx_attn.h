@@ -92,13 +92,14 @@ typedef struct r9vx_rope_kv_args {
  * their slots.  Columns from rot on are copied.  A slot other than -1 outside
  * the cache writes nothing and sets R9VX_STATUS_BAD_SLOT; of two rows with one
  * slot either may be kept, 16 bytes by 16 bytes.  Pointers 16-byte aligned,
- * strides such that every head is. */
+ * strides such that every head is; rows of q_out, of k_cache and of v_cache
+ * apart from each other. */
 int r9vx_rope_kv_launch(const r9vx_rope_kv_static *st, const r9vx_rope_kv_args *args, r9vx_stream_t stream);
 
 /* ----------------------------------------------------------- attention */
 
 typedef struct r9vx_attn_static {
-    uint32_t b_bucket;     /* the launch's b <= b_bucket */
+    uint32_t b_bucket;     /* the launch's b <= b_bucket < 2^16 */
     uint32_t t_bucket;     /* decode: new tokens of each sequence, 1 .. 8; prefill: the launch's t <= t_bucket */
     uint32_t len_bucket;   /* the longest length; the table has a column for each of its pages */
     uint32_t heads;        /* a multiple of kv_heads */
@@ -126,8 +127,8 @@ typedef struct r9vx_attn_args {
     uint8_t *workspace;     /* r9vx_attn_*_workspace_bytes, 256-byte aligned; NULL when 0 */
     uint32_t *status;       /* or NULL */
     uint64_t q_stride[3];   /* of a sequence (decode), of a token, of a head */
-    uint64_t out_stride[3];
-    uint64_t k_stride[3];   /* of a page, of a token, of a head */
+    uint64_t out_stride[3]; /* rows apart from each other */
+    uint64_t k_stride[3];   /* of a page, of a token (below 2^27), of a head; all strides multiples of 8 below 2^40 */
     uint64_t v_stride[3];
     uint64_t table_stride;  /* of a sequence */
     uint32_t pages;

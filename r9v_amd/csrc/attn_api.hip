@@ -36,6 +36,22 @@ uint64_t span(const uint64_t (&stride)[N], const uint64_t (&size)[N], uint64_t c
     return (last + columns) * bytes;
 }
 
+/* Whether an output's rows stand apart: by ascending strides, each row behind the last one's end. */
+template <int N>
+bool rows_apart(const uint64_t (&stride)[N], const uint64_t (&size)[N], uint64_t columns) {
+    bool done[N] = {};
+    for (int n = 0; n < N; ++n) {
+        int least = -1;
+        for (int i = 0; i < N; ++i)
+            if (!done[i] && size[i] > 1 && (least < 0 || stride[i] < stride[least])) least = i;
+        if (least < 0) return true;
+        if (stride[least] < columns) return false;
+        columns += (size[least] - 1) * stride[least];
+        done[least] = true;
+    }
+    return true;
+}
+
 template <int N>
 void check_strides(const char *name, const uint64_t (&stride)[N], uint64_t bytes, Problems &pr) {
     for (int i = 0; i < N; ++i) {
@@ -114,6 +130,9 @@ void check_groups(const r9vx_attn_static *st, bool decode, Problems &pr) {
     const uint64_t groups = decode ? r9vx_attn_decode_groups(p) : r9vx_attn_prefill_groups(p);
     if (groups >= (1u << 24) || (!decode && (uint64_t)st->t_bucket * p.group >= (1u << 31)))
         pr.add(R9VX_ERR_UNSUPPORTED, "b_bucket=%u, t_bucket=%u of %u heads have more tiles than a launch", st->b_bucket, st->t_bucket, st->heads);
+    const uint64_t rows = (decode ? (uint64_t)st->b_bucket : 1ull) * st->t_bucket * st->heads;
+    if (p.splits > 1 && r9vx_attn_join_groups(p, rows) >= (1u << 24))
+        pr.add(R9VX_ERR_UNSUPPORTED, "b_bucket=%u, t_bucket=%u of %u heads and len_bucket=%u: more rows to join than a launch has", st->b_bucket, st->t_bucket, st->heads, st->len_bucket);
 }
 
 size_t attn_workspace_bytes(const r9vx_attn_static *st, bool decode) {
@@ -175,6 +194,7 @@ int attn_launch(const char *op, bool decode, const r9vx_attn_static *st, const r
             overlap(a->out, ny, a->table, nt) || overlap(a->out, ny, a->lengths, 4ull * a->b) || overlap(a->out, ny, a->offsets, 4ull * a->b + 4) ||
             overlap(a->out, ny, a->starts, 4 * tokens) || overlap(a->out, ny, a->prefix, 4ull * a->b) || overlap(a->out, ny, a->slopes, 4ull * st->heads))
             pr.add(R9VX_ERR_INVALID, "out must not overlap an operand");
+        if (!rows_apart(a->out_stride, rows, st->head_dim)) pr.add(R9VX_ERR_INVALID, "rows of out overlap each other");
         if (overlap(a->workspace, ws, a->q, nq) || overlap(a->workspace, ws, a->out, ny) || overlap(a->workspace, ws, a->k_cache, nk) ||
             overlap(a->workspace, ws, a->v_cache, nv) || overlap(a->workspace, ws, a->table, nt) || overlap(a->workspace, ws, a->lengths, 4ull * a->b) ||
             overlap(a->workspace, ws, a->offsets, 4ull * a->b + 4) || overlap(a->workspace, ws, a->starts, 4 * tokens) ||
@@ -247,6 +267,7 @@ int r9vx_rope_kv_launch(const r9vx_rope_kv_static *st, const r9vx_rope_kv_args *
         if (!in_place && overlap(a->q_out, ny, a->q, nq)) pr.add(R9VX_ERR_INVALID, "q_out must not overlap q (it may be q, with q's strides and type)");
         if (overlap(a->q_out, ny, a->positions, 4ull * a->t) || overlap(a->q_out, ny, a->freqs, 4ull * st->rot) || overlap(a->q_out, ny, a->slots, 8ull * a->t))
             pr.add(R9VX_ERR_INVALID, "q_out must not overlap positions, freqs or slots");
+        if (!rows_apart(a->q_out_stride, rows, st->head_dim)) pr.add(R9VX_ERR_INVALID, "rows of q_out overlap each other");
         if (cache) {
             const uint64_t nk = span(a->k_stride, kv, st->head_dim, in), nv = span(a->v_stride, kv, st->head_dim, in);
             const uint64_t nkc = span(a->k_cache_stride, pages, st->head_dim, out), nvc = span(a->v_cache_stride, pages, st->head_dim, out);
@@ -259,6 +280,9 @@ int r9vx_rope_kv_launch(const r9vx_rope_kv_static *st, const r9vx_rope_kv_args *
             if (overlap(a->k_cache, nkc, a->positions, 4ull * a->t) || overlap(a->k_cache, nkc, a->freqs, 4ull * st->rot) || overlap(a->k_cache, nkc, a->slots, 8ull * a->t) ||
                 overlap(a->v_cache, nvc, a->positions, 4ull * a->t) || overlap(a->v_cache, nvc, a->freqs, 4ull * st->rot) || overlap(a->v_cache, nvc, a->slots, 8ull * a->t))
                 pr.add(R9VX_ERR_INVALID, "the cache must not overlap positions, freqs or slots");
+            /* (keys and values may take turns in one allocation) */
+            if (!rows_apart(a->k_cache_stride, pages, st->head_dim) || !rows_apart(a->v_cache_stride, pages, st->head_dim) || (nkc && a->k_cache == a->v_cache))
+                pr.add(R9VX_ERR_INVALID, "rows of the cache overlap each other");
         }
     }
     const int rc = pr.finish("rope_kv");

@@ -11,12 +11,19 @@
  * Scores are taken transposed, S^T = K Q^T by 16 x 16 x 32 products, with a
  * block's keys dealt to the two tiles so that what a lane holds of S^T, 8
  * neighbouring keys of one row, is what the second product O^T = V^T P^T
- * takes from it: probabilities never leave their lane.  Values are loaded as they
- * stand, a lane 8 keys x head_dim / 16 columns, and turned in registers
- * (half a v_perm an element).  Nothing but the joins goes through LDS.
+ * takes from it: probabilities never leave their lane.  Keys and values are loaded
+ * by whole lines, a lane head_dim / 16 columns of 8 neighbouring keys; keys are
+ * dealt out through a part of LDS that is the wave's own (loaded in the operand's
+ * order, 16 rows at once, the same bytes took 116 us instead of 107 at 131072 keys
+ * and 136 instead of 106 for 48 ragged sequences), values are turned in registers
+ * (half a v_perm an element).
  *
  * Bound by the keys' and values' bytes: a wave keeps a block's keys or values on
- * their way while it works on the others.
+ * their way while it works on the others.  131072 keys of 8 kv heads of 128 columns,
+ * 537 MB, 86 us (6.2 TB/s: part of them is still in the last cache) and 5 for the
+ * join; 45 sequences of 100 to 8192 keys, 348 MB, 80 us, since the parts of the
+ * longest end late.  Few keys cost 7 us from the launch on: a table's page, a block
+ * and the waves' join, one after another (517 keys of 2 kv heads of 256 columns).
  */
 #include "r9vx_attn_kernels.h"
 
@@ -39,7 +46,7 @@ struct DecodeShape {
     static constexpr int KP = D + 8;
     static constexpr int kArea = kBlock * KP * 2; /* bytes of a wave: a block's keys, or after them its sums of 16 rows */
     static_assert(16 * (D + 4) * 4 <= kArea);
-    /* waves a SIMD that the registers are to leave room for */
+    /* waves a SIMD that the registers are to leave room for (256 columns: 366 of 512 for one) */
     static constexpr int kWavesASimd(int rt) { return D > 192 || D * rt > 256 ? 1 : D * rt > 96 ? 2 : 3; }
 };
 
@@ -388,7 +395,7 @@ __device__ __forceinline__ uint16_t *join_out(const r9vx_attn_problem &a, uint64
 /* A row's parts, by a workgroup for each 32 columns:
  * each wave takes the parts' maxima and sums, then four columns a thread are added
  * up, several parts side by side, and those through LDS.  Bound by a launch and
- * two loads in turn. */
+ * two loads in turn: 64 parts of 32 rows of 128 columns 5.1 us. */
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, const float2 *ml) {
     __shared__ float weight[kMostParts];
@@ -443,8 +450,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, con
 
 /* The same of at most kFewParts parts, by a wave, which has all its loads on their way
  * at once: lane i % 16 part i's maximum and sum, and every lane four columns of
- * the parts lane / (D / 4), one in 256 / D.  (13 parts of 4800 rows of 256 columns,
- * 64 MB: 15.5 us by workgroups; 5 parts of 16 rows: 4.2) */
+ * the parts lane / (D / 4), one in 256 / D.  13 parts of 4800 rows of 256 columns,
+ * 64 MB, take 12 us (15.5 by a workgroup a row). */
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_join_few_kernel(r9vx_attn_problem a, const float2 *ml, uint64_t rows) {
     constexpr int kWidth = D / 4, kSide = 64 / kWidth, kMost = (kFewParts + kSide - 1) / kSide;
@@ -566,6 +573,8 @@ void r9vx_attn_decode_plan(r9vx_attn_problem &p) {
     p.splits = (most + per - 1) / per;
     if (p.splits < p.parts) p.splits = p.parts;
 }
+
+uint64_t r9vx_attn_join_groups(const r9vx_attn_problem &p, uint64_t rows) { return p.splits > (uint32_t)kFewParts ? rows * (p.head_dim / 32) : (rows + 3) / 4; }
 
 int r9vx_launch_attn_join(const r9vx_attn_problem &p, uint64_t rows, hipStream_t stream) {
     const float2 *ml = reinterpret_cast<const float2 *>(p.partial + (p.offsets ? (uint64_t)p.t_bucket : (uint64_t)p.b_bucket * p.t_bucket) * p.heads * p.splits * p.head_dim);

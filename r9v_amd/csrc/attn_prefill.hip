@@ -12,6 +12,14 @@
  * product O^T = V^T P^T takes, so that probabilities stay in registers; V^T
  * comes from LDS by the transposing read.  Where the rows are too few to fill the
  * card the keys are cut into parts, joined by a further launch.
+ *
+ * A tile's 1024 cycles of matrix instructions and its 700 or so of exponentials,
+ * maxima and conversions overlap only where the two workgroups of a CU are at different
+ * phases: 8192 causal tokens of 32 heads of 128 columns 532 to 564 us, 0.98 to 1.03
+ * PFLOP/s, about half of the matrix unit's cycles (a large product reaches 1.47).
+ * Eight waves at opposite phases behind shared barriers took 568 when this form
+ * took 561, a tile's products in halves around the softmax no less: registers spilt.
+ * A workgroup takes 5 us before its first tile is done: 17 tokens 12 us.
  */
 #include "r9vx_attn_kernels.h"
 

@@ -45,6 +45,7 @@ int r9vx_launch_attn_decode(const r9vx_attn_problem &p, hipStream_t stream);
 int r9vx_launch_attn_prefill(const r9vx_attn_problem &p, hipStream_t stream);
 /* out from the parts of rows [0, rows): row r is token r / heads, head r % heads. */
 int r9vx_launch_attn_join(const r9vx_attn_problem &p, uint64_t rows, hipStream_t stream);
+uint64_t r9vx_attn_join_groups(const r9vx_attn_problem &p, uint64_t rows);
 /* Workgroups a launch of these sizes has (the API refuses more than 32 bits of threads). */
 uint64_t r9vx_attn_decode_groups(const r9vx_attn_problem &p);
 uint64_t r9vx_attn_prefill_groups(const r9vx_attn_problem &p);

@@ -83,7 +83,9 @@ NO_CACHE = dict(kv_heads=0, k=None, v=None, k_cache=None, v_cache=None, slots=No
     (dict(q_out=APART["q"]), INVALID, "q_out must not overlap q"), (dict(q_out=APART["k"]), INVALID, "overlap k or v"),
     (dict(q_out=APART["q"], q_out_stride=(1536, 128), in_dtype=ffi.F32), INVALID, "q_out must not overlap q"),
     (dict(k_cache=APART["q"] + 4096), INVALID, "cache must not overlap"), (dict(v_cache=APART["q_out"]), INVALID, "cache must not overlap"),
-    (dict(v_cache=APART["slots"]), INVALID, "cache must not overlap positions"), (dict(q_out=APART["freqs"]), INVALID, "positions, freqs or slots")])
+    (dict(v_cache=APART["slots"]), INVALID, "cache must not overlap positions"), (dict(q_out=APART["freqs"]), INVALID, "positions, freqs or slots"),
+    (dict(q_out_stride=(0, 128)), INVALID, "rows of q_out overlap"), (dict(k_cache_stride=(4096, 128, 128)), INVALID, "rows of the cache overlap"),
+    (dict(v_cache_stride=(2048, 256, 128)), INVALID, "rows of the cache overlap"), (dict(v_cache=APART["k_cache"]), INVALID, "rows of the cache overlap")])
 def test_rope_refusals(kw, code, text):
     refused(lib.r9vx_rope_kv_launch, *rope(**kw), code=code, text=text)
 
@@ -124,10 +126,13 @@ BOTH = [
     (dict(workspace=ATTN["workspace"] + 16), ALIGN, "256-byte"), (dict(table_stride=31), INVALID, "columns apart"),
     (dict(out=ATTN["q"]), INVALID, "out must not overlap"), (dict(out=ATTN["v_cache"] + 4096), INVALID, "out must not overlap"),
     (dict(out=ATTN["lengths"]), INVALID, "out must not overlap"), (dict(workspace=ATTN["out"], len_bucket=600), INVALID, "workspace must not overlap"),
-    (dict(workspace=ATTN["table"], len_bucket=600), INVALID, "workspace must not overlap")]
+    (dict(workspace=ATTN["table"], len_bucket=600), INVALID, "workspace must not overlap"),
+    (dict(out_stride=(2048, 0, 128)), INVALID, "rows of out overlap"), (dict(out_stride=(2048, 1024, 120)), INVALID, "rows of out overlap")]
 DECODE = [(dict(t_bucket=0), UNSUPPORTED, "1 to 8"), (dict(t_bucket=9), UNSUPPORTED, "1 to 8"), (dict(causal=0), INVALID, "causal"), (dict(t=2), INVALID, "t=2"),
           (dict(offsets=ATTN["offsets"]), INVALID, "prefill's"), (dict(prefix=ATTN["prefix"]), INVALID, "prefill's"),
-          (dict(b_bucket=65535, heads=1024, kv_heads=512), UNSUPPORTED, "more tiles than a launch")]
+          (dict(b_bucket=65535, heads=1024, kv_heads=512), UNSUPPORTED, "more tiles than a launch"),
+          (dict(b_bucket=65535, t_bucket=8, heads=256, kv_heads=1, len_bucket=1 << 23), UNSUPPORTED, "more rows to join"),
+          (dict(out_stride=(0, 1024, 128)), INVALID, "rows of out overlap"), (dict(out_stride=(1024, 1024, 128)), INVALID, "rows of out overlap")]
 PREFILL = [(dict(t_bucket=(1 << 24) + 1), UNSUPPORTED, "2^24"), (dict(t=101), INVALID, "t=101"), (dict(offsets=None), NULL, "offsets"),
            (dict(causal=0, prefix=ATTN["prefix"]), INVALID, "prefix without"), (dict(t_bucket=1 << 24, heads=1024, kv_heads=4), UNSUPPORTED, "more tiles")]
 
@@ -273,7 +278,9 @@ def attn(decode, threads=None, **kw):
     st = dict(b_bucket=4, t_bucket=1 if decode else 100, len_bucket=4096, heads=8, kv_heads=2, head_dim=128, page_size=16, dtype=ffi.BF16, causal=1,
               window=0, scale_bits=0x3F800000, softcap_bits=0)
     st.update(kw)
-    a = ffi.AttnArgs(*APART[:5], None if decode else APART[5], None, None, None, APART[6], APART[7], None, (0, 1024, 128), (0, 1024, 128),
+    token = st["heads"] * st["head_dim"]
+    rows = (st["t_bucket"] * token, token, st["head_dim"])
+    a = ffi.AttnArgs(*APART[:5], None if decode else APART[5], None, None, None, APART[6], APART[7], None, rows, rows,
                      (4096, 256, 128), (4096, 256, 128), 1 << 20, 1000, st["b_bucket"], 0 if decode else st["t_bucket"], 0)
     f = L.r9vx_attn_decode_launch if decode else L.r9vx_attn_prefill_launch
     return f(ctypes.byref(ffi.AttnStatic(**st)), ctypes.byref(a), None)
