@@ -29,7 +29,7 @@ namespace {
 
 constexpr int kRows = 128; /* of a workgroup */
 constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kThreads = 64 * kWaves; /* times the halves */
 
 typedef short attn_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) attn_s4 attn_lds_s4;
@@ -65,6 +65,13 @@ __device__ __forceinline__ void attn_copy16(uint32_t at, const uint16_t *base, u
                  : "=&s"(all) : "v"(off), "s"(base), "s"(at), "s"(lanes) : "m0", "scc");
 }
 
+/* `lanes` or none, as attn_copy16 takes them: in scalar registers. */
+__device__ __forceinline__ uint64_t attn_lanes(bool on, uint64_t lanes) {
+    uint32_t lo = __builtin_amdgcn_readfirstlane(on ? (uint32_t)lanes : 0u), hi = __builtin_amdgcn_readfirstlane(on ? (uint32_t)(lanes >> 32) : 0u);
+    asm volatile("" : "+s"(lo), "+s"(hi));
+    return (uint64_t)hi << 32 | lo;
+}
+
 /* Holds what makes x before what follows: pure arithmetic is otherwise moved to its use,
  * behind the barriers that part the phases. */
 template <class X>
@@ -89,11 +96,12 @@ __device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
     return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
 }
 
-template <int D>
+template <int D, int H>
 struct PrefillShared {
-    __attribute__((aligned(1024))) uint16_t kv[4][PrefillShape<D>::TILE]; /* keys of two tiles, values of two */
+    __attribute__((aligned(1024))) uint16_t kv[H][4][PrefillShape<D>::TILE]; /* keys of two tiles, values of two; in the end the second half's sums */
     int bounds[kWaves];
-    uint32_t redo, odds[2]; /* odds: keys of a tile with values that are not finite */
+    uint32_t redo, odds[H][2]; /* odds: keys of a tile with values that are not finite */
+    float tops[H - 1 ? kThreads : 1], sums[H - 1 ? kThreads : 1];
 };
 
 /* A workgroup's rows.  CAREFUL: the second way through, which a workgroup takes where
@@ -101,16 +109,16 @@ struct PrefillShared {
  * brought it in through a probability of zero.  It takes such values out of LDS, and
  * adds each to the rows that see its key (times a probability, a NaN or an infinity is
  * itself).  Returns whether the second way has to be taken (nothing is written then). */
-template <class T, int D, bool CAREFUL>
-__device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, uint32_t tiles, PrefillShared<D> &sh) {
+template <class T, int D, int H, bool CAREFUL>
+__device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, uint32_t tiles, PrefillShared<D, H> &sh) {
     using S = PrefillShape<D>;
     typedef typename T::x8 x8;
     constexpr int KT = S::KT, NK = KT / 32;
-    auto &kv = sh.kv;
+    const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h2 = lane >> 5;
+    const int half = H == 1 ? 0 : wave8 / kWaves, wave = H == 1 ? wave8 : wave8 % kWaves;
+    auto &kv = sh.kv[half];
     auto &bounds = sh.bounds;
-    auto &odds = sh.odds;
-
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h2 = lane >> 5;
+    auto &odds = sh.odds[half];
     uint32_t id = blockIdx.x;
     const uint32_t kvh = id % a.kv_heads;
     id /= a.kv_heads;
@@ -119,7 +127,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 
     if (tile == 0 && kvh == 0 && split == 0 && a.status) {
         bool odd = false;
-        for (uint32_t i = threadIdx.x; i < a.b; i += kThreads) odd |= a.offsets[i] < 0 || a.offsets[i] > a.offsets[i + 1] || (int64_t)a.offsets[i + 1] > a.t;
+        for (uint32_t i = threadIdx.x; i < a.b; i += H * kThreads) odd |= a.offsets[i] < 0 || a.offsets[i] > a.offsets[i + 1] || (int64_t)a.offsets[i + 1] > a.t;
         if (odd) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
     }
     AttnTile part;
@@ -177,8 +185,9 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 
     /* this part's tiles */
     const int t0 = ulo < uhi ? ulo / KT : 0, t1 = ulo < uhi ? (uhi + KT - 1) / KT : 0;
-    int begin, end;
-    attn_part(t0, t1, 1, a.parts, a.part_blocks, split, begin, end);
+    int first, last; /* of the workgroup; then of this half */
+    attn_part(t0, t1, 1, a.parts, a.part_blocks, split, first, last);
+    const int steps = (last - first + H - 1) / H, begin = first + half * steps, end = H == 1 ? last : min(begin + steps, last);
 
     const AttnScore score(a);
     const uint16_t *kbase = a.k + kvh * a.k_stride[2], *vbase = a.v + kvh * a.v_stride[2];
@@ -193,24 +202,25 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 
     /* Lane j of every wave has the page of the tile's j-th eight keys (page 0 where
      * nothing of them is seen or the cache has no such page: something has to be
-     * copied, and is replaced in LDS).  Copy i of a wave has rows R (wave + 4 i) ..
-     * of the tile, all in one eight and at the same place in it for every i. */
+     * copied, and is replaced in LDS); of two halves lane 32 + j the other half's.  Copy i
+     * of a wave has rows R (wave + 4 i) .. of the tile, all in one eight and at the same
+     * place in it for every i. */
     const int lrow = lane / S::CH, lpiece = lane % S::CH; /* (beyond the rows for lanes that copy nothing) */
     const int inside = S::R * wave % 8 + lrow;
     const uint32_t kstep = (uint32_t)(inside * a.k_stride[1] * 2), vstep = (uint32_t)(inside * a.v_stride[1] * 2);
     /* (nothing is done with what is loaded until the tile is copied: a wait here would be
      * one for the copies under way) */
+    const int place8 = H == 1 ? 8 * lane : 8 * c32 + (h2 ? (half ? -steps : steps) * KT : 0);
+    const int bound = H == 1 ? uhi : min(uhi, ((half ^ h2) ? last : first + steps) * KT);
+    auto in_tile = [&](int key) { return (H == 1 ? lane : c32) < KT / 8 && key < bound && key + 8 > ulo; };
     auto page_of = [&](int t) -> uint32_t {
-        const int key = t * KT + 8 * lane;
-        return (uint32_t)table[(lane < KT / 8 && key < uhi && key + 8 > ulo ? key : ulo) >> a.page_shift];
+        const int key = t * KT + place8;
+        return (uint32_t)table[(in_tile(key) ? key : ulo) >> a.page_shift];
     };
-    auto no_page = [&](int t, uint32_t page) -> bool {
-        const int key = t * KT + 8 * lane;
-        return lane < KT / 8 && key < uhi && key + 8 > ulo && page >= a.pages;
-    };
+    auto no_page = [&](int t, uint32_t page) -> uint64_t { return __ballot(in_tile(t * KT + place8) && page >= a.pages); };
     /* where tile t's eights begin, in lane j's registers; copy i of them into a buffer */
     auto source = [&](int t, uint32_t page, const uint16_t *base, const uint64_t *stride) -> uint64_t {
-        const uint32_t place = (uint32_t)(t * KT + 8 * lane) & mask, from = page < a.pages ? page : 0u;
+        const uint32_t place = (uint32_t)(t * KT + place8) & mask, from = page < a.pages ? page : 0u;
         return (uint64_t)(base + from * stride[0] + place * stride[1]);
     };
     auto copy = [&](int i, uint64_t p, uint32_t step, uint32_t at, uint64_t on) {
@@ -224,7 +234,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     const int vkey = 4 * h2 + (lane & 15) / 4, vpiece = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ S::swizzle(vkey);
     const int vrow = S::row(vkey) + 4 * (lane & 1);
 
-    const int n = end - begin;
+    const int n = end - begin; /* (of the second half steps or one less) */
     constexpr int kEach = (2 * S::N + D / 16 - 1) / (D / 16); /* copies beside a score's step */
     static_assert(kEach * (D / 16) >= 2 * S::N);
 
@@ -238,13 +248,15 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 
     /* Tile t (of n) has landed.  What stands beside the keys that are seen is no value, a
      * key of a page that is not there makes NaN of the scores that see it. */
-    auto landed = [&](int t, uint32_t no) {
+    auto landed = [&](int t, uint64_t nos) {
         const int key0 = (begin + t) * KT;
-        if (!(CAREFUL || no || key0 < ulo || key0 + KT > uhi)) return;
-        if (CAREFUL && threadIdx.x == 0) odds[0] = odds[1] = 0;
-        if (no && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
+        const uint32_t no = (uint32_t)nos;
+        /* (both halves come here or none: there are barriers) */
+        if (!(CAREFUL || nos || (first + t) * KT < ulo || (H == 1 ? key0 : (first + steps + t) * KT) + KT > uhi)) return;
+        if (CAREFUL && wave == 0 && lane == 0) odds[0] = odds[1] = 0;
+        if (no && wave == 0 && lane == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_PAGE);
         if (CAREFUL) __syncthreads();
-        if (S::LANES == 64 || lane < S::LANES) {
+        if ((S::LANES == 64 || lane < S::LANES) && (H == 1 || t < n)) {
 #pragma unroll 1
             for (int i = 0; i < S::N; ++i) {
                 const int c = wave + kWaves * i, r = S::R * c + lrow;
@@ -272,14 +284,15 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
         __syncthreads();
     };
 
-    if (n > 0) {
+    if (steps > 0) {
         uint32_t page = page_of(begin);
         uint64_t kp = source(begin, page, kbase, a.k_stride), vp = source(begin, page, vbase, a.v_stride);
-        uint32_t no = (uint32_t)__ballot(no_page(begin, page));
+        uint64_t no = no_page(begin, page);
+        const uint64_t lanes0 = attn_lanes(H == 1 || n > 0, kLanes);
 #pragma unroll
-        for (int i = 0; i < S::N; ++i) copy(i, kp, kstep, 0, kLanes), copy(i, vp, vstep, 2 * kTileBytes, kLanes);
+        for (int i = 0; i < S::N; ++i) copy(i, kp, kstep, 0, lanes0), copy(i, vp, vstep, 2 * kTileBytes, lanes0);
         page = page_of(begin + 1);
-        for (int t = 0; t < n; ++t) {
+        for (int t = 0; t < steps; ++t) {
             const int buf = t & 1, key0 = (begin + t) * KT;
             /* this tile has landed, and every wave is done with the other buffers */
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -287,11 +300,12 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
             __syncthreads();
             landed(t, no);
             const bool more = t + 1 < n;
-            no = more ? (uint32_t)__ballot(no_page(begin + t + 1, page)) : 0u;
+            no = H == 2 || more ? no_page(begin + t + 1, page) : 0u;
             const uint32_t to = (buf ^ 1) * kTileBytes;
-            const uint64_t lanes = (uint64_t)__builtin_amdgcn_readfirstlane(more ? (uint32_t)(kLanes >> 32) : 0u) << 32 | __builtin_amdgcn_readfirstlane(more ? ~0u : 0u);
+            const uint64_t lanes = attn_lanes(more, kLanes);
             kp = source(begin + t + 1, page, kbase, a.k_stride), vp = source(begin + t + 1, page, vbase, a.v_stride);
             page = page_of(begin + t + 2);
+            if (H == 2 && t >= n) break; /* (the last step) */
             const uint16_t *ks = kv[buf];
             uint16_t *vs = kv[2 + buf];
             attn_priority<D, 1>();
@@ -404,20 +418,48 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
         }
     }
     l += attn_swap32(l);
+    if constexpr (H == 2) { /* the second half's sums through LDS to the first */
+        r9vx_f32x4 *far = reinterpret_cast<r9vx_f32x4 *>(sh.kv[0][0]) + wave * (D / 8 * 64) + lane;
+        static_assert(kWaves * (D / 8) * 64 * 16 <= (int)sizeof(sh.kv));
+        __syncthreads(); /* the last tiles have been read */
+        if (half) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) far[(4 * d + e / 4) * 64] = r9vx_f32x4{o[d][e], o[d][e + 1], o[d][e + 2], o[d][e + 3]};
+            sh.tops[wave * 64 + lane] = m, sh.sums[wave * 64 + lane] = l;
+        }
+        __syncthreads();
+        if (!half) {
+            const float m1 = sh.tops[wave * 64 + lane], top = fmaxf(m, m1);
+            /* a half that saw nothing (or scores of -infinity alone) has zeros, or a NaN of NaN scores */
+            const float f0 = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top), f1 = m1 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m1 - top);
+            l = l * f0 + sh.sums[wave * 64 + lane] * f1;
+            m = top;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const r9vx_f32x4 y = far[(4 * d + e / 4) * 64];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[d][e + i] = o[d][e + i] * f0 + y[i] * f1;
+                }
+        }
+    }
     if (!CAREFUL) {
         float zero = l * 0.0f; /* or a NaN where something is not finite */
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) zero = fmaf(o[d][e], 0.0f, zero);
-        if (__any(zero != 0.0f && there) && lane == 0) sh.redo = 1;
+        if (!half && __any(zero != 0.0f && there) && lane == 0) sh.redo = 1;
         __syncthreads();
         if (sh.redo) return true;
     }
-    if (!there) return false;
+    if (!there || half) return false;
     float sum = l, top = m;
     if (bad_length || (sum != sum && top == -INFINITY)) top = 0.0f; /* a NaN that counts beside any other part */
-    if (bad_length || (sum == 0.0f && top == -INFINITY && max(lo, begin * KT) < min(hi, end * KT))) sum = __builtin_nanf("");
+    if (bad_length || (sum == 0.0f && top == -INFINITY && max(lo, first * KT) < min(hi, last * KT))) sum = __builtin_nanf("");
     if (a.splits == 1) {
         const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
         uint16_t *y = a.out + at * a.out_stride[1] + head * a.out_stride[2];
@@ -447,29 +489,35 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 typedef __attribute__((address_space(4))) const r9vx_attn_problem attn_kernel_args;
 
 /* Out of line: nothing of it takes registers of the first way's loop. */
-template <class T, int D>
-__device__ __attribute__((noinline)) void attn_prefill_careful(attn_kernel_args *args, uint32_t tiles, __attribute__((address_space(3))) PrefillShared<D> *sh) {
+template <class T, int D, int H>
+__device__ __attribute__((noinline)) void attn_prefill_careful(attn_kernel_args *args, uint32_t tiles, __attribute__((address_space(3))) PrefillShared<D, H> *sh) {
     const r9vx_attn_problem a = *(const r9vx_attn_problem *)args;
-    attn_prefill_rows<T, D, true>(a, tiles, *(PrefillShared<D> *)sh);
+    attn_prefill_rows<T, D, H, true>(a, tiles, *(PrefillShared<D, H> *)sh);
+}
+
+template <class T, int D, int H>
+__global__ __launch_bounds__(H * kThreads, 2) void attn_prefill_kernel(r9vx_attn_problem a, uint32_t tiles) {
+    __shared__ PrefillShared<D, H> sh;
+    if (attn_prefill_rows<T, D, H, false>(a, tiles, sh))
+        attn_prefill_careful<T, D, H>((attn_kernel_args *)__builtin_amdgcn_kernarg_segment_ptr(), tiles, (__attribute__((address_space(3))) PrefillShared<D, H> *)&sh);
 }
 
 template <class T, int D>
-__global__ __launch_bounds__(kThreads, 2) void attn_prefill_kernel(r9vx_attn_problem a, uint32_t tiles) {
-    __shared__ PrefillShared<D> sh;
-    if (attn_prefill_rows<T, D, false>(a, tiles, sh))
-        attn_prefill_careful<T, D>((attn_kernel_args *)__builtin_amdgcn_kernarg_segment_ptr(), tiles, (__attribute__((address_space(3))) PrefillShared<D> *)&sh);
+void launch_columns(const r9vx_attn_problem &p, hipStream_t stream) {
+    const uint32_t tiles = attn_tiles(p.t, p.b, p.group, kRows);
+    const dim3 grid((unsigned)r9vx_attn_prefill_groups(p));
+    if (p.halves == 2) hipLaunchKernelGGL((attn_prefill_kernel<T, D, 2>), grid, dim3(2 * kThreads), 0, stream, p, tiles);
+    else hipLaunchKernelGGL((attn_prefill_kernel<T, D, 1>), grid, dim3(kThreads), 0, stream, p, tiles);
 }
 
 template <class T>
 int launch_prefill(const r9vx_attn_problem &p, hipStream_t stream) {
-    const uint32_t tiles = attn_tiles(p.t, p.b, p.group, kRows);
-    const dim3 grid((unsigned)r9vx_attn_prefill_groups(p)), block(kThreads);
     switch (p.head_dim) {
-    case 64: hipLaunchKernelGGL((attn_prefill_kernel<T, 64>), grid, block, 0, stream, p, tiles); break;
-    case 96: hipLaunchKernelGGL((attn_prefill_kernel<T, 96>), grid, block, 0, stream, p, tiles); break;
-    case 128: hipLaunchKernelGGL((attn_prefill_kernel<T, 128>), grid, block, 0, stream, p, tiles); break;
-    case 192: hipLaunchKernelGGL((attn_prefill_kernel<T, 192>), grid, block, 0, stream, p, tiles); break;
-    default: hipLaunchKernelGGL((attn_prefill_kernel<T, 256>), grid, block, 0, stream, p, tiles); break;
+    case 64: launch_columns<T, 64>(p, stream); break;
+    case 96: launch_columns<T, 96>(p, stream); break;
+    case 128: launch_columns<T, 128>(p, stream); break;
+    case 192: launch_columns<T, 192>(p, stream); break;
+    default: launch_columns<T, 256>(p, stream); break;
     }
     return (int)hipGetLastError();
 }
@@ -480,11 +528,21 @@ uint64_t r9vx_attn_prefill_groups(const r9vx_attn_problem &p) { return (uint64_t
 
 void r9vx_attn_prefill_plan(r9vx_attn_problem &p) {
     const uint64_t groups = (uint64_t)attn_tiles(p.t_bucket, p.b_bucket, p.group, kRows) * p.kv_heads;
-    const uint64_t fill = 2ull * r9vx_device_cus();
-    const uint64_t most = ((uint64_t)p.len_bucket + 255) / 256; /* keys of a part: 256 or more */
-    uint64_t s = groups ? fill / groups : 1;
-    if (s > most) s = most;
-    if (s > 64) s = 64;
+    /* Where the rows are few: parts of 256 keys or more, so that there are two workgroups a
+     * CU; or half as many parts for workgroups of two halves, one a CU, which join two in LDS:
+     * half the sums to write and to join.  (us by parts and by halves: 300 tokens of 16 heads
+     * of 256 columns onto 4096, 13 or 6 parts, 60 and 52; 700 tokens of 32 heads of 128, 2 or
+     * 1, 31 and 22.)  Not where that leaves more CUs idle (512 tokens of 32 heads of 128 onto
+     * 16384, 3 or 1: 183 and 244), nor where all parts are under way at once and are joined by
+     * a launch in any case (4 x 40 tokens of 16 heads of 64 onto 2000, 8 or 4: 16.6 and 18). */
+    const uint64_t fill = r9vx_device_cus(), keys = p.len_bucket;
+    auto parts = [&](uint64_t places, uint64_t least) {
+        const uint64_t s = groups ? places / groups : 1, most = (keys + least - 1) / least;
+        return s < most ? (s < 64 ? s : 64) : most < 64 ? most : 64;
+    };
+    const uint64_t whole = parts(2 * fill, 256), halved = parts(fill, 512);
+    p.halves = whole > 1 && 20 * halved >= 9 * whole && (halved == 1 || groups * whole > fill) ? 2 : 1;
+    const uint64_t s = p.halves == 2 ? halved : whole;
     p.splits = p.parts = s > 1 ? (uint32_t)s : 1u;
     p.part_blocks = 1u << 27; /* no limit */
 }

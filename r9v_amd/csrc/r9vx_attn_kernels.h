@@ -36,9 +36,10 @@ struct r9vx_attn_problem {
     uint64_t q_stride[3], out_stride[3], k_stride[3], v_stride[3], table_stride;
     uint32_t pages, b, t, b_bucket, t_bucket, len_bucket, heads, kv_heads, group, group_magic, head_dim, page_shift, dtype, causal, window;
     uint32_t splits, parts, part_blocks; /* parts of a row's keys in the grid; those a row is cut into, of at most part_blocks blocks (attn_part) */
+    uint32_t halves; /* prefill: of a part's keys, for four waves each */
     float scale, softcap;
 };
-/* Sets splits, parts and part_blocks: by the static alone. */
+/* Sets splits, parts, part_blocks and halves: by the static alone. */
 void r9vx_attn_decode_plan(r9vx_attn_problem &p);
 void r9vx_attn_prefill_plan(r9vx_attn_problem &p);
 int r9vx_launch_attn_decode(const r9vx_attn_problem &p, hipStream_t stream);

@@ -240,3 +240,81 @@ def test_a_long_tail_of_small_probabilities(kind, score):
     q[..., 0] = score
     out = attn.prefill(q, k, v, table, ints([3001]), offsets_of([4]), scale=1.0)
     check(out, q, k, v, table, [3001], [4], scale=1.0)
+
+
+# Buckets of 6 heads on 2 of kv that pick two halves of the keys a workgroup: of each of several parts, and alone.
+HALVES = [1152, 4138]
+
+
+@pytest.mark.parametrize("t_bucket", HALVES)
+@pytest.mark.parametrize("dim,kind", [(64, "bf16"), (96, "f16"), (128, "bf16"), (192, "bf16"), (256, "f16")])
+def test_halves_of_the_keys(dim, kind, t_bucket):
+    before, new = [1100, 0, 60], [70, 33, 0]
+    lengths = [a + b for a, b in zip(before, new)]
+    k, v, table = pool(lengths, 16, 2, dim, DT[kind], 141)
+    q = queries((sum(new), 6, dim), DT[kind], 142)
+    slopes = torch.linspace(0.3, 0.01, 6, device="cuda")
+    starts = ints([t // 40 * 40 for t in range(70)] + [0] * 20 + [12] * 13)
+    for kw in (dict(), dict(window=300), dict(causal=False), dict(softcap=10.0, slopes=slopes, window=33), dict(starts=starts, prefix=ints([1140, 5, 3]))):
+        out = attn.prefill(q, k, v, table, ints(lengths), offsets_of(new), b_bucket=3, t_bucket=t_bucket, **kw)
+        check(out, q, k, v, table, lengths, new, rows=20, **kw)
+
+
+@pytest.mark.parametrize("t_bucket", HALVES)
+@pytest.mark.parametrize("length", [1, 31, 64, 65, 128, 129, 500, 513])
+def test_halves_of_few_keys(length, t_bucket):
+    """From no tile for the second half on."""
+    for dim in (128, 256):
+        k, v, table = pool([length, 1500], 16, 2, dim, torch.bfloat16, 151)
+        q = queries((min(length, 9), 6, dim), torch.bfloat16, 152)
+        out = attn.prefill(q, k, v, table[:1], ints([length]), offsets_of([len(q)]), b_bucket=3, t_bucket=t_bucket)
+        check(out, q, k, v, table[:1], [length], [len(q)])
+
+
+@pytest.mark.parametrize("t_bucket", HALVES)
+def test_halves_with_faults(t_bucket):
+    """NaN where a row sees it or not, pages that are not there, in either half; captured and replayed."""
+    before, new = [1000, 0], [60, 100]
+    lengths, dim = [1060, 100], 128
+    k, v, table = pool(lengths, 16, 2, dim, torch.float16, 161)
+    q = queries((160, 6, dim), torch.float16, 162)
+    table = torch.cat((table, torch.full((2, 30), -1, dtype=torch.int32, device="cuda")), 1)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    n, off, out = ints(lengths), offsets_of(new), torch.zeros_like(q)
+
+    def call(values, pages, y=None):
+        return attn.prefill(q, k, values, pages, n, off, window=500, out=y, status=status, b_bucket=3, t_bucket=t_bucket)
+
+    clean = call(v, table)
+    check(clean, q, k, v, table, lengths, new, window=500, rows=20)
+    assert ffi.status_read(status) == 0
+    for p in (530, 540, 700, 1030, 1059):
+        v2 = v.clone()
+        v2[table[0, p // 16].long(), p % 16, :, 7] = float("inf")
+        y = call(v2, table)
+        sees = [t for t in range(60) if 1000 + t >= p > 500 + t]
+        rest = [t for t in range(160) if t not in sees]
+        assert torch.equal(y[rest], clean[rest]) and (not sees or not y[sees][..., 7].isfinite().any())
+        assert torch.equal(y[..., 8:], clean[..., 8:])
+    assert ffi.status_read(status) == 0
+    for page in (40, 50, 60, 66):
+        t2 = table.clone()
+        t2[0, page] = k.shape[0]
+        status.zero_()
+        y = call(v, t2)
+        assert ffi.status_read(status) == ffi.STATUS_BAD_PAGE
+        sees = [t for t in range(60) if 16 * page <= 1000 + t and 16 * page + 15 > 500 + t]
+        rest = [t for t in range(160) if t not in sees]
+        assert y[sees].isnan().all() and torch.equal(y[rest], clean[rest])
+    status.zero_()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(v, table, out)
+    for lens in (lengths, [60, 100], [1060, 100]):
+        n.copy_(ints(lens))
+        out.zero_()
+        g.replay()
+        want = call(v, table)
+        assert torch.equal(out, want)
+    assert torch.equal(out, clean) and ffi.status_read(status) == 0
