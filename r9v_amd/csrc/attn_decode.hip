@@ -47,7 +47,7 @@ struct DecodeShape {
     static constexpr int kArea = kBlock * KP * 2; /* bytes of a wave: a block's keys, or after them its sums of 16 rows */
     static_assert(16 * (D + 4) * 4 <= kArea);
     /* waves a SIMD that the registers are to leave room for (256 columns: 366 of 512 for one) */
-    static constexpr int kWavesASimd(int rt) { return D > 192 || D * rt > 256 ? 1 : D * rt > 96 ? 2 : 3; }
+    static constexpr int kWavesASimd(int rt) { return D > 192 ? 1 : D * rt > 96 ? 2 : 3; }
 };
 
 /* DW words in LDS. */
@@ -90,11 +90,13 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
      * then parts, so that it is not always the same dies whose sequences have ended;
      * and with each part the sequences move on, so that a long one's parts are not all
      * on one die (24 of 300 to 16384 keys, 2 kv heads of 256 columns: 86 us without it). */
-    const uint32_t split = blockIdx.z;
-    uint32_t b = blockIdx.y;
-    if (split) b = (b + (gridDim.y - 1) % 8 * split) % gridDim.y;
-    uint32_t kvh = blockIdx.x, tile = 0;
-    if (row_tiles > 1) kvh = blockIdx.x / row_tiles, tile = blockIdx.x - kvh * row_tiles;
+    uint32_t split = blockIdx.z, b = blockIdx.y, kvh = blockIdx.x, tile = 0;
+    if (row_tiles > 1) { /* the tiles of the same keys one after another on one die (40 rows, 4 x 8192 keys of 256 columns: 34 us; beside each other on several 44) */
+        const uint32_t slot = blockIdx.x / 8, turn = slot / row_tiles, group = turn * 8 + blockIdx.x % 8, seqs = group / a.kv_heads;
+        tile = slot - turn * row_tiles, kvh = group - seqs * a.kv_heads, split = seqs / a.b, b = seqs - split * a.b;
+        if (split >= a.splits) return;
+    }
+    if (split) b = (b + (a.b - 1) % 8 * split) % a.b;
     const int rows = (int)(a.t_bucket * a.group);
     const int row0 = (int)tile * RT * 16;
     const int length = a.lengths[b];
@@ -494,21 +496,12 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(r9vx_attn_problem a,
     *reinterpret_cast<four *>(y + c) = four{(typename T::elem)(o[0] * f), (typename T::elem)(o[1] * f), (typename T::elem)(o[2] * f), (typename T::elem)(o[3] * f)};
 }
 
-/* blocks of the longest row */
-uint32_t decode_blocks(const r9vx_attn_problem &p) {
-    const uint32_t whole = (p.len_bucket + kBlock - 1) / kBlock, seen = (p.window + p.t_bucket - 1) / kBlock + 2;
-    return seen < whole ? seen : whole > 0 ? whole : 1;
-}
-
-/* 32 rows a workgroup halve what is read through the caches, but beyond 128 columns
- * they take all registers of a SIMD and longer to begin: only where every wave has
- * several blocks (256 columns, 2 kv heads at 8192 keys, 32 rows: one sequence 25 us
- * with 16 rows and 30 with 32, four 34 and 37, eight 54 and 50; 65536 keys and 64
- * rows 94 and 74; 192 columns, 40 rows, one sequence 19 and 22, eight with 4 kv
- * heads and 32 rows 67 and 53). */
+/* 32 rows a workgroup work on each block of keys half as often (64 rows of 64 columns, 16 x 4096
+ * keys: 32 us against 38; 32 of 128, 8 x 8192: 37 against 40).  Beyond 128 columns they take
+ * all registers of a SIMD: slower (8 x 8192 keys of 256 columns, 32 rows: 50 us against 40). */
 uint32_t decode_row_tiles(const r9vx_attn_problem &p, uint32_t &rt) {
     const uint32_t rows = p.t_bucket * p.group;
-    rt = rows > 16 && (p.head_dim <= 128 || (uint64_t)p.b_bucket * p.kv_heads * decode_blocks(p) >= 16ull * r9vx_device_cus()) ? 2 : 1;
+    rt = rows > 16 && p.head_dim <= 128 ? 2 : 1;
     return (rows + 16 * rt - 1) / (16 * rt);
 }
 
@@ -528,9 +521,15 @@ template <class T, int D>
 int launch_decode(const r9vx_attn_problem &p, hipStream_t stream) {
     uint32_t rt;
     const uint32_t tiles = decode_row_tiles(p, rt);
-    const dim3 grid(p.kv_heads * tiles, p.b, p.splits);
-    if (rt == 2) hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
-    else hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+    const uint64_t groups = r9vx_attn_decode_groups(p);
+    const dim3 grid = tiles > 1 ? dim3((unsigned)groups) : dim3(p.kv_heads, p.b, p.splits);
+    if constexpr (D <= 128) {
+        if (rt == 2) {
+            hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+            return (int)hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
     return (int)hipGetLastError();
 }
 
@@ -549,14 +548,17 @@ int launch_decode_type(const r9vx_attn_problem &p, hipStream_t stream) {
 
 uint64_t r9vx_attn_decode_groups(const r9vx_attn_problem &p) {
     uint32_t rt;
-    return (uint64_t)p.b * p.kv_heads * decode_row_tiles(p, rt) * p.splits;
+    const uint64_t tiles = decode_row_tiles(p, rt), groups = (uint64_t)p.b * p.kv_heads * p.splits;
+    return tiles > 1 ? (groups + 7) / 8 * 8 * tiles : groups;
 }
 
 void r9vx_attn_decode_plan(r9vx_attn_problem &p) {
     uint32_t rt;
     const uint64_t groups = (uint64_t)p.b_bucket * p.kv_heads * decode_row_tiles(p, rt);
-    const uint64_t fill = (p.head_dim > 192 || p.head_dim * rt > 256 ? 1ull : p.head_dim * rt > 96 ? 2ull : 3ull) * r9vx_device_cus();
-    const uint32_t most = decode_blocks(p);
+    const uint64_t fill = (p.head_dim > 192 ? 1ull : p.head_dim * rt > 96 ? 2ull : 3ull) * r9vx_device_cus();
+    /* blocks of the longest row */
+    const uint32_t whole = (p.len_bucket + kBlock - 1) / kBlock, seen = (p.window + p.t_bucket - 1) / kBlock + 2;
+    const uint32_t most = seen < whole ? seen : whole > 0 ? whole : 1;
     uint64_t parts = groups ? fill / groups : 1;
     if (parts > (most + kWaves - 1) / kWaves) parts = (most + kWaves - 1) / kWaves;
     if (parts > kMostParts) parts = kMostParts;
