@@ -134,19 +134,20 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     if (!attn_tile(a.offsets, a.b, a.t, a.group, kRows, tile, part)) return false;
     const uint32_t b = part.b, r0 = part.row;
     const int off = part.offset, news = part.n;
-    const int length = a.lengths[b];
+    const int length = a.lengths[b], prefix = a.prefix ? a.prefix[b] : 0;
     const bool bad_length = length < 0 || length > (int)a.len_bucket;
     if (bad_length && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
 
-    /* this lane's row */
-    const uint32_t row = r0 + wave * 32 + c32;
-    const bool there = row < (uint64_t)news * a.group;
-    const int token = there ? (int)(row / a.group) : 0;
-    const uint32_t head = kvh * a.group + (there ? row - token * a.group : 0);
+    /* this lane's row: the token and the head that row r0 + i is */
+    const uint32_t rows = (uint32_t)news * a.group, i0 = wave * 32, t0 = r0 / a.group, h0 = r0 - t0 * a.group;
+    auto token_of = [&](uint32_t i) { return (int)t0 + attn_token(h0 + i, a.group_magic); };
+    const bool there = r0 + i0 + c32 < rows;
+    const int token = there ? token_of(i0 + c32) : 0;
+    const uint32_t head = kvh * a.group + (there ? h0 + i0 + c32 - (token - t0) * a.group : 0);
     const uint64_t at = (uint64_t)off + token;
     const int pos = length - news + token;
     int lo, hi;
-    attn_seen(a.window, a.causal, pos, length, a.starts ? a.starts[at] : 0, a.prefix ? a.prefix[b] : 0, lo, hi);
+    attn_seen(a.window, a.causal, pos, length, a.starts ? a.starts[at] : 0, prefix, lo, hi);
     if (!there || bad_length) lo = hi = 0;
     const bool some = lo < hi;
     x8 q[D / 16];
@@ -161,15 +162,13 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 
     /* keys that all rows of the wave see, and those that some of the workgroup do: where
      * they begin and end grows with the token, but for the tokens' own starts */
-    const uint32_t rows = (uint32_t)news * a.group, w0 = r0 + wave * 32, w1 = (w0 + 32 < rows ? w0 + 32 : rows) - 1; /* (w0 >= rows: nothing is there) */
+    const uint32_t n0 = rows - r0 < (uint32_t)kRows ? rows - r0 : (uint32_t)kRows, n1 = i0 + 32 < n0 ? i0 + 32 : n0; /* rows of the workgroup; up to this wave's last (i0 >= n0: none is there) */
     int ulo, uhi, wfl, wfh, any;
-    auto seen_by = [&](uint32_t r, int &from, int &to) {
-        attn_seen(a.window, a.causal, length - news + (int)(r / a.group), length, 0, a.prefix ? a.prefix[b] : 0, from, to);
-    };
-    seen_by(r0, ulo, any);
-    seen_by((r0 + kRows < rows ? r0 + kRows : rows) - 1, any, uhi);
-    seen_by(w0 < rows ? w0 : 0, any, wfh);
-    seen_by(w0 < rows ? w1 : 0, wfl, any);
+    auto seen_by = [&](uint32_t i, int &from, int &to) { attn_seen(a.window, a.causal, length - news + token_of(i), length, 0, prefix, from, to); };
+    seen_by(0, ulo, any);
+    seen_by(n0 - 1, any, uhi);
+    seen_by(i0 < n0 ? i0 : 0, any, wfh);
+    seen_by(i0 < n0 ? n1 - 1 : 0, wfl, any);
     if (!CAREFUL && threadIdx.x == 0) sh.redo = 0; /* (the second way is on while other waves read it) */
     if (a.starts) {
         int most = there ? lo : 0, least = some ? lo : INT32_MAX;
@@ -184,9 +183,9 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     if (bad_length) ulo = uhi = 0;
 
     /* this part's tiles */
-    const int t0 = ulo < uhi ? ulo / KT : 0, t1 = ulo < uhi ? (uhi + KT - 1) / KT : 0;
+    const int k0 = ulo < uhi ? ulo / KT : 0, k1 = ulo < uhi ? (uhi + KT - 1) / KT : 0;
     int first, last; /* of the workgroup; then of this half */
-    attn_part(t0, t1, 1, a.parts, a.part_blocks, split, first, last);
+    attn_part(k0, k1, 1, a.parts, a.part_blocks, split, first, last);
     const int steps = (last - first + H - 1) / H, begin = first + half * steps, end = H == 1 ? last : min(begin + steps, last);
 
     const AttnScore score(a);
