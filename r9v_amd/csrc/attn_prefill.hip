@@ -11,7 +11,8 @@
  * S^T = K Q^T: a lane then holds 16 keys of one row in the order that the second
  * product O^T = V^T P^T takes, so that probabilities stay in registers; V^T
  * comes from LDS by the transposing read.  Where the rows are too few to fill the
- * card the keys are cut into parts, joined by a further launch.
+ * card the keys are cut into parts, joined by a further launch, or into halves of
+ * parts for two times four waves, joined through LDS.
  *
  * A tile's 1024 cycles of matrix instructions and its 700 or so of exponentials,
  * maxima and conversions overlap only where the two workgroups of a CU are at different
