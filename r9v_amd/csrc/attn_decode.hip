@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     /* Consecutive workgroups go to the eight dies in turn.  Heads, then sequences,
      * then parts, so that it is not always the same dies whose sequences have ended;
      * and with each part the sequences move on, so that a long one's parts are not all
-     * on one die (24 of 300 to 16384 keys, 2 kv heads of 256 columns: 86 us without it). */
+     * on one die (24 of 300 to 16384 keys, 2 kv heads of 256 columns: 73 us, 86 without it). */
     uint32_t split = blockIdx.z, b = blockIdx.y, kvh = blockIdx.x, tile = 0;
     if (row_tiles > 1) { /* the tiles of the same keys one after another on one die (40 rows, 4 x 8192 keys of 256 columns: 34 us; beside each other on several 44) */
         const uint32_t slot = blockIdx.x / 8, turn = slot / row_tiles, group = turn * 8 + blockIdx.x % 8, seqs = group / a.kv_heads;
@@ -561,6 +561,11 @@ void r9vx_attn_decode_plan(r9vx_attn_problem &p) {
     const uint32_t most = seen < whole ? seen : whole > 0 ? whole : 1;
     uint64_t parts = groups ? fill / groups : 1;
     if (parts > (most + kWaves - 1) / kWaves) parts = (most + kWaves - 1) / kWaves;
+    /* two or three blocks a wave cost what the launch of a join does (one part or one for
+     * each four blocks, in a graph and in calls from Python: 200 keys of 128 columns 7.4 us
+     * against 8.7 and 9.2 against 13.6, 350 9.0 against 9.0 and 9.1 against 13.8; 200 of
+     * 256 columns 10.2 against 11.5, 350 12.7 against 11.6, 517 of 128 11.7 against 9.0) */
+    if (most <= (p.head_dim > 128 ? 2u : 3u) * kWaves) parts = 1;
     if (parts > kMostParts) parts = kMostParts;
     if (parts < 1) parts = 1;
     uint32_t per = (uint32_t)((most + parts - 1) / parts);
