@@ -132,3 +132,27 @@ def test_prompts_chunks_tokens_and_drafts(dim, kw):
         assert all(torch.equal(a, c) for a, c in zip((q, y, z), again[1:]))
         # a draft that was not kept stands behind the next step's first tokens until it is overwritten
         done = [d + n for d, n in zip(done, kept)]
+
+
+def test_two_streams_at_once():
+    """Calls beside each other, each with memory of its stream, on one cache that both read."""
+    lengths, new = [3000, 40, 1700], 2
+    layer = Layer(128, lengths, 3000)
+    g = torch.Generator().manual_seed(11)
+    for c in (layer.k, layer.v):
+        c.copy_(torch.randn(c.shape, generator=g))
+    q = torch.randn(3, new, HEADS, 128, generator=g).to(torch.bfloat16).cuda()
+    p = torch.randn(90, HEADS, 128, generator=g).to(torch.bfloat16).cuda()
+    n, off = ints(lengths), ints([0, 50, 60, 90])
+
+    def calls(stream):
+        return [attn.decode(q, layer.k, layer.v, layer.table, n, stream=stream), attn.prefill(p, layer.k, layer.v, layer.table, n, off, stream=stream)]
+
+    want = calls(None)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [calls(s) for _ in range(8) for s in streams]
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for pair in got for a, b in zip(pair, want))
