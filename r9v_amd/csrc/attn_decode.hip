@@ -60,18 +60,20 @@ __device__ __forceinline__ void store_words(uint16_t *p, const uint32_t (&w)[DW]
     } else *reinterpret_cast<r9vx_u32x4 *>(p) = r9vx_u32x4{w[0], w[1], w[2], w[3]};
 }
 
+/* DW words of global memory.  Said so: a pointer that may be a row of zeros is loaded
+ * through otherwise as one that may be LDS, whose waits are then those for these loads. */
 template <int DW>
 __device__ __forceinline__ void load_words(const uint16_t *p, uint32_t (&w)[DW]) {
     static_assert(DW >= 2 && DW <= 4);
     if constexpr (DW == 2) {
-        const r9vx_u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const r9vx_u32x2 *>(p));
+        const r9vx_u32x2 v = __builtin_nontemporal_load((const __attribute__((address_space(1))) r9vx_u32x2 *)p);
         w[0] = v.x, w[1] = v.y;
     } else if constexpr (DW == 3) { /* 12 bytes: dword alignment */
         typedef attn_u32x3 vec __attribute__((aligned(4)));
-        const attn_u32x3 v = *reinterpret_cast<const vec *>(p);
+        const attn_u32x3 v = *(const __attribute__((address_space(1))) vec *)p;
         w[0] = v.x, w[1] = v.y, w[2] = v.z;
     } else {
-        const r9vx_u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const r9vx_u32x4 *>(p));
+        const r9vx_u32x4 v = __builtin_nontemporal_load((const __attribute__((address_space(1))) r9vx_u32x4 *)p);
         w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     }
 }

@@ -154,7 +154,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     x8 q[D / 16];
     const uint16_t *qrow = (there ? a.q + at * a.q_stride[1] + head * a.q_stride[2] : reinterpret_cast<const uint16_t *>(kAttnZeroRow)) + h2 * 8;
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) q[s] = *reinterpret_cast<const x8 *>(qrow + s * 16);
+    for (int s = 0; s < D / 16; ++s) q[s] = *(const __attribute__((address_space(1))) x8 *)(qrow + s * 16);
     if (a.scale <= 0.0f) {
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) q[s] = attn_signed<T>(a, q[s]);
