@@ -59,10 +59,13 @@ struct PrefillShape {
 /* 16 bytes of each lane of `lanes` from `base` + `off` (bytes) in global memory to LDS at
  * `at` + 16 * lane.  Within straight-line code: a branch around it would cut the
  * schedule in pieces.  (No "memory": it writes a buffer that is read behind the next
- * barrier alone, and may stand among reads of the other.) */
+ * barrier alone, and may stand among reads of the other.)  `base` comes from v_readlane:
+ * a scalar register that a vector instruction wrote is a memory instruction's to read
+ * five wait states later, which neither the hardware nor, in here, the compiler sees
+ * to.  Two are the instructions before the load, three s_nop's. */
 __device__ __forceinline__ void attn_copy16(uint32_t at, const uint16_t *base, uint32_t off, uint64_t lanes) {
     uint64_t all;
-    asm volatile("s_mov_b32 m0, %3\n\ts_and_saveexec_b64 %0, %4\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, %0"
+    asm volatile("s_mov_b32 m0, %3\n\ts_and_saveexec_b64 %0, %4\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, %0"
                  : "=&s"(all) : "v"(off), "s"(base), "s"(at), "s"(lanes) : "m0", "scc");
 }
 
