@@ -32,7 +32,9 @@
  * Probabilities are rounded to the cache's type before they are multiplied with
  * values (by up to 2^-8 of each for bf16, 2^-11 for f16: as much again as the
  * output's own rounding); attn_decode keeps a bf16 probability as two bf16
- * numbers.  One rounding to the output.
+ * numbers.  One rounding to the output.  A cap adds up to 5 * 2^-23 of itself to a
+ * score's error, one above 128 at most 21 * 2^-23 of the score; one above 2^100 is
+ * taken as 2^100.
  *
  * Faulty data.  A page that is not in the cache, or a length below 0 or above
  * len_bucket, makes that sequence's outputs NaN, as far as they were to see it,

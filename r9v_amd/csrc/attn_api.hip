@@ -116,7 +116,8 @@ r9vx_attn_problem attn_problem(const r9vx_attn_static *st, bool decode) {
     p.causal = st->causal;
     p.window = st->window && st->window < kAttnNoWindow ? st->window : kAttnNoWindow;
     p.scale = as_float(st->scale_bits);
-    p.softcap = as_float(st->softcap_bits);
+    /* (a cap of 2^100 leaves scores up to 2^88 as they are, and scale / cap a normal number) */
+    p.softcap = fminf(as_float(st->softcap_bits), 0x1p100f);
     p.b = st->b_bucket;
     p.t = st->t_bucket;
     if (decode) r9vx_attn_decode_plan(p);

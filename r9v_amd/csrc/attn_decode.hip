@@ -78,7 +78,9 @@ __device__ __forceinline__ void load_words(const uint16_t *p, uint32_t (&w)[DW])
     }
 }
 
-template <class T, int D, int RT>
+/* FAR: of a cap above kAttnShortCap (both formulas in one loop took 19.2 us for a token and
+ * four drafts at 8191 keys, without a cap, where one takes 18.7). */
+template <class T, int D, int RT, bool FAR>
 __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void attn_decode_kernel(r9vx_attn_problem a, uint32_t row_tiles) {
     using S = DecodeShape<D>;
     typedef typename T::x8 x8;
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
                 for (int e = 0; e < 8; ++e) x[e] = sc[r][e >> 2][e & 3];
                 if (a.softcap > 0.0f) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = score.capped(x[e]);
+                    for (int e = 0; e < 8; ++e) x[e] = FAR ? score.capped_far(x[e]) : score.capped(x[e]);
                 }
                 if (a.slopes) {
                     const float far = (float)(pos[r] - k8);
@@ -519,6 +521,13 @@ int launch_join(const r9vx_attn_problem &p, const float2 *ml, uint64_t rows, hip
     return (int)hipGetLastError();
 }
 
+template <class T, int D, int RT>
+int launch_decode_rows(const r9vx_attn_problem &p, dim3 grid, uint32_t tiles, hipStream_t stream) {
+    if (p.softcap > kAttnShortCap) hipLaunchKernelGGL((attn_decode_kernel<T, D, RT, true>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+    else hipLaunchKernelGGL((attn_decode_kernel<T, D, RT, false>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
+    return (int)hipGetLastError();
+}
+
 template <class T, int D>
 int launch_decode(const r9vx_attn_problem &p, hipStream_t stream) {
     uint32_t rt;
@@ -526,13 +535,9 @@ int launch_decode(const r9vx_attn_problem &p, hipStream_t stream) {
     const uint64_t groups = r9vx_attn_decode_groups(p);
     const dim3 grid = tiles > 1 ? dim3((unsigned)groups) : dim3(p.kv_heads, p.b, p.splits);
     if constexpr (D <= 128) {
-        if (rt == 2) {
-            hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
-            return (int)hipGetLastError();
-        }
+        if (rt == 2) return launch_decode_rows<T, D, 2>(p, grid, tiles, stream);
     }
-    hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, dim3(64 * kWaves), 0, stream, p, tiles);
-    return (int)hipGetLastError();
+    return launch_decode_rows<T, D, 1>(p, grid, tiles, stream);
 }
 
 template <class T>

@@ -11,10 +11,12 @@ F32 = 2.0 ** -23  # twice an f32 rounding: a step of the matrix unit or of a har
 
 
 def cap_error(s, softcap):
-    """Of softcap * tanh(s / softcap), absolutely.  cap - 2 cap / (e + 1):
+    """Of softcap * tanh(s / softcap), absolutely.  Caps up to 128, cap - 2 cap / (e + 1):
     e's argument (2 roundings and exp2) moves it by at most cap F32, e + 1 and the
-    reciprocal by 1.5 F32 of 2 cap, the sum and the cap by F32 of cap: 5 cap F32."""
-    return 5 * softcap * F32
+    reciprocal by 1.5 F32 of 2 cap, the sum and the cap by F32 of cap: 5 cap F32.  Above,
+    where |s| < cap / 4, s times a series: 8 roundings of s; elsewhere cap < 4.1 |out|:
+    21 F32 of it."""
+    return 5 * softcap * F32 if softcap <= 128 else 21 * np.abs(softcap * np.tanh(s / softcap)) * F32
 
 
 def attention(q, keys, values, seen, p, scale, softcap, slope, dtype, decode, rounded=None):

@@ -7,8 +7,8 @@ import torch
 from attn_cases import DT
 
 WINDOW = 6
-CASES = [dict(), dict(scale=-0.1), dict(softcap=0.3), dict(softcap=2.0), dict(softcap=20.0), dict(softcap=50.0), dict(softcap=128.0),
-         dict(slopes=True), dict(softcap=2.0, slopes=True)]
+CASES = [dict(), dict(scale=-0.1), dict(softcap=0.3), dict(softcap=2.0), dict(softcap=20.0), dict(softcap=50.0), dict(softcap=128.0), dict(softcap=129.0),
+         dict(softcap=1e4), dict(softcap=1e7), dict(softcap=1e30), dict(slopes=True), dict(softcap=2.0, slopes=True), dict(softcap=1e5, slopes=True)]
 
 
 def inputs(dim, kind, t, length, heads, kv=1, seed=17):

@@ -32,3 +32,15 @@ def test_f16_probabilities_rounded_to_bf16_are_not_within_it(dim, kw, decode):
         coarse = B.attention(*args, rounded=rounding(torch.bfloat16))[0]
         missed += int((np.abs(coarse - want) > tol).any())
     assert missed >= 4
+
+
+def test_an_f32_of_the_short_form_is_not_within_it_at_large_caps():
+    """1 - 2 / (e + 1) in f32 throughout, at the caps that take the series."""
+    f = np.float32
+    s = np.linspace(-4, 4, 1001)
+    for cap, holds in ((0.3, True), (20.0, True), (50.0, True), (128.0, True), (1e4, False), (1e7, False)):
+        with np.errstate(over="ignore"):
+            e = np.exp2((s.astype(f) * f(2 * 1.4426950408889634 / cap)).astype(f)).astype(f)
+            short = f(cap) - f(2 * cap) / (e + f(1))
+        err = np.abs(short.astype(np.float64) - cap * np.tanh(s / cap))
+        assert (err <= B.cap_error(s, cap) + B.F32).all() == holds, cap

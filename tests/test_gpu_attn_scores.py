@@ -63,7 +63,7 @@ def test_prefill(kw, dim, kind):
     check(out, q, k, v, table, lengths, new, False, **more)
 
 
-@pytest.mark.parametrize("softcap", [50.0])
+@pytest.mark.parametrize("softcap", [50.0, 1e4, 1e7])
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 def test_caps_of_many_keys(softcap, kind):
     """Every key seen, in parts that are joined; scores of up to 50, so that the caps of 50 are reached."""
