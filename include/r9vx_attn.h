@@ -95,7 +95,8 @@ typedef struct r9vx_rope_kv_args {
  * the cache writes nothing and sets R9VX_STATUS_BAD_SLOT; of two rows with one
  * slot either may be kept, 16 bytes by 16 bytes.  Pointers 16-byte aligned,
  * strides such that every head is; rows of q_out, of k_cache and of v_cache
- * apart from each other. */
+ * apart from each other.  q in place may stand among k's and v's rows (of the same
+ * token stride) and be none of them. */
 int r9vx_rope_kv_launch(const r9vx_rope_kv_static *st, const r9vx_rope_kv_args *args, r9vx_stream_t stream);
 
 /* ----------------------------------------------------------- attention */

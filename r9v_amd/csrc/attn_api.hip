@@ -52,6 +52,54 @@ bool rows_apart(const uint64_t (&stride)[N], const uint64_t (&size)[N], uint64_t
     return true;
 }
 
+/* A strided operand's rows: of `columns` elements, `size` of them `stride` apart on each axis. */
+template <int N>
+struct Rows {
+    uintptr_t at;
+    uint64_t stride[N], size[N], columns, bytes;
+    __int128 extent(int axis) const { /* from an element to behind the last of the axes from `axis` on */
+        __int128 last = 0;
+        for (int i = axis; i < N; ++i) last += (__int128)(size[i] - 1) * stride[i];
+        return (last + columns) * bytes;
+    }
+};
+
+/* Whether no row of x meets one of y, whose first element is `d` bytes behind x's.  Axes
+ * go from the widest stride on.  Where both have the same stride, longer than what is
+ * inside it, y's inner rows are between two of x's, the distance modulo the stride apart:
+ * those are looked at in turn.  (Rows that may be apart and are not of this kind
+ * count as meeting.) */
+template <int N>
+bool apart(const Rows<N> &x, const Rows<N> &y, __int128 d, int axis = 0) {
+    if (d >= x.extent(axis) || -d >= y.extent(axis)) return true;
+    if (axis == N) return false;
+    const bool many = x.size[axis] > 1, also = y.size[axis] > 1;
+    if (!many && !also) return apart(x, y, d, axis + 1);
+    const __int128 stride = (__int128)(many ? x.stride[axis] : y.stride[axis]) * x.bytes;
+    if ((many && also && x.stride[axis] != y.stride[axis]) || stride < x.extent(axis + 1) || stride < y.extent(axis + 1)) return false;
+    const __int128 r = (d % stride + stride) % stride;
+    return apart(x, y, r, axis + 1) && apart(x, y, r - stride, axis + 1);
+}
+
+template <int N>
+bool apart(const void *px, const uint64_t (&sx)[N], const uint64_t (&nx)[N], const void *py, const uint64_t (&sy)[N], const uint64_t (&ny)[N], uint64_t columns,
+           uint64_t bytes) {
+    Rows<N> x{(uintptr_t)px, {}, {}, columns, bytes}, y{(uintptr_t)py, {}, {}, columns, bytes};
+    bool done[N] = {};
+    for (int n = 0; n < N; ++n) {
+        int widest = -1;
+        uint64_t most = 0;
+        for (int i = 0; i < N; ++i) {
+            if (!nx[i] || !ny[i]) return true;
+            const uint64_t s = nx[i] > 1 ? sx[i] : ny[i] > 1 ? sy[i] : 0;
+            if (!done[i] && (widest < 0 || s > most)) widest = i, most = s;
+        }
+        done[widest] = true;
+        x.stride[n] = sx[widest], x.size[n] = nx[widest], y.stride[n] = sy[widest], y.size[n] = ny[widest];
+    }
+    return apart(x, y, (__int128)y.at - (__int128)x.at);
+}
+
 template <int N>
 void check_strides(const char *name, const uint64_t (&stride)[N], uint64_t bytes, Problems &pr) {
     for (int i = 0; i < N; ++i) {
@@ -272,8 +320,9 @@ int r9vx_rope_kv_launch(const r9vx_rope_kv_static *st, const r9vx_rope_kv_args *
         if (cache) {
             const uint64_t nk = span(a->k_stride, kv, st->head_dim, in), nv = span(a->v_stride, kv, st->head_dim, in);
             const uint64_t nkc = span(a->k_cache_stride, pages, st->head_dim, out), nvc = span(a->v_cache_stride, pages, st->head_dim, out);
-            /* q in place may stand among k's and v's rows, as one projection leaves them */
-            if (!in_place && (overlap(a->q_out, ny, a->k, nk) || overlap(a->q_out, ny, a->v, nv)))
+            /* q in place may stand among k's and v's rows, as one projection leaves them, but be none of them */
+            if (in_place ? !apart(a->q_out, a->q_out_stride, rows, a->k, a->k_stride, kv, st->head_dim, in) || !apart(a->q_out, a->q_out_stride, rows, a->v, a->v_stride, kv, st->head_dim, in)
+                         : overlap(a->q_out, ny, a->k, nk) || overlap(a->q_out, ny, a->v, nv))
                 pr.add(R9VX_ERR_INVALID, "q_out must not overlap k or v");
             if (overlap(a->k_cache, nkc, a->q, nq) || overlap(a->k_cache, nkc, a->k, nk) || overlap(a->k_cache, nkc, a->v, nv) || overlap(a->k_cache, nkc, a->q_out, ny) ||
                 overlap(a->v_cache, nvc, a->q, nq) || overlap(a->v_cache, nvc, a->k, nk) || overlap(a->v_cache, nvc, a->v, nv) || overlap(a->v_cache, nvc, a->q_out, ny))
