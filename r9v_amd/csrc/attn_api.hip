@@ -331,7 +331,8 @@ int r9vx_rope_kv_launch(const r9vx_rope_kv_static *st, const r9vx_rope_kv_args *
                 overlap(a->v_cache, nvc, a->positions, 4ull * a->t) || overlap(a->v_cache, nvc, a->freqs, 4ull * st->rot) || overlap(a->v_cache, nvc, a->slots, 8ull * a->t))
                 pr.add(R9VX_ERR_INVALID, "the cache must not overlap positions, freqs or slots");
             /* (keys and values may take turns in one allocation) */
-            if (!rows_apart(a->k_cache_stride, pages, st->head_dim) || !rows_apart(a->v_cache_stride, pages, st->head_dim) || (nkc && a->k_cache == a->v_cache))
+            if (!rows_apart(a->k_cache_stride, pages, st->head_dim) || !rows_apart(a->v_cache_stride, pages, st->head_dim) ||
+                !apart(a->k_cache, a->k_cache_stride, pages, a->v_cache, a->v_cache_stride, pages, st->head_dim, out))
                 pr.add(R9VX_ERR_INVALID, "rows of the cache overlap each other");
         }
     }

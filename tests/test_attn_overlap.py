@@ -73,3 +73,49 @@ RECORDS = pytest.mark.skipif(not launch_record.LIB.exists() or shutil.which("gcc
 @RECORDS
 def test_q_in_place_beside_k_and_v(tmp_path, monkeypatch):
     accepted(tmp_path, monkeypatch, BESIDE)
+
+
+PAGE, PAGES = 16, 10
+TOKEN, WHOLE = KV * D, PAGE * KV * D
+K = APART["k_cache"]
+
+
+def caches(v, k_stride, v_stride=None, **kw):
+    """v_cache `v` elements behind k_cache."""
+    return dict(v_cache=K + 2 * v, k_cache_stride=k_stride, v_cache_stride=v_stride or k_stride, **kw)
+
+
+DENSE = (WHOLE, TOKEN, D)
+MEETING = {
+    "a page on": caches(WHOLE, DENSE),
+    "a token on": caches(TOKEN, DENSE),
+    "a head on": caches(D, DENSE),
+    "half a head on": caches(64, (2 * WHOLE, 2 * TOKEN, 2 * D)),
+    "the last page is the first": caches((PAGES - 1) * WHOLE, DENSE),
+    "another order in the same pages": caches(D, (2 * WHOLE, 2 * TOKEN, 2 * D), (2 * WHOLE, D, PAGE * D)),
+    "half of the second's tokens in the first's": caches(PAGE // 2 * TOKEN, (2 * WHOLE, TOKEN, D)),
+    "a page before": caches(-WHOLE, DENSE),
+}
+APART_CACHES = {
+    "one after the other": caches(PAGES * WHOLE, DENSE),
+    "pages in turn": caches(WHOLE, (2 * WHOLE, TOKEN, D)),
+    "pages in turn, values first": caches(-WHOLE, (2 * WHOLE, TOKEN, D)),
+    "tokens in turn": caches(TOKEN, (2 * WHOLE, 2 * TOKEN, D)),
+    "heads in turn": caches(D, (2 * WHOLE, 2 * TOKEN, 2 * D)),
+    "heads first, then tokens in turn": caches(D, (2 * WHOLE, 2 * D, 2 * PAGE * D)),
+    "heads first in halves of a page": caches(PAGE * D, (2 * WHOLE, D, 2 * PAGE * D)),
+    "tokens and heads of each in an order of its own, pages in turn": caches(WHOLE, (2 * WHOLE, TOKEN, D), (2 * WHOLE, D, PAGE * D)),
+    "one kv head, tokens in turn": caches(D, (2 * PAGE * D, 2 * D, 0), kv_heads=1),
+    "one page": caches(TOKEN, (0, 2 * TOKEN, D), pages=1),
+    "no page": caches(0, DENSE, pages=0),
+}
+
+
+@pytest.mark.parametrize("name", MEETING)
+def test_caches_that_meet(name):
+    refused(lib.r9vx_rope_kv_launch, *rope(**MEETING[name]), code=INVALID, text="rows of the cache overlap each other")
+
+
+@RECORDS
+def test_caches_beside_each_other(tmp_path, monkeypatch):
+    accepted(tmp_path, monkeypatch, APART_CACHES)
