@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import functools
 import math
+import numbers
 import struct
 
 from . import ffi
@@ -111,7 +112,7 @@ def _plan(key, make, *args):
 
 
 def _number(name, x):
-    if type(x) not in (int, float):
+    if not isinstance(x, numbers.Real) or isinstance(x, bool):
         raise R9vxError(-103, f"{name}={x!r} is no number")
     return _bits(x)
 
