@@ -93,21 +93,23 @@ def _bits(x):
 
 # A decode step makes these calls in every layer and each takes a few microseconds
 # on the GPU.  What a call checks and fills in goes by its operands' shapes, strides,
-# types and devices and by its numbers alone: it is kept by those (ffi._fp8_statics,
-# beside the statics), and a further call of the same ones packs its pointers.
+# types and devices and by its numbers alone: it is kept by those, and a further call of
+# the same ones packs its pointers.
+
+_plans = {}  # of these calls alone: a server whose every prompt has a new length fills it
+
 
 def _meta(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
 def _plan(key, make, *args):
-    plans = ffi._fp8_statics
-    got = plans.get(key)
+    got = _plans.get(key)
     if got is None:
         got = make(*args)
-        if len(plans) >= 4096:  # a caller that never repeats a size
-            plans.clear()
-        plans[key] = got
+        if len(_plans) >= 4096:  # a caller that never repeats a size
+            _plans.clear()
+        _plans[key] = got
     return got
 
 

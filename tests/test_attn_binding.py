@@ -27,3 +27,15 @@ def test_numbers_of_any_type_are_taken(x, on_cpu, monkeypatch):  # noqa: F811
 def test_what_is_no_number_is_refused(x):
     with pytest.raises(ffi.R9vxError, match="is no number"):
         attn._number("softcap", x)
+
+
+def test_plans_are_of_these_calls_alone(on_cpu, monkeypatch):  # noqa: F811
+    """A caller that never repeats a size leaves what the e4m3 calls keep."""
+    monkeypatch.setattr(attn.ffi, "_fp8_operands", lambda *o: 0)
+    kept = {("a static", i): i for i in range(4000)}
+    monkeypatch.setattr(ffi, "_fp8_statics", dict(kept))
+    monkeypatch.setattr(attn, "_plans", {}, raising=False)
+    with on_cpu:
+        for i in range(5000):
+            CALLS["rope"](amplitude=1.0 + i)
+    assert ffi._fp8_statics == kept and 0 < len(attn._plans) <= 4096
