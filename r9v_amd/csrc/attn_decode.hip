@@ -278,13 +278,13 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 #pragma unroll
                         for (int j = 0; j < S::DL; ++j) o[r][c][j] *= f;
                 }
-                const float ref = (m[r] == -INFINITY ? 0.0f : m[r]) - T::kBits;
+                const float ref = (m[r] == -INFINITY ? 0.0f : m[r]) - T::kTop;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float pe = __builtin_amdgcn_exp2f(fmaf(x[e], score.factor, -ref));
                     l[r] += pe;
                     ph[r][e] = (typename T::elem)pe;
-                    if constexpr (T::kBits == 0.0f) pl[r][e] = (typename T::elem)(pe - (float)ph[r][e]);
+                    if constexpr (T::kWide) pl[r][e] = (typename T::elem)(pe - (float)ph[r][e]);
                 }
             }
             if (key0 < vlo || key0 + kBlock > vhi) { /* what stands behind the last key, or is not to be seen */
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
                         o[r][c][j] = T::mma16(vt, ph[r], o[r][c][j]);
-                        if constexpr (T::kBits == 0.0f) o[r][c][j] = T::mma16(vt, pl[r], o[r][c][j]);
+                        if constexpr (T::kWide) o[r][c][j] = T::mma16(vt, pl[r], o[r][c][j]);
                     }
                 }
             if (more) {

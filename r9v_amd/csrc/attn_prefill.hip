@@ -96,7 +96,7 @@ __device__ __forceinline__ void attn_priority() {
 /* Bits of a pair of elements whose exponent is that of an infinity or a NaN. */
 template <class T>
 __device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
-    constexpr uint32_t e = T::kBits == 0.0f ? 0x7F80u : 0x7C00u;
+    constexpr uint32_t e = T::kWide ? 0x7F80u : 0x7C00u;
     return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
 }
 
@@ -379,7 +379,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[d][e] *= f;
             }
-            const float ref = (m == -INFINITY ? 0.0f : m) - T::kBits;
+            const float ref = (m == -INFINITY ? 0.0f : m) - (T::kTop - kAttnSlack);
 #pragma unroll
             for (int s = 0; s < KT / 16; ++s) {
 #pragma unroll

@@ -70,12 +70,14 @@ constexpr float kAttnSlack = 8.0f;
  * 32 heads of 128 columns take 727 us at a cap of 50 and 830 at one of 1000. */
 constexpr float kAttnShortCap = 128.0f;
 
-/* The two element types.  kBits is added to every exponent of a probability:
- * f16 holds 2^-24 at the least, so they are made up to 2^15 there. */
+/* The two element types.  kTop is the exponent that the largest probability of a row is
+ * given at most: f16 holds 2^-24 at the least, so 15 there (the largest is 2^7 to 2^15 where
+ * the reference lags by kAttnSlack). */
 struct AttnBf16 {
     typedef r9vx_bf16x8 x8;
     typedef __bf16 elem;
-    static constexpr float kBits = 0.0f;
+    static constexpr bool kWide = true; /* f32's exponents */
+    static constexpr float kTop = 0.0f;
     static constexpr uint32_t kNan = 0x7FC07FC0u;
     /* c and the eight elements, in f32 */
     static __device__ __forceinline__ float add8(x8 x, float c) {
@@ -90,7 +92,8 @@ struct AttnBf16 {
 struct AttnF16 {
     typedef attn_f16x8 x8;
     typedef _Float16 elem;
-    static constexpr float kBits = 15.0f - kAttnSlack;
+    static constexpr bool kWide = false;
+    static constexpr float kTop = 15.0f;
     static constexpr uint32_t kNan = 0x7E007E00u;
     static __device__ __forceinline__ float add8(x8 x, float c) {
         const r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, x);

@@ -52,6 +52,6 @@ def attention(q, keys, values, seen, p, scale, softcap, slope, dtype, decode, ro
     else:
         tol = tol + 2.0 ** -16 * (w @ np.abs(v))
     tol = tol + (n + 64) * F32 * (w @ np.abs(v) + np.abs(out))  # sums of n terms, parts and waves
-    if dtype == R.torch.float16:  # probabilities of 2^7 to 2^15 at the largest, in steps of 2^-24 below 2^-14
-        tol = tol + 2.0 ** -32 * w.max() * (np.abs(v).sum(0) + n * np.abs(out)) + 2.0 ** -25
+    if dtype == R.torch.float16:  # probabilities of 2^15 at the largest (prefill 2^7 to 2^15), in steps of 2^-24 below 2^-14
+        tol = tol + 2.0 ** (-40 if decode else -32) * w.max() * (np.abs(v).sum(0) + n * np.abs(out)) + 2.0 ** -25
     return out, tol * (1 + 2.0 ** -10)

@@ -74,3 +74,22 @@ def test_caps_of_many_keys(softcap, kind):
         check(out[0], q[0], k, v, table, [2000], [2], True, softcap=softcap, scale=scale)
         out = attn.prefill(q[0], k, v, table, ints([2000]), ints([0, 2]), softcap=softcap, scale=scale)
         check(out, q[0], k, v, table, [2000], [2], False, softcap=softcap, scale=scale)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("score", [17.0, 21.0, 23.0])
+def test_a_tail_whose_values_are_large(score, new):
+    """One key of value 0, and those behind it that weigh 2^-24 to 2^-33 of it and have values of 60000."""
+    for length in (384, 3000):
+        k, v, table = pool([length], 16, 1, 64, torch.float16, 177)
+        k.mul_(0.0), k.nan_to_num_(0.0)
+        v.mul_(0.0).nan_to_num_(0.0).add_(60000.0)
+        page = table[0, 0].long()
+        k[page, 7, 0, 0] = 1.0
+        v[page, 7] = 0.0
+        q = torch.zeros(1, new, 2, 64, dtype=torch.float16, device="cuda")
+        q[..., 0] = score
+        out = attn.decode(q, k, v, table, ints([length]), scale=1.0)
+        check(out[0], q[0], k, v, table, [length], [new], True, scale=1.0)
+        out = attn.prefill(q[0], k, v, table, ints([length]), ints([0, new]), scale=1.0)
+        check(out, q[0], k, v, table, [length], [new], False, scale=1.0)
