@@ -72,12 +72,13 @@ constexpr float kAttnShortCap = 128.0f;
 
 /* The two element types.  kTop is the exponent that the largest probability of a row is
  * given at most: f16 holds 2^-24 at the least, so 15 there (the largest is 2^7 to 2^15 where
- * the reference lags by kAttnSlack). */
+ * the reference lags by kAttnSlack); bf16 has f32's exponents, and -32 keeps the sums of
+ * 2^30 values of any size finite. */
 struct AttnBf16 {
     typedef r9vx_bf16x8 x8;
     typedef __bf16 elem;
     static constexpr bool kWide = true; /* f32's exponents */
-    static constexpr float kTop = 0.0f;
+    static constexpr float kTop = -32.0f;
     static constexpr uint32_t kNan = 0x7FC07FC0u;
     /* c and the eight elements, in f32 */
     static __device__ __forceinline__ float add8(x8 x, float c) {
