@@ -26,7 +26,8 @@
  *     out = sum over the seen j of softmax(s)[j] * v[j]
  * A query that sees no key gets zeros.  What is not seen has no part in a row,
  * whatever its place in the cache holds (NaN and infinities too); a NaN that is
- * seen, or a softmax that is none (+infinity, all -infinity), makes the row NaN.
+ * seen, or a softmax that is none (+infinity, all -infinity), makes the row NaN.  An
+ * infinite value that is seen makes its column infinite, however small its probability.
  *
  * Numbers.  Products are summed in f32; scores, their maximum and sum are f32.
  * Probabilities are rounded to the cache's type before they are multiplied with

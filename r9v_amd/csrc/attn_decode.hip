@@ -78,15 +78,27 @@ __device__ __forceinline__ void load_words(const uint16_t *p, uint32_t (&w)[DW])
     }
 }
 
-/* FAR: of a cap above kAttnShortCap (both formulas in one loop took 19.2 us for a token and
- * four drafts at 8191 keys, without a cap, where one takes 18.7). */
-template <class T, int D, int RT, bool FAR>
-__global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void attn_decode_kernel(r9vx_attn_problem a, uint32_t row_tiles) {
+template <int D>
+struct DecodeShared {
+    float jm[kWaves][16], jl[kWaves][16];
+    __attribute__((aligned(16))) uint8_t area[kWaves][DecodeShape<D>::kArea];
+    uint32_t redo;
+};
+
+/* A workgroup's rows.  FAR: of a cap above kAttnShortCap (both formulas in one loop took
+ * 19.2 us for a token and four drafts at 8191 keys, without a cap, where one takes 18.7).
+ * CAREFUL: the second way, which a workgroup takes where the first one gave a NaN or an
+ * infinity: a key that another token alone sees may have brought it in through a
+ * probability of zero, and one that is seen makes a NaN of a probability's second half of
+ * zero.  It goes through the keys once for each token, and adds values that are not
+ * finite by a product of their own, with ones.  Returns whether the second way has to be taken. */
+template <class T, int D, int RT, bool FAR, bool CAREFUL>
+__device__ __forceinline__ bool attn_decode_rows(const r9vx_attn_problem &a, uint32_t row_tiles, DecodeShared<D> &sh) {
     using S = DecodeShape<D>;
     typedef typename T::x8 x8;
-    __shared__ float jm[kWaves][16], jl[kWaves][16];
-    __shared__ __attribute__((aligned(16))) uint8_t area[kWaves][S::kArea];
-    __shared__ uint32_t redo;
+    auto &jm = sh.jm;
+    auto &jl = sh.jl;
+    auto &area = sh.area;
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = lane >> 4;
@@ -98,7 +110,7 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     if (row_tiles > 1) { /* the tiles of the same keys one after another on one die (40 rows, 4 x 8192 keys of 256 columns: 34 us; beside each other on several 44) */
         const uint32_t slot = blockIdx.x / 8, turn = slot / row_tiles, group = turn * 8 + blockIdx.x % 8, seqs = group / a.kv_heads;
         tile = slot - turn * row_tiles, kvh = group - seqs * a.kv_heads, split = seqs / a.b, b = seqs - split * a.b;
-        if (split >= a.splits) return;
+        if (split >= a.splits) return false;
     }
     if (split) b = (b + (a.b - 1) % 8 * split) % a.b;
     const int rows = (int)(a.t_bucket * a.group);
@@ -197,18 +209,17 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
     float m[RT], l[RT];
     r9vx_f32x4 o[RT][S::VC][S::DL];
 
-    /* Keys [vlo, vhi) have values; a second pass for each token follows only where
-     * the first gave a NaN or an infinity, which a key that another token alone
-     * sees may have brought in through a probability of zero. */
+    /* keys [vlo, vhi) have values: those that some row sees, or of the second way those that its token does */
     int vlo = ulo, vhi = uhi;
-    if (threadIdx.x == 0) redo = 0;
-    for (int pass = -1; pass <= last; ++pass) {
-        if (pass >= 0) {
-            if (pass < first) continue;
+    if (!CAREFUL && threadIdx.x == 0) sh.redo = 0;
+    for (int pass = CAREFUL ? first : last; pass <= last; ++pass) {
+        if (CAREFUL) {
             attn_seen(a.window, 1, p0 + pass, length, start, 0, vlo, vhi);
-            __syncthreads(); /* the sums of the pass before have been read */
-            first_page();
-            first_block();
+            if (pass > first) {
+                __syncthreads(); /* the sums of the pass before have been read */
+                first_page();
+                first_block();
+            }
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -270,7 +281,8 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
                 top = fmaxf(top, __shfl_xor(top, 32, R9VX_WAVE)) * score.factor;
                 if (__any(top > m[r])) {
                     const float now = fmaxf(m[r], top);
-                    const float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - now);
+                    float f = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - now);
+                    if (CAREFUL) f = attn_some(f);
                     m[r] = now;
                     l[r] *= f;
 #pragma unroll
@@ -304,6 +316,18 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         w[i] = __builtin_amdgcn_perm(v[2 * i + 1][c][j >> 1], v[2 * i][c][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+                    if (CAREFUL) { /* what is not finite apart from what is */
+                        const r9vx_u32x4 ones = {T::kOnes, T::kOnes, T::kOnes, T::kOnes};
+                        r9vx_u32x4 not_finite;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t bits = attn_odd<T>(w[i]);
+                            not_finite[i] = w[i] & bits;
+                            w[i] &= ~bits;
+                        }
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) o[r][c][j] = T::mma16(__builtin_bit_cast(x8, not_finite), __builtin_bit_cast(x8, ones), o[r][c][j]);
+                    }
                     const x8 vt = __builtin_bit_cast(x8, w);
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
@@ -337,7 +361,7 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
             for (int i = threadIdx.x; i < 16 * D / 4; i += 64 * kWaves) {
                 const int in = i / (D / 4), c = i % (D / 4) * 4, row = row0 + r * 16 + in;
                 const int tok = attn_token(row, a.group_magic);
-                if (row >= rows || (pass >= 0 && tok != pass)) continue;
+                if (row >= rows || (CAREFUL && tok != pass)) continue;
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) top = fmaxf(top, jm[w][in]);
@@ -345,7 +369,8 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) {
                     /* a wave that saw nothing (or scores of -infinity alone) has zeros, or a NaN of NaN scores */
-                    const float f = jm[w][in] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(jm[w][in] - top);
+                    float f = jm[w][in] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(jm[w][in] - top);
+                    if (CAREFUL) f = attn_some(f);
                     sum += jl[w][in] * f;
                     y += *reinterpret_cast<const r9vx_f32x4 *>(reinterpret_cast<const float *>(area[w]) + in * (D + 4) + c) * f;
                 }
@@ -370,13 +395,26 @@ __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void 
                 }
             }
         }
-        if (pass < 0) {
-            if (first == last) break;
-            if (odd) redo = 1;
+        if (!CAREFUL) {
+            if (odd) sh.redo = 1;
             __syncthreads();
-            if (!redo) break;
         }
     }
+    return !CAREFUL && sh.redo;
+}
+
+/* Out of line: nothing of it takes registers of the first way's loop. */
+template <class T, int D, int RT, bool FAR>
+__device__ __attribute__((noinline)) void attn_decode_careful(attn_kernel_args *args, uint32_t row_tiles, __attribute__((address_space(3))) DecodeShared<D> *sh) {
+    const r9vx_attn_problem a = *(const r9vx_attn_problem *)args;
+    attn_decode_rows<T, D, RT, FAR, true>(a, row_tiles, *(DecodeShared<D> *)sh);
+}
+
+template <class T, int D, int RT, bool FAR>
+__global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void attn_decode_kernel(r9vx_attn_problem a, uint32_t row_tiles) {
+    __shared__ DecodeShared<D> sh;
+    if (attn_decode_rows<T, D, RT, FAR, false>(a, row_tiles, sh))
+        attn_decode_careful<T, D, RT, FAR>((attn_kernel_args *)__builtin_amdgcn_kernarg_segment_ptr(), row_tiles, (__attribute__((address_space(3))) DecodeShared<D> *)&sh);
 }
 
 constexpr uint32_t kMostParts = 256;
@@ -427,7 +465,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(r9vx_attn_problem a, con
     for (int i = 0; i < N; ++i) {
         const float w = x[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x[i].x - m);
         if (x[i].x != -INFINITY || m == -INFINITY) sum += x[i].y * (m == -INFINITY ? 1.0f : w);
-        if (threadIdx.x < 64) weight[lane + 64 * i] = w;
+        if (threadIdx.x < 64) weight[lane + 64 * i] = x[i].x == -INFINITY ? 0.0f : attn_some(w);
     }
     for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off, R9VX_WAVE);
     __syncthreads();
@@ -478,14 +516,14 @@ __global__ __launch_bounds__(256) void attn_join_few_kernel(r9vx_attn_problem a,
     float m = x.x;
 #pragma unroll
     for (int off = 1; off < kFewParts; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, R9VX_WAVE));
-    const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - m);
+    const float w = x.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(x.x - m), some = x.x == -INFINITY ? 0.0f : attn_some(w);
     float sum = x.x != -INFINITY || m == -INFINITY ? x.y * (m == -INFINITY ? 1.0f : w) : 0.0f;
 #pragma unroll
     for (int off = 1; off < kFewParts; off <<= 1) sum += __shfl_xor(sum, off, R9VX_WAVE);
     r9vx_f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kMost; ++j) {
-        const float f = __shfl(w, (side + j * kSide) % kFewParts, R9VX_WAVE);
+        const float f = __shfl(some, (side + j * kSide) % kFewParts, R9VX_WAVE);
         if (f != 0.0f || f != f) o += v[j] * f; /* not 0 times what a part without weight left */
     }
 #pragma unroll

@@ -93,13 +93,6 @@ __device__ __forceinline__ void attn_priority() {
     if constexpr (D % 128) __builtin_amdgcn_s_setprio(P);
 }
 
-/* Bits of a pair of elements whose exponent is that of an infinity or a NaN. */
-template <class T>
-__device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
-    constexpr uint32_t e = T::kWide ? 0x7F80u : 0x7C00u;
-    return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
-}
-
 template <int D, int H>
 struct PrefillShared {
     __attribute__((aligned(1024))) uint16_t kv[H][4][PrefillShape<D>::TILE]; /* keys of two tiles, values of two; in the end the second half's sums */
@@ -371,7 +364,8 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
              * probabilities are then up to 2^8, and sums are rescaled seldom */
             const bool grown = top > m + kAttnSlack;
             if (__any(grown)) {
-                const float f = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 1.0f; /* (sums before the first score: zeros, or what is no number) */
+                float f = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 1.0f; /* (sums before the first score: zeros, or what is no number) */
+                if (CAREFUL) f = attn_some(f);
                 m = grown ? top : m;
                 l *= f;
 #pragma unroll
@@ -438,7 +432,8 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
         if (!half) {
             const float m1 = sh.tops[wave * 64 + lane], top = fmaxf(m, m1);
             /* a half that saw nothing (or scores of -infinity alone) has zeros, or a NaN of NaN scores */
-            const float f0 = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top), f1 = m1 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m1 - top);
+            float f0 = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top), f1 = m1 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m1 - top);
+            if (CAREFUL) f0 = attn_some(f0), f1 = attn_some(f1);
             l = l * f0 + sh.sums[wave * 64 + lane] * f1;
             m = top;
 #pragma unroll
@@ -490,8 +485,6 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     }
     return false;
 }
-
-typedef __attribute__((address_space(4))) const r9vx_attn_problem attn_kernel_args;
 
 /* Out of line: nothing of it takes registers of the first way's loop. */
 template <class T, int D, int H, bool FAR>

@@ -79,12 +79,12 @@ struct AttnBf16 {
     typedef __bf16 elem;
     static constexpr bool kWide = true; /* f32's exponents */
     static constexpr float kTop = -32.0f;
-    static constexpr uint32_t kNan = 0x7FC07FC0u;
+    static constexpr uint32_t kNan = 0x7FC07FC0u, kOnes = 0x3F803F80u;
     /* c and the eight elements, in f32 */
     static __device__ __forceinline__ float add8(x8 x, float c) {
         const r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c = r9vx_dot2_bf16(w[i], 0x3F803F80u, c);
+        for (int i = 0; i < 4; ++i) c = r9vx_dot2_bf16(w[i], kOnes, c);
         return c;
     }
     static __device__ __forceinline__ r9vx_f32x4 mma16(x8 a, x8 b, r9vx_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -95,11 +95,11 @@ struct AttnF16 {
     typedef _Float16 elem;
     static constexpr bool kWide = false;
     static constexpr float kTop = 15.0f;
-    static constexpr uint32_t kNan = 0x7E007E00u;
+    static constexpr uint32_t kNan = 0x7E007E00u, kOnes = 0x3C003C00u;
     static __device__ __forceinline__ float add8(x8 x, float c) {
         const r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c = r9vx_dot2_f16(w[i], 0x3C003C00u, c);
+        for (int i = 0; i < 4; ++i) c = r9vx_dot2_f16(w[i], kOnes, c);
         return c;
     }
     static __device__ __forceinline__ r9vx_f32x4 mma16(x8 a, x8 b, r9vx_f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -172,6 +172,19 @@ __device__ __forceinline__ const uint16_t *attn_row(AttnPlace where, const uint1
     const uint16_t *p = base + page * stride[0] + place * stride[1];
     return where == kAttnKept ? p : where == kAttnBad ? attn_nan_row<T>() : reinterpret_cast<const uint16_t *>(kAttnZeroRow);
 }
+
+/* Bits of a pair of elements whose exponent is that of an infinity or a NaN. */
+template <class T>
+__device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
+    constexpr uint32_t e = T::kWide ? 0x7F80u : 0x7C00u;
+    return ((w & e) == e ? 0xFFFFu : 0u) | ((w >> 16 & e) == e ? 0xFFFF0000u : 0u);
+}
+
+/* A weight of a sum that may hold an infinity: 0 times it would be none.  (Times a
+ * finite sum the least number adds nothing that counts.) */
+__device__ __forceinline__ float attn_some(float f) { return f < 0x1p-149f ? 0x1p-149f : f; }
+
+typedef __attribute__((address_space(4))) const r9vx_attn_problem attn_kernel_args; /* a kernel's first argument, for what it calls out of line */
 
 /* The larger of the two half waves' values. */
 __device__ __forceinline__ float attn_max32(float x) {
