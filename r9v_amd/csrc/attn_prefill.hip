@@ -16,11 +16,13 @@
  *
  * A tile's 1024 cycles of matrix instructions and its 700 or so of exponentials,
  * maxima and conversions overlap only where the two workgroups of a CU are at different
- * phases: 8192 causal tokens of 32 heads of 128 columns 532 to 564 us, 0.98 to 1.03
- * PFLOP/s, about half of the matrix unit's cycles (a large product reaches 1.47).
+ * phases: 8192 causal tokens of 32 heads of 128 columns 532 to 583 us, 0.94 to 1.03 of
+ * the matrix unit's 2.5 PFLOP/s (a large product reaches 1.47).
  * Eight waves at opposite phases behind shared barriers took 568 when this form
  * took 561, a tile's products in halves around the softmax no less: registers spilt.
- * A workgroup takes 5 us before its first tile is done: 17 tokens 12 us.
+ * A workgroup takes 5 us before its first tile is done: 17 tokens 12 us.  Heads of 256
+ * columns fill the 256 registers: a wave reloads two of those it spilt each tile (four
+ * of workgroups of two halves); the other widths spill none outside the second way.
  */
 #include "r9vx_attn_kernels.h"
 
@@ -74,15 +76,6 @@ __device__ __forceinline__ uint64_t attn_lanes(bool on, uint64_t lanes) {
     uint32_t lo = __builtin_amdgcn_readfirstlane(on ? (uint32_t)lanes : 0u), hi = __builtin_amdgcn_readfirstlane(on ? (uint32_t)(lanes >> 32) : 0u);
     asm volatile("" : "+s"(lo), "+s"(hi));
     return (uint64_t)hi << 32 | lo;
-}
-
-/* Holds what makes x before what follows: pure arithmetic is otherwise moved to its use,
- * behind the barriers that part the phases. */
-template <class X>
-__device__ __forceinline__ void attn_pin(X &x) {
-    r9vx_u32x4 w = __builtin_bit_cast(r9vx_u32x4, x);
-    asm volatile("" : "+v"(w));
-    x = __builtin_bit_cast(X, w);
 }
 
 /* A wave at its products goes before one at its softmax (8192 causal tokens, 96
@@ -361,7 +354,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
                 for (int e = 0; e < 16; ++e) top = fmaxf(top, sc[k][e]);
             top = attn_max32(top) * score.factor;
             /* a row's reference moves only where its largest score has grown by 2^8:
-             * probabilities are then up to 2^8, and sums are rescaled seldom */
+             * probabilities are then up to 2^8 times the reference's, and sums are rescaled seldom */
             const bool grown = top > m + kAttnSlack;
             if (__any(grown)) {
                 float f = grown && m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 1.0f; /* (sums before the first score: zeros, or what is no number) */
@@ -374,12 +367,14 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
                     for (int e = 0; e < 16; ++e) o[d][e] *= f;
             }
             const float ref = (m == -INFINITY ? 0.0f : m) - (T::kTop - kAttnSlack);
+            /* One number each: second halves would make half as many products again of a tile's, for
+             * 1.6e-3 from the definition instead of 2.1e-3 (bf16, 8192 tokens). */
 #pragma unroll
             for (int s = 0; s < KT / 16; ++s) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     p[s][e] = (typename T::elem)__builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], score.factor, -ref));
-                l = T::add8(p[s], l); /* of what is multiplied, in f32 */
+                l = T::add8(p[s], l); /* of what is multiplied, in f32: a rounding moves the weights among each other alone */
             }
             attn_priority<D, 1>();
 #pragma unroll
