@@ -102,15 +102,18 @@ __device__ __forceinline__ bool attn_decode_rows(const r9vx_attn_problem &a, uin
     auto &jl = sh.jl;
     auto &area = sh.area;
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t thread = threadIdx.x, bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
+    if (CAREFUL) /* worked out anew: what the first way's loop would keep for this one is reloaded in it */
+        asm volatile("" : "+v"(thread), "+s"(bx), "+s"(by), "+s"(bz));
+    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6);
     const int col = lane & 15, g4 = lane >> 4;
     /* Consecutive workgroups go to the eight dies in turn.  Heads, then sequences,
      * then parts, so that it is not always the same dies whose sequences have ended;
      * and with each part the sequences move on, so that a long one's parts are not all
      * on one die (24 of 300 to 16384 keys, 2 kv heads of 256 columns: 73 us, 86 without it). */
-    uint32_t split = blockIdx.z, b = blockIdx.y, kvh = blockIdx.x, tile = 0;
+    uint32_t split = bz, b = by, kvh = bx, tile = 0;
     if (row_tiles > 1) { /* the tiles of the same keys one after another on one die (40 rows, 4 x 8192 keys of 256 columns: 34 us; beside each other on several 44) */
-        const uint32_t slot = blockIdx.x / 8, turn = slot / row_tiles, group = turn * 8 + blockIdx.x % 8, seqs = group / a.kv_heads;
+        const uint32_t slot = bx / 8, turn = slot / row_tiles, group = turn * 8 + bx % 8, seqs = group / a.kv_heads;
         tile = slot - turn * row_tiles, kvh = group - seqs * a.kv_heads, split = seqs / a.b, b = seqs - split * a.b;
         if (split >= a.splits) return false;
     }
@@ -119,7 +122,7 @@ __device__ __forceinline__ bool attn_decode_rows(const r9vx_attn_problem &a, uin
     const int row0 = (int)tile * RT * 16;
     const int length = a.lengths[b];
     const bool bad_length = length < 0 || length > (int)a.len_bucket;
-    if (bad_length && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
+    if (bad_length && thread == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
     const int start = a.starts ? a.starts[b] : 0;
     const int p0 = length - (int)a.t_bucket; /* of token 0 */
 
@@ -213,7 +216,7 @@ __device__ __forceinline__ bool attn_decode_rows(const r9vx_attn_problem &a, uin
 
     /* keys [vlo, vhi) have values: those that some row sees, or of the second way those that its token does */
     int vlo = ulo, vhi = uhi;
-    if (!CAREFUL && threadIdx.x == 0) sh.redo = 0;
+    if (!CAREFUL && thread == 0) sh.redo = 0;
     for (int pass = CAREFUL ? first : last; pass <= last; ++pass) {
         if (CAREFUL) {
             attn_seen(a.window, 1, p0 + pass, length, start, 0, vlo, vhi);
@@ -362,7 +365,7 @@ __device__ __forceinline__ bool attn_decode_rows(const r9vx_attn_problem &a, uin
                     for (int j = 0; j < S::DL; j += 2)
                         *reinterpret_cast<float2 *>(sums + col * (D + 4) + c * S::CW + S::DL * (4 * g4 + e) + j) = make_float2(o[r][c][j][e], o[r][c][j + 1][e]);
             __syncthreads();
-            for (int i = threadIdx.x; i < 16 * D / 4; i += 64 * kWaves) {
+            for (int i = thread; i < 16 * D / 4; i += 64 * kWaves) {
                 const int in = i / (D / 4), c = i % (D / 4) * 4, row = row0 + r * 16 + in;
                 const int tok = attn_token(row, a.group_magic);
                 if (row >= rows || (CAREFUL && tok != pass)) continue;
@@ -407,18 +410,15 @@ __device__ __forceinline__ bool attn_decode_rows(const r9vx_attn_problem &a, uin
     return !CAREFUL && sh.redo;
 }
 
-/* Out of line: nothing of it takes registers of the first way's loop. */
-template <class T, int D, int RT, bool FAR>
-__device__ __attribute__((noinline)) void attn_decode_careful(attn_kernel_args *args, uint32_t row_tiles, __attribute__((address_space(3))) DecodeShared<D> *sh) {
-    const r9vx_attn_problem a = *(const r9vx_attn_problem *)args;
-    attn_decode_rows<T, D, RT, FAR, true>(a, row_tiles, *(DecodeShared<D> *)sh);
-}
-
 template <class T, int D, int RT, bool FAR>
 __global__ __launch_bounds__(64 * kWaves, DecodeShape<D>::kWavesASimd(RT)) void attn_decode_kernel(r9vx_attn_problem a, uint32_t row_tiles) {
     __shared__ DecodeShared<D> sh;
-    if (attn_decode_rows<T, D, RT, FAR, false>(a, row_tiles, sh))
-        attn_decode_careful<T, D, RT, FAR>((attn_kernel_args *)__builtin_amdgcn_kernarg_segment_ptr(), row_tiles, (__attribute__((address_space(3))) DecodeShared<D> *)&sh);
+    if (!attn_decode_rows<T, D, RT, FAR, false>(a, row_tiles, sh)) return;
+    /* (in line: as a function it takes 0.3 to 1 KB of scratch a lane, 480 MB of a card's memory) */
+    uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args), "+s"(row_tiles));
+    const r9vx_attn_problem again = *(const r9vx_attn_problem *)(attn_kernel_args *)args;
+    attn_decode_rows<T, D, RT, FAR, true>(again, row_tiles, sh);
 }
 
 constexpr uint32_t kMostParts = 256;
