@@ -21,8 +21,7 @@
  * Eight waves at opposite phases behind shared barriers took 568 when this form
  * took 561, a tile's products in halves around the softmax no less: registers spilt.
  * A workgroup takes 5 us before its first tile is done: 17 tokens 12 us.  Heads of 256
- * columns fill the 256 registers: a wave reloads two of those it spilt each tile (four
- * of workgroups of two halves); the other widths spill none outside the second way.
+ * columns fill the 256 registers and spill some; the other widths spill none.
  */
 #include "r9vx_attn_kernels.h"
 
@@ -106,12 +105,13 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     using S = PrefillShape<D>;
     typedef typename T::x8 x8;
     constexpr int KT = S::KT, NK = KT / 32;
-    const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c32 = lane & 31, h2 = lane >> 5;
+    uint32_t thread = threadIdx.x, id = blockIdx.x;
+    if (CAREFUL) asm volatile("" : "+v"(thread), "+s"(id)); /* worked out anew: nothing is kept for this way through the first one's loop */
+    const int lane = thread & 63, wave8 = __builtin_amdgcn_readfirstlane(thread >> 6), c32 = lane & 31, h2 = lane >> 5;
     const int half = H == 1 ? 0 : wave8 / kWaves, wave = H == 1 ? wave8 : wave8 % kWaves;
     auto &kv = sh.kv[half];
     auto &bounds = sh.bounds;
     auto &odds = sh.odds[half];
-    uint32_t id = blockIdx.x;
     const uint32_t kvh = id % a.kv_heads;
     id /= a.kv_heads;
     const uint32_t split = id % a.splits;
@@ -119,7 +119,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
 
     if (tile == 0 && kvh == 0 && split == 0 && a.status) {
         bool odd = false;
-        for (uint32_t i = threadIdx.x; i < a.b; i += H * kThreads) odd |= a.offsets[i] < 0 || a.offsets[i] > a.offsets[i + 1] || (int64_t)a.offsets[i + 1] > a.t;
+        for (uint32_t i = thread; i < a.b; i += H * kThreads) odd |= a.offsets[i] < 0 || a.offsets[i] > a.offsets[i + 1] || (int64_t)a.offsets[i + 1] > a.t;
         if (odd) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
     }
     AttnTile part;
@@ -128,7 +128,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     const int off = part.offset, news = part.n;
     const int length = a.lengths[b], prefix = a.prefix ? a.prefix[b] : 0;
     const bool bad_length = length < 0 || length > (int)a.len_bucket;
-    if (bad_length && threadIdx.x == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
+    if (bad_length && thread == 0 && a.status) atomicOr(a.status, R9VX_STATUS_BAD_LENGTH);
 
     /* this lane's row: the token and the head that row r0 + i is */
     const uint32_t rows = (uint32_t)news * a.group, i0 = wave * 32, t0 = r0 / a.group, h0 = r0 - t0 * a.group;
@@ -161,7 +161,7 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     seen_by(n0 - 1, any, uhi);
     seen_by(i0 < n0 ? i0 : 0, any, wfh);
     seen_by(i0 < n0 ? n1 - 1 : 0, wfl, any);
-    if (!CAREFUL && threadIdx.x == 0) sh.redo = 0; /* (the second way is on while other waves read it) */
+    if (!CAREFUL && thread == 0) sh.redo = 0; /* (the second way is on while other waves read it) */
     if (a.starts) {
         int most = there ? lo : 0, least = some ? lo : INT32_MAX;
 #pragma unroll
@@ -481,18 +481,16 @@ __device__ __forceinline__ bool attn_prefill_rows(const r9vx_attn_problem &a, ui
     return false;
 }
 
-/* Out of line: nothing of it takes registers of the first way's loop. */
-template <class T, int D, int H, bool FAR>
-__device__ __attribute__((noinline)) void attn_prefill_careful(attn_kernel_args *args, uint32_t tiles, __attribute__((address_space(3))) PrefillShared<D, H> *sh) {
-    const r9vx_attn_problem a = *(const r9vx_attn_problem *)args;
-    attn_prefill_rows<T, D, H, FAR, true>(a, tiles, *(PrefillShared<D, H> *)sh);
-}
-
 template <class T, int D, int H, bool FAR>
 __global__ __launch_bounds__(H * kThreads, 2) void attn_prefill_kernel(r9vx_attn_problem a, uint32_t tiles) {
     __shared__ PrefillShared<D, H> sh;
-    if (attn_prefill_rows<T, D, H, FAR, false>(a, tiles, sh))
-        attn_prefill_careful<T, D, H, FAR>((attn_kernel_args *)__builtin_amdgcn_kernarg_segment_ptr(), tiles, (__attribute__((address_space(3))) PrefillShared<D, H> *)&sh);
+    if (!attn_prefill_rows<T, D, H, FAR, false>(a, tiles, sh)) return;
+    /* (in line: as a function it took 300 to 790 bytes of scratch a lane, 390 MB of a card's memory, and
+     * registers that left 64 columns two waves a SIMD instead of three: 8192 tokens 375 us, 355 so) */
+    uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args), "+s"(tiles));
+    const r9vx_attn_problem again = *(const r9vx_attn_problem *)(attn_kernel_args *)args;
+    attn_prefill_rows<T, D, H, FAR, true>(again, tiles, sh);
 }
 
 template <class T, int D, bool FAR>

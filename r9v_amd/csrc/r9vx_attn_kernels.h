@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t attn_odd(uint32_t w) {
  * finite sum the least number adds nothing that counts.) */
 __device__ __forceinline__ float attn_some(float f) { return f < 0x1p-149f ? 0x1p-149f : f; }
 
-typedef __attribute__((address_space(4))) const r9vx_attn_problem attn_kernel_args; /* a kernel's first argument, for what it calls out of line */
+typedef __attribute__((address_space(4))) const r9vx_attn_problem attn_kernel_args; /* a kernel's first argument, read again */
 
 /* The larger of the two half waves' values. */
 __device__ __forceinline__ float attn_max32(float x) {
